@@ -66,6 +66,31 @@ class HcPostArgs(C.Structure):
     _fields_ = [("R_old", c_void_p), ("post", c_void_p), ("comb", c_void_p), ("R_new", c_void_p)]
 
 
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_sum", c_void_p),
+                ("table", c_void_p), ("table_ld", c_int), ("n_blocks", c_int), ("n_kv", c_int), ("head_dim", c_int)]
+
+
+class AttnBatchDesc(C.Structure):
+    _fields_ = [("start", c_void_p), ("kv_len", c_void_p), ("n_seq", c_int), ("n_tokens", c_int), ("max_new", c_int), ("max_len", c_int)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("ld_q", c_int64), ("ld_k", c_int64), ("ld_v", c_int64),
+                ("is_bf16", c_int), ("n_q", c_int), ("q_w", c_void_p), ("k_w", c_void_p), ("eps", c_float), ("cos", c_void_p),
+                ("sin", c_void_p), ("pos", c_void_p), ("n_pos", c_int), ("rot_dim", c_int), ("pairs", c_int), ("q_out", c_void_p)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [("q", c_void_p), ("ld_q", c_int64), ("is_bf16", c_int), ("n_q", c_int), ("scale", c_float), ("window", c_int),
+                ("sel", c_void_p), ("n_sel", c_int), ("out", c_void_p), ("lse", c_void_p)]
+
+
+class SelectArgs(C.Structure):
+    _fields_ = [("q", c_void_p), ("ld_q", c_int64), ("is_bf16", c_int), ("n_q", c_int), ("n_first", c_int), ("n_last", c_int),
+                ("n_sel", c_int), ("sel", c_void_p)]
+
+
 _SIGNATURES = {
     "maya_version": (C.c_char_p, []),
     "maya_last_cuda_error": (c_int, []),
@@ -144,6 +169,12 @@ _SIGNATURES = {
     "maya_peer_buffer_close": (c_int, [c_void_p]),
     "maya_peer_buffer_destroy": (c_int, [c_void_p]),
     "maya_quantize_weights_host": (c_int, [c_int, c_void_p, c_int64, c_int64, c_void_p]),
+    "maya_qk_norm_rope_append": (c_int, [C.POINTER(KvCacheDesc), C.POINTER(AttnBatchDesc), C.POINTER(RopeArgs), c_void_p]),
+    "maya_kv_read": (c_int, [C.POINTER(KvCacheDesc), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "maya_attn_scratch_bytes": (c_size_t, [C.POINTER(KvCacheDesc), c_int, c_int]),
+    "maya_attn_q8": (c_int, [C.POINTER(KvCacheDesc), C.POINTER(AttnBatchDesc), C.POINTER(AttnArgs), c_void_p, c_size_t, c_void_p]),
+    "maya_attn_error": (c_int, [c_void_p, c_void_p]),
+    "maya_block_select": (c_int, [C.POINTER(KvCacheDesc), C.POINTER(AttnBatchDesc), C.POINTER(SelectArgs), c_void_p]),
     "maya_synth_weights": (c_int, [c_int, c_uint64, c_float, c_int64, c_int64, c_void_p, c_void_p]),
 }
 

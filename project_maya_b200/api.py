@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import ExpertLayout, HcPostArgs, MmqProduct, MoeLayerDesc, MoePlan, MoeWin
+from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RopeArgs, SelectArgs
 
 Q8_0, Q4_K, IQ3_S, IQ2_S = 8, 12, 21, 22
 Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ1_S, IQ4_XS = 13, 14, 16, 18, 19, 23      # decode paths only (see maya_ggml_type in the header)
@@ -622,3 +622,174 @@ class MoePrefill:
         if code:
             self.chain.zero_()
         return code
+
+
+# ---------------------------------------------------------------- attention over a paged 8-bit cache
+KV_BLOCK = 64                # tokens of a block (MAYA_KV_BLOCK)
+
+
+class KvCache:
+    """The keys and values of a layer's sequences in 8 bits: blocks of 64 tokens with an f32 scale a block and key/value head
+    (include/maya_attn.h states the layout).  A handle over the caller's tensors; KvCache.empty allocates them.
+
+    k uint8 [n_blocks, n_kv, head_dim / 64, 64, 64] (the last two: token, value), v uint8 [n_blocks, n_kv, head_dim, 64], k_scale and
+    v_scale f32 [n_blocks, n_kv], table i32 [n_seq, blocks of a sequence] (which block holds tokens 64 b .. of sequence s), k_sum
+    int16 [n_blocks, n_kv, head_dim] or None (block selection needs it).  Entries of `table` may be changed between calls; where its
+    first dimension is longer than a batch, the batch's sequences are its first rows."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, k_sum=None):
+        n_blocks, n_kv, panels, tokens, width = k.shape
+        head_dim = 64 * panels
+        assert (tokens, width) == (KV_BLOCK, 64) and v.shape == (n_blocks, n_kv, head_dim, KV_BLOCK) and table.dim() == 2
+        assert k_scale.shape == v_scale.shape == (n_blocks, n_kv) and (k_sum is None or k_sum.shape == (n_blocks, n_kv, head_dim))
+        assert k.dtype == v.dtype == torch.uint8 and k_scale.dtype == v_scale.dtype == torch.float32 and table.dtype == torch.int32
+        assert k_sum is None or k_sum.dtype == torch.int16
+        self.k, self.v, self.k_scale, self.v_scale, self.table, self.k_sum = k, v, k_scale, v_scale, table, k_sum
+        self.n_blocks, self.n_kv, self.head_dim = n_blocks, n_kv, head_dim
+        self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), _ptr(k_sum), _ptr(table), table.shape[1], n_blocks, n_kv,
+                                head_dim)
+        self._ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_blocks: int, n_kv: int, head_dim: int, table, sums: bool = True):
+        """A cache of n_blocks blocks on the table's device; its contents are whatever the memory held."""
+        dev = table.device
+        return cls(torch.empty((n_blocks, n_kv, head_dim // 64, KV_BLOCK, 64), dtype=torch.uint8, device=dev),
+                   torch.empty((n_blocks, n_kv, head_dim, KV_BLOCK), dtype=torch.uint8, device=dev),
+                   torch.empty((n_blocks, n_kv), dtype=torch.float32, device=dev), torch.empty((n_blocks, n_kv), dtype=torch.float32, device=dev),
+                   table, torch.empty((n_blocks, n_kv, head_dim), dtype=torch.int16, device=dev) if sums else None)
+
+    def read(self, blocks, counts=None, k=None, v=None, mean=None, dtype=torch.bfloat16, stream=None):
+        """Blocks (i32 [n]) as the values they stand for: k and v [n, 64, n_kv, head_dim], and the mean key [n, n_kv, head_dim] of each
+        block's first counts[i] tokens (None without sums); tokens from counts[i] on are zeros."""
+        n, dev = blocks.numel(), blocks.device
+        if k is None:
+            k = torch.empty((n, KV_BLOCK, self.n_kv, self.head_dim), dtype=dtype, device=dev)
+        if v is None:
+            v = torch.empty((n, KV_BLOCK, self.n_kv, self.head_dim), dtype=dtype, device=dev)
+        if mean is None and self.k_sum is not None:
+            mean = torch.empty((n, self.n_kv, self.head_dim), dtype=dtype, device=dev)
+        assert k.dtype == v.dtype and (mean is None or mean.dtype == k.dtype) and k.dtype in (torch.float32, torch.bfloat16)
+        assert blocks.dtype == torch.int32 and (counts is None or (counts.dtype == torch.int32 and counts.numel() == n))
+        _check("kv_read", _lib.load().maya_kv_read(self._ref, _ptr(blocks), _ptr(counts), n, int(k.dtype == torch.bfloat16), _ptr(k), _ptr(v),
+                                                   _ptr(mean), _stream(stream)))
+        return k, v, mean
+
+
+class AttnBatch:
+    """The new tokens of a pass: those of sequence s are rows start[s] .. start[s + 1] - 1 (i32 [n_seq + 1]) and the last of its
+    kv_len[s] tokens (i32 [n_seq]; it counts them).  n_tokens = start[n_seq]; max_new and max_len: upper bounds of the new tokens and
+    of kv_len of any sequence, which size the launches."""
+
+    def __init__(self, start, kv_len, n_tokens: int, max_new: int, max_len: int):
+        assert start.dtype == kv_len.dtype == torch.int32 and start.numel() == kv_len.numel() + 1
+        self.start, self.kv_len, self.n_tokens = start, kv_len, n_tokens
+        self.desc = AttnBatchDesc(_ptr(start), _ptr(kv_len), kv_len.numel(), n_tokens, max_new, max_len)
+        self._ref = C.byref(self.desc)
+
+    @classmethod
+    def of(cls, new, kv_len, device="cuda"):
+        """From host lists: the new tokens of every sequence and its tokens with them."""
+        start = [0]
+        for n in new:
+            start.append(start[-1] + n)
+        return cls(torch.tensor(start, dtype=torch.int32, device=device), torch.tensor(list(kv_len), dtype=torch.int32, device=device),
+                   start[-1], max(new, default=0), max(kv_len, default=0))
+
+
+class Rope:
+    """What stands between a layer's projections and its attention: cos and sin f32 [positions, rot_dim / 2] (None: no rotation), the
+    weights f32 [head_dim] of the queries' and keys' RMS norms (None: no norm).  pairs: value 2 i turns with 2 i + 1, else i with
+    i + rot_dim / 2."""
+
+    def __init__(self, cos=None, sin=None, q_w=None, k_w=None, eps: float = 1e-6, pairs: bool = False):
+        for t in (cos, sin, q_w, k_w):
+            assert t is None or t.dtype == torch.float32
+        assert (cos is None) == (sin is None) and (cos is None or cos.shape == sin.shape)
+        self.cos, self.sin, self.q_w, self.k_w, self.eps, self.pairs = cos, sin, q_w, k_w, eps, pairs
+        self.n_pos, self.rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
+
+
+def _rows(x, heads: int, head_dim: int):
+    """(address, elements between rows) of [tokens, heads, head_dim] whose heads lie side by side: a view into wider rows is fine."""
+    assert x.is_cuda and x.dim() == 3 and x.shape[1:] == (heads, head_dim) and x.stride(2) == 1 and (heads == 1 or x.stride(1) == head_dim)
+    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else heads * head_dim
+
+
+class KvAttention:
+    """The attention of one layer over a KvCache: n_q query heads, the first n_q / n_kv of which share key/value head 0, and so on.
+
+    append(batch, q, k, v, rope) normalises and rotates the new tokens' queries and keys and puts keys and values into the cache;
+    forward(batch, q) attends over it; select(batch, q) chooses the n_sel blocks each token reads and forward(batch, q, sel=...) attends over those
+    alone.  f32 or bf16; q, k, v [n_tokens, heads, head_dim], views into rows of projections among them.  scale: of the scores
+    (head_dim ** -0.5); window > 0: a token sees the last `window` positions.  The scratch belongs to this object: one stream at a
+    time."""
+
+    def __init__(self, cache: KvCache, n_q: int, scale: float | None = None, window: int = 0, n_sel: int = 0, n_first: int = 1,
+                 n_last: int = 2, max_tokens: int = 65536):
+        self.cache, self.n_q, self.n_sel = cache, n_q, n_sel
+        nbytes = int(_lib.load().maya_attn_scratch_bytes(cache._ref, n_q, max_tokens))
+        if nbytes == 0:
+            raise MayaError("attn_scratch_bytes", -1)
+        self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=cache.k.device)
+        self.scratch[:1 << 19].zero_()                      # the error word and the counters
+        self._attn = AttnArgs(None, 0, 0, n_q, cache.head_dim ** -0.5 if scale is None else scale, window, None, 0, None, None)
+        self._select = SelectArgs(None, 0, 0, n_q, n_first, n_last, n_sel, None)
+        self._rope = RopeArgs(n_q=n_q)
+        self._refs = C.byref(self._attn), C.byref(self._select), C.byref(self._rope)
+
+    def _act(self, batch, x):
+        assert x.shape[0] == batch.n_tokens and x.dtype in (torch.float32, torch.bfloat16)
+        assert batch.desc.n_seq <= self.cache.table.shape[0]
+        return int(x.dtype == torch.bfloat16)
+
+    def append(self, batch: AttnBatch, q, k, v, rope: Rope, pos=None, q_out=None, stream=None):
+        """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
+        (None: the tokens' positions)."""
+        a, c = self._rope, self.cache
+        a.is_bf16 = self._act(batch, q)
+        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
+        if k is not None:
+            assert k.dtype == v.dtype == q.dtype and k.shape[0] == v.shape[0] == batch.n_tokens
+            a.k, a.ld_k = _rows(k, c.n_kv, c.head_dim)
+            a.v, a.ld_v = _rows(v, c.n_kv, c.head_dim)
+        else:
+            a.k = a.v = None
+        q_out = q_out if q_out is not None else torch.empty((batch.n_tokens, self.n_q, c.head_dim), dtype=q.dtype, device=q.device)
+        assert q_out.dtype == q.dtype and (pos is None or (pos.dtype == torch.int32 and pos.numel() == batch.n_tokens))
+        a.q_w, a.k_w, a.eps = _ptr(rope.q_w), _ptr(rope.k_w), rope.eps
+        a.cos, a.sin, a.pos, a.n_pos, a.rot_dim, a.pairs = _ptr(rope.cos), _ptr(rope.sin), _ptr(pos), rope.n_pos, rope.rot_dim, int(rope.pairs)
+        a.q_out = _ptr(q_out)
+        _check("qk_norm_rope_append", _lib.load().maya_qk_norm_rope_append(c._ref, batch._ref, self._refs[2], _stream(stream)))
+        return q_out
+
+    def forward(self, batch: AttnBatch, q, sel=None, out=None, lse=None, stream=None):
+        """out [n_tokens, n_q, head_dim] of q's type.  sel i32 [n_tokens, n_kv, n_sel] (select's): the blocks each token reads.
+        lse f32 [n_tokens, n_q]: ln of the sum of exp(scores), for joining with attention over other tokens."""
+        a, c = self._attn, self.cache
+        a.is_bf16 = self._act(batch, q)
+        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
+        out = out if out is not None else torch.empty((batch.n_tokens, self.n_q, c.head_dim), dtype=q.dtype, device=q.device)
+        assert out.dtype == q.dtype and out.shape == (batch.n_tokens, self.n_q, c.head_dim)
+        assert lse is None or (lse.dtype == torch.float32 and lse.shape == (batch.n_tokens, self.n_q))
+        if sel is not None:
+            assert sel.dtype == torch.int32 and sel.shape[:2] == (batch.n_tokens, c.n_kv)
+            a.n_sel = sel.shape[2]
+        a.sel, a.out, a.lse = _ptr(sel), _ptr(out), _ptr(lse)
+        _check("attn_q8", _lib.load().maya_attn_q8(c._ref, batch._ref, self._refs[0], self.scratch.data_ptr(), self.scratch.numel(), _stream(stream)))
+        return out
+
+    def select(self, batch: AttnBatch, q, sel=None, stream=None):
+        """i32 [n_tokens, n_kv, n_sel]: the blocks each token reads, ascending, -1 behind the last."""
+        a, c = self._select, self.cache
+        a.is_bf16 = self._act(batch, q)
+        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
+        sel = sel if sel is not None else torch.empty((batch.n_tokens, c.n_kv, self.n_sel), dtype=torch.int32, device=q.device)
+        assert sel.dtype == torch.int32 and sel.shape == (batch.n_tokens, c.n_kv, self.n_sel)
+        a.sel = _ptr(sel)
+        _check("block_select", _lib.load().maya_block_select(c._ref, batch._ref, self._refs[1], _stream(stream)))
+        return sel
+
+    def error(self, stream=None) -> int:
+        """1 after a call whose bounded wait ran out (its outputs are not valid; sticky); synchronises the stream."""
+        return int(_lib.load().maya_attn_error(self.scratch.data_ptr(), _stream(stream)))

@@ -1,0 +1,39 @@
+// kv_attn.cuh - attention over the paged 8-bit cache, what its kernels share: arguments, work tiles, partial results and their join.
+//
+// softmax(scale q.K) V over one tile of query rows in one pass over the cache: running maximum m (base 2), sum l and output O in f32.
+//   s_j = (q . k_j) * scale * k_scale[block] * log2(e)          p_j = 2^(s_j - m)          O = sum p_j v_j,  l = sum p_j
+// The codes of K and V become f16 exactly (|code| <= 127); a query row is multiplied by a power of two that brings its largest
+// value to 2^11 .. 2^12 and rounded to f16, or for f32 activations split in two f16 terms (22 bits); P likewise, as 2^12 p
+// times v_scale[block] / (the largest v_scale so far), which keeps it in f16's range whatever the scales.  Products are summed in f32.
+#pragma once
+
+#include "maya_kv.cuh"
+#include "maya_stream.cuh"
+
+namespace maya {
+
+constexpr float kPBias = 12.0f;                  // P is kept as 2^12 p
+constexpr float kNone = -INFINITY;
+
+struct AttnView {
+    const void* q;
+    int64_t ld_q;
+    void* out;
+    float* lse;
+    const int* sel;
+    int n_sel, n_q, group, window, wide_q;
+    float scale_log2;                            // scale * log2(e)
+    int row_tiles;                               // tiles of a sequence (of a token, with sel)
+    int split_blocks, n_split;                   // cache blocks a split takes, splits of the longest tile
+    unsigned* error;
+    unsigned* counters;                          // one a (tile, head): partials that have been written
+    float* part_o;                               // [tile][head][split][rows][D]
+    float2* part_ml;                             // [tile][head][split][rows]
+};
+
+// The scratch: a 256-byte head (the error word), the counters, the partials.
+constexpr size_t kAttnHead = 256;
+constexpr int kCountersMost = 1 << 16;           // (tile, head) pairs that can be split
+constexpr int kPartRows = 296 * 4 * 64;          // rows of partials: four splits a resident block of the widest tiles, see attn_q8's rule
+
+}  // namespace maya
