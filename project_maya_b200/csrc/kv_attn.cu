@@ -426,13 +426,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, RW>::ctas) attn_kernel(c
 }
 
 template<int D, bool F32, int RW>
-int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, uint8_t* scratch, size_t scratch_bytes, cudaStream_t s) {
+int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, size_t scratch_bytes, cudaStream_t s) {
     using K = Cfg<D, F32, RW>;
-    AttnView A{};
-    A.q = a.q; A.ld_q = a.ld_q; A.out = a.out; A.lse = a.lse; A.sel = a.sel; A.n_sel = a.n_sel; A.n_q = a.n_q; A.group = a.n_q / c.n_kv;
-    A.window = a.window;
-    A.wide_q = rows_wide(a.q, a.ld_q, F32 ? 4 : 2);
-    A.scale_log2 = a.scale * 1.4426950408889634f;
     const long long rows = a.sel ? A.group : (long long) b.max_new * A.group;
     A.row_tiles = (int) ((rows + K::rows - 1) / K::rows);
     const long long tiles = (long long) A.row_tiles * (a.sel ? b.n_tokens : b.n_seq);
@@ -459,7 +454,6 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
     }
     A.split_blocks = (int) per;
     A.n_split = (int) n_split;
-    A.error = (unsigned*) scratch;
     A.counters = (unsigned*) (scratch + kAttnHead);
     A.part_ml = (float2*) (scratch + kAttnHead + kCountersMost * 4);
     A.part_o = (float*) (A.part_ml + pairs * n_split * K::rows);
@@ -471,11 +465,12 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
 }
 
 template<int D, bool F32>
-int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, uint8_t* scratch, size_t bytes, cudaStream_t s) {
+int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, uint8_t* scratch, size_t bytes,
+            cudaStream_t s) {
     const long long rows = (long long) (a.sel ? 1 : b.max_new) * (a.n_q / c.n_kv);
-    if (rows <= 16) return launch_attn<D, F32, 1>(c, b, a, scratch, bytes, s);
-    if (rows <= 32) return launch_attn<D, F32, 2>(c, b, a, scratch, bytes, s);
-    return launch_attn<D, F32, 4>(c, b, a, scratch, bytes, s);
+    if (rows <= 16) return launch_attn<D, F32, 1>(c, b, a, A, scratch, bytes, s);
+    if (rows <= 32) return launch_attn<D, F32, 2>(c, b, a, A, scratch, bytes, s);
+    return launch_attn<D, F32, 4>(c, b, a, A, scratch, bytes, s);
 }
 
 }  // namespace
@@ -501,7 +496,15 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     if ((a->sel && a->n_sel > MAYA_MAX_SELECTED) || c->n_kv > 65535) return refuse(MAYA_ERR_LIMIT);
     if (!scratch || ((uintptr_t) scratch & 255u) || scratch_bytes < kAttnHead + kCountersMost * 4) return refuse(MAYA_ERR_ARG);
     cudaStream_t s = as_stream(stream);
-#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, (uint8_t*) scratch, scratch_bytes, s) : by_rows<D, true>(*c, *b, *a, (uint8_t*) scratch, scratch_bytes, s)
+    AttnView A{};
+    A.q = a->q; A.ld_q = a->ld_q; A.out = a->out; A.lse = a->lse; A.sel = a->sel; A.n_sel = a->n_sel; A.n_q = a->n_q; A.group = a->n_q / c->n_kv;
+    A.window = a->window;
+    A.wide_q = rows_wide(a->q, a->ld_q, a->is_bf16 ? 2 : 4);
+    A.scale_log2 = a->scale * 1.4426950408889634f;
+    A.error = (unsigned*) scratch;
+    st = attn_prompt(*c, *b, A, a->is_bf16 != 0, s);
+    if (st != kNotTaken) return st;
+#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, (uint8_t*) scratch, scratch_bytes, s) : by_rows<D, true>(*c, *b, *a, A, (uint8_t*) scratch, scratch_bytes, s)
     switch (c->head_dim) {
         case 64: return ATTN(64);
         case 128: return ATTN(128);

@@ -36,4 +36,8 @@ constexpr size_t kAttnHead = 256;
 constexpr int kCountersMost = 1 << 16;           // (tile, head) pairs that can be split
 constexpr int kPartRows = 296 * 4 * 64;          // rows of partials: four splits a resident block of the widest tiles, see attn_q8's rule
 
+constexpr int kNotTaken = 1;
+// Attention of a prompt's rows on tcgen05 (kv_attn_prompt.cu); kNotTaken: not that kernel's call, nothing launched.
+int attn_prompt(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, cudaStream_t s);
+
 }  // namespace maya

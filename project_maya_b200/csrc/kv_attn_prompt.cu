@@ -1,0 +1,439 @@
+// kv_attn_prompt.cu - attention over the paged 8-bit cache for prompts (many query rows a sequence), on tcgen05.  bf16 activations, head sizes
+// 64 and 128.
+//
+// A thread block owns 256 rows - (token, head of the group) pairs of one key/value head, two tiles of 128 - and walks over the cache
+// blocks they see, 128 tokens a step:
+//   warps 0..3, 4..7   softmax of tile 0, 1: a thread a row.  64 scores at a time (a cache block: one scale) from tensor memory, 2^x, P back
+//                      to tensor memory as f16 over the scores it came from.
+//   warps 8..11        expand the codes of K and V to f16 into the swizzled shared-memory tiles that the tensor cores read, one step
+//                      ahead (codes come straight to registers: staging them would cost shared-memory bandwidth the products need).
+//   warp 12            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory).  (Warps 13..15 only
+//                      complete the group whose registers the others take.)
+// The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
+// tensor pipe (D = 128) and 2048 of the exponential's pipe.
+//
+// Numbers.  A query row is scaled by a power of two into f16 (exact for bf16).  With vs the block's scale of V,
+//   P = 2^(s + log2 vs - m + 4),  O = sum P code,  l = sum P / vs:
+// V's scale rides in the exponent, so P is in f16's range whatever the scales.  m is raised only when a row's maximum passes it by more than 8 (P
+// then stays below 2^12): O in tensor memory is rescaled a few times a row instead of at every step.
+#include <cuda_fp16.h>
+
+#include "kv_attn.cuh"
+#include "maya_tcgen05.cuh"
+
+namespace maya {
+namespace {
+
+constexpr int kPThreads = 16 * 32;
+// Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 176 + 128 * 104 + 128 * 48 = 64512.
+constexpr int kRegsSoftmax = 176, kRegsExpand = 104, kRegsIssue = 48;
+constexpr float kRise = 8.0f, kUp = 4.0f;
+constexpr float kVsLeast = 1e-30f;               // a scale of 0 is this in the exponent: its P is 0 in f16 and right in l
+constexpr int kMetaRing = 4;
+
+struct StepMeta {                                // of the two cache blocks of a step
+    int lb[2];
+    float ks[2], lv[2], ivs[2];
+};
+
+template<int D> struct PCfg {
+    static constexpr int panels = D / 64;
+    static constexpr int tile = 128 * D * 2;     // bytes of a 128-row f16 tile (Q, K; V transposed the same)
+    static constexpr int q = 0, k = 2 * tile, v = 4 * tile, end = 6 * tile;
+    static constexpr size_t smem = (size_t) end + 1024;      // + the start's rounding to 1024
+    static constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t) (128 >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
+    static constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t) (D >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
+    static constexpr int col_s = 0, col_o = 256; // tensor memory: S of tile x at 128 x, O at 256 + D x
+};
+
+__device__ __forceinline__ float ex2p(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*) &h;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// One K = 16 product, operands in shared memory (SS) or A in tensor memory (TS); `acc` = 0 overwrites.  By one elected lane of a converged warp.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+
+template<int D>
+__global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, const BatchView B, const AttnView A) {
+    using K = PCfg<D>;
+    constexpr int P = K::panels;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_ready[2][2], pv_first[2], o_done[2], q_ready[2];
+    __shared__ StepMeta meta[kMetaRing];
+    __shared__ uint32_t tmem_base;
+    __shared__ int lost;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint8_t* smem = (uint8_t*) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_free[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4); mbar_init(&pv_first[i], 1); mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
+        }
+        lost = 0;
+        mbar_fence_init();
+    }
+    if (warp == 12) tmem_alloc(&tmem_base, 512);
+    grid_launch_dependents();
+    grid_dependency_wait();
+
+    // ---- the rows, and the cache blocks they see
+    const int h = blockIdx.y, si = blockIdx.x / A.row_tiles, r0 = (A.row_tiles - 1 - blockIdx.x % A.row_tiles) * 256;   // the longest rows first
+    const Seq s = seq_of(B, si);
+    const int n_rows = s.n_new * A.group, first = s.len - s.n_new;
+    const bool here = r0 < n_rows;
+    const int last_row = min(r0 + 256, n_rows) - 1;
+    const int pos_lo = first + r0 / A.group, pos_hi = here ? first + last_row / A.group : -1;
+    const int b_lo = A.window > 0 ? max(0, pos_lo - A.window + 1) / kKvBlock : 0;
+    const int n_blocks = pos_hi < 0 ? 0 : max(0, pos_hi / kKvBlock + 1 - b_lo);
+    const int steps = (n_blocks + 1) / 2;
+    const int tiles = here && n_rows - r0 > 128 ? 2 : 1;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity)) return true;
+        lost = 1;
+        return false;
+    };
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    // (each part sets its registers in a branch of its own: where paths meet the smallest number holds)
+    if (warp >= 8 && warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
+        // ================================================================ codes -> f16 operands
+        const int ct = tid - 256;
+        constexpr int pieces = 128 * D / 16 / 128;                      // 16-byte pieces of a tile a thread takes
+        int batch = -1;
+        int my_phys = -1, my_lb = -1;
+        float my_ks = 0.0f, my_vs = 0.0f;
+        auto look_up = [&](int b) {                                     // cache block b_lo + b of this range: 32 at a time, a lane each
+            if ((b >> 5) != batch) {
+                batch = b >> 5;
+                const int x = (batch << 5) + lane;
+                my_lb = x < n_blocks ? b_lo + x : -1;
+                my_phys = my_lb >= 0 ? block_of(C, si, my_lb) : -1;
+                my_ks = my_vs = 0.0f;
+                if (my_phys >= 0) {
+                    const size_t bh = (size_t) my_phys * C.n_kv + h;
+                    my_ks = C.k_scale[bh];
+                    my_vs = C.v_scale[bh];
+                }
+            }
+        };
+        uint4 cur[pieces], nxt[pieces];
+        int phys[2];
+        auto load = [&](uint4 (&w)[pieces], const uint8_t* base) {
+#pragma unroll
+            for (int i = 0; i < pieces; ++i) {
+                const int q = i * 128 + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16);
+                w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                if (phys[x] >= 0) w[i] = *((const uint4*) (base + ((size_t) phys[x] * C.n_kv + h) * (kKvBlock * D)) + in);
+            }
+        };
+        auto store = [&](const uint4 (&w)[pieces], uint8_t* dst, bool val) {
+#pragma unroll
+            for (int i = 0; i < pieces; ++i) {
+                const int q = i * 128 + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16), c4 = in & 3;
+                // keys: panel = 64 values, row = token; values: panel = the block's 64 tokens, row = value
+                const int panel = val ? x : in / 256, row = val ? in / 4 : x * 64 + (in % 256) / 4;
+                uint8_t* p = dst + panel * ((val ? D : 128) * 128) + row * 128;
+                uint32_t o[8];
+                codes_to_half(w[i].x, o[0], o[1]); codes_to_half(w[i].y, o[2], o[3]);
+                codes_to_half(w[i].z, o[4], o[5]); codes_to_half(w[i].w, o[6], o[7]);
+                *(uint4*) (p + (((2 * c4) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *(uint4*) (p + (((2 * c4 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            fence_proxy_async();
+            __syncwarp();
+        };
+        auto find = [&](int j) {                                        // the step's two blocks
+            StepMeta m;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                look_up(2 * j + x);
+                const int src = (2 * j + x) & 31;
+                phys[x] = __shfl_sync(0xffffffffu, my_phys, src);
+                m.lb[x] = phys[x] >= 0 ? __shfl_sync(0xffffffffu, my_lb, src) : -1;
+                m.ks[x] = __shfl_sync(0xffffffffu, my_ks, src);
+                const float vs = fmaxf(__shfl_sync(0xffffffffu, my_vs, src), kVsLeast);
+                m.lv[x] = log2f(vs);
+                m.ivs[x] = 1.0f / vs;
+            }
+            return m;
+        };
+        if (here && steps > 0) {
+            StepMeta m = find(0);
+            load(cur, C.k);
+            for (int j = 0; j < steps; ++j) {
+                load(nxt, C.v);                                         // this step's values, under the conversion of its keys
+                if (j >= 2 && !wait(&k_free[j & 1], ((j >> 1) - 1) & 1)) break;
+                if (ct == 0) meta[j % kMetaRing] = m;
+                store(cur, smem + K::k + (j & 1) * K::tile, false);
+                if (lane == 0) mbar_arrive_one(&k_full[j & 1]);
+                if (j + 1 < steps) {
+                    m = find(j + 1);
+                    load(cur, C.k);
+                }
+                if (j >= 2 && !wait(&v_free[j & 1], ((j >> 1) - 1) & 1)) break;
+                store(nxt, smem + K::v + (j & 1) * K::tile, true);
+                if (lane == 0) mbar_arrive_one(&v_full[j & 1]);
+            }
+        }
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (here && warp == 12) {
+            // ================================================================ products
+            const uint32_t base = smem_u32(smem);
+            auto scores = [&](int x, int j) {
+                const uint32_t qa = base + K::q + x * K::tile, ka = base + K::k + (j & 1) * K::tile;
+    #pragma unroll
+                for (int p = 0; p < P; ++p)
+    #pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ss(tmem + K::col_s + 128 * x, smem_desc_sw128(qa + p * (128 * 128) + k * 32), smem_desc_sw128(ka + p * (128 * 128) + k * 32),
+                               K::idesc_s, p + k > 0);
+                mma_commit_elect(smem_u32(&s_full[x]));
+            };
+            bool ok = steps == 0 || (wait(&k_full[0], 0) && wait(&q_ready[0], 0) && (tiles == 1 || wait(&q_ready[1], 0)));
+            tc_fence_after();
+            if (ok && steps > 0) {
+                for (int x = 0; x < tiles; ++x) scores(x, 0);
+                mma_commit_elect(smem_u32(&k_free[0]));
+            }
+            for (int j = 0; j < steps && ok; ++j) {
+                ok = wait(&v_full[j & 1], (j >> 1) & 1);
+                if (ok && j + 1 < steps) ok = wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+                for (int x = 0; x < tiles && ok; ++x) {
+                    const uint32_t va = base + K::v + (j & 1) * K::tile;
+    #pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        ok = ok && wait(&p_ready[x][c], j & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma_ts(tmem + K::col_o + D * x, tmem + K::col_s + 128 * x + 64 * c + 8 * k, smem_desc_sw128(va + c * (D * 128) + k * 32),
+                                   K::idesc_o, j + c + k > 0);
+                        if (c == 0) mma_commit_elect(smem_u32(&pv_first[x]));
+                    }
+                    if (!ok) break;
+                    if (j + 1 == steps) mma_commit_elect(smem_u32(&o_done[x]));
+                    if (x + 1 == tiles) mma_commit_elect(smem_u32(&v_free[j & 1]));
+                    if (j + 1 < steps) scores(x, j + 1);
+                }
+                if (ok && j + 1 < steps) mma_commit_elect(smem_u32(&k_free[(j + 1) & 1]));
+            }
+            if (!ok && steps > 0) {                                         // what has been issued ends before the memory is given back
+                mma_commit_elect(smem_u32(&o_done[0]));
+                mbar_wait(&o_done[0], 0);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        if (here && warp < 4 * tiles) {
+            // ================================================================ softmax, a row a thread
+            const int x = warp >> 2, row = r0 + tid;
+            // ---- queries into shared memory: row r of tile x is thread 128 x + r
+            float qinv;
+            {
+                uint8_t* dst = smem + K::q + (warp >> 2) * K::tile;
+                const int r = tid & 127;
+                uint32_t w[D / 2];
+                if (row < n_rows) {
+                    const uint16_t* src = (const uint16_t*) A.q + (size_t) (s.row + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D;
+                    if (A.wide_q) {
+        #pragma unroll
+                        for (int i = 0; i < D / 8; ++i) *(uint4*) &w[4 * i] = ((const uint4*) src)[i];
+                    } else {
+        #pragma unroll
+                        for (int i = 0; i < D / 2; ++i) w[i] = src[2 * i] | (uint32_t) src[2 * i + 1] << 16;
+                    }
+                } else {
+        #pragma unroll
+                    for (int i = 0; i < D / 2; ++i) w[i] = 0u;
+                }
+                float amax = 0.0f;
+        #pragma unroll
+                for (int i = 0; i < D / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+                const int e2 = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;    // amax * 2^e2 in [2^11, 2^12)
+                const float up = __uint_as_float((uint32_t) (127 + e2) << 23);
+                qinv = __uint_as_float((uint32_t) (127 - e2) << 23) * A.scale_log2;
+        #pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4 o;
+                    uint32_t* ow = (uint32_t*) &o;
+        #pragma unroll
+                    for (int i = 0; i < 4; ++i) ow[i] = half2_of(__uint_as_float(w[4 * c + i] << 16) * up, __uint_as_float(w[4 * c + i] & 0xFFFF0000u) * up);
+                    *(uint4*) (dst + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = o;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_one(&q_ready[warp >> 2]);
+            }
+            const uint32_t lane_base = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
+            const uint32_t at_s = lane_base + K::col_s + 128 * x, at_o = lane_base + K::col_o + D * x;
+            const int pos = row < n_rows ? first + row / A.group : 0x3fffffff;
+            const int wlo = __reduce_min_sync(0xffffffffu, pos), whi = first + min(last_row, r0 + warp * 32 + 31) / A.group;
+            float m = kNone, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < steps && ok; ++j) {
+                if (!wait(&s_full[x], j & 1)) { ok = false; break; }
+                tc_fence_after();
+    #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const StepMeta& sm = meta[j % kMetaRing];
+                    const int lb = sm.lb[c];
+                    const float lv = sm.lv[c], ivs = sm.ivs[c];
+                    float f = qinv * sm.ks[c];
+                    uint32_t v[64];
+                    tmem_ld32(at_s + 64 * c, *(uint32_t(*)[32]) &v[0]);
+                    tmem_ld32(at_s + 64 * c + 32, *(uint32_t(*)[32]) &v[32]);
+                    tmem_wait_ld();
+                    const int tb = lb * kKvBlock;
+                    if (lb < 0) {
+    #pragma unroll
+                        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(kNone);
+                        f = 1.0f;
+                    } else if (tb + kKvBlock - 1 > wlo || (A.window > 0 && tb <= whi - A.window)) {
+    #pragma unroll
+                        for (int i = 0; i < 64; ++i) {
+                            const bool seen = tb + i <= pos && (A.window <= 0 || tb + i > pos - A.window || pos == 0x3fffffff);
+                            v[i] = __float_as_uint(seen ? __uint_as_float(v[i]) * f : kNone);
+                        }
+                        f = 1.0f;
+                    }
+                    float mx[4] = {kNone, kNone, kNone, kNone};
+    #pragma unroll
+                    for (int i = 0; i < 64; i += 4)
+    #pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(v[i + e]));
+                    const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
+                    if (__any_sync(0xffffffffu, top > m + kRise || (m == kNone && top > kNone))) {      // the warp's rows are rescaled together
+                        const bool mine = top > m + kRise || m == kNone;
+                        const float up = mine ? top : m;
+                        const float alpha = !mine ? 1.0f : m == kNone ? 0.0f : ex2p(m - up);
+                        m = up;
+                        l *= alpha;
+                        if (j + c > 0) {
+                            if (c == 1 && !wait(&pv_first[x], j & 1)) { ok = false; break; }            // (at c = 0 the scores came after it)
+                            tc_fence_after();
+    #pragma unroll
+                            for (int d = 0; d < D; d += 16) {
+                                float o[16];
+                                tmem_ld16(at_o + d, o);
+                                uint32_t ow[16];
+    #pragma unroll
+                                for (int i = 0; i < 16; ++i) ow[i] = __float_as_uint(o[i] * alpha);
+                                tmem_st16(at_o + d, ow);
+                            }
+                            tmem_wait_st();
+                        }
+                    }
+                    const float off = m == kNone ? kNone : lv - m + kUp;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll
+                    for (int i = 0; i < 64; i += 32) {
+                        uint32_t p[16];
+    #pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float a = ex2p(fmaf(__uint_as_float(v[i + e]), f, off)), b = ex2p(fmaf(__uint_as_float(v[i + e + 1]), f, off));
+                            sum[e & 2] += a;
+                            sum[(e & 2) + 1] += b;
+                            p[e / 2] = half2_of(a, b);
+                        }
+                        tmem_st16(at_s + 64 * c + i / 2, p);
+                    }
+                    l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ivs, l);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_one(&p_ready[x][c]);
+                }
+            }
+            // ---- O / l
+            if (ok && steps > 0) ok = wait(&o_done[x], 0);
+            tc_fence_after();
+            if (ok) {                                                       // (warp-uniform: a wait runs out for a whole warp)
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const int n = s.row + row / A.group, hq = h * A.group + row % A.group;
+                uint16_t* dst = (uint16_t*) A.out + ((size_t) n * A.n_q + hq) * D;
+    #pragma unroll
+                for (int d = 0; d < D; d += 16) {
+                    float o[16];
+                    if (steps > 0) tmem_ld16(at_o + d, o);
+                    else
+    #pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+                    if (row < n_rows) {
+                        uint32_t w[8];
+    #pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(l > 0.0f ? o[2 * i] * inv : 0.0f, l > 0.0f ? o[2 * i + 1] * inv : 0.0f);
+                            w[i] = *(const uint32_t*) &b;
+                        }
+                        ((uint4*) (dst + d))[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                        ((uint4*) (dst + d))[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                }
+                if (A.lse != nullptr && row < n_rows)
+                    A.lse[(size_t) n * A.n_q + hq] = l > 0.0f ? (m + log2f(l) - kUp) * 0.69314718055994531f : kNone;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (tid == 0 && lost) atomicExch(A.error, 1u);
+}
+
+template<int D> int launch_prompt(const maya_kv_cache& c, const maya_attn_batch& b, AttnView A, cudaStream_t s) {
+    const long long rows = (long long) b.max_new * A.group;
+    A.row_tiles = (int) ((rows + 255) / 256);
+    const long long tiles = (long long) A.row_tiles * b.n_seq;
+    if (tiles > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
+    static SmemLimit limit;
+    if (!limit.raise((const void*) prompt_kernel<D>, PCfg<D>::smem)) return note_launch("kv prompt attention smem attribute");
+    launch_dependent(prompt_kernel<D>, dim3((unsigned) tiles, (unsigned) c.n_kv), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
+    return note_launch("attn_q8 prompt");
+}
+
+}  // namespace
+
+// Attention of a prompt's rows on tcgen05; kNotTaken: not this kernel's call, nothing launched.
+int attn_prompt(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, cudaStream_t s) {
+    if (!bf16 || A.sel != nullptr || (c.head_dim != 64 && c.head_dim != 128)) return kNotTaken;
+    if ((long long) b.max_new * A.group < 128) return kNotTaken;
+    return c.head_dim == 64 ? launch_prompt<64>(c, b, A, s) : launch_prompt<128>(c, b, A, s);
+}
+
+}  // namespace maya

@@ -155,6 +155,58 @@ def test_long_sequence_is_split_and_joined(cuda, bf16):
     assert T.equal(out, again)                # whichever split is last
 
 
+PROMPTS = [
+    # the same columns; 128 rows (tokens * group) of a sequence and more in bf16: the tensor-core kernel's tiles of 256
+    ([128], [128], 1, 1, 128, 0),
+    ([129], [129], 2, 1, 64, 0),
+    ([256], [300], 1, 1, 128, 0),
+    ([43, 0, 100, 1], [43, 70, 1000, 900], 2, 6, 128, 0),
+    ([300], [300], 1, 2, 64, 0),
+    ([130], [64], 1, 1, 128, 0),             # 66 rows before the sequence: one tile sees nothing at all
+    ([200], [777], 1, 3, 128, 130),
+    ([257, 20], [257, 300], 1, 7, 64, 64),
+    ([17], [2100], 1, 16, 128, 0),
+    ([150], [400], 1, 1, 128, 1),
+]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_prompts(cuda, case, bf16):
+    import torch as T
+    new, lens, n_kv, group, dim, window = PROMPTS[case]
+    rng = np.random.default_rng(400 + case)
+    cache, host = make_cache(T, rng, lens, n_kv, dim)
+    q = T.from_numpy(rng.standard_normal((sum(new), n_kv * group, dim)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32)
+    want = plain_attention(host, new, lens, q.double().numpy(), n_kv, dim ** -0.5, window)
+    out, lse = attend(T, cache, new, lens, q.cuda(), window)
+    check(out, lse, want, bf16)
+    again, _ = attend(T, cache, new, lens, q.cuda(), window, lse=False)
+    assert T.equal(out, again)
+
+
+def test_prompt_with_large_scores_and_scales_far_apart(cuda):
+    """Rows whose maximum rises late and by much, value scales 1e-20 .. 1 and 0, blocks the table does not have, unaligned queries."""
+    import torch as T
+    rng = np.random.default_rng(17)
+    lens, new = [1000], [160]
+    cache, host = make_cache(T, rng, lens, 1, 128)
+    for b in range(16):
+        host["ks"][host["table"][0, b]] = 0.002 * 1.3 ** b
+        host["vs"][host["table"][0, b]] = (0.0, 1e-20, 1.0, 1e-3)[b % 4]
+    cache.k_scale.copy_(T.from_numpy(host["ks"]))
+    cache.v_scale.copy_(T.from_numpy(host["vs"]))
+    rows = T.from_numpy(4 * rng.standard_normal((160, 131)).astype(np.float32)).bfloat16().cuda()
+    for off in (0, 3):
+        q = rows[:, off:off + 128].unflatten(1, (1, 128))
+        out, lse = attend(T, cache, new, lens, q)
+        check(out, lse, plain_attention(host, new, lens, q.double().cpu().numpy(), 1, 128 ** -0.5), True)
+    cache.table[0, 3] = -1
+    cache.table[0, 8:10] = cache.n_blocks
+    out, lse = attend(T, cache, new, lens, q)
+    check(out, lse, plain_attention(host, new, lens, q.double().cpu().numpy(), 1, 128 ** -0.5, absent=((0, 3), (0, 8), (0, 9))), True)
+
+
 def test_strided_and_unaligned_queries(cuda):
     import torch as T
     rng = np.random.default_rng(6)
