@@ -732,7 +732,7 @@ class KvAttention:
         if nbytes == 0:
             raise MayaError("attn_scratch_bytes", -1)
         self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=cache.k.device)
-        self.scratch[:1 << 19].zero_()                      # the error word and the counters
+        self.scratch[:1 << 12].zero_()                      # the error word and the counters
         self._attn = AttnArgs(None, 0, 0, n_q, cache.head_dim ** -0.5 if scale is None else scale, window, None, 0, None, None)
         self._select = SelectArgs(None, 0, 0, n_q, n_first, n_last, n_sel, None)
         self._rope = RopeArgs(n_q=n_q)

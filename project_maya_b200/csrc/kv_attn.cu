@@ -1,20 +1,25 @@
 // kv_attn.cu - attention over the paged 8-bit cache for single tokens, windows and short prompts, on mma.sync (m16n8k16, f16 into f32).
 //
 // What bounds it is the cache's bytes: 2 * head_dim bytes a token and key/value head, read once for the group of query heads
-// that shares them.  So everything is made to keep copies in flight: a thread block is four warps with a ring of half-block slots
-// (64 tokens of keys, 64 tokens of values: 64 * D contiguous bytes each, one bulk copy), two thread blocks an SM.
-//   RW warps share a ring and take 16 rows each; BW = 4 / RW rings take every BW-th cache block.  One token of up to 16 heads a
-//   group: RW = 1, every warp on its own; 17..32 rows: 2 x 2; more: one ring, 64 rows.
-// Between HBM and the tensor cores a code costs a byte permute and half a subtraction (codes_to_half); no value is written back.
+// that shares them.  So everything is made to keep copies in flight: a thread block is four warps with rings of 4 KB pieces (64 tokens of 64 key
+// values, or 64 values of 64 tokens: contiguous in the cache, one bulk copy each), three thread blocks an SM.
+//   RW warps share a ring and take 8 NT rows each; BW = 4 / RW rings take every BW-th cache block.  One token of up to 8 (16) heads a
+//   group: RW = 1, NT = 1 (2), every warp on its own; 17..32 rows: 2 x 2; more: one ring, 64 rows.
+//
+// The codes are the first operand of both products, the queries and P the second: S^T = K Q^T and O^T = V^T P^T.  Rows are then tokens (values), of which
+// there are always enough, and columns come in eights, so that a group of 8 heads wastes nothing (with queries as rows of 16 it took twice the
+// products, exponentials and registers: 1165 warp instructions a block against ...).  Between HBM and the tensor cores a code costs a byte permute and half
+// a subtraction (codes_to_half).
 //
 // Fragments.  The contraction index of m16n8k16 may be permuted as long as both operands agree, and the cache's layout is chosen for
 // it: lane (g, t) of a warp owns values 16 t .. 16 t + 15 of every 64 in a key row (four K = 16 steps of four values from one
-// 16-byte load), and tokens 16 t .. 16 t + 15 of the block in a value column.  Keys enter as columns in the order that leaves the
-// scores where P wants its tokens: column n of tile j is token 16 (n >> 1) + 4 (j >> 1) + 2 (j & 1) + (n & 1).  Every shared-memory
-// load is 16 bytes a lane, a quarter warp on 128 consecutive bytes.
+// 16-byte load), and tokens 16 t .. 16 t + 15 of the block in a value row.  Row g of S^T's tile s is token 16 (g >> 1) + 4 s + (g & 1), row g + 8 the
+// token two further: turned over by movmatrix, P^T's columns are the tokens of V's step s.  Every shared-memory load is 16 bytes a lane, a
+// quarter warp on 128 consecutive bytes.
 //
-// A tile whose cache blocks are split over several thread blocks leaves (m, l, O) partials; the last of them to arrive joins
-// all in the order of the splits, so the bits do not depend on who was last.
+// All (tile, head, cache block) triples of a call are one list, and every resident thread block takes an even stretch of it, whatever the
+// sequences' lengths (they are known on the device only); copies run ahead from one tile into the next.  A (tile, head) that lies in the
+// stretches of several thread blocks leaves (m, l, O) parts, which a second launch joins in the order of the list, a warp a row.
 #include <cuda_fp16.h>
 
 #include "kv_attn.cuh"
@@ -23,15 +28,17 @@ namespace maya {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
-constexpr int kMeta = 256;                        // cache blocks looked up at a time
+constexpr int kMeta = 128;                        // cache blocks looked up at a time
+constexpr int kPiece = 4096;                      // bytes of a ring's slot: 64 tokens x 64 values of K or of V
+constexpr int kTilesMost = 256;                   // tiles whose blocks a thread block adds up
 
 struct Meta {
-    int phys, lb;
+    int bh, lb;                                   // block and head in the cache (-1: none); place in the sequence
     float ks, vs;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4 a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
@@ -44,39 +51,73 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *(const uint32_t*) &h;
 }
+__device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 matrix of f16, a row's pair a lane
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 // what f16 left of a and b
 __device__ __forceinline__ uint32_t pack_rest(uint32_t hi, float a, float b) {
     const float2 f = __half22float2(*(const __half2*) &hi);
     return pack_half(a - f.x, b - f.y);
 }
 
-template<int D, bool F32, int RW> struct Cfg {
+template<int D, bool F32, int NT, int RW> struct Cfg {
     static constexpr int BW = kWarps / RW;
-    static constexpr int rows = 16 * RW;
-    static constexpr int slot = kKvBlock * D;                                    // bytes: keys or values of one block
-    // slots of a ring: 96 KB a thread block; D = 256: one thread block an SM, what the queries leave of its shared memory
-    static constexpr int slots = D == 64 ? 6 * RW : D == 128 ? 3 * RW : D == 192 ? 2 * RW : RW == 1 ? 3 : RW == 2 ? 5 : 9;
-    static constexpr int ctas = D == 256 ? 1 : 2;                                // thread blocks an SM
-    static constexpr int ring = BW * slots * slot;
-    static constexpr int merge = kWarps * 16 * D * 4;                            // the warps' outputs, over the ring's bytes
-    static constexpr int frag = RW * (D / 64) * 4 * 512;                         // queries as fragments
-    static constexpr int body = ring > merge ? ring : merge;
-    static constexpr size_t smem = (size_t) body + (F32 ? 2 : 1) * frag;
+    static constexpr int rows = 8 * NT * RW;
+    static constexpr int ctas = D == 64 ? (F32 && NT == 2 ? 2 : 3) : D == 128 ? (F32 || NT == 2 ? 2 : 3) : F32 ? 1 : 2;   // thread blocks an SM
+    static constexpr int room = ctas == 3 ? 71680 : ctas == 2 ? 108544 : 212992; // and shared memory of each
+    static constexpr int frag = RW * NT * (D / 64) * 2 * 512;                    // queries as fragments
+    static constexpr int wide = 64 + 4;                                          // floats of a row where outputs meet, 64 values at a time
+    static constexpr int merge = (RW > 2 ? RW : 2) * 8 * NT * wide * 4;
+    static constexpr int desk = (F32 ? 2 : 1) * frag > merge ? (F32 ? 2 : 1) * frag : merge;   // the queries, and after them the outputs that meet
+    static constexpr int slots = (room - desk) / kPiece / BW;                    // of a ring
+    static constexpr int body = BW * slots * kPiece;
+    static constexpr size_t smem = (size_t) body + desk;
 };
 
-template<int D, bool F32, int RW>
-__global__ void __launch_bounds__(kThreads, Cfg<D, F32, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
-    using K = Cfg<D, F32, RW>;
-    constexpr int BW = K::BW, P = D / 64, V = D / 32;
+// Cache blocks that a tile's rows see, from block b_lo on; rows r0 .. of unit `unit`.
+struct Tile {
+    Seq s;
+    int si, i0, r0, n_rows, first, pos_lo, pos_hi, b_lo, n_blocks;
+};
+__device__ __forceinline__ Tile tile_of(const BatchView& B, const AttnView& A, int tile, int rows) {
+    Tile t;
+    const int unit = tile / A.row_tiles;
+    t.r0 = (A.row_tiles - 1 - tile % A.row_tiles) * rows;                        // the longest rows of a prompt first
+    t.si = A.sel != nullptr ? seq_of_row(B, unit) : unit;
+    t.s = seq_of(B, t.si);
+    t.i0 = A.sel != nullptr ? unit - t.s.row : 0;                                // the unit's first new token
+    t.n_rows = A.sel != nullptr ? (t.i0 < t.s.n_new ? A.group : 0) : t.s.n_new * A.group;
+    t.first = t.s.len - t.s.n_new;
+    t.pos_lo = t.first + t.i0 + t.r0 / A.group;
+    t.pos_hi = t.first + t.i0 + (min(t.r0 + rows, t.n_rows) - 1) / A.group;
+    t.b_lo = A.sel != nullptr || A.window <= 0 ? 0 : max(0, t.pos_lo - A.window + 1) / kKvBlock;
+    // (a tile whose rows see nothing has one block to look at, which is none: its zeros have to be written all the same)
+    t.n_blocks = t.r0 >= t.n_rows ? 0 : A.sel != nullptr ? A.n_sel : t.pos_hi < 0 ? 1 : max(1, t.pos_hi / kKvBlock + 1 - t.b_lo);
+    return t;
+}
+__device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int h, int r) {      // row r of the tile in `out`
+    const int row = T.r0 + r;
+    return (size_t) (T.s.row + T.i0 + row / A.group) * A.n_q + h * A.group + row % A.group;
+}
+// O is P V with P = 2^12 p, l the sum of P (V's scale taken out again)
+__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.0f ? (m + log2f(l) - kPBias) * 0.69314718055994531f : kNone; }
+
+template<int D, bool F32, int NT, int RW>
+__global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
+    using K = Cfg<D, F32, NT, RW>;
+    constexpr int BW = K::BW, P = D / 64, V = D / 32, TF = F32 ? 2 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Meta meta[kMeta];
     __shared__ __align__(8) uint64_t full[BW][K::slots], empty[BW][K::slots];
-    __shared__ float qinv[K::rows], sm_m[kWarps][16], sm_l[kWarps][16], sm_vr[kWarps];
-    __shared__ int lost, arrived;
+    __shared__ float qinv[K::rows], sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT], sm_vr[kWarps];
+    __shared__ int pre[kTilesMost + 1];                                          // blocks (of one head) in front of each tile
+    __shared__ int lost;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int bw = warp / RW, rw = warp % RW;
-    uint8_t* ring = smem + (size_t) bw * K::slots * K::slot;
-    uint8_t* fragq = smem + K::body;
+    uint8_t* ring = smem + (size_t) bw * K::slots * kPiece;
+    uint8_t* desk = smem + K::body;
 
     if (tid == 0) {
         for (int b = 0; b < BW; ++b)
@@ -87,390 +128,621 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, RW>::ctas) attn_kernel(c
     grid_launch_dependents();
     grid_dependency_wait();
 
-    // ---- the tile: rows r0 .. of (new token, head of the group) pairs of one sequence, or of one token with a list
-    const int split = blockIdx.z, h = blockIdx.y;
-    const int unit = blockIdx.x / A.row_tiles, r0 = (A.row_tiles - 1 - blockIdx.x % A.row_tiles) * K::rows;   // the longest rows of a prompt first
-    const int si = A.sel != nullptr ? seq_of_row(B, unit) : unit;
-    const Seq s = seq_of(B, si);
-    const int i0 = A.sel != nullptr ? unit - s.row : 0;                          // the unit's first new token
-    const int n_rows = A.sel != nullptr ? A.group : s.n_new * A.group;
-    if (r0 >= n_rows || i0 >= s.n_new) return;
-    const int first = s.len - s.n_new;
-    const int last_row = min(r0 + K::rows, n_rows) - 1;
-    const int pos_lo = first + i0 + r0 / A.group, pos_hi = first + i0 + last_row / A.group;
-    const int* list = A.sel != nullptr ? A.sel + ((size_t) unit * C.n_kv + h) * A.n_sel : nullptr;
-    const int b_lo = list != nullptr || A.window <= 0 ? 0 : max(0, pos_lo - A.window + 1) / kKvBlock;
-    const int n_blocks = list != nullptr ? A.n_sel : max(0, (pos_hi < 0 ? -1 : pos_hi / kKvBlock) + 1 - b_lo);
-    const int block_hi = pos_hi < 0 ? -1 : pos_hi / kKvBlock;
-    const int my0 = split * A.split_blocks, my1 = min(my0 + A.split_blocks, n_blocks);
-    const int splits = max(1, (n_blocks + A.split_blocks - 1) / A.split_blocks);  // of this tile
-    if (split >= splits) return;
-
-    // ---- queries: scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
-    for (int r = warp; r < K::rows; r += kWarps) {
-        const int row = r0 + r, i = i0 + row / A.group, hq = h * A.group + row % A.group;
-        float x[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = 0.0f;
-        if (row < n_rows) ld_acts<!F32, V>(A.q, (size_t) (s.row + i) * A.ld_q + (size_t) hq * D + lane * V, A.wide_q, x);
-        float amax = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(x[e]));
-        amax = warp_max(amax);
-        const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
-        const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
-        if (lane == 0) qinv[r] = __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2;
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-            const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
-            uint8_t* f = fragq + ((((r >> 4) * P + (d >> 6)) * 4 + st) * 32 + (r & 7) * 4 + tt) * 16 + (((w >> 1) * 2) + ((r >> 3) & 1)) * 4;
-            const uint32_t hi = pack_half(x[e] * up, x[e + 1] * up);
-            *(uint32_t*) f = hi;
-            if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, x[e] * up, x[e + 1] * up);
+    // ---- this thread block's share of all (tile, head, cache block) triples, in that order
+    unsigned total = 0;                                                          // blocks of one head over all tiles
+    if (A.direct) {
+        __syncthreads();
+    } else if (A.sel != nullptr) {
+        total = (unsigned) A.tiles * (unsigned) A.n_sel;
+        __syncthreads();
+    } else {
+        const int each = (A.tiles + kThreads - 1) / kThreads;
+        int sum = 0;
+        for (int i = 0; i < each; ++i) {
+            const int x = tid * each + i;
+            if (x < A.tiles) { pre[x] = sum; sum += tile_of(B, A, x, K::rows).n_blocks; }
         }
+        int up = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) { const int y = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += y; }
+        if (lane == 31) sm_l[0][warp] = __int_as_float(up);
+        __syncthreads();
+        int before = up - sum, all = 0;
+        for (int w = 0; w < kWarps; ++w) { const int y = __float_as_int(sm_l[0][w]); if (w < warp) before += y; all += y; }
+        for (int i = 0; i < each; ++i) {
+            const int x = tid * each + i;
+            if (x < A.tiles) pre[x] += before;
+        }
+        if (tid == 0) pre[A.tiles] = all;
+        total = (unsigned) all;
+        __syncthreads();
     }
-
-    float o[D / 8][4];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m[2] = {kNone, kNone}, l[2] = {0.0f, 0.0f}, vr = 0.0f;
-    int pos[2];                                                                  // last visible position of rows g, g + 8 (rows beyond the tile's: all, not kept)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int row = r0 + rw * 16 + g + 8 * e;
-        pos[e] = row < n_rows ? first + i0 + row / A.group : 0x3fffffff;
+    const unsigned work = total * (unsigned) C.n_kv;
+    unsigned share = (work + gridDim.x - 1) / gridDim.x;
+    share = max((unsigned) BW, (share + BW - 1) / BW * BW);                      // whole rounds of the rings
+    unsigned w0 = min(work, blockIdx.x * share), w1 = min(work, w0 + share);
+    if (A.direct) {
+        w0 = 0;
+        w1 = (unsigned) tile_of(B, A, (int) (blockIdx.x / C.n_kv), K::rows).n_blocks;
+    } else if (blockIdx.x == 0) {                                                // for the join
+        if (A.sel == nullptr)
+            for (int i = tid; i <= A.tiles; i += kThreads) A.pre[i] = pre[i];
+        if (tid == 0) *A.share = share;
     }
-    const int wpos_lo = __reduce_min_sync(0xffffffffu, min(pos[0], pos[1]));     // over the warp's rows
-    const int wpos_hi = first + i0 + min(last_row, r0 + rw * 16 + 15) / A.group;
+    if (w0 >= w1) return;
+    // triple w: its tile (the last whose first triple is not behind it), head and block
+    auto find = [&](unsigned w, int& tile, int& h, int& b, int& nb) {
+        if (A.direct) {
+            tile = (int) (blockIdx.x / C.n_kv);
+            h = (int) (blockIdx.x % C.n_kv);
+            b = (int) w;
+            nb = (int) w1;
+            return;
+        }
+        if (A.sel != nullptr) {
+            const unsigned pair = w / (unsigned) A.n_sel;
+            tile = (int) (pair / (unsigned) C.n_kv);
+            h = (int) (pair % (unsigned) C.n_kv);
+            b = (int) (w % (unsigned) A.n_sel);
+            nb = A.n_sel;
+            return;
+        }
+        int lo = 0, hi = A.tiles - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((unsigned) pre[mid] * (unsigned) C.n_kv <= w) lo = mid; else hi = mid - 1;
+        }
+        tile = lo;
+        nb = pre[lo + 1] - pre[lo];
+        const unsigned in = w - (unsigned) pre[lo] * (unsigned) C.n_kv;
+        h = (int) (in / (unsigned) nb);
+        b = (int) (in % (unsigned) nb);
+    };
 
-    unsigned u_put = 0, u_get = 0;                                               // half-block slots asked for and taken so far by this ring
+    float o[NT][D / 16][4], m[NT][2], l[NT][2], vr = F32 ? 0.0f : 1.0f;          // columns 2 t, 2 t + 1
+    int pos[NT][2], wpos_lo = 0, wpos_hi = 0;
+    unsigned u_put = 0, u_get = 0;                                               // pieces asked for and taken so far by this ring
     bool ok = true;
-    for (int c0 = my0; c0 < my1 && ok; c0 += kMeta) {
-        const int nc = min(kMeta, my1 - c0);
-        __syncthreads();                                                         // queries (first round); everybody is done with meta
+    Tile T;
+    int tile = 0, h = 0;
+    unsigned seg0 = w0, seg1 = w0;                                               // the (tile, head) at hand: its triples
+    constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
+    float qx[U][V];
+    auto ask_rows = [&](int r4) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = T.r0 + r4 + u * kWarps;
+#pragma unroll
+            for (int e = 0; e < V; ++e) qx[u][e] = 0.0f;
+            if (row < T.n_rows)
+                ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
+        }
+    };
+    auto begin = [&](unsigned w) {                                               // the (tile, head) of triple w: its first queries are asked for
+        int b, nb;
+        find(w, tile, h, b, nb);
+        T = tile_of(B, A, tile, K::rows);
+        seg0 = w - (unsigned) b;
+        seg1 = seg0 + (unsigned) nb;
+        ask_rows(warp);
+    };
+    begin(w0);                                                                   // (in front of the copies, behind which they would have to wait)
+    bool fresh = true;
+    for (unsigned c0 = w0; c0 < w1; c0 += kMeta) {
+        const int nc = (int) min((unsigned) kMeta, w1 - c0);
+        __syncthreads();                                                         // everybody is done with meta
         if (lost) break;
         for (int i = tid; i < nc; i += kThreads) {
-            Meta x;
-            x.lb = list != nullptr ? list[c0 + i] : b_lo + c0 + i;
-            x.phys = x.lb >= 0 && x.lb <= block_hi ? block_of(C, si, x.lb) : -1;
-            x.ks = x.vs = 0.0f;
-            if (x.phys >= 0) {
-                const size_t bh = (size_t) x.phys * C.n_kv + h;
-                x.ks = C.k_scale[bh];
-                x.vs = C.v_scale[bh];
-            }
-            meta[i] = x;
+            int ti, hh, b, nb;
+            find(c0 + i, ti, hh, b, nb);
+            const Tile x = tile_of(B, A, ti, K::rows);
+            const int lb = A.sel != nullptr ? x.n_rows > 0 ? A.sel[((size_t) (ti / A.row_tiles) * C.n_kv + hh) * A.n_sel + b] : -1 : x.b_lo + b;
+            const int phys = lb >= 0 && x.pos_hi >= 0 && lb <= x.pos_hi / kKvBlock ? block_of(C, x.si, lb) : -1;
+            Meta e;
+            e.lb = lb;
+            e.bh = phys >= 0 ? phys * C.n_kv + hh : -1;
+            e.ks = e.vs = 0.0f;
+            if (phys >= 0) { e.ks = C.k_scale[e.bh]; e.vs = C.v_scale[e.bh]; }
+            meta[i] = e;
         }
         __syncthreads();
 
-        // copies of this ring's blocks: keys and values by turns, as many half blocks ahead as there are slots
-        int put = bw;                                                            // next block to ask for
-        bool put_v = false;
-        auto ask = [&](unsigned limit) {                                         // by the ring's first warp, until `limit` halves are asked for
+        // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots, whichever tile they are for
+        int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
+        auto ask = [&](unsigned limit) {                                         // by the ring's first warp, until `limit` pieces are asked for
             while (put < nc && u_put < limit) {
-                const Meta x = meta[put];
-                if (x.phys < 0) { put += BW; continue; }
+                const int bh = meta[put].bh;
+                if (bh < 0) { put += BW; continue; }
                 const unsigned sl = u_put % K::slots;
                 if (u_put >= K::slots && RW > 1 && !mbar_wait(&empty[bw][sl], ((u_put / K::slots) - 1) & 1)) { ok = false; return; }
                 if (lane == 0) {
-                    mbar_expect_tx(&full[bw][sl], K::slot);
-                    bulk_load(ring + sl * K::slot, (put_v ? C.v : C.k) + ((size_t) x.phys * C.n_kv + h) * K::slot, K::slot, &full[bw][sl]);
+                    mbar_expect_tx(&full[bw][sl], kPiece);
+                    bulk_load(ring + sl * kPiece, (put_at >= P ? C.v + (size_t) (put_at - P) * kPiece : C.k + (size_t) put_at * kPiece) + (size_t) bh * (P * kPiece), kPiece, &full[bw][sl]);
                 }
                 ++u_put;
-                if (put_v) put += BW;
-                put_v = !put_v;
+                if (++put_at == 2 * P) { put_at = 0; put += BW; }
             }
+        };
+        auto take = [&]() -> const uint8_t* {                                    // the ring's next piece, once it is there
+            const unsigned sl = u_get % K::slots;
+            if (!mbar_wait(&full[bw][sl], (u_get / K::slots) & 1)) { ok = false; return nullptr; }
+            return ring + sl * kPiece;
+        };
+        auto leave = [&]() {                                                     // and its room for another
+            __syncwarp();
+            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][u_get % K::slots]);
+            ++u_get;
+            if (rw == 0) ask(u_get + K::slots);
         };
         if (rw == 0) ask(u_get + K::slots);
 
-        for (int b = bw; b < nc && ok; b += BW) {
-            const Meta x = meta[b];
-            if (x.phys < 0) continue;
-            // ---- S = Q K^T
-            unsigned sl = u_get % K::slots;
-            if (!mbar_wait(&full[bw][sl], (u_get / K::slots) & 1)) { ok = false; break; }
-            float sc[8][4];
+        for (int i0 = 0; i0 < nc;) {                                             // the stretches of this part of the share that are one (tile, head)'s
+            if (fresh || c0 + i0 == seg1) {                                      // ---- a new one: its queries
+                if (!fresh) begin(c0 + i0);
+                fresh = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[j][e] = 0.0f;
-            const uint8_t* kp = ring + sl * K::slot + (16 * (g >> 1) + (g & 1)) * 64 + t * 16;
+                    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                uint4 a[4], a2[F32 ? 4 : 1];
+                        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    a[st] = *(const uint4*) (fragq + (((rw * P + p) * 4 + st) * 32 + lane) * 16);
-                    if constexpr (F32) a2[st] = *(const uint4*) (fragq + K::frag + (((rw * P + p) * 4 + st) * 32 + lane) * 16);
+                    for (int e = 0; e < 2; ++e) {
+                        m[n][e] = kNone;
+                        l[n][e] = 0.0f;
+                        const int row = T.r0 + (rw * NT + n) * 8 + 2 * t + e;    // last visible position (rows beyond the tile's: all, not kept)
+                        pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
+                    }
                 }
+                vr = F32 ? 0.0f : 1.0f;
+                int low = min(pos[0][0], pos[0][1]);
+                if constexpr (NT == 2) low = min(low, min(pos[1][0], pos[1][1]));
+                wpos_lo = __reduce_min_sync(0xffffffffu, low);                   // over the warp's rows
+                wpos_hi = T.first + T.i0 + min(min(T.r0 + K::rows, T.n_rows) - 1, T.r0 + (rw + 1) * NT * 8 - 1) / A.group;
+                // scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
+                for (int r4 = warp; r4 < K::rows; r4 += kWarps * U) {
+                    if (r4 != warp) ask_rows(r4);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint4 w = *(const uint4*) (kp + p * (kKvBlock * 64) + (4 * (j >> 1) + 2 * (j & 1)) * 64);
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int u = 0; u < U; ++u) {
+                        const int r = r4 + u * kWarps;
+                        float amax = 0.0f;
 #pragma unroll
-                    for (int st = 0; st < 4; ++st) {
-                        uint32_t b0, b1;
-                        codes_to_half(ww[st], b0, b1);
-                        if constexpr (F32) {
-                            mma16816(part, a2[st], b0, b1);
-                            mma16816(part, a[st], b0, b1);
-                        } else {
-                            mma16816(sc[j], a[st], b0, b1);
+                        for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
+                        amax = warp_max(amax);
+                        const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
+                        const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
+                        if (lane == 0) qinv[r] = __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2;
+#pragma unroll
+                        for (int e = 0; e < V; e += 2) {
+                            const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
+                            uint8_t* f = desk + ((((r >> 3) * P + (d >> 6)) * 2 + (st >> 1)) * 32 + (r & 7) * 4 + tt) * 16 + ((st & 1) * 2 + (w >> 1)) * 4;
+                            const uint32_t hi = pack_half(qx[u][e] * up, qx[u][e + 1] * up);
+                            *(uint32_t*) f = hi;
+                            if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, qx[u][e] * up, qx[u][e + 1] * up);
                         }
                     }
-                    if constexpr (F32)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[j][e] += part[e];
                 }
+                __syncthreads();
             }
-            __syncwarp();
-            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][sl]);
-            ++u_get;
-            if (rw == 0) ask(u_get + K::slots);
-
-            // ---- running maximum, P
-            const int tb = x.lb * kKvBlock;
-            float c[2];
+            const int i1 = (int) min((unsigned) nc, seg1 - c0);
+            for (int b = i0 + (int) ((unsigned) (bw - i0) % (unsigned) BW); b < i1 && ok; b += BW) {
+                const Meta x = meta[b];
+                if (x.bh < 0) continue;
+                // ---- S^T = K Q^T: rows of tile s are tokens, columns the queries
+                float sc[NT][4][4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) c[e] = qinv[rw * 16 + g + 8 * e] * x.ks;
-            if (tb + kKvBlock - 1 > wpos_lo || (A.window > 0 && tb <= wpos_hi - A.window)) {      // the block is not visible to every row in whole
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                    for (int s = 0; s < 4; ++s)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = tb + 16 * t + 4 * (j >> 1) + 2 * (j & 1) + (e & 1), to = pos[e >> 1];
-                        sc[j][e] = at <= to && (A.window <= 0 || at > to - A.window || to == 0x3fffffff) ? sc[j][e] * c[e >> 1] : kNone;
+                        for (int e = 0; e < 4; ++e) sc[n][s][e] = 0.0f;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const uint8_t* kp = take();
+                    if (!ok) break;
+                    kp += (16 * (g >> 1) + (g & 1)) * 64 + t * 16;
+                    uint4 q[TF][NT][2];
+#pragma unroll
+                    for (int f = 0; f < TF; ++f)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                q[f][n][i] = *(const uint4*) (desk + f * K::frag + ((((rw * NT + n) * P + p) * 2 + i) * 32 + lane) * 16);
+                    constexpr int SG = NT == 1 ? 4 : 2;                          // tiles side by side: one's wait for the product before is another's turn
+#pragma unroll
+                    for (int s0 = 0; s0 < 4; s0 += SG) {
+                        uint32_t wa[SG][4], wb[SG][4];
+#pragma unroll
+                        for (int i = 0; i < SG; ++i) {
+                            *(uint4*) wa[i] = *(const uint4*) (kp + 4 * (s0 + i) * 64);
+                            *(uint4*) wb[i] = *(const uint4*) (kp + (4 * (s0 + i) + 2) * 64);
+                        }
+                        // (f32: 64 values' products are summed by themselves and added with a rounded add - the tensor cores cut what falls off a sum,
+                        // always towards zero, and over a long axis that adds up)
+                        float part[NT][SG][4];
+                        if constexpr (F32)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < SG; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) part[n][i][e] = 0.0f;
+#pragma unroll
+                        for (int st = 0; st < 4; ++st)
+#pragma unroll
+                            for (int i = 0; i < SG; ++i) {
+                                uint4 a;
+                                codes_to_half(wa[i][st], a.x, a.z);
+                                codes_to_half(wb[i][st], a.y, a.w);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int f = TF - 1; f >= 0; --f) {
+                                        const uint4 y = q[f][n][st >> 1];
+                                        mma16816(F32 ? part[n][i] : sc[n][s0 + i], a, st & 1 ? y.z : y.x, st & 1 ? y.w : y.y);
+                                    }
+                            }
+                        if constexpr (F32)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < SG; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) sc[n][s0 + i][e] += part[n][i][e];
                     }
-                c[0] = c[1] = 1.0f;
-            }
-            float mx[2] = {kNone, kNone};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                mx[0] = fmaxf(mx[0], fmaxf(sc[j][0], sc[j][1]));
-                mx[1] = fmaxf(mx[1], fmaxf(sc[j][2], sc[j][3]));
-            }
-            const bool vgrew = x.vs > vr;
-            float beta = 1.0f;
-            if (vgrew) { beta = __fdividef(vr, x.vs); vr = x.vs; }
-            const float wv = vr > 0.0f ? x.vs == vr ? 1.0f : __fdiv_rn(x.vs, vr) : 0.0f;
-            float alpha[2], off[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                const float mn = fmaxf(m[e], mx[e] * c[e]);
-                const float use = mn == kNone ? 0.0f : mn;
-                alpha[e] = ex2(m[e] - use);
-                off[e] = kPBias - use;
-                m[e] = mn;
-                l[e] *= alpha[e];
-                alpha[e] *= beta;
-            }
-            if (!F32 && __any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
-                    o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
+                    leave();
                 }
+                if (!ok) break;
+
+                // ---- running maximum, P^T
+                const int tb = x.lb * kKvBlock;
+                const bool cut = tb + kKvBlock - 1 > wpos_lo || (A.window > 0 && tb <= wpos_hi - A.window);      // not visible to every row in whole
+                // V's scale: bf16: in P's exponent (m is then of s + log2 vs, and l takes it out again); f32, where that would cost bits: a factor
+                // against the largest one so far
+                float beta = 1.0f, wv = 1.0f, lv = 0.0f, ivs = 1.0f;
+                if constexpr (F32) {
+                    if (x.vs > vr) { beta = __fdividef(vr, x.vs); vr = x.vs; }
+                    wv = vr > 0.0f ? x.vs == vr ? 1.0f : __fdiv_rn(x.vs, vr) : 0.0f;
+                } else {
+                    const float vs = fmaxf(x.vs, kVsLeast);
+                    lv = __log2f(vs);
+                    ivs = __fdividef(1.0f, vs);
+                }
+                float alpha[NT][2];
+                bool moved = false;
+                uint32_t pb[TF][NT][4][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float off[2], c[2], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) c[e] = qinv[(rw * NT + n) * 8 + 2 * t + e] * x.ks;
+                    if (cut) {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int at = tb + 16 * (g >> 1) + 4 * s + (g & 1) + (e & 2), to = pos[n][e & 1];
+                                sc[n][s][e] = at <= to && (A.window <= 0 || at > to - A.window || to == 0x3fffffff) ? sc[n][s][e] * c[e & 1] : kNone;
+                            }
+                        c[0] = c[1] = 1.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(sc[n][0][e], sc[n][0][e + 2]);
+#pragma unroll
+                        for (int s = 1; s < 4; ++s) mx = fmaxf(mx, fmaxf(sc[n][s][e], sc[n][s][e + 2]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(m[n][e], fmaf(mx, c[e], lv));
+                        const float use = mn == kNone ? 0.0f : mn;
+                        const float al = ex2(m[n][e] - use);
+                        off[e] = kPBias + lv - use;
+                        m[n][e] = mn;
+                        l[n][e] *= al;
+                        alpha[n][e] = al * beta;
+                        moved = moved || alpha[n][e] != 1.0f;
+                    }
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {                         // rows g, g + 8
+                            const float p0 = ex2(fmaf(sc[n][s][2 * hh], c[0], off[0])), p1 = ex2(fmaf(sc[n][s][2 * hh + 1], c[1], off[1]));
+                            sum[0] += p0;
+                            sum[1] += p1;
+                            if constexpr (F32) {
+                                const uint32_t hi = pack_half(p0 * wv, p1 * wv);
+                                pb[0][n][s][hh] = turned(hi);
+                                pb[TF - 1][n][s][hh] = turned(pack_rest(hi, p0 * wv, p1 * wv));
+                            } else {
+                                pb[0][n][s][hh] = turned(pack_half(p0, p1));
+                            }
+                        }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], ivs, l[n][e]);
+                }
+                if (!F32 && __any_sync(0xffffffffu, moved))
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha[n][e & 1];
+
+                // ---- O^T += V^T P^T: rows are values
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const uint8_t* vp = take();
+                    if (!ok) break;
+                    vp += g * kKvBlock + t * 16;
+#pragma unroll
+                    for (int i0 = 0; i0 < 4; i0 += 2) {
+                        uint32_t wa[2][4], wb[2][4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            *(uint4*) wa[i] = *(const uint4*) (vp + 16 * (i0 + i) * kKvBlock);
+                            *(uint4*) wb[i] = *(const uint4*) (vp + (16 * (i0 + i) + 8) * kKvBlock);
+                        }
+                        float part[NT][2][4];
+                        if constexpr (F32)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) part[n][i][e] = 0.0f;
+#pragma unroll
+                        for (int st = 0; st < 4; ++st)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                uint4 a;
+                                codes_to_half(wa[i][st], a.x, a.z);
+                                codes_to_half(wb[i][st], a.y, a.w);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int f = TF - 1; f >= 0; --f)
+                                        mma16816(F32 ? part[n][i] : o[n][4 * p + i0 + i], a, pb[f][n][st][0], pb[f][n][st][1]);
+                            }
+                        if constexpr (F32)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        float& y = o[n][4 * p + i0 + i][e];
+                                        y = fmaf(y, alpha[n][e & 1], part[n][i][e]);
+                                    }
+                    }
+                    leave();
+                }
+                if (!ok) break;
             }
-            uint4 pa[4], pr[F32 ? 4 : 1];
+            if (!ok) lost = 1;
+            i0 = i1;
+            if (c0 + i1 != seg1 && c0 + i1 != w1) continue;                      // the (tile, head) goes on in the next part of the share
+
+            // ---- the rings' results meet: the upper half of them hands its rows over, until the first has all
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                uint32_t hi[4], rest[4];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {                                    // rows g, g + 8
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int q2 = 0; q2 < 2; ++q2) {                             // tokens + {0, 1}, + {2, 3}
-                        const float p0 = ex2(fmaf(sc[2 * st + q2][2 * e], c[e], off[e])), p1 = ex2(fmaf(sc[2 * st + q2][2 * e + 1], c[e], off[e]));
-                        l[e] += p0 + p1;
-                        hi[q2 * 2 + e] = pack_half(p0 * wv, p1 * wv);
-                        if constexpr (F32) rest[q2 * 2 + e] = pack_rest(hi[q2 * 2 + e], p0 * wv, p1 * wv);
+                    for (int x = 4; x < 32; x *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+            float* buf = (float*) desk;                                          // [warp of two, or of RW][8 NT][wide]
+            auto lay = [&](int place, int p) {                                   // 64 values of this warp's rows
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            buf[((place * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][4 * p + i][e];
+            };
+#pragma unroll
+            for (int half = BW / 2; half >= 1; half /= 2) {
+                const bool gives = bw >= half && bw < 2 * half, takes = bw < half;
+                const int place = (gives ? bw - half : bw) * RW + rw;            // of the pair: 0 or 1
+                if (gives && g == 0) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
+                    sm_vr[warp] = vr;
+                }
+                float mine[NT][2], theirs[NT][2];
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    __syncthreads();                                             // the desk is free (queries are done with; the values before have been taken)
+                    if (gives) lay(place, p);
+                    __syncthreads();
+                    if (takes) {
+                        const int from = warp + half * RW;
+                        if (p == 0) {
+                            const float v2 = sm_vr[from], vm = fmaxf(vr, v2), a = F32 ? vm > 0.0f ? __fdividef(vr, vm) : 0.0f : 1.0f,
+                                        b = F32 ? vm > 0.0f ? __fdividef(v2, vm) : 0.0f : 1.0f;
+                            vr = vm;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float m2 = sm_m[from][n * 8 + 2 * t + e], mn = fmaxf(m[n][e], m2), use = mn == kNone ? 0.0f : mn;
+                                    mine[n][e] = ex2(m[n][e] - use);
+                                    theirs[n][e] = ex2(m2 - use);
+                                    l[n][e] = l[n][e] * mine[n][e] + sm_l[from][n * 8 + 2 * t + e] * theirs[n][e];
+                                    m[n][e] = mn;
+                                    mine[n][e] *= a;
+                                    theirs[n][e] *= b;
+                                }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    float& y = o[n][4 * p + i][e];
+                                    y = y * mine[n][e & 1] + buf[((place * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] * theirs[n][e & 1];
+                                }
                     }
                 }
-                pa[st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if constexpr (F32) pr[st] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
             }
-
-            // ---- O += P V
-            sl = u_get % K::slots;
-            if (!mbar_wait(&full[bw][sl], (u_get / K::slots) & 1)) { ok = false; break; }
-            const uint8_t* vp = ring + sl * K::slot + g * kKvBlock + t * 16;
+            if (BW == 1) __syncthreads();                                        // every warp is done with the queries
+            // ---- out, or a part of it, row by row over the desk
+            const bool whole = seg0 >= w0 && seg1 <= w1;
+            // a thread block has parts of two (tile, head)s at most: one that began in front of its share, one that goes on behind it
+            const size_t part_at = (size_t) (2 * blockIdx.x + (seg0 < w0 ? 0 : 1)) * K::rows;
+            if (bw == 0 && !lost) {
+                if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const uint4 w = *(const uint4*) (vp + i * 8 * kKvBlock);
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                // f32: a block's products are summed by themselves and added with a rounded add - the tensor cores cut what falls off a
-                // sum, always towards zero, and over a long axis that adds up (so do those of 64 values of a score)
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    uint32_t b0, b1;
-                    codes_to_half(ww[st], b0, b1);
-                    if constexpr (F32) {
-                        mma16816(part, pr[st], b0, b1);
-                        mma16816(part, pa[st], b0, b1);
-                    } else {
-                        mma16816(o[i], pa[st], b0, b1);
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = (rw * NT + n) * 8 + 2 * t + e;
+                            sm_l[warp][n * 8 + 2 * t + e] = whole ? l[n][e] == 0.0f ? 0.0f : vr / l[n][e] : vr;
+                            if (T.r0 + r < T.n_rows) {
+                                if (!whole) A.part_ml[part_at + r] = make_float2(m[n][e], l[n][e]);
+                                else if (A.lse != nullptr) A.lse[out_row(A, T, h, r)] = lse_of(m[n][e], l[n][e]);
+                            }
+                        }
+                }
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    __syncwarp();
+                    lay(rw, p);
+                    __syncwarp();
+#pragma unroll
+                    for (int r2 = 0; r2 < 8 * NT; r2 += 2) {
+                        const int r = r2 + (lane >> 4), at_tile = rw * NT * 8 + r, d = (lane & 15) * 4;
+                        if (T.r0 + at_tile >= T.n_rows) continue;
+                        float4 y = *(const float4*) (buf + (rw * NT * 8 + r) * K::wide + d);
+                        const float f = sm_l[warp][r];
+                        y.x *= f; y.y *= f; y.z *= f; y.w *= f;
+                        if (!whole) *(float4*) (A.part_o + (part_at + at_tile) * D + 64 * p + d) = y;
+                        else if constexpr (F32) *(float4*) ((float*) A.out + out_row(A, T, h, at_tile) * D + 64 * p + d) = y;
+                        else {
+                            const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+                            *(uint2*) ((uint16_t*) A.out + out_row(A, T, h, at_tile) * D + 64 * p + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
+                        }
                     }
                 }
-                if constexpr (F32)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], alpha[e >> 1], part[e]);
             }
-            __syncwarp();
-            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][sl]);
-            ++u_get;
-            if (rw == 0) ask(u_get + K::slots);
+            __syncthreads();                                                     // the desk is free for the next queries
+            if (lost) break;
         }
-        if (!ok) lost = 1;
+        if (lost || !ok) break;
     }
-    if (!ok) {                                                                   // a copy that did not land in time: none may land after the end
-        lost = 1;
-        if (rw == 0)
-            for (unsigned u = u_put > K::slots ? u_put - K::slots : 0; u < u_put; ++u) mbar_wait(&full[bw][u % K::slots], (u / K::slots) & 1);
-    }
-
-    // ---- the warps' results meet in shared memory (the ring is done with)
+    if (!ok && rw == 0)                                                          // a copy that did not land in time: none may land after the end
+        for (unsigned u = u_put > K::slots ? u_put - K::slots : 0; u < u_put; ++u) mbar_wait(&full[bw][u % K::slots], (u / K::slots) & 1);
     __syncthreads();
-    if (lost) {
-        if (tid == 0) atomicExch(A.error, 1u);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        if (t == 0) { sm_m[warp][g + 8 * e] = m[e]; sm_l[warp][g + 8 * e] = l[e]; }
-    }
-    if (lane == 0) sm_vr[warp] = vr;
-    float* mo = (float*) smem;                                                   // [warp][16][D]
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-        *(float2*) (mo + (warp * 16 + g) * D + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
-        *(float2*) (mo + (warp * 16 + g + 8) * D + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
-    }
-    __syncthreads();
-    const size_t slot_id = (size_t) blockIdx.x * C.n_kv + h;
-    const int tile_rows = min(K::rows, n_rows - r0);
-    auto put_row = [&](int r, int d, float4 v, float total) {                    // four values of row r, divided by the sum
-        const int row = r0 + r, i = i0 + row / A.group, hq = h * A.group + row % A.group;
-        const size_t at = ((size_t) (s.row + i) * A.n_q + hq) * D + d;
-        const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-        v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-        if constexpr (F32) *(float4*) ((float*) A.out + at) = v;
-        else {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-            *(uint2*) ((uint16_t*) A.out + at) = make_uint2(*(const uint32_t*) &x, *(const uint32_t*) &y);
-        }
-    };
-    auto put_lse = [&](int r, float mm, float total) {
-        const int row = r0 + r, i = i0 + row / A.group, hq = h * A.group + row % A.group;
-        if (A.lse != nullptr) A.lse[(size_t) (s.row + i) * A.n_q + hq] = total > 0.0f ? (mm + log2f(total) - kPBias) * 0.69314718055994531f : kNone;
-    };
-    for (int i = tid; i < tile_rows * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = r & 15, w0 = r >> 4;      // the row's warps: w0 + RW * b
-        float mm = kNone, total = 0.0f;
-#pragma unroll
-        for (int b = 0; b < BW; ++b) mm = fmaxf(mm, sm_m[w0 + RW * b][rr]);
-        const float use = mm == kNone ? 0.0f : mm;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int b = 0; b < BW; ++b) {
-            const int w = w0 + RW * b;
-            const float f = ex2(sm_m[w][rr] - use), fv = f * sm_vr[w];
-            total += sm_l[w][rr] * f;
-            const float4 y = *(const float4*) (mo + (w * 16 + rr) * D + d);
-            v.x += y.x * fv; v.y += y.y * fv; v.z += y.z * fv; v.w += y.w * fv;
-        }
-        if (splits == 1) {
-            put_row(r, d, v, total);
-            if (d == 0) put_lse(r, mm, total);
-        } else {
-            const size_t at = (slot_id * A.n_split + split) * K::rows + r;
-            *(float4*) (A.part_o + at * D + d) = v;
-            if (d == 0) A.part_ml[at] = make_float2(mm, total);
-        }
-    }
-    if (splits == 1) return;
-
-    // ---- the last of the tile's splits joins them
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        arrived = (int) atomicAdd(A.counters + slot_id, 1u);
-        __threadfence();
-    }
-    __syncthreads();
-    if (arrived != splits - 1) return;
-    if (tid == 0) A.counters[slot_id] = 0;
-    for (int i = tid; i < tile_rows * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        const size_t at = slot_id * A.n_split * K::rows + r;
-        float mm = kNone, total = 0.0f;
-        for (int k = 0; k < splits; ++k) mm = fmaxf(mm, __ldcg(A.part_ml + at + (size_t) k * K::rows).x);
-        const float use = mm == kNone ? 0.0f : mm;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < splits; ++k) {
-            const float2 ml = __ldcg(A.part_ml + at + (size_t) k * K::rows);
-            const float f = ex2(ml.x - use);
-            const float4 y = __ldcg((const float4*) (A.part_o + (at + (size_t) k * K::rows) * D + d));
-            total += ml.y * f;
-            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-        }
-        put_row(r, d, v, total);
-        if (d == 0) put_lse(r, mm, total);
-    }
+    if (lost && tid == 0) atomicExch(A.error, 1u);
 }
 
-template<int D, bool F32, int RW>
-int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, size_t scratch_bytes, cudaStream_t s) {
-    using K = Cfg<D, F32, RW>;
+// The rows of (tile, head)s that lie in several thread blocks' shares, from their parts in the order of the list: a warp a row.
+template<int D, bool F32>
+__global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows) {
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    const long long id = (long long) blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int r = (int) (id % rows), h = (int) (id / rows % C.n_kv), tile = (int) (id / rows / C.n_kv);
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (tile >= A.tiles) return;
+    const unsigned share = *A.share, nb = A.sel != nullptr ? (unsigned) A.n_sel : (unsigned) (A.pre[tile + 1] - A.pre[tile]);
+    if (nb == 0) return;
+    const unsigned w = A.sel != nullptr ? ((unsigned) tile * (unsigned) C.n_kv + h) * nb : (unsigned) A.pre[tile] * (unsigned) C.n_kv + (unsigned) h * nb;
+    const unsigned cta0 = w / share, cta1 = (w + nb - 1) / share;
+    if (cta0 == cta1) return;
+    const Tile T = tile_of(B, A, tile, rows);
+    if (T.r0 + r >= T.n_rows) return;
+    auto slot_of = [&](unsigned c) { return (size_t) (2 * c + (c == cta0 ? 1 : 0)) * rows + r; };
+    float mm = kNone, total = 0.0f;
+    for (unsigned c = cta0 + lane; c <= cta1; c += 32) mm = fmaxf(mm, A.part_ml[slot_of(c)].x);
+    mm = warp_max(mm);
+    const float use = mm == kNone ? 0.0f : mm;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    for (unsigned c32 = cta0; c32 <= cta1; c32 += 32) {
+        float f = 0.0f;
+        if (c32 + lane <= cta1) {
+            const float2 x = A.part_ml[slot_of(c32 + lane)];
+            f = ex2(x.x - use);
+            total += x.y * f;
+        }
+        const int n = (int) min(32u, cta1 - c32 + 1);
+#pragma unroll 16
+        for (int k = 0; k < n; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float* src = A.part_o + slot_of(c32 + k) * D + lane * V;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 y = *(const float2*) (src + e);
+                acc[e] += y.x * fk;
+                acc[e + 1] += y.y * fk;
+            }
+        }
+    }
+    total = warp_sum(total);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const size_t at = out_row(A, T, h, r);
+#pragma unroll
+    for (int e = 0; e < V; ++e) st_act<!F32>(A.out, at * D + lane * V + e, acc[e] * inv);
+    if (A.lse != nullptr && lane == 0) A.lse[at] = lse_of(mm, total);
+}
+
+template<int D, bool F32, int NT, int RW>
+int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, cudaStream_t s) {
+    using K = Cfg<D, F32, NT, RW>;
+    static_assert(K::slots >= 2, "a ring holds a piece in use and one on its way");
     const long long rows = a.sel ? A.group : (long long) b.max_new * A.group;
     A.row_tiles = (int) ((rows + K::rows - 1) / K::rows);
     const long long tiles = (long long) A.row_tiles * (a.sel ? b.n_tokens : b.n_seq);
-    if (tiles > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
-    // cache blocks of the longest tile
-    long long most = a.sel ? a.n_sel : (b.max_len + kKvBlock - 1) / kKvBlock;
+    long long most = a.sel ? a.n_sel : (b.max_len + kKvBlock - 1) / kKvBlock;    // cache blocks of the longest tile
     if (!a.sel && a.window > 0) {
         const long long reach = (a.window + (K::rows + A.group - 1) / A.group + 2 * kKvBlock) / kKvBlock;
         if (reach < most) most = reach;
     }
     if (most < 1) most = 1;
-    // Splits: as many as fill the chip once with the longest tiles, none below one block a ring or, to keep ragged batches even, above 64.
-    const long long room = (long long) sm_count() * K::ctas, pairs = tiles * c.n_kv;
-    long long per = (most * pairs + room - 1) / room;
-    if (per < K::BW) per = K::BW;
-    if (per > 64) per = 64;
-    long long n_split = (most + per - 1) / per;
-    const size_t parts = scratch_bytes > kAttnHead + kCountersMost * 4 ? (scratch_bytes - kAttnHead - kCountersMost * 4) / ((D + 2) * 4) : 0;
-    if (pairs > kCountersMost || pairs * n_split * K::rows > (long long) parts) {   // no room for the partials: as many as there is room for
-        n_split = pairs > kCountersMost ? 1 : (long long) parts / (pairs * K::rows);
-        if (n_split < 1) n_split = 1;
-        per = (most + n_split - 1) / n_split;
-        n_split = (most + per - 1) / per;
+    // As many thread blocks as are on the chip at once, each with an even share of the cache blocks; none with less than a round of its rings.
+    // With more tiles than a thread block adds up in one go, one a (tile, head): there are enough of them to fill the chip.
+    A.tiles = (int) tiles;
+    A.direct = (!a.sel && tiles > kTilesMost) || tiles * most * c.n_kv >= 0x7fffffffll;
+    long long grid = tiles * c.n_kv;
+    if (grid > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
+    if (!A.direct) {
+        const long long rounds = (tiles * most * c.n_kv + K::BW - 1) / K::BW;
+        grid = (long long) sm_count() * K::ctas;
+        if (grid > kCtasMost) grid = kCtasMost;
+        if (grid > rounds) grid = rounds;
     }
-    A.split_blocks = (int) per;
-    A.n_split = (int) n_split;
-    A.counters = (unsigned*) (scratch + kAttnHead);
-    A.part_ml = (float2*) (scratch + kAttnHead + kCountersMost * 4);
-    A.part_o = (float*) (A.part_ml + pairs * n_split * K::rows);
+    A.share = (unsigned*) (scratch + 16);
+    A.pre = (int*) (scratch + kAttnHead);
+    A.part_ml = (float2*) (scratch + kAttnHead + kAttnPre);
+    A.part_o = (float*) (A.part_ml + 2 * kCtasMost * K::rows);
     static SmemLimit limit;
-    if (!limit.raise((const void*) attn_kernel<D, F32, RW>, K::smem)) return note_launch("kv attention smem attribute");
-    launch_dependent(attn_kernel<D, F32, RW>, dim3((unsigned) tiles, (unsigned) c.n_kv, (unsigned) n_split), dim3(kThreads), K::smem, s, kv_view(c),
-                     batch_view(b), A);
-    return note_launch("attn_q8");
+    if (!limit.raise((const void*) attn_kernel<D, F32, NT, RW>, K::smem)) return note_launch("kv attention smem attribute");
+    launch_dependent(attn_kernel<D, F32, NT, RW>, dim3((unsigned) grid), dim3(kThreads), K::smem, s, kv_view(c), batch_view(b), A);
+    const int st = note_launch("attn_q8");
+    if (st != MAYA_OK || A.direct || grid == 1) return st;
+    launch_dependent(join_kernel<D, F32>, dim3((unsigned) ((tiles * c.n_kv * K::rows + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows);
+    return note_launch("attn_q8 join");
 }
 
 template<int D, bool F32>
-int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, uint8_t* scratch, size_t bytes,
-            cudaStream_t s) {
+int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, uint8_t* scratch, cudaStream_t s) {
     const long long rows = (long long) (a.sel ? 1 : b.max_new) * (a.n_q / c.n_kv);
-    if (rows <= 16) return launch_attn<D, F32, 1>(c, b, a, A, scratch, bytes, s);
-    if (rows <= 32) return launch_attn<D, F32, 2>(c, b, a, A, scratch, bytes, s);
-    return launch_attn<D, F32, 4>(c, b, a, A, scratch, bytes, s);
+    if (rows <= 8) return launch_attn<D, F32, 1, 1>(c, b, a, A, scratch, s);
+    if constexpr (D <= 128) {
+        if (rows <= 16) return launch_attn<D, F32, 2, 1>(c, b, a, A, scratch, s);
+        if (rows <= 32) return launch_attn<D, F32, 2, 2>(c, b, a, A, scratch, s);
+        return launch_attn<D, F32, 2, 4>(c, b, a, A, scratch, s);
+    } else {                                                                     // (two columns of outputs of these sizes do not fit the registers)
+        if (rows <= 16) return launch_attn<D, F32, 1, 2>(c, b, a, A, scratch, s);
+        return launch_attn<D, F32, 1, 4>(c, b, a, A, scratch, s);
+    }
 }
 
 }  // namespace
@@ -480,7 +752,7 @@ using namespace maya;
 
 extern "C" size_t maya_attn_scratch_bytes(const maya_kv_cache* c, int n_q, int max_tokens) {
     if (kv_check(c) != MAYA_OK || n_q <= 0 || n_q % c->n_kv != 0 || max_tokens <= 0) return 0;
-    return kAttnHead + (size_t) kCountersMost * 4 + (size_t) kPartRows * (c->head_dim + 2) * 4;
+    return kAttnHead + kAttnPre + (size_t) 2 * kCtasMost * 64 * (c->head_dim + 2) * 4;
 }
 
 extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, const maya_attn_args* a, void* scratch, size_t scratch_bytes,
@@ -494,7 +766,7 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     if (a->ld_q < (int64_t) a->n_q * c->head_dim || !aligned16(a->out)) return refuse(MAYA_ERR_ARG);
     if (a->sel && a->n_sel <= 0) return refuse(MAYA_ERR_ARG);
     if ((a->sel && a->n_sel > MAYA_MAX_SELECTED) || c->n_kv > 65535) return refuse(MAYA_ERR_LIMIT);
-    if (!scratch || ((uintptr_t) scratch & 255u) || scratch_bytes < kAttnHead + kCountersMost * 4) return refuse(MAYA_ERR_ARG);
+    if (!scratch || ((uintptr_t) scratch & 255u) || scratch_bytes < maya_attn_scratch_bytes(c, a->n_q, 1)) return refuse(MAYA_ERR_ARG);
     cudaStream_t s = as_stream(stream);
     AttnView A{};
     A.q = a->q; A.ld_q = a->ld_q; A.out = a->out; A.lse = a->lse; A.sel = a->sel; A.n_sel = a->n_sel; A.n_q = a->n_q; A.group = a->n_q / c->n_kv;
@@ -504,7 +776,7 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     A.error = (unsigned*) scratch;
     st = attn_prompt(*c, *b, A, a->is_bf16 != 0, s);
     if (st != kNotTaken) return st;
-#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, (uint8_t*) scratch, scratch_bytes, s) : by_rows<D, true>(*c, *b, *a, A, (uint8_t*) scratch, scratch_bytes, s)
+#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, (uint8_t*) scratch, s) : by_rows<D, true>(*c, *b, *a, A, (uint8_t*) scratch, s)
     switch (c->head_dim) {
         case 64: return ATTN(64);
         case 128: return ATTN(128);

@@ -4,7 +4,7 @@
 //   s_j = (q . k_j) * scale * k_scale[block] * log2(e)          p_j = 2^(s_j - m)          O = sum p_j v_j,  l = sum p_j
 // The codes of K and V become f16 exactly (|code| <= 127); a query row is multiplied by a power of two that brings its largest
 // value to 2^11 .. 2^12 and rounded to f16, or for f32 activations split in two f16 terms (22 bits); P likewise, as 2^12 p
-// times v_scale[block] / (the largest v_scale so far), which keeps it in f16's range whatever the scales.  Products are summed in f32.
+// with v_scale[block] in its exponent or as a factor against the largest one so far, which keeps it in f16's range whatever the scales.  Products are summed in f32.
 #pragma once
 
 #include "maya_kv.cuh"
@@ -24,18 +24,19 @@ struct AttnView {
     int n_sel, n_q, group, window, wide_q;
     float scale_log2;                            // scale * log2(e)
     int row_tiles;                               // tiles of a sequence (of a token, with sel)
-    int split_blocks, n_split;                   // cache blocks a split takes, splits of the longest tile
+    int tiles;                                   // of all sequences (tokens)
+    bool direct;                                 // a thread block a (tile, head), not an even share of all
     unsigned* error;
-    unsigned* counters;                          // one a (tile, head): partials that have been written
-    float* part_o;                               // [tile][head][split][rows][D]
-    float2* part_ml;                             // [tile][head][split][rows]
+    unsigned* share;                             // triples of a thread block, and
+    int* pre;                                    // blocks in front of each tile: for the join
+    float* part_o;                               // [thread block][2][rows][D]
+    float2* part_ml;                             // [thread block][2][rows]
 };
 
-// The scratch: a 256-byte head (the error word), the counters, the partials.
-constexpr size_t kAttnHead = 256;
-constexpr int kCountersMost = 1 << 16;           // (tile, head) pairs that can be split
-constexpr int kPartRows = 296 * 4 * 64;          // rows of partials: four splits a resident block of the widest tiles, see attn_q8's rule
-
+// The scratch: a 256-byte head (the error word, the share), the prefix, the parts.
+constexpr size_t kAttnHead = 256, kAttnPre = 2048;
+constexpr int kCtasMost = 448;                   // thread blocks that share out the work: three an SM
+constexpr float kVsLeast = 1e-30f;               // a value scale of 0 is this in P's exponent: P is 0 in f16 and right in l
 constexpr int kNotTaken = 1;
 // Attention of a prompt's rows on tcgen05 (kv_attn_prompt.cu); kNotTaken: not that kernel's call, nothing launched.
 int attn_prompt(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, cudaStream_t s);

@@ -28,7 +28,6 @@ constexpr int kPThreads = 16 * 32;
 // Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 176 + 128 * 104 + 128 * 48 = 64512.
 constexpr int kRegsSoftmax = 176, kRegsExpand = 104, kRegsIssue = 48;
 constexpr float kRise = 8.0f, kUp = 4.0f;
-constexpr float kVsLeast = 1e-30f;               // a scale of 0 is this in the exponent: its P is 0 in f16 and right in l
 constexpr int kMetaRing = 4;
 
 struct StepMeta {                                // of the two cache blocks of a step
