@@ -30,6 +30,7 @@ namespace {
 constexpr int kThreads = 128, kWarps = 4;
 constexpr int kMeta = 128;                        // cache blocks looked up at a time
 constexpr int kPiece = 4096;                      // bytes of a ring's slot: 64 tokens x 64 values of K or of V
+constexpr long long kWarm = 1 << 20;              // bytes of queries, and of the table, that are asked into L2 ahead
 constexpr int kTilesMost = 256;                   // tiles whose blocks a thread block adds up
 
 struct Meta {
@@ -68,11 +69,12 @@ template<int D, bool F32, int NT, int RW> struct Cfg {
     static constexpr int ctas = D == 64 ? (F32 && NT == 2 ? 2 : 3) : D == 128 ? (F32 || NT == 2 ? 2 : 3) : F32 ? 1 : 2;   // thread blocks an SM
     static constexpr int room = ctas == 3 ? 71680 : ctas == 2 ? 108544 : 212992; // and shared memory of each
     static constexpr int frag = RW * NT * (D / 64) * 2 * 512;                    // queries as fragments
-    static constexpr int wide = 64 + 4;                                          // floats of a row where outputs meet, 64 values at a time
-    static constexpr int merge = (RW > 2 ? RW : 2) * 8 * NT * wide * 4;
-    static constexpr int desk = (F32 ? 2 : 1) * frag > merge ? (F32 ? 2 : 1) * frag : merge;   // the queries, and after them the outputs that meet
+    static constexpr int wide = D + 4;                                           // floats of a row where the rings' outputs meet, over the rings
+    static constexpr int merge = kWarps * 8 * NT * wide * 4;
+    static constexpr int desk = (F32 ? 2 : 1) * frag;
     static constexpr int slots = (room - desk) / kPiece / BW;                    // of a ring
     static constexpr int body = BW * slots * kPiece;
+    static_assert(merge <= body, "outputs meet in the rings' memory");
     static constexpr size_t smem = (size_t) body + desk;
 };
 
@@ -104,6 +106,39 @@ __device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int 
 // O is P V with P = 2^12 p, l the sum of P (V's scale taken out again)
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.0f ? (m + log2f(l) - kPBias) * 0.69314718055994531f : kNone; }
 
+// How the list of `work` triples is cut into stretches, one a thread block: whole rounds of `bw` blocks, as even as they go; or, with lists that are
+// fewer than thread blocks, every list into as many stretches as there are thread blocks for it (a stretch of two lists pays for two ends).
+struct Shares {
+    unsigned work, count, unit, per, more;       // stretches; rounds of each, the first `more` of them one more
+    unsigned parts, each, len;                   // of a list: stretches, blocks of each, blocks in all
+    __device__ __forceinline__ unsigned start(unsigned i) const {
+        if (parts > 0) return i / parts * len + min(i % parts * each, len);
+        return min(work, (i * per + min(i, more)) * unit);
+    }
+    __device__ __forceinline__ unsigned of(unsigned w) const {                   // the stretch that triple w is in
+        if (parts > 0) return w / len * parts + w % len / each;
+        const unsigned u = w / unit, big = more * (per + 1);
+        return u < big ? u / (per + 1) : more + (u - big) / per;
+    }
+};
+__device__ __forceinline__ Shares shares_of(const AttnView& A, unsigned work, int bw) {
+    Shares s{};
+    s.work = work;
+    s.unit = (unsigned) bw;
+    if (A.sel != nullptr && A.list_parts > 0) {
+        s.len = (unsigned) A.n_sel;
+        s.each = (s.len + A.list_parts - 1) / A.list_parts;
+        s.parts = (s.len + s.each - 1) / s.each;
+        s.count = work / s.len * s.parts;
+        return s;
+    }
+    const unsigned all = (work + s.unit - 1) / s.unit;
+    s.count = max(1u, min(A.grid, all));                                         // (no stretch is empty: the join takes parts from all of them)
+    s.per = all / s.count;
+    s.more = all % s.count;
+    return s;
+}
+
 template<int D, bool F32, int NT, int RW>
 __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
     using K = Cfg<D, F32, NT, RW>;
@@ -126,6 +161,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
         mbar_fence_init();
     }
     grid_launch_dependents();
+    // what the way to the first copies reads, asked into L2 (the launch in front may still be writing some of it: nothing is read)
+    for (unsigned i = blockIdx.x * kThreads + tid; i < A.warm_q + A.warm_table; i += gridDim.x * kThreads) {
+        const char* p = i < A.warm_q ? (const char*) A.q + (size_t) i * 128 : (const char*) C.table + (size_t) (i - A.warm_q) * 128;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    }
+    if (tid < 2) asm volatile("prefetch.global.L2 [%0];" ::"l"(tid == 0 ? B.start : B.kv_len));
     grid_dependency_wait();
 
     // ---- this thread block's share of all (tile, head, cache block) triples, in that order
@@ -157,26 +198,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
         total = (unsigned) all;
         __syncthreads();
     }
-    const unsigned work = total * (unsigned) C.n_kv;
-    unsigned share = (work + gridDim.x - 1) / gridDim.x;
-    share = max((unsigned) BW, (share + BW - 1) / BW * BW);                      // whole rounds of the rings
-    unsigned w0 = min(work, blockIdx.x * share), w1 = min(work, w0 + share);
-    if (A.direct) {
-        w0 = 0;
-        w1 = (unsigned) tile_of(B, A, (int) (blockIdx.x / C.n_kv), K::rows).n_blocks;
-    } else if (blockIdx.x == 0) {                                                // for the join
+    const Shares shares = shares_of(A, total * (unsigned) C.n_kv, BW);
+    if (!A.direct && blockIdx.x == 0) {                                          // for the join
         if (A.sel == nullptr)
             for (int i = tid; i <= A.tiles; i += kThreads) A.pre[i] = pre[i];
-        if (tid == 0) *A.share = share;
+        if (tid == 0) *A.work = shares.work;
     }
-    if (w0 >= w1) return;
     // triple w: its tile (the last whose first triple is not behind it), head and block
     auto find = [&](unsigned w, int& tile, int& h, int& b, int& nb) {
         if (A.direct) {
             tile = (int) (blockIdx.x / C.n_kv);
             h = (int) (blockIdx.x % C.n_kv);
             b = (int) w;
-            nb = (int) w1;
+            nb = tile_of(B, A, tile, K::rows).n_blocks;
             return;
         }
         if (A.sel != nullptr) {
@@ -205,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
     bool ok = true;
     Tile T;
     int tile = 0, h = 0;
-    unsigned seg0 = w0, seg1 = w0;                                               // the (tile, head) at hand: its triples
+    unsigned seg0 = 0, seg1 = 0;                                                 // the (tile, head) at hand: its triples
     constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
     float qx[U][V];
     auto ask_rows = [&](int r4) {
@@ -226,7 +260,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
         seg1 = seg0 + (unsigned) nb;
         ask_rows(warp);
     };
-    begin(w0);                                                                   // (in front of the copies, behind which they would have to wait)
+    unsigned w0 = 0, w1 = 0;
+    if (A.direct) {
+        w1 = (unsigned) tile_of(B, A, (int) (blockIdx.x / C.n_kv), K::rows).n_blocks;
+    } else if (blockIdx.x < shares.count) {
+        w0 = shares.start(blockIdx.x);
+        w1 = shares.start(blockIdx.x + 1);
+    }
+    if (w0 < w1) begin(w0);                                                      // (its queries in front of the copies, behind which they would have to wait)
     bool fresh = true;
     for (unsigned c0 = w0; c0 < w1; c0 += kMeta) {
         const int nc = (int) min((unsigned) kMeta, w1 - c0);
@@ -238,19 +279,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
             const Tile x = tile_of(B, A, ti, K::rows);
             const int lb = A.sel != nullptr ? x.n_rows > 0 ? A.sel[((size_t) (ti / A.row_tiles) * C.n_kv + hh) * A.n_sel + b] : -1 : x.b_lo + b;
             const int phys = lb >= 0 && x.pos_hi >= 0 && lb <= x.pos_hi / kKvBlock ? block_of(C, x.si, lb) : -1;
-            Meta e;
-            e.lb = lb;
-            e.bh = phys >= 0 ? phys * C.n_kv + hh : -1;
-            e.ks = e.vs = 0.0f;
-            if (phys >= 0) { e.ks = C.k_scale[e.bh]; e.vs = C.v_scale[e.bh]; }
-            meta[i] = e;
+            meta[i].lb = lb;
+            meta[i].bh = phys >= 0 ? phys * C.n_kv + hh : -1;
         }
         __syncthreads();
 
-        // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots, whichever tile they are for
-        int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
+        // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots
+        int put = 0, put_to = 0, put_at = 0;                                     // next block to ask for, where to stop, its next piece
         auto ask = [&](unsigned limit) {                                         // by the ring's first warp, until `limit` pieces are asked for
-            while (put < nc && u_put < limit) {
+            while (put < put_to && u_put < limit) {
                 const int bh = meta[put].bh;
                 if (bh < 0) { put += BW; continue; }
                 const unsigned sl = u_put % K::slots;
@@ -274,12 +311,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
             ++u_get;
             if (rw == 0) ask(u_get + K::slots);
         };
-        if (rw == 0) ask(u_get + K::slots);
-
+        bool scaled = false;
         for (int i0 = 0; i0 < nc;) {                                             // the stretches of this part of the share that are one (tile, head)'s
-            if (fresh || c0 + i0 == seg1) {                                      // ---- a new one: its queries
-                if (!fresh) begin(c0 + i0);
-                fresh = false;
+            const bool first_part = fresh || c0 + i0 == seg1;
+            if (first_part && !fresh) begin(c0 + i0);
+            fresh = false;
+            const int i1 = (int) min((unsigned) nc, seg1 - c0), mine0 = i0 + (int) ((unsigned) (bw - i0) % (unsigned) BW);
+            put = mine0;
+            put_to = i1;
+            put_at = 0;
+            if (rw == 0) ask(u_get + K::slots);
+            if (!scaled) {                                                       // the scales, behind the first copies
+                scaled = true;
+                for (int i = tid; i < nc; i += kThreads) {
+                    const int bh = meta[i].bh;
+                    meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
+                    meta[i].vs = bh >= 0 ? C.v_scale[bh] : 0.0f;
+                }
+                if (!first_part) __syncthreads();
+            }
+            if (first_part) {                                                    // ---- a new one: its queries
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -324,8 +375,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                 }
                 __syncthreads();
             }
-            const int i1 = (int) min((unsigned) nc, seg1 - c0);
-            for (int b = i0 + (int) ((unsigned) (bw - i0) % (unsigned) BW); b < i1 && ok; b += BW) {
+            for (int b = mine0; b < i1 && ok; b += BW) {
                 const Meta x = meta[b];
                 if (x.bh < 0) continue;
                 // ---- S^T = K Q^T: rows of tile s are tokens, columns the queries
@@ -524,113 +574,66 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
             i0 = i1;
             if (c0 + i1 != seg1 && c0 + i1 != w1) continue;                      // the (tile, head) goes on in the next part of the share
 
-            // ---- the rings' results meet: the upper half of them hands its rows over, until the first has all
+            // ---- the rings' results meet in the rings' memory (nothing is on its way into it), a thread four values of a row
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-            float* buf = (float*) desk;                                          // [warp of two, or of RW][8 NT][wide]
-            auto lay = [&](int place, int p) {                                   // 64 values of this warp's rows
+            if (g == 0) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            buf[((place * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][4 * p + i][e];
-            };
-#pragma unroll
-            for (int half = BW / 2; half >= 1; half /= 2) {
-                const bool gives = bw >= half && bw < 2 * half, takes = bw < half;
-                const int place = (gives ? bw - half : bw) * RW + rw;            // of the pair: 0 or 1
-                if (gives && g == 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
-                    sm_vr[warp] = vr;
-                }
-                float mine[NT][2], theirs[NT][2];
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    __syncthreads();                                             // the desk is free (queries are done with; the values before have been taken)
-                    if (gives) lay(place, p);
-                    __syncthreads();
-                    if (takes) {
-                        const int from = warp + half * RW;
-                        if (p == 0) {
-                            const float v2 = sm_vr[from], vm = fmaxf(vr, v2), a = F32 ? vm > 0.0f ? __fdividef(vr, vm) : 0.0f : 1.0f,
-                                        b = F32 ? vm > 0.0f ? __fdividef(v2, vm) : 0.0f : 1.0f;
-                            vr = vm;
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const float m2 = sm_m[from][n * 8 + 2 * t + e], mn = fmaxf(m[n][e], m2), use = mn == kNone ? 0.0f : mn;
-                                    mine[n][e] = ex2(m[n][e] - use);
-                                    theirs[n][e] = ex2(m2 - use);
-                                    l[n][e] = l[n][e] * mine[n][e] + sm_l[from][n * 8 + 2 * t + e] * theirs[n][e];
-                                    m[n][e] = mn;
-                                    mine[n][e] *= a;
-                                    theirs[n][e] *= b;
-                                }
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    float& y = o[n][4 * p + i][e];
-                                    y = y * mine[n][e & 1] + buf[((place * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] * theirs[n][e & 1];
-                                }
-                    }
-                }
+                    for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
+                if (t == 0) sm_vr[warp] = vr;
             }
-            if (BW == 1) __syncthreads();                                        // every warp is done with the queries
-            // ---- out, or a part of it, row by row over the desk
-            const bool whole = seg0 >= w0 && seg1 <= w1;
-            // a thread block has parts of two (tile, head)s at most: one that began in front of its share, one that goes on behind it
-            const size_t part_at = (size_t) (2 * blockIdx.x + (seg0 < w0 ? 0 : 1)) * K::rows;
-            if (bw == 0 && !lost) {
-                if (g == 0) {
+            __syncthreads();                                                     // every ring is empty
+            float* buf = (float*) smem;                                          // [warp][8 NT][wide]
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int r = (rw * NT + n) * 8 + 2 * t + e;
-                            sm_l[warp][n * 8 + 2 * t + e] = whole ? l[n][e] == 0.0f ? 0.0f : vr / l[n][e] : vr;
-                            if (T.r0 + r < T.n_rows) {
-                                if (!whole) A.part_ml[part_at + r] = make_float2(m[n][e], l[n][e]);
-                                else if (A.lse != nullptr) A.lse[out_row(A, T, h, r)] = lse_of(m[n][e], l[n][e]);
-                            }
-                        }
-                }
+                for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    __syncwarp();
-                    lay(rw, p);
-                    __syncwarp();
-#pragma unroll
-                    for (int r2 = 0; r2 < 8 * NT; r2 += 2) {
-                        const int r = r2 + (lane >> 4), at_tile = rw * NT * 8 + r, d = (lane & 15) * 4;
-                        if (T.r0 + at_tile >= T.n_rows) continue;
-                        float4 y = *(const float4*) (buf + (rw * NT * 8 + r) * K::wide + d);
-                        const float f = sm_l[warp][r];
-                        y.x *= f; y.y *= f; y.z *= f; y.w *= f;
-                        if (!whole) *(float4*) (A.part_o + (part_at + at_tile) * D + 64 * p + d) = y;
-                        else if constexpr (F32) *(float4*) ((float*) A.out + out_row(A, T, h, at_tile) * D + 64 * p + d) = y;
-                        else {
-                            const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-                            *(uint2*) ((uint16_t*) A.out + out_row(A, T, h, at_tile) * D + 64 * p + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
-                        }
-                    }
-                }
-            }
-            __syncthreads();                                                     // the desk is free for the next queries
+                    for (int e = 0; e < 4; ++e) buf[((warp * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][i][e];
+            __syncthreads();
             if (lost) break;
+            const bool whole = seg0 >= w0 && seg1 <= w1;
+            // a stretch has parts of two (tile, head)s at most: one that began in front of it, one that goes on behind it
+            const size_t part_at = (size_t) (2 * blockIdx.x + (seg0 < w0 ? 0 : 1)) * K::rows;
+            for (int i = tid; i < K::rows * (D / 4); i += kThreads) {
+                const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = r % (8 * NT), x0 = r / (8 * NT);      // the row's warps: x0 + RW * b
+                if (T.r0 + r >= T.n_rows) break;
+                float mm = kNone, total = 0.0f;
+#pragma unroll
+                for (int b = 0; b < BW; ++b) mm = fmaxf(mm, sm_m[x0 + RW * b][rr]);
+                const float use = mm == kNone ? 0.0f : mm;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int b = 0; b < BW; ++b) {
+                    const int x = x0 + RW * b;
+                    const float f = ex2(sm_m[x][rr] - use), fv = F32 ? f * sm_vr[x] : f;
+                    total += sm_l[x][rr] * f;
+                    const float4 z = *(const float4*) (buf + (x * 8 * NT + rr) * K::wide + d);
+                    y.x += z.x * fv; y.y += z.y * fv; y.z += z.z * fv; y.w += z.w * fv;
+                }
+                if (!whole) {
+                    *(float4*) (A.part_o + (part_at + r) * D + d) = y;
+                    if (d == 0) A.part_ml[part_at + r] = make_float2(mm, total);
+                    continue;
+                }
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+                const size_t at = out_row(A, T, h, r);
+                if constexpr (F32) *(float4*) ((float*) A.out + at * D + d) = y;
+                else {
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+                    *(uint2*) ((uint16_t*) A.out + at * D + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
+                }
+                if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total);
+            }
+            fence_proxy_async();                                                 // the next copies write where this was read
+            __syncthreads();
         }
         if (lost || !ok) break;
     }
@@ -640,52 +643,76 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
     if (lost && tid == 0) atomicExch(A.error, 1u);
 }
 
-// The rows of (tile, head)s that lie in several thread blocks' shares, from their parts in the order of the list: a warp a row.
-template<int D, bool F32>
-__global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long id = (long long) blockIdx.x * kWarps + (threadIdx.x >> 5);
+// The rows of (tile, head)s that lie in several stretches, from their parts in the order of the list: a thread block a row (WIDE: few rows, each of many
+// parts), or a warp.
+template<int D, bool F32, bool WIDE>
+__global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows, int bw) {
+    constexpr int V = D / 32, W = WIDE ? kWarps : 1;
+    __shared__ float acc_of[WIDE ? kWarps : 1][D], l_of[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = WIDE ? warp : 0;
+    const long long id = WIDE ? (long long) blockIdx.x : (long long) blockIdx.x * kWarps + warp;
     const int r = (int) (id % rows), h = (int) (id / rows % C.n_kv), tile = (int) (id / rows / C.n_kv);
     grid_launch_dependents();
     grid_dependency_wait();
     if (tile >= A.tiles) return;
-    const unsigned share = *A.share, nb = A.sel != nullptr ? (unsigned) A.n_sel : (unsigned) (A.pre[tile + 1] - A.pre[tile]);
+    const Shares shares = shares_of(A, *A.work, bw);
+    const unsigned nb = A.sel != nullptr ? (unsigned) A.n_sel : (unsigned) (A.pre[tile + 1] - A.pre[tile]);
     if (nb == 0) return;
     const unsigned w = A.sel != nullptr ? ((unsigned) tile * (unsigned) C.n_kv + h) * nb : (unsigned) A.pre[tile] * (unsigned) C.n_kv + (unsigned) h * nb;
-    const unsigned cta0 = w / share, cta1 = (w + nb - 1) / share;
-    if (cta0 == cta1) return;
+    const unsigned s0 = shares.of(w), s1 = shares.of(w + nb - 1);
+    if (s0 == s1) return;
     const Tile T = tile_of(B, A, tile, rows);
     if (T.r0 + r >= T.n_rows) return;
-    auto slot_of = [&](unsigned c) { return (size_t) (2 * c + (c == cta0 ? 1 : 0)) * rows + r; };
+    auto slot_of = [&](unsigned c) { return (size_t) (2 * c + (c == s0 ? 1 : 0)) * rows + r; };
     float mm = kNone, total = 0.0f;
-    for (unsigned c = cta0 + lane; c <= cta1; c += 32) mm = fmaxf(mm, A.part_ml[slot_of(c)].x);
+    for (unsigned c = s0 + lane; c <= s1; c += 32) mm = fmaxf(mm, A.part_ml[slot_of(c)].x);
     mm = warp_max(mm);
     const float use = mm == kNone ? 0.0f : mm;
     float acc[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-    for (unsigned c32 = cta0; c32 <= cta1; c32 += 32) {
+    for (unsigned c32 = s0 + part * 32; c32 <= s1; c32 += 32 * W) {
         float f = 0.0f;
-        if (c32 + lane <= cta1) {
+        if (c32 + lane <= s1) {
             const float2 x = A.part_ml[slot_of(c32 + lane)];
             f = ex2(x.x - use);
             total += x.y * f;
         }
-        const int n = (int) min(32u, cta1 - c32 + 1);
-#pragma unroll 16
-        for (int k = 0; k < n; ++k) {
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float* src = A.part_o + slot_of(c32 + k) * D + lane * V;
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 y = *(const float2*) (src + e);
-                acc[e] += y.x * fk;
-                acc[e + 1] += y.y * fk;
+        for (int k0 = 0; k0 < 32; k0 += 16) {                                    // sixteen parts in flight
+            if (c32 + k0 > s1) break;
+            float y[16][V];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float* src = A.part_o + slot_of(min(c32 + k0 + k, s1)) * D + lane * V;
+#pragma unroll
+                for (int e = 0; e < V; e += 2) *(float2*) &y[k][e] = *(const float2*) (src + e);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k0 + k);            // (0 behind the last)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] = fmaf(y[k][e], fk, acc[e]);
             }
         }
     }
     total = warp_sum(total);
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc_of[warp][lane * V + e] = acc[e];
+        if (lane == 0) l_of[warp] = total;
+        __syncthreads();
+        if (warp != 0) return;
+        total = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) total += l_of[x];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            acc[e] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < kWarps; ++x) acc[e] += acc_of[x][lane * V + e];
+        }
+    }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const size_t at = out_row(A, T, h, r);
 #pragma unroll
@@ -718,16 +745,25 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
         if (grid > kCtasMost) grid = kCtasMost;
         if (grid > rounds) grid = rounds;
     }
-    A.share = (unsigned*) (scratch + 16);
+    A.grid = (unsigned) grid;
+    A.list_parts = a.sel && !A.direct ? (unsigned) (grid / (tiles * c.n_kv)) : 0u;
+    const long long q_bytes = ((long long) (b.n_tokens - 1) * a.ld_q + (long long) a.n_q * D) * (F32 ? 4 : 2), table_bytes = (long long) b.n_seq * c.table_ld * 4;
+    A.warm_q = (unsigned) ((q_bytes < kWarm ? q_bytes : kWarm) / 128);
+    A.warm_table = (unsigned) ((table_bytes < kWarm ? table_bytes : kWarm) / 128);
+    A.work = (unsigned*) (scratch + 16);
     A.pre = (int*) (scratch + kAttnHead);
     A.part_ml = (float2*) (scratch + kAttnHead + kAttnPre);
-    A.part_o = (float*) (A.part_ml + 2 * kCtasMost * K::rows);
+    A.part_o = (float*) (A.part_ml + kPartRows);
     static SmemLimit limit;
     if (!limit.raise((const void*) attn_kernel<D, F32, NT, RW>, K::smem)) return note_launch("kv attention smem attribute");
     launch_dependent(attn_kernel<D, F32, NT, RW>, dim3((unsigned) grid), dim3(kThreads), K::smem, s, kv_view(c), batch_view(b), A);
     const int st = note_launch("attn_q8");
     if (st != MAYA_OK || A.direct || grid == 1) return st;
-    launch_dependent(join_kernel<D, F32>, dim3((unsigned) ((tiles * c.n_kv * K::rows + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows);
+    const long long all_rows = tiles * c.n_kv * K::rows;
+    if (all_rows <= 4 * sm_count())
+        launch_dependent(join_kernel<D, F32, true>, dim3((unsigned) all_rows), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
+    else
+        launch_dependent(join_kernel<D, F32, false>, dim3((unsigned) ((all_rows + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
     return note_launch("attn_q8 join");
 }
 
@@ -752,7 +788,7 @@ using namespace maya;
 
 extern "C" size_t maya_attn_scratch_bytes(const maya_kv_cache* c, int n_q, int max_tokens) {
     if (kv_check(c) != MAYA_OK || n_q <= 0 || n_q % c->n_kv != 0 || max_tokens <= 0) return 0;
-    return kAttnHead + kAttnPre + (size_t) 2 * kCtasMost * 64 * (c->head_dim + 2) * 4;
+    return kAttnHead + kAttnPre + (size_t) kPartRows * (c->head_dim + 2) * 4;
 }
 
 extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, const maya_attn_args* a, void* scratch, size_t scratch_bytes,

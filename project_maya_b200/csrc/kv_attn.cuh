@@ -27,15 +27,18 @@ struct AttnView {
     int tiles;                                   // of all sequences (tokens)
     bool direct;                                 // a thread block a (tile, head), not an even share of all
     unsigned* error;
-    unsigned* share;                             // triples of a thread block, and
+    unsigned grid, list_parts;                   // thread blocks; stretches of a list (0: even shares of all)
+    unsigned warm_q, warm_table;                 // lines of 128 bytes
+    unsigned* work;                              // all triples, and
     int* pre;                                    // blocks in front of each tile: for the join
-    float* part_o;                               // [thread block][2][rows][D]
-    float2* part_ml;                             // [thread block][2][rows]
+    float* part_o;                               // [stretch][2][rows][D]
+    float2* part_ml;                             // [stretch][2][rows]
 };
 
-// The scratch: a 256-byte head (the error word, the share), the prefix, the parts.
+// The scratch: a 256-byte head (the error word, the work), the prefix, the parts.
 constexpr size_t kAttnHead = 256, kAttnPre = 2048;
 constexpr int kCtasMost = 448;                   // thread blocks that share out the work: three an SM
+constexpr int kPartRows = 2 * kCtasMost * 64;      // rows of parts
 constexpr float kVsLeast = 1e-30f;               // a value scale of 0 is this in P's exponent: P is 0 in f16 and right in l
 constexpr int kNotTaken = 1;
 // Attention of a prompt's rows on tcgen05 (kv_attn_prompt.cu); kNotTaken: not that kernel's call, nothing launched.
