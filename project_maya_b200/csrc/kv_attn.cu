@@ -17,9 +17,9 @@
 // token two further: turned over by movmatrix, P^T's columns are the tokens of V's step s.  Every shared-memory load is 16 bytes a lane, a
 // quarter warp on 128 consecutive bytes.
 //
-// All (tile, head, cache block) triples of a call are one list, and every resident thread block takes an even stretch of it, whatever the
-// sequences' lengths (they are known on the device only); copies run ahead from one tile into the next.  A (tile, head) that lies in the
-// stretches of several thread blocks leaves (m, l, O) parts, which a second launch joins in the order of the list, a warp a row.
+// Long sequences are cut into pieces of a few dozen blocks, and the resident thread blocks take one after the other, whatever the sequences' lengths (they
+// are known on the device only).  The pieces of a (tile, head) leave (m, l, O) parts, which a second launch joins in order, a warp or a thread block a
+// row, so that the bits do not depend on who worked on what.
 #include <cuda_fp16.h>
 
 #include "kv_attn.cuh"
@@ -106,38 +106,15 @@ __device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int 
 // O is P V with P = 2^12 p, l the sum of P (V's scale taken out again)
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.0f ? (m + log2f(l) - kPBias) * 0.69314718055994531f : kNone; }
 
-// How the list of `work` triples is cut into stretches, one a thread block: whole rounds of `bw` blocks, as even as they go; or, with lists that are
-// fewer than thread blocks, every list into as many stretches as there are thread blocks for it (a stretch of two lists pays for two ends).
-struct Shares {
-    unsigned work, count, unit, per, more;       // stretches; rounds of each, the first `more` of them one more
-    unsigned parts, each, len;                   // of a list: stretches, blocks of each, blocks in all
-    __device__ __forceinline__ unsigned start(unsigned i) const {
-        if (parts > 0) return i / parts * len + min(i % parts * each, len);
-        return min(work, (i * per + min(i, more)) * unit);
-    }
-    __device__ __forceinline__ unsigned of(unsigned w) const {                   // the stretch that triple w is in
-        if (parts > 0) return w / len * parts + w % len / each;
-        const unsigned u = w / unit, big = more * (per + 1);
-        return u < big ? u / (per + 1) : more + (u - big) / per;
-    }
-};
-__device__ __forceinline__ Shares shares_of(const AttnView& A, unsigned work, int bw) {
-    Shares s{};
-    s.work = work;
-    s.unit = (unsigned) bw;
-    if (A.sel != nullptr && A.list_parts > 0) {
-        s.len = (unsigned) A.n_sel;
-        s.each = (s.len + A.list_parts - 1) / A.list_parts;
-        s.parts = (s.len + s.each - 1) / s.each;
-        s.count = work / s.len * s.parts;
-        return s;
-    }
-    const unsigned all = (work + s.unit - 1) / s.unit;
-    s.count = max(1u, min(A.grid, all));                                         // (no stretch is empty: the join takes parts from all of them)
-    s.per = all / s.count;
-    s.more = all % s.count;
-    return s;
+// A (tile, head)'s cache blocks are cut into pieces of about `q`, of which a thread block works on one at a time: about six a thread block where there are
+// many blocks (the SMs are not equally fast: with even shares fixed beforehand the last of 444 thread blocks ended at 147 us, the middle one at 113), none
+// below a round of 16, or more than there is room for parts of.
+__device__ __forceinline__ unsigned piece_of(const AttnView& A, unsigned blocks, int bw) {
+    const unsigned turns = max(1u, min(6u, blocks / A.grid / 16)), share = A.grid * turns;
+    const unsigned q = max((blocks + share - 1) / share, blocks / (A.parts_most - A.pairs) + 1);
+    return (q + bw - 1) / bw * bw;
 }
+__device__ __forceinline__ unsigned pieces_of(unsigned nb, unsigned q) { return (nb + q - 1) / q; }
 
 template<int D, bool F32, int NT, int RW>
 __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
@@ -147,7 +124,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
     __shared__ Meta meta[kMeta];
     __shared__ __align__(8) uint64_t full[BW][K::slots], empty[BW][K::slots];
     __shared__ float qinv[K::rows], sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT], sm_vr[kWarps];
-    __shared__ int pre[kTilesMost + 1];                                          // blocks (of one head) in front of each tile
+    __shared__ int pre[kTilesMost + 1];
+    __shared__ unsigned sums[kWarps], upcoming;
     __shared__ int lost;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int bw = warp / RW, rw = warp % RW;
@@ -169,69 +147,49 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
     if (tid < 2) asm volatile("prefetch.global.L2 [%0];" ::"l"(tid == 0 ? B.start : B.kv_len));
     grid_dependency_wait();
 
-    // ---- this thread block's share of all (tile, head, cache block) triples, in that order
-    unsigned total = 0;                                                          // blocks of one head over all tiles
+    // ---- the pieces in front of each tile (of one head)
+    unsigned units = 0;
     if (A.direct) {
         __syncthreads();
     } else if (A.sel != nullptr) {
-        total = (unsigned) A.tiles * (unsigned) A.n_sel;
+        units = (unsigned) A.tiles * pieces_of((unsigned) A.n_sel, piece_of(A, (unsigned) A.tiles * (unsigned) C.n_kv * (unsigned) A.n_sel, BW));
         __syncthreads();
     } else {
         const int each = (A.tiles + kThreads - 1) / kThreads;
-        int sum = 0;
-        for (int i = 0; i < each; ++i) {
-            const int x = tid * each + i;
-            if (x < A.tiles) { pre[x] = sum; sum += tile_of(B, A, x, K::rows).n_blocks; }
-        }
-        int up = sum;
+        unsigned nb[kTilesMost / kThreads], sum = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) { const int y = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += y; }
-        if (lane == 31) sm_l[0][warp] = __int_as_float(up);
-        __syncthreads();
-        int before = up - sum, all = 0;
-        for (int w = 0; w < kWarps; ++w) { const int y = __float_as_int(sm_l[0][w]); if (w < warp) before += y; all += y; }
-        for (int i = 0; i < each; ++i) {
-            const int x = tid * each + i;
-            if (x < A.tiles) pre[x] += before;
+        for (int i = 0; i < kTilesMost / kThreads; ++i) {
+            nb[i] = i < each && tid * each + i < A.tiles ? (unsigned) tile_of(B, A, tid * each + i, K::rows).n_blocks : 0u;
+            sum += nb[i];
         }
-        if (tid == 0) pre[A.tiles] = all;
-        total = (unsigned) all;
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) sums[warp] = sum;
         __syncthreads();
-    }
-    const Shares shares = shares_of(A, total * (unsigned) C.n_kv, BW);
-    if (!A.direct && blockIdx.x == 0) {                                          // for the join
-        if (A.sel == nullptr)
+        unsigned all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) all += sums[w];
+        const unsigned q = piece_of(A, all * (unsigned) C.n_kv, BW);
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < kTilesMost / kThreads; ++i) sum += pieces_of(nb[i], q);
+        unsigned up = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) { const unsigned y = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += y; }
+        __syncthreads();
+        if (lane == 31) sums[warp] = up;
+        __syncthreads();
+        unsigned before = up - sum;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sums[w]; units += sums[w]; }
+#pragma unroll
+        for (int i = 0; i < kTilesMost / kThreads; ++i)
+            if (i < each && tid * each + i < A.tiles) { pre[tid * each + i] = (int) before; before += pieces_of(nb[i], q); }
+        if (tid == 0) pre[A.tiles] = (int) units;
+        __syncthreads();
+        if (blockIdx.x == 0)                                                     // for the join
             for (int i = tid; i <= A.tiles; i += kThreads) A.pre[i] = pre[i];
-        if (tid == 0) *A.work = shares.work;
     }
-    // triple w: its tile (the last whose first triple is not behind it), head and block
-    auto find = [&](unsigned w, int& tile, int& h, int& b, int& nb) {
-        if (A.direct) {
-            tile = (int) (blockIdx.x / C.n_kv);
-            h = (int) (blockIdx.x % C.n_kv);
-            b = (int) w;
-            nb = tile_of(B, A, tile, K::rows).n_blocks;
-            return;
-        }
-        if (A.sel != nullptr) {
-            const unsigned pair = w / (unsigned) A.n_sel;
-            tile = (int) (pair / (unsigned) C.n_kv);
-            h = (int) (pair % (unsigned) C.n_kv);
-            b = (int) (w % (unsigned) A.n_sel);
-            nb = A.n_sel;
-            return;
-        }
-        int lo = 0, hi = A.tiles - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if ((unsigned) pre[mid] * (unsigned) C.n_kv <= w) lo = mid; else hi = mid - 1;
-        }
-        tile = lo;
-        nb = pre[lo + 1] - pre[lo];
-        const unsigned in = w - (unsigned) pre[lo] * (unsigned) C.n_kv;
-        h = (int) (in / (unsigned) nb);
-        b = (int) (in % (unsigned) nb);
-    };
+    units *= (unsigned) C.n_kv;
 
     float o[NT][D / 16][4], m[NT][2], l[NT][2], vr = F32 ? 0.0f : 1.0f;          // columns 2 t, 2 t + 1
     int pos[NT][2], wpos_lo = 0, wpos_hi = 0;
@@ -252,42 +210,86 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                 ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
         }
     };
-    auto begin = [&](unsigned w) {                                               // the (tile, head) of triple w: its first queries are asked for
-        int b, nb;
-        find(w, tile, h, b, nb);
-        T = tile_of(B, A, tile, K::rows);
-        seg0 = w - (unsigned) b;
-        seg1 = seg0 + (unsigned) nb;
-        ask_rows(warp);
-    };
-    unsigned w0 = 0, w1 = 0;
+    // ---- one piece after the other: the thread block's own number first, then whichever is next
+    for (unsigned unit = blockIdx.x;;) {
+    if (!A.direct && unit >= units) break;
+    unsigned next = 0xffffffffu, pieces = 1, piece = 0;
+    if (tid == 0 && !A.direct) next = gridDim.x + atomicAdd(A.taken, 1u);        // (its number arrives meanwhile)
+    int tile, h;
     if (A.direct) {
-        w1 = (unsigned) tile_of(B, A, (int) (blockIdx.x / C.n_kv), K::rows).n_blocks;
-    } else if (blockIdx.x < shares.count) {
-        w0 = shares.start(blockIdx.x);
-        w1 = shares.start(blockIdx.x + 1);
+        tile = (int) (unit / (unsigned) C.n_kv);
+        h = (int) (unit % (unsigned) C.n_kv);
+    } else {
+        unsigned in;
+        if (A.sel != nullptr) {
+            pieces = units / ((unsigned) A.tiles * (unsigned) C.n_kv);
+            tile = (int) (unit / (pieces * (unsigned) C.n_kv));
+            in = unit % (pieces * (unsigned) C.n_kv);
+        } else {
+            int lo = 0, hi = A.tiles - 1;                                        // the last tile whose first piece is not behind it
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if ((unsigned) pre[mid] * (unsigned) C.n_kv <= unit) lo = mid; else hi = mid - 1;
+            }
+            tile = lo;
+            pieces = (unsigned) (pre[lo + 1] - pre[lo]);
+            in = unit - (unsigned) pre[lo] * (unsigned) C.n_kv;
+        }
+        h = (int) (in / pieces);
+        piece = in % pieces;
     }
-    if (w0 < w1) begin(w0);                                                      // (its queries in front of the copies, behind which they would have to wait)
-    bool fresh = true;
-    for (unsigned c0 = w0; c0 < w1; c0 += kMeta) {
-        const int nc = (int) min((unsigned) kMeta, w1 - c0);
-        __syncthreads();                                                         // everybody is done with meta
+    const Tile T = tile_of(B, A, tile, K::rows);
+    const unsigned base = (unsigned) T.n_blocks / pieces, rest = (unsigned) T.n_blocks % pieces;
+    const int w0 = (int) (piece * base + min(piece, rest)), w1 = w0 + (int) (base + (piece < rest ? 1u : 0u));
+    constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
+    float qx[U][V];
+    auto ask_rows = [&](int r4) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = T.r0 + r4 + u * kWarps;
+#pragma unroll
+            for (int e = 0; e < V; ++e) qx[u][e] = 0.0f;
+            if (row < T.n_rows)
+                ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
+        }
+    };
+    ask_rows(warp);                                                              // (in front of the copies, behind which they would have to wait)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[n][e] = kNone;
+            l[n][e] = 0.0f;
+            const int row = T.r0 + (rw * NT + n) * 8 + 2 * t + e;                // last visible position (rows beyond the tile's: all, not kept)
+            pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
+        }
+    }
+    vr = F32 ? 0.0f : 1.0f;
+    int low = min(pos[0][0], pos[0][1]);
+    if constexpr (NT == 2) low = min(low, min(pos[NT - 1][0], pos[NT - 1][1]));
+    const int wpos_lo = __reduce_min_sync(0xffffffffu, low);                     // over the warp's rows
+    const int wpos_hi = T.first + T.i0 + min(min(T.r0 + K::rows, T.n_rows) - 1, T.r0 + (rw + 1) * NT * 8 - 1) / A.group;
+
+    for (int c0 = w0; c0 < w1; c0 += kMeta) {
+        const int nc = min(kMeta, w1 - c0);
+        if (c0 > w0) __syncthreads();                                            // everybody is done with meta
         if (lost) break;
         for (int i = tid; i < nc; i += kThreads) {
-            int ti, hh, b, nb;
-            find(c0 + i, ti, hh, b, nb);
-            const Tile x = tile_of(B, A, ti, K::rows);
-            const int lb = A.sel != nullptr ? x.n_rows > 0 ? A.sel[((size_t) (ti / A.row_tiles) * C.n_kv + hh) * A.n_sel + b] : -1 : x.b_lo + b;
-            const int phys = lb >= 0 && x.pos_hi >= 0 && lb <= x.pos_hi / kKvBlock ? block_of(C, x.si, lb) : -1;
+            const int lb = A.sel != nullptr ? T.n_rows > 0 ? A.sel[((size_t) (tile / A.row_tiles) * C.n_kv + h) * A.n_sel + c0 + i] : -1 : T.b_lo + c0 + i;
+            const int phys = lb >= 0 && T.pos_hi >= 0 && lb <= T.pos_hi / kKvBlock ? block_of(C, T.si, lb) : -1;
             meta[i].lb = lb;
-            meta[i].bh = phys >= 0 ? phys * C.n_kv + hh : -1;
+            meta[i].bh = phys >= 0 ? phys * C.n_kv + h : -1;
         }
         __syncthreads();
 
         // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots
-        int put = 0, put_to = 0, put_at = 0;                                     // next block to ask for, where to stop, its next piece
+        int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
         auto ask = [&](unsigned limit) {                                         // by the ring's first warp, until `limit` pieces are asked for
-            while (put < put_to && u_put < limit) {
+            while (put < nc && u_put < limit) {
                 const int bh = meta[put].bh;
                 if (bh < 0) { put += BW; continue; }
                 const unsigned sl = u_put % K::slots;
@@ -311,71 +313,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
             ++u_get;
             if (rw == 0) ask(u_get + K::slots);
         };
-        bool scaled = false;
-        for (int i0 = 0; i0 < nc;) {                                             // the stretches of this part of the share that are one (tile, head)'s
-            const bool first_part = fresh || c0 + i0 == seg1;
-            if (first_part && !fresh) begin(c0 + i0);
-            fresh = false;
-            const int i1 = (int) min((unsigned) nc, seg1 - c0), mine0 = i0 + (int) ((unsigned) (bw - i0) % (unsigned) BW);
-            put = mine0;
-            put_to = i1;
-            put_at = 0;
-            if (rw == 0) ask(u_get + K::slots);
-            if (!scaled) {                                                       // the scales, behind the first copies
-                scaled = true;
-                for (int i = tid; i < nc; i += kThreads) {
-                    const int bh = meta[i].bh;
-                    meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
-                    meta[i].vs = bh >= 0 ? C.v_scale[bh] : 0.0f;
-                }
-                if (!first_part) __syncthreads();
-            }
-            if (first_part) {                                                    // ---- a new one: its queries
+        if (rw == 0) ask(u_get + K::slots);
+        for (int i = tid; i < nc; i += kThreads) {                               // the scales, behind the first copies
+            const int bh = meta[i].bh;
+            meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
+            meta[i].vs = bh >= 0 ? C.v_scale[bh] : 0.0f;
+        }
+        if (c0 == w0) {
+            // scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
+            for (int r4 = warp; r4 < K::rows; r4 += kWarps * U) {
+                if (r4 != warp) ask_rows(r4);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int u = 0; u < U; ++u) {
+                    const int r = r4 + u * kWarps;
+                    float amax = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
+                    for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
+                    amax = warp_max(amax);
+                    const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
+                    const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
+                    if (lane == 0) qinv[r] = __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        m[n][e] = kNone;
-                        l[n][e] = 0.0f;
-                        const int row = T.r0 + (rw * NT + n) * 8 + 2 * t + e;    // last visible position (rows beyond the tile's: all, not kept)
-                        pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
+                    for (int e = 0; e < V; e += 2) {
+                        const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
+                        uint8_t* f = desk + ((((r >> 3) * P + (d >> 6)) * 2 + (st >> 1)) * 32 + (r & 7) * 4 + tt) * 16 + ((st & 1) * 2 + (w >> 1)) * 4;
+                        const uint32_t hi = pack_half(qx[u][e] * up, qx[u][e + 1] * up);
+                        *(uint32_t*) f = hi;
+                        if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, qx[u][e] * up, qx[u][e + 1] * up);
                     }
                 }
-                vr = F32 ? 0.0f : 1.0f;
-                int low = min(pos[0][0], pos[0][1]);
-                if constexpr (NT == 2) low = min(low, min(pos[1][0], pos[1][1]));
-                wpos_lo = __reduce_min_sync(0xffffffffu, low);                   // over the warp's rows
-                wpos_hi = T.first + T.i0 + min(min(T.r0 + K::rows, T.n_rows) - 1, T.r0 + (rw + 1) * NT * 8 - 1) / A.group;
-                // scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
-                for (int r4 = warp; r4 < K::rows; r4 += kWarps * U) {
-                    if (r4 != warp) ask_rows(r4);
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int r = r4 + u * kWarps;
-                        float amax = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
-                        amax = warp_max(amax);
-                        const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
-                        const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
-                        if (lane == 0) qinv[r] = __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2;
-#pragma unroll
-                        for (int e = 0; e < V; e += 2) {
-                            const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
-                            uint8_t* f = desk + ((((r >> 3) * P + (d >> 6)) * 2 + (st >> 1)) * 32 + (r & 7) * 4 + tt) * 16 + ((st & 1) * 2 + (w >> 1)) * 4;
-                            const uint32_t hi = pack_half(qx[u][e] * up, qx[u][e + 1] * up);
-                            *(uint32_t*) f = hi;
-                            if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, qx[u][e] * up, qx[u][e + 1] * up);
-                        }
-                    }
-                }
-                __syncthreads();
             }
-            for (int b = mine0; b < i1 && ok; b += BW) {
+        }
+        __syncthreads();
+
+            for (int b = bw; b < nc && ok; b += BW) {
                 const Meta x = meta[b];
                 if (x.bh < 0) continue;
                 // ---- S^T = K Q^T: rows of tile s are tokens, columns the queries
@@ -571,8 +542,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                 if (!ok) break;
             }
             if (!ok) lost = 1;
-            i0 = i1;
-            if (c0 + i1 != seg1 && c0 + i1 != w1) continue;                      // the (tile, head) goes on in the next part of the share
+    }
 
             // ---- the rings' results meet in the rings' memory (nothing is on its way into it), a thread four values of a row
 #pragma unroll
@@ -598,9 +568,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                     for (int e = 0; e < 4; ++e) buf[((warp * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][i][e];
             __syncthreads();
             if (lost) break;
-            const bool whole = seg0 >= w0 && seg1 <= w1;
-            // a stretch has parts of two (tile, head)s at most: one that began in front of it, one that goes on behind it
-            const size_t part_at = (size_t) (2 * blockIdx.x + (seg0 < w0 ? 0 : 1)) * K::rows;
+            const bool whole = pieces == 1;
+            const size_t part_at = (size_t) unit * K::rows;
             for (int i = tid; i < K::rows * (D / 4); i += kThreads) {
                 const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = r % (8 * NT), x0 = r / (8 * NT);      // the row's warps: x0 + RW * b
                 if (T.r0 + r >= T.n_rows) break;
@@ -633,17 +602,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                 if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total);
             }
             fence_proxy_async();                                                 // the next copies write where this was read
+            if (A.direct) break;
+            if (tid == 0) upcoming = next;
             __syncthreads();
-        }
-        if (lost || !ok) break;
+            unit = upcoming;
     }
     if (!ok && rw == 0)                                                          // a copy that did not land in time: none may land after the end
         for (unsigned u = u_put > K::slots ? u_put - K::slots : 0; u < u_put; ++u) mbar_wait(&full[bw][u % K::slots], (u / K::slots) & 1);
     __syncthreads();
-    if (lost && tid == 0) atomicExch(A.error, 1u);
+    if (tid == 0) {
+        if (lost) atomicExch(A.error, 1u);
+        if (!A.direct) {                                                         // the last to leave sets the counters back
+            __threadfence();
+            if (atomicAdd(A.taken + 1, 1u) == gridDim.x - 1) A.taken[0] = A.taken[1] = 0u;
+        }
+    }
 }
 
-// The rows of (tile, head)s that lie in several stretches, from their parts in the order of the list: a thread block a row (WIDE: few rows, each of many
+// The rows of (tile, head)s that were cut into pieces, from their parts in order: a thread block a row (WIDE: few rows, each of many
 // parts), or a warp.
 template<int D, bool F32, bool WIDE>
 __global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows, int bw) {
@@ -655,15 +631,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const Ba
     grid_launch_dependents();
     grid_dependency_wait();
     if (tile >= A.tiles) return;
-    const Shares shares = shares_of(A, *A.work, bw);
-    const unsigned nb = A.sel != nullptr ? (unsigned) A.n_sel : (unsigned) (A.pre[tile + 1] - A.pre[tile]);
-    if (nb == 0) return;
-    const unsigned w = A.sel != nullptr ? ((unsigned) tile * (unsigned) C.n_kv + h) * nb : (unsigned) A.pre[tile] * (unsigned) C.n_kv + (unsigned) h * nb;
-    const unsigned s0 = shares.of(w), s1 = shares.of(w + nb - 1);
-    if (s0 == s1) return;
+    unsigned pieces, s0;
+    if (A.sel != nullptr) {
+        pieces = pieces_of((unsigned) A.n_sel, piece_of(A, (unsigned) A.tiles * (unsigned) C.n_kv * (unsigned) A.n_sel, bw));
+        s0 = ((unsigned) tile * (unsigned) C.n_kv + h) * pieces;
+    } else {
+        const unsigned p0 = (unsigned) A.pre[tile];
+        pieces = (unsigned) A.pre[tile + 1] - p0;
+        s0 = p0 * (unsigned) C.n_kv + h * pieces;
+    }
+    if (pieces <= 1) return;
+    const unsigned s1 = s0 + pieces - 1;
     const Tile T = tile_of(B, A, tile, rows);
     if (T.r0 + r >= T.n_rows) return;
-    auto slot_of = [&](unsigned c) { return (size_t) (2 * c + (c == s0 ? 1 : 0)) * rows + r; };
+    auto slot_of = [&](unsigned c) { return (size_t) c * rows + r; };
     float mm = kNone, total = 0.0f;
     for (unsigned c = s0 + lane; c <= s1; c += 32) mm = fmaxf(mm, A.part_ml[slot_of(c)].x);
     mm = warp_max(mm);
@@ -746,11 +727,14 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
         if (grid > rounds) grid = rounds;
     }
     A.grid = (unsigned) grid;
-    A.list_parts = a.sel && !A.direct ? (unsigned) (grid / (tiles * c.n_kv)) : 0u;
+    A.pairs = (unsigned) (tiles * c.n_kv);
+    A.parts_most = (unsigned) (kPartRows / K::rows);
+    if (A.pairs >= A.parts_most / 2) A.direct = true;                            // many (tile, head)s: whole ones, as many thread blocks
+    if (A.direct) grid = tiles * c.n_kv;
     const long long q_bytes = ((long long) (b.n_tokens - 1) * a.ld_q + (long long) a.n_q * D) * (F32 ? 4 : 2), table_bytes = (long long) b.n_seq * c.table_ld * 4;
     A.warm_q = (unsigned) ((q_bytes < kWarm ? q_bytes : kWarm) / 128);
     A.warm_table = (unsigned) ((table_bytes < kWarm ? table_bytes : kWarm) / 128);
-    A.work = (unsigned*) (scratch + 16);
+    A.taken = (unsigned*) (scratch + 16);
     A.pre = (int*) (scratch + kAttnHead);
     A.part_ml = (float2*) (scratch + kAttnHead + kAttnPre);
     A.part_o = (float*) (A.part_ml + kPartRows);

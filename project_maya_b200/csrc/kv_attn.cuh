@@ -25,17 +25,17 @@ struct AttnView {
     float scale_log2;                            // scale * log2(e)
     int row_tiles;                               // tiles of a sequence (of a token, with sel)
     int tiles;                                   // of all sequences (tokens)
-    bool direct;                                 // a thread block a (tile, head), not an even share of all
+    bool direct;                                 // a thread block a (tile, head), in one piece
     unsigned* error;
-    unsigned grid, list_parts;                   // thread blocks; stretches of a list (0: even shares of all)
+    unsigned grid, pairs, parts_most;            // thread blocks; (tile, head)s; parts there is room for
     unsigned warm_q, warm_table;                 // lines of 128 bytes
-    unsigned* work;                              // all triples, and
-    int* pre;                                    // blocks in front of each tile: for the join
-    float* part_o;                               // [stretch][2][rows][D]
-    float2* part_ml;                             // [stretch][2][rows]
+    unsigned* taken;                             // pieces taken beyond each thread block's first; thread blocks that have left
+    int* pre;                                    // pieces of a head in front of each tile: for the join
+    float* part_o;                               // [piece][rows][D]
+    float2* part_ml;                             // [piece][rows]
 };
 
-// The scratch: a 256-byte head (the error word, the work), the prefix, the parts.
+// The scratch: a 256-byte head (the error word, the counters), the prefix, the parts.
 constexpr size_t kAttnHead = 256, kAttnPre = 2048;
 constexpr int kCtasMost = 448;                   // thread blocks that share out the work: three an SM
 constexpr int kPartRows = 2 * kCtasMost * 64;      // rows of parts
