@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             for (int j = 0; j < steps && ok; ++j) {
                 if (!wait(&s_full[x], j & 1)) { ok = false; break; }
                 tc_fence_after();
-    #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+    #pragma unroll 1
+                for (int c = 0; c < 2; ++c) {                           // (not unrolled: the parts' code side by side is more than the instruction cache holds)
                     const StepMeta& sm = meta[j % kMetaRing];
                     const int lb = sm.lb[c];
                     const float lv = sm.lv[c], ivs = sm.ivs[c];
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         if (j + c > 0) {
                             if (c == 1 && !wait(&pv_first[x], j & 1)) { ok = false; break; }            // (at c = 0 the scores came after it)
                             tc_fence_after();
-    #pragma unroll
+    #pragma unroll 1
                             for (int d = 0; d < D; d += 16) {
                                 float o[16];
                                 tmem_ld16(at_o + d, o);
