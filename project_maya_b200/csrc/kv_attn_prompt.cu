@@ -5,10 +5,9 @@
 // blocks they see, 128 tokens a step:
 //   warps 0..3, 4..7   softmax of tile 0, 1: a thread a row.  64 scores at a time (a cache block: one scale) from tensor memory, 2^x, P back
 //                      to tensor memory as f16 over the scores it came from.
-//   warps 8..11        expand the codes of K and V to f16 into the swizzled shared-memory tiles that the tensor cores read, one step
+//   warps 8..14        expand the codes of K and V to f16 into the swizzled shared-memory tiles that the tensor cores read, one step
 //                      ahead (codes come straight to registers: staging them would cost shared-memory bandwidth the products need).
-//   warp 12            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory).  (Warps 13..15 only
-//                      complete the group whose registers the others take.)
+//   warp 15            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory).
 // The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
 // tensor pipe (D = 128) and 2048 of the exponential's pipe.
 //
@@ -25,10 +24,11 @@ namespace maya {
 namespace {
 
 constexpr int kPThreads = 16 * 32;
-// Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 176 + 128 * 104 + 128 * 48 = 64512.
-constexpr int kRegsSoftmax = 176, kRegsExpand = 104, kRegsIssue = 48;
+constexpr int kExpandWarps = 7, kExpandThreads = 32 * kExpandWarps, kIssueWarp = 15;
+// Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 168 + 256 * 88 = 65536.
+constexpr int kRegsSoftmax = 168, kRegsOther = 88;
 constexpr float kRise = 8.0f, kUp = 4.0f;
-constexpr int kMetaRing = 4;
+constexpr int kMetaRing = 4;                     // (a step's numbers are written while the softmax may be three steps behind)
 
 struct StepMeta {                                // of the two cache blocks of a step
     int lb[2];
@@ -49,6 +49,22 @@ __device__ __forceinline__ float ex2p(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two f32 operations at once; the largest of three
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(unsigned long long*) &d) : "l"(*(unsigned long long*) &a), "l"(*(unsigned long long*) &b), "l"(*(unsigned long long*) &c));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*) &d) : "l"(*(unsigned long long*) &a), "l"(*(unsigned long long*) &b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -94,13 +110,13 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_free[i], 1);
+            mbar_init(&k_full[i], kExpandWarps); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], kExpandWarps); mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4); mbar_init(&pv_first[i], 1); mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
         }
         lost = 0;
         mbar_fence_init();
     }
-    if (warp == 12) tmem_alloc(&tmem_base, 512);
+    if (warp == kIssueWarp) tmem_alloc(&tmem_base, 512);
     grid_launch_dependents();
     grid_dependency_wait();
 
@@ -127,11 +143,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     const uint32_t tmem = tmem_base;
 
     // (each part sets its registers in a branch of its own: where paths meet the smallest number holds)
-    if (warp >= 8 && warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (warp != kIssueWarp) {
         // ================================================================ codes -> f16 operands
         const int ct = tid - 256;
-        constexpr int pieces = 128 * D / 16 / 128;                      // 16-byte pieces of a tile a thread takes
+        constexpr int all = 128 * D / 16, pieces = (all + kExpandThreads - 1) / kExpandThreads;    // 16-byte pieces of a tile; a thread takes
         int batch = -1;
         int my_phys = -1, my_lb = -1;
         float my_ks = 0.0f, my_vs = 0.0f;
@@ -154,15 +171,16 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
         auto load = [&](uint4 (&w)[pieces], const uint8_t* base) {
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
-                const int q = i * 128 + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16);
+                const int q = i * kExpandThreads + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16);
                 w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (phys[x] >= 0) w[i] = *((const uint4*) (base + ((size_t) phys[x] * C.n_kv + h) * (kKvBlock * D)) + in);
+                if (q < all && (x == 0 ? phys[0] : phys[1]) >= 0) w[i] = *((const uint4*) (base + ((size_t) (x == 0 ? phys[0] : phys[1]) * C.n_kv + h) * (kKvBlock * D)) + in);
             }
         };
         auto store = [&](const uint4 (&w)[pieces], uint8_t* dst, bool val) {
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
-                const int q = i * 128 + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16), c4 = in & 3;
+                const int q = i * kExpandThreads + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16), c4 = in & 3;
+                if (q >= all) break;
                 // keys: panel = 64 values, row = token; values: panel = the block's 64 tokens, row = value
                 const int panel = val ? x : in / 256, row = val ? in / 4 : x * 64 + (in % 256) / 4;
                 uint8_t* p = dst + panel * ((val ? D : 128) * 128) + row * 128;
@@ -176,31 +194,30 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             __syncwarp();
         };
         auto find = [&](int j) {                                        // the step's two blocks
-            StepMeta m;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 look_up(2 * j + x);
-                const int src = (2 * j + x) & 31;
-                phys[x] = __shfl_sync(0xffffffffu, my_phys, src);
-                m.lb[x] = phys[x] >= 0 ? __shfl_sync(0xffffffffu, my_lb, src) : -1;
-                m.ks[x] = __shfl_sync(0xffffffffu, my_ks, src);
-                const float vs = fmaxf(__shfl_sync(0xffffffffu, my_vs, src), kVsLeast);
-                m.lv[x] = log2f(vs);
-                m.ivs[x] = 1.0f / vs;
+                phys[x] = __shfl_sync(0xffffffffu, my_phys, (2 * j + x) & 31);
             }
-            return m;
+            if (warp == 8 && ((2 * j) & 31) == (lane & 30)) {           // their numbers, from the two lanes that have them
+                StepMeta& m = meta[j % kMetaRing];
+                const float vs = fmaxf(my_vs, kVsLeast);
+                m.lb[lane & 1] = my_phys >= 0 ? my_lb : -1;
+                m.ks[lane & 1] = my_ks;
+                m.lv[lane & 1] = __log2f(vs);
+                m.ivs[lane & 1] = __fdividef(1.0f, vs);
+            }
         };
         if (here && steps > 0) {
-            StepMeta m = find(0);
+            find(0);
             load(cur, C.k);
             for (int j = 0; j < steps; ++j) {
                 load(nxt, C.v);                                         // this step's values, under the conversion of its keys
                 if (j >= 2 && !wait(&k_free[j & 1], ((j >> 1) - 1) & 1)) break;
-                if (ct == 0) meta[j % kMetaRing] = m;
                 store(cur, smem + K::k + (j & 1) * K::tile, false);
                 if (lane == 0) mbar_arrive_one(&k_full[j & 1]);
                 if (j + 1 < steps) {
-                    m = find(j + 1);
+                    find(j + 1);
                     load(cur, C.k);
                 }
                 if (j >= 2 && !wait(&v_free[j & 1], ((j >> 1) - 1) & 1)) break;
@@ -208,9 +225,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 if (lane == 0) mbar_arrive_one(&v_full[j & 1]);
             }
         }
-    } else if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-        if (here && warp == 12) {
+        } else if (here) {
             // ================================================================ products
             const uint32_t base = smem_u32(smem);
             auto scores = [&](int x, int j) {
@@ -331,11 +346,13 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         }
                         f = 1.0f;
                     }
-                    float mx[4] = {kNone, kNone, kNone, kNone};
-    #pragma unroll
-                    for (int i = 0; i < 64; i += 4)
-    #pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(v[i + e]));
+                    float mx[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 4]));
+#pragma unroll
+                    for (int i = 8; i < 64; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
                     const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
                     if (__any_sync(0xffffffffu, top > m + kRise || (m == kNone && top > kNone))) {      // the warp's rows are rescaled together
                         const bool mine = top > m + kRise || m == kNone;
@@ -359,20 +376,23 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         }
                     }
                     const float off = m == kNone ? kNone : lv - m + kUp;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    #pragma unroll
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+#pragma unroll
                     for (int i = 0; i < 64; i += 32) {
                         uint32_t p[16];
-    #pragma unroll
+#pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float a = ex2p(fmaf(__uint_as_float(v[i + e]), f, off)), b = ex2p(fmaf(__uint_as_float(v[i + e + 1]), f, off));
-                            sum[e & 2] += a;
-                            sum[(e & 2) + 1] += b;
-                            p[e / 2] = half2_of(a, b);
+                            float2 y = fma2(make_float2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1])), f2, off2);
+                            y.x = ex2p(y.x);
+                            y.y = ex2p(y.y);
+                            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], y);
+                            p[e / 2] = half2_of(y.x, y.y);
                         }
                         tmem_st16(at_s + 64 * c + i / 2, p);
                     }
-                    l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ivs, l);
+                    sum[0] = add2(sum[0], sum[1]);
+                    l = fmaf(sum[0].x + sum[0].y, ivs, l);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -411,7 +431,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == kIssueWarp) tmem_dealloc(tmem, 512);
     if (tid == 0 && lost) atomicExch(A.error, 1u);
 }
 
