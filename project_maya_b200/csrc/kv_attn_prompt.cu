@@ -40,9 +40,9 @@ template<int D> struct PCfg {
     static constexpr int tile = 128 * D * 2;     // bytes of a 128-row f16 tile (Q, K; V transposed the same)
     static constexpr int q = 0, k = 2 * tile, v = 4 * tile, end = 6 * tile;
     static constexpr size_t smem = (size_t) end + 1024;      // + the start's rounding to 1024
-    static constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t) (128 >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
+    static constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t) (64 >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t) (D >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
-    static constexpr int col_s = 0, col_o = 256; // tensor memory: S of tile x at 128 x, O at 256 + D x
+    static constexpr int col_s = 0, col_o = 256; // tensor memory: S of tile x's even blocks at 128 x, of odd ones at 128 x + 64, O at 256 + D x
 };
 
 __device__ __forceinline__ float ex2p(float x) {
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     using K = PCfg<D>;
     constexpr int P = K::panels;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_ready[2][2], pv_first[2], o_done[2], q_ready[2];
+    __shared__ __align__(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2], q_ready[2];
     __shared__ StepMeta meta[kMetaRing];
     __shared__ uint32_t tmem_base;
     __shared__ int lost;
@@ -111,7 +111,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], kExpandWarps); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], kExpandWarps); mbar_init(&v_free[i], 1);
-            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4); mbar_init(&pv_first[i], 1); mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
+            mbar_init(&s_full[i][0], 1); mbar_init(&s_full[i][1], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4);
+            mbar_init(&pv_done[i], 1); mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
         }
         lost = 0;
         mbar_fence_init();
@@ -228,48 +229,50 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
         } else if (here) {
             // ================================================================ products
             const uint32_t base = smem_u32(smem);
-            auto scores = [&](int x, int j) {
-                const uint32_t qa = base + K::q + x * K::tile, ka = base + K::k + (j & 1) * K::tile;
-    #pragma unroll
+            // k counts cache blocks of 64 tokens; even and odd ones have their own scores, so that the next block's are there when the softmax of
+            // this one ends.  (Products run in the order they are issued in: P of block k - 1 has been read before S of k + 1 takes its place.)
+            const int blocks = 2 * steps;
+            auto scores = [&](int x, int k) {
+                const uint32_t qa = base + K::q + x * K::tile, ka = base + K::k + ((k >> 1) & 1) * K::tile + (k & 1) * (64 * 128);
+#pragma unroll
                 for (int p = 0; p < P; ++p)
-    #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ss(tmem + K::col_s + 128 * x, smem_desc_sw128(qa + p * (128 * 128) + k * 32), smem_desc_sw128(ka + p * (128 * 128) + k * 32),
-                               K::idesc_s, p + k > 0);
-                mma_commit_elect(smem_u32(&s_full[x]));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_ss(tmem + K::col_s + 128 * x + 64 * (k & 1), smem_desc_sw128(qa + p * (128 * 128) + i * 32), smem_desc_sw128(ka + p * (128 * 128) + i * 32),
+                               K::idesc_s, p + i > 0);
+                mma_commit_elect(smem_u32(&s_full[x][k & 1]));
             };
             bool ok = steps == 0 || (wait(&k_full[0], 0) && wait(&q_ready[0], 0) && (tiles == 1 || wait(&q_ready[1], 0)));
             tc_fence_after();
-            if (ok && steps > 0) {
+            if (ok && steps > 0)
                 for (int x = 0; x < tiles; ++x) scores(x, 0);
-                mma_commit_elect(smem_u32(&k_free[0]));
-            }
-            for (int j = 0; j < steps && ok; ++j) {
-                ok = wait(&v_full[j & 1], (j >> 1) & 1);
-                if (ok && j + 1 < steps) ok = wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-                for (int x = 0; x < tiles && ok; ++x) {
-                    const uint32_t va = base + K::v + (j & 1) * K::tile;
-    #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        ok = ok && wait(&p_ready[x][c], j & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-    #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_ts(tmem + K::col_o + D * x, tmem + K::col_s + 128 * x + 64 * c + 8 * k, smem_desc_sw128(va + c * (D * 128) + k * 32),
-                                   K::idesc_o, j + c + k > 0);
-                        if (c == 0) mma_commit_elect(smem_u32(&pv_first[x]));
-                    }
+            for (int k = 0; k < blocks && ok; ++k) {
+                const int j = k >> 1;
+                if (k + 1 < blocks) {
+                    const int j1 = (k + 1) >> 1;
+                    if (j1 != j) ok = wait(&k_full[j1 & 1], (j1 >> 1) & 1);
                     if (!ok) break;
-                    if (j + 1 == steps) mma_commit_elect(smem_u32(&o_done[x]));
-                    if (x + 1 == tiles) mma_commit_elect(smem_u32(&v_free[j & 1]));
-                    if (j + 1 < steps) scores(x, j + 1);
+                    tc_fence_after();
+                    for (int x = 0; x < tiles; ++x) scores(x, k + 1);
+                    if (j1 == j) mma_commit_elect(smem_u32(&k_free[j & 1]));
                 }
-                if (ok && j + 1 < steps) mma_commit_elect(smem_u32(&k_free[(j + 1) & 1]));
+                if ((k & 1) == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
+                const uint32_t va = base + K::v + (j & 1) * K::tile + (k & 1) * (D * 128);
+                for (int x = 0; x < tiles && ok; ++x) {
+                    ok = wait(&p_ready[x][k & 1], j & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_ts(tmem + K::col_o + D * x, tmem + K::col_s + 128 * x + 64 * (k & 1) + 8 * i, smem_desc_sw128(va + i * 32), K::idesc_o, k + i > 0);
+                    mma_commit_elect(smem_u32(&pv_done[x]));
+                    if (k + 1 == blocks) mma_commit_elect(smem_u32(&o_done[x]));
+                }
+                if (ok && (k & 1)) mma_commit_elect(smem_u32(&v_free[j & 1]));
             }
             if (!ok && steps > 0) {                                         // what has been issued ends before the memory is given back
-                mma_commit_elect(smem_u32(&o_done[0]));
-                mbar_wait(&o_done[0], 0);
+                mma_commit_elect(smem_u32(&o_done[1]));
+                mbar_wait(&o_done[1], 0);
             }
         }
     } else {
@@ -320,30 +323,24 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             const int wlo = __reduce_min_sync(0xffffffffu, pos), whi = first + min(last_row, r0 + warp * 32 + 31) / A.group;
             float m = kNone, l = 0.0f;
             bool ok = true;
-            for (int j = 0; j < steps && ok; ++j) {
-                if (!wait(&s_full[x], j & 1)) { ok = false; break; }
-                tc_fence_after();
-    #pragma unroll 1
-                for (int c = 0; c < 2; ++c) {                           // (not unrolled: the parts' code side by side is more than the instruction cache holds)
-                    const StepMeta& sm = meta[j % kMetaRing];
-                    const int lb = sm.lb[c];
-                    const float lv = sm.lv[c], ivs = sm.ivs[c];
-                    float f = qinv * sm.ks[c];
+#pragma unroll 1
+            for (int k = 0; k < 2 * steps; ++k) {                       // (not unrolled: the parts' code side by side is more than the instruction cache holds)
+                    if (!wait(&s_full[x][k & 1], (k >> 1) & 1)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at_k = at_s + 64 * (k & 1);
+                    const StepMeta& sm = meta[(k >> 1) % kMetaRing];
+                    const int lb = sm.lb[k & 1];
+                    const float lv = sm.lv[k & 1], ivs = sm.ivs[k & 1];
+                    float f = qinv * sm.ks[k & 1];
                     uint32_t v[64];
-                    tmem_ld32(at_s + 64 * c, *(uint32_t(*)[32]) &v[0]);
-                    tmem_ld32(at_s + 64 * c + 32, *(uint32_t(*)[32]) &v[32]);
+                    tmem_ld32(at_k, *(uint32_t(*)[32]) &v[0]);
+                    tmem_ld32(at_k + 32, *(uint32_t(*)[32]) &v[32]);
                     tmem_wait_ld();
-                    const int tb = lb * kKvBlock;
-                    if (lb < 0) {
-    #pragma unroll
-                        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(kNone);
-                        f = 1.0f;
-                    } else if (tb + kKvBlock - 1 > wlo || (A.window > 0 && tb <= whi - A.window)) {
-    #pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            const bool seen = tb + i <= pos && (A.window <= 0 || tb + i > pos - A.window || pos == 0x3fffffff);
-                            v[i] = __float_as_uint(seen ? __uint_as_float(v[i]) * f : kNone);
-                        }
+                    const int tb = lb >= 0 ? lb * kKvBlock : 0x3ffffffe;    // (no block: behind every row)
+                    if (tb + kKvBlock - 1 > wlo || (A.window > 0 && tb <= whi - A.window)) {      // not visible to every row in whole
+                        const int from = A.window > 0 && pos != 0x3fffffff ? pos - A.window - tb : -1, to = lb >= 0 ? pos - tb : -1;
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(i <= to && i > from ? __uint_as_float(v[i]) * f : kNone);
                         f = 1.0f;
                     }
                     float mx[4];
@@ -360,15 +357,15 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         const float alpha = !mine ? 1.0f : m == kNone ? 0.0f : ex2p(m - up);
                         m = up;
                         l *= alpha;
-                        if (j + c > 0) {
-                            if (c == 1 && !wait(&pv_first[x], j & 1)) { ok = false; break; }            // (at c = 0 the scores came after it)
+                        if (k > 0) {
+                            if (!wait(&pv_done[x], (k - 1) & 1)) { ok = false; break; }       // (the one before it ended in front of these scores)
                             tc_fence_after();
-    #pragma unroll 1
+#pragma unroll 1
                             for (int d = 0; d < D; d += 16) {
                                 float o[16];
                                 tmem_ld16(at_o + d, o);
                                 uint32_t ow[16];
-    #pragma unroll
+#pragma unroll
                                 for (int i = 0; i < 16; ++i) ow[i] = __float_as_uint(o[i] * alpha);
                                 tmem_st16(at_o + d, ow);
                             }
@@ -389,15 +386,14 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                             sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], y);
                             p[e / 2] = half2_of(y.x, y.y);
                         }
-                        tmem_st16(at_s + 64 * c + i / 2, p);
+                        tmem_st16(at_k + i / 2, p);
                     }
                     sum[0] = add2(sum[0], sum[1]);
                     l = fmaf(sum[0].x + sum[0].y, ivs, l);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_one(&p_ready[x][c]);
-                }
+                    if (lane == 0) mbar_arrive_one(&p_ready[x][k & 1]);
             }
             // ---- O / l
             if (ok && steps > 0) ok = wait(&o_done[x], 0);
@@ -406,16 +402,16 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 const int n = s.row + row / A.group, hq = h * A.group + row % A.group;
                 uint16_t* dst = (uint16_t*) A.out + ((size_t) n * A.n_q + hq) * D;
-    #pragma unroll
+#pragma unroll
                 for (int d = 0; d < D; d += 16) {
                     float o[16];
                     if (steps > 0) tmem_ld16(at_o + d, o);
                     else
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = 0.0f;
                     if (row < n_rows) {
                         uint32_t w[8];
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const __nv_bfloat162 b = __floats2bfloat162_rn(l > 0.0f ? o[2 * i] * inv : 0.0f, l > 0.0f ? o[2 * i + 1] * inv : 0.0f);
                             w[i] = *(const uint32_t*) &b;
