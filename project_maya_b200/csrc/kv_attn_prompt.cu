@@ -24,7 +24,7 @@ namespace maya {
 namespace {
 
 constexpr int kPThreads = 16 * 32;
-constexpr int kExpandWarps = 7, kExpandThreads = 32 * kExpandWarps, kIssueWarp = 15;
+constexpr int kExpandWarps = 7, kIssueWarp = 15;
 // Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 168 + 256 * 88 = 65536.
 constexpr int kRegsSoftmax = 168, kRegsOther = 88;
 constexpr float kRise = 8.0f, kUp = 4.0f;
@@ -148,48 +148,49 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp != kIssueWarp) {
         // ================================================================ codes -> f16 operands
-        const int ct = tid - 256;
-        constexpr int all = 128 * D / 16, pieces = (all + kExpandThreads - 1) / kExpandThreads;    // 16-byte pieces of a tile; a thread takes
+        // A warp takes every seventh group of eight rows of a tile, a lane 16 codes of it: group u lies 1024 u bytes into the f16 tile, for keys
+        // (panel, block, tokens) and for values (block, values) alike.
+        constexpr int groups = 128 * D / 512, pieces = (groups + kExpandWarps - 1) / kExpandWarps;
+        const int cw = warp - 8, r8 = lane >> 2, c4 = lane & 3;
+        const uint32_t to0 = r8 * 128 + (((2 * c4) ^ r8) << 4), to1 = r8 * 128 + (((2 * c4 + 1) ^ r8) << 4);
         int batch = -1;
-        int my_phys = -1, my_lb = -1;
+        int my_bh = -1, my_lb = -1;
         float my_ks = 0.0f, my_vs = 0.0f;
         auto look_up = [&](int b) {                                     // cache block b_lo + b of this range: 32 at a time, a lane each
             if ((b >> 5) != batch) {
                 batch = b >> 5;
                 const int x = (batch << 5) + lane;
                 my_lb = x < n_blocks ? b_lo + x : -1;
-                my_phys = my_lb >= 0 ? block_of(C, si, my_lb) : -1;
-                my_ks = my_vs = 0.0f;
-                if (my_phys >= 0) {
-                    const size_t bh = (size_t) my_phys * C.n_kv + h;
-                    my_ks = C.k_scale[bh];
-                    my_vs = C.v_scale[bh];
-                }
+                const int phys = my_lb >= 0 ? block_of(C, si, my_lb) : -1;
+                my_bh = phys >= 0 ? phys * C.n_kv + h : -1;
+                my_ks = my_bh >= 0 ? C.k_scale[my_bh] : 0.0f;
+                my_vs = my_bh >= 0 ? C.v_scale[my_bh] : 0.0f;
             }
         };
         uint4 cur[pieces], nxt[pieces];
-        int phys[2];
-        auto load = [&](uint4 (&w)[pieces], const uint8_t* base) {
+        int bh[2];                                                      // the step's blocks and head in the cache, -1: none
+        auto load = [&](uint4 (&w)[pieces], const uint8_t* cache, bool val) {
+            const uint8_t* src[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) src[x] = cache + (size_t) max(bh[x], 0) * (kKvBlock * D) + lane * 16;
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
-                const int q = i * kExpandThreads + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16);
+                const int u = cw + i * kExpandWarps, x = val ? u / (D / 8) : (u >> 3) & 1;
+                const int at = val ? u % (D / 8) : (u >> 4) * 8 + (u & 7);                             // group of the block's 512-byte groups
                 w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (q < all && (x == 0 ? phys[0] : phys[1]) >= 0) w[i] = *((const uint4*) (base + ((size_t) (x == 0 ? phys[0] : phys[1]) * C.n_kv + h) * (kKvBlock * D)) + in);
+                if (u < groups && (x == 0 ? bh[0] : bh[1]) >= 0) w[i] = *(const uint4*) ((x == 0 ? src[0] : src[1]) + at * 512);
             }
         };
-        auto store = [&](const uint4 (&w)[pieces], uint8_t* dst, bool val) {
+        auto store = [&](const uint4 (&w)[pieces], uint8_t* dst) {
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
-                const int q = i * kExpandThreads + ct, x = q / (kKvBlock * D / 16), in = q % (kKvBlock * D / 16), c4 = in & 3;
-                if (q >= all) break;
-                // keys: panel = 64 values, row = token; values: panel = the block's 64 tokens, row = value
-                const int panel = val ? x : in / 256, row = val ? in / 4 : x * 64 + (in % 256) / 4;
-                uint8_t* p = dst + panel * ((val ? D : 128) * 128) + row * 128;
+                const int u = cw + i * kExpandWarps;
+                if (u >= groups) break;
                 uint32_t o[8];
                 codes_to_half(w[i].x, o[0], o[1]); codes_to_half(w[i].y, o[2], o[3]);
                 codes_to_half(w[i].z, o[4], o[5]); codes_to_half(w[i].w, o[6], o[7]);
-                *(uint4*) (p + (((2 * c4) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *(uint4*) (p + (((2 * c4 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                *(uint4*) (dst + u * 1024 + to0) = make_uint4(o[0], o[1], o[2], o[3]);
+                *(uint4*) (dst + u * 1024 + to1) = make_uint4(o[4], o[5], o[6], o[7]);
             }
             fence_proxy_async();
             __syncwarp();
@@ -198,12 +199,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 look_up(2 * j + x);
-                phys[x] = __shfl_sync(0xffffffffu, my_phys, (2 * j + x) & 31);
+                bh[x] = __shfl_sync(0xffffffffu, my_bh, (2 * j + x) & 31);
             }
             if (warp == 8 && ((2 * j) & 31) == (lane & 30)) {           // their numbers, from the two lanes that have them
                 StepMeta& m = meta[j % kMetaRing];
                 const float vs = fmaxf(my_vs, kVsLeast);
-                m.lb[lane & 1] = my_phys >= 0 ? my_lb : -1;
+                m.lb[lane & 1] = my_bh >= 0 ? my_lb : -1;
                 m.ks[lane & 1] = my_ks;
                 m.lv[lane & 1] = __log2f(vs);
                 m.ivs[lane & 1] = __fdividef(1.0f, vs);
@@ -211,18 +212,18 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
         };
         if (here && steps > 0) {
             find(0);
-            load(cur, C.k);
+            load(cur, C.k, false);
             for (int j = 0; j < steps; ++j) {
-                load(nxt, C.v);                                         // this step's values, under the conversion of its keys
+                load(nxt, C.v, true);                                         // this step's values, under the conversion of its keys
                 if (j >= 2 && !wait(&k_free[j & 1], ((j >> 1) - 1) & 1)) break;
-                store(cur, smem + K::k + (j & 1) * K::tile, false);
+                store(cur, smem + K::k + (j & 1) * K::tile);
                 if (lane == 0) mbar_arrive_one(&k_full[j & 1]);
                 if (j + 1 < steps) {
                     find(j + 1);
-                    load(cur, C.k);
+                    load(cur, C.k, false);
                 }
                 if (j >= 2 && !wait(&v_free[j & 1], ((j >> 1) - 1) & 1)) break;
-                store(nxt, smem + K::v + (j & 1) * K::tile, true);
+                store(nxt, smem + K::v + (j & 1) * K::tile);
                 if (lane == 0) mbar_arrive_one(&v_full[j & 1]);
             }
         }
