@@ -645,7 +645,7 @@ class KvCache:
         assert k.dtype == v.dtype == torch.uint8 and k_scale.dtype == v_scale.dtype == torch.float32 and table.dtype == torch.int32
         assert k_sum is None or k_sum.dtype == torch.int16
         self.k, self.v, self.k_scale, self.v_scale, self.table, self.k_sum = k, v, k_scale, v_scale, table, k_sum
-        self.n_blocks, self.n_kv, self.head_dim = n_blocks, n_kv, head_dim
+        self.n_blocks, self.n_kv, self.head_dim, self.n_seq = n_blocks, n_kv, head_dim, table.shape[0]
         self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), _ptr(k_sum), _ptr(table), table.shape[1], n_blocks, n_kv,
                                 head_dim)
         self._ref = C.byref(self.desc)
@@ -683,7 +683,7 @@ class AttnBatch:
 
     def __init__(self, start, kv_len, n_tokens: int, max_new: int, max_len: int):
         assert start.dtype == kv_len.dtype == torch.int32 and start.numel() == kv_len.numel() + 1
-        self.start, self.kv_len, self.n_tokens = start, kv_len, n_tokens
+        self.start, self.kv_len, self.n_tokens, self.n_seq = start, kv_len, n_tokens, kv_len.numel()
         self.desc = AttnBatchDesc(_ptr(start), _ptr(kv_len), kv_len.numel(), n_tokens, max_new, max_len)
         self._ref = C.byref(self.desc)
 
@@ -706,14 +706,17 @@ class Rope:
         for t in (cos, sin, q_w, k_w):
             assert t is None or t.dtype == torch.float32
         assert (cos is None) == (sin is None) and (cos is None or cos.shape == sin.shape)
-        self.cos, self.sin, self.q_w, self.k_w, self.eps, self.pairs = cos, sin, q_w, k_w, eps, pairs
-        self.n_pos, self.rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
+        n_pos, rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
+        self._keep = cos, sin, q_w, k_w
+        self.args = RopeArgs(q_w=_ptr(q_w), k_w=_ptr(k_w), eps=eps, cos=_ptr(cos), sin=_ptr(sin), n_pos=n_pos, rot_dim=rot_dim, pairs=int(pairs))
+        self._ref = C.byref(self.args)
 
 
-def _rows(x, heads: int, head_dim: int):
-    """(address, elements between rows) of [tokens, heads, head_dim] whose heads lie side by side: a view into wider rows is fine."""
-    assert x.is_cuda and x.dim() == 3 and x.shape[1:] == (heads, head_dim) and x.stride(2) == 1 and (heads == 1 or x.stride(1) == head_dim)
-    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else heads * head_dim
+def _rows(x, n: int, heads: int, head_dim: int):
+    """(address, elements between rows) of [n, heads, head_dim] whose heads lie side by side: a view into wider rows is fine."""
+    row, head, one = x.stride()
+    assert x.is_cuda and x.shape == (n, heads, head_dim) and one == 1 and (heads == 1 or head == head_dim)
+    return x.data_ptr(), row if n > 1 else heads * head_dim
 
 
 class KvAttention:
@@ -735,42 +738,44 @@ class KvAttention:
         self.scratch[:1 << 12].zero_()                      # the error word and the counters
         self._attn = AttnArgs(None, 0, 0, n_q, cache.head_dim ** -0.5 if scale is None else scale, window, None, 0, None, None)
         self._select = SelectArgs(None, 0, 0, n_q, n_first, n_last, n_sel, None)
-        self._rope = RopeArgs(n_q=n_q)
-        self._refs = C.byref(self._attn), C.byref(self._select), C.byref(self._rope)
+        self._refs = C.byref(self._attn), C.byref(self._select)
 
-    def _act(self, batch, x):
-        assert x.shape[0] == batch.n_tokens and x.dtype in (torch.float32, torch.bfloat16)
-        assert batch.desc.n_seq <= self.cache.table.shape[0]
-        return int(x.dtype == torch.bfloat16)
+    def _queries(self, a, batch, q):
+        """The queries of a call into its arguments; returns their type."""
+        dtype, c = q.dtype, self.cache
+        assert dtype is torch.float32 or dtype is torch.bfloat16
+        assert batch.n_seq <= c.n_seq
+        a.is_bf16 = dtype is torch.bfloat16
+        a.q, a.ld_q = _rows(q, batch.n_tokens, self.n_q, c.head_dim)
+        return dtype
 
     def append(self, batch: AttnBatch, q, k, v, rope: Rope, pos=None, q_out=None, stream=None):
         """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
         (None: the tokens' positions)."""
-        a, c = self._rope, self.cache
-        a.is_bf16 = self._act(batch, q)
-        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
+        a, c, n = rope.args, self.cache, batch.n_tokens
+        dtype = self._queries(a, batch, q)
+        a.n_q = self.n_q
         if k is not None:
-            assert k.dtype == v.dtype == q.dtype and k.shape[0] == v.shape[0] == batch.n_tokens
-            a.k, a.ld_k = _rows(k, c.n_kv, c.head_dim)
-            a.v, a.ld_v = _rows(v, c.n_kv, c.head_dim)
+            assert k.dtype is dtype and v.dtype is dtype
+            a.k, a.ld_k = _rows(k, n, c.n_kv, c.head_dim)
+            a.v, a.ld_v = _rows(v, n, c.n_kv, c.head_dim)
         else:
             a.k = a.v = None
-        q_out = q_out if q_out is not None else torch.empty((batch.n_tokens, self.n_q, c.head_dim), dtype=q.dtype, device=q.device)
-        assert q_out.dtype == q.dtype and (pos is None or (pos.dtype == torch.int32 and pos.numel() == batch.n_tokens))
-        a.q_w, a.k_w, a.eps = _ptr(rope.q_w), _ptr(rope.k_w), rope.eps
-        a.cos, a.sin, a.pos, a.n_pos, a.rot_dim, a.pairs = _ptr(rope.cos), _ptr(rope.sin), _ptr(pos), rope.n_pos, rope.rot_dim, int(rope.pairs)
-        a.q_out = _ptr(q_out)
-        _check("qk_norm_rope_append", _lib.load().maya_qk_norm_rope_append(c._ref, batch._ref, self._refs[2], _stream(stream)))
+        if q_out is None:
+            q_out = torch.empty((n, self.n_q, c.head_dim), dtype=dtype, device=q.device)
+        assert q_out.dtype is dtype and q_out.shape == (n, self.n_q, c.head_dim) and (pos is None or (pos.dtype == torch.int32 and pos.numel() == n))
+        a.pos, a.q_out = _ptr(pos), _ptr(q_out)
+        _check("qk_norm_rope_append", _lib.load().maya_qk_norm_rope_append(c._ref, batch._ref, rope._ref, _stream(stream)))
         return q_out
 
     def forward(self, batch: AttnBatch, q, sel=None, out=None, lse=None, stream=None):
         """out [n_tokens, n_q, head_dim] of q's type.  sel i32 [n_tokens, n_kv, n_sel] (select's): the blocks each token reads.
         lse f32 [n_tokens, n_q]: ln of the sum of exp(scores), for joining with attention over other tokens."""
         a, c = self._attn, self.cache
-        a.is_bf16 = self._act(batch, q)
-        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
-        out = out if out is not None else torch.empty((batch.n_tokens, self.n_q, c.head_dim), dtype=q.dtype, device=q.device)
-        assert out.dtype == q.dtype and out.shape == (batch.n_tokens, self.n_q, c.head_dim)
+        dtype = self._queries(a, batch, q)
+        if out is None:
+            out = torch.empty((batch.n_tokens, self.n_q, c.head_dim), dtype=dtype, device=q.device)
+        assert out.dtype is dtype and out.shape == (batch.n_tokens, self.n_q, c.head_dim)
         assert lse is None or (lse.dtype == torch.float32 and lse.shape == (batch.n_tokens, self.n_q))
         if sel is not None:
             assert sel.dtype == torch.int32 and sel.shape[:2] == (batch.n_tokens, c.n_kv)
@@ -782,9 +787,9 @@ class KvAttention:
     def select(self, batch: AttnBatch, q, sel=None, stream=None):
         """i32 [n_tokens, n_kv, n_sel]: the blocks each token reads, ascending, -1 behind the last."""
         a, c = self._select, self.cache
-        a.is_bf16 = self._act(batch, q)
-        a.q, a.ld_q = _rows(q, self.n_q, c.head_dim)
-        sel = sel if sel is not None else torch.empty((batch.n_tokens, c.n_kv, self.n_sel), dtype=torch.int32, device=q.device)
+        self._queries(a, batch, q)
+        if sel is None:
+            sel = torch.empty((batch.n_tokens, c.n_kv, self.n_sel), dtype=torch.int32, device=q.device)
         assert sel.dtype == torch.int32 and sel.shape == (batch.n_tokens, c.n_kv, self.n_sel)
         a.sel = _ptr(sel)
         _check("block_select", _lib.load().maya_block_select(c._ref, batch._ref, self._refs[1], _stream(stream)))
