@@ -26,6 +26,7 @@ STATUS = {0: "ok", -1: "bad argument", -2: "unsupported ggml type", -3: "CUDA la
           -5: "no sm_100 device"}
 LAYER_CHOICE, LAYER_FUSED, LAYER_TOKEN, LAYER_STAGED = 0, 1, 2, 3        # maya_layer_kernel
 INF = float("inf")
+MAX_COLS = 8                 # activation columns of native_mmvq (MAYA_MAX_COLS)
 
 
 class MayaError(RuntimeError):
