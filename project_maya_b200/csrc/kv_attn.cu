@@ -28,6 +28,7 @@ namespace maya {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
+template<bool F32> constexpr float kBias = F32 ? 12.0f : 4.0f;                  // P is kept as 2^bias p
 constexpr int kMeta = 128;                        // cache blocks looked up at a time
 constexpr int kPiece = 4096;                      // bytes of a ring's slot: 64 tokens x 64 values of K or of V
 constexpr long long kWarm = 1 << 20;              // bytes of queries, and of the table, that are asked into L2 ahead
@@ -103,8 +104,8 @@ __device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int 
     const int row = T.r0 + r;
     return (size_t) (T.s.row + T.i0 + row / A.group) * A.n_q + h * A.group + row % A.group;
 }
-// O is P V with P = 2^12 p, l the sum of P (V's scale taken out again)
-__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.0f ? (m + log2f(l) - kPBias) * 0.69314718055994531f : kNone; }
+// O is P V, l the sum of P (V's scale taken out again)
+__device__ __forceinline__ float lse_of(float m, float l, float bias) { return l > 0.0f ? (m + log2f(l) - bias) * 0.69314718055994531f : kNone; }
 
 // A (tile, head)'s cache blocks are cut into pieces of about `q`, of which a thread block works on one at a time: about six a thread block where there are
 // many blocks (the SMs are not equally fast: with even shares fixed beforehand the last of 444 thread blocks ended at 147 us, the middle one at 113), none
@@ -120,6 +121,7 @@ template<int D, bool F32, int NT, int RW>
 __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
     using K = Cfg<D, F32, NT, RW>;
     constexpr int BW = K::BW, P = D / 64, V = D / 32, TF = F32 ? 2 : 1;
+    constexpr float bias = kBias<F32>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Meta meta[kMeta];
     __shared__ __align__(8) uint64_t full[BW][K::slots], empty[BW][K::slots];
@@ -193,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
 
     float o[NT][D / 16][4], m[NT][2], l[NT][2], vr = F32 ? 0.0f : 1.0f;          // columns 2 t, 2 t + 1
     int pos[NT][2], wpos_lo = 0, wpos_hi = 0;
-    unsigned u_put = 0, u_get = 0;                                               // pieces asked for and taken so far by this ring
+    unsigned u_put = 0, put_phase = 0, get_phase = 0;                            // pieces this ring has asked for; the phases of
+    int put_slot = 0, get_slot = 0;                                              // the slots that the next one goes into, and is taken from
     bool ok = true;
     Tile T;
     int tile = 0, h = 0;
@@ -288,32 +291,36 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
 
         // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots
         int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
-        auto ask = [&](unsigned limit) {                                         // by the ring's first warp, until `limit` pieces are asked for
-            while (put < nc && u_put < limit) {
-                const int bh = meta[put].bh;
-                if (bh < 0) { put += BW; continue; }
-                const unsigned sl = u_put % K::slots;
-                if (u_put >= K::slots && RW > 1 && !mbar_wait(&empty[bw][sl], ((u_put / K::slots) - 1) & 1)) { ok = false; return; }
-                if (lane == 0) {
-                    mbar_expect_tx(&full[bw][sl], kPiece);
-                    bulk_load(ring + sl * kPiece, (put_at >= P ? C.v + (size_t) (put_at - P) * kPiece : C.k + (size_t) put_at * kPiece) + (size_t) bh * (P * kPiece), kPiece, &full[bw][sl]);
-                }
-                ++u_put;
-                if (++put_at == 2 * P) { put_at = 0; put += BW; }
+        const uint8_t* src = nullptr;                                            // the piece
+        auto ask = [&]() {                                                       // one piece, by the ring's first warp
+            if (put_at == 0) {
+                while (put < nc && meta[put].bh < 0) put += BW;
+                if (put < nc) src = C.k + (size_t) meta[put].bh * (P * kPiece);
             }
+            if (put >= nc) return;
+            if (RW > 1 && u_put >= K::slots && !mbar_wait(&empty[bw][put_slot], put_phase ^ 1u)) { ok = false; return; }
+            if (lane == 0) {
+                mbar_expect_tx(&full[bw][put_slot], kPiece);
+                bulk_load(ring + put_slot * kPiece, src, kPiece, &full[bw][put_slot]);
+            }
+            ++u_put;
+            if (++put_slot == K::slots) { put_slot = 0; put_phase ^= 1u; }
+            src += kPiece;
+            if (++put_at == P) src += C.v - C.k - P * kPiece;
+            if (put_at == 2 * P) { put_at = 0; put += BW; }
         };
         auto take = [&]() -> const uint8_t* {                                    // the ring's next piece, once it is there
-            const unsigned sl = u_get % K::slots;
-            if (!mbar_wait(&full[bw][sl], (u_get / K::slots) & 1)) { ok = false; return nullptr; }
-            return ring + sl * kPiece;
+            if (!mbar_wait(&full[bw][get_slot], get_phase)) { ok = false; return nullptr; }
+            return ring + get_slot * kPiece;
         };
         auto leave = [&]() {                                                     // and its room for another
             __syncwarp();
-            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][u_get % K::slots]);
-            ++u_get;
-            if (rw == 0) ask(u_get + K::slots);
+            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][get_slot]);
+            if (++get_slot == K::slots) { get_slot = 0; get_phase ^= 1u; }
+            if (rw == 0) ask();
         };
-        if (rw == 0) ask(u_get + K::slots);
+        if (rw == 0)
+            for (int i = 0; i < K::slots && ok; ++i) ask();
         for (int i = tid; i < nc; i += kThreads) {                               // the scales, behind the first copies
             const int bh = meta[i].bh;
             meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
@@ -456,14 +463,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m[n][e], fmaf(mx, c[e], lv));
-                        const float use = mn == kNone ? 0.0f : mn;
-                        const float al = ex2(m[n][e] - use);
-                        off[e] = kPBias + lv - use;
-                        m[n][e] = mn;
-                        l[n][e] *= al;
-                        alpha[n][e] = al * beta;
-                        moved = moved || alpha[n][e] != 1.0f;
+                        const float top = fmaf(mx, c[e], lv);
+                        if constexpr (F32) {
+                            const float mn = fmaxf(m[n][e], top), use = mn == kNone ? 0.0f : mn, al = ex2(m[n][e] - use);
+                            off[e] = bias + lv - use;
+                            m[n][e] = mn;
+                            l[n][e] *= al;
+                            alpha[n][e] = al * beta;
+                        } else {                                                 // m is raised only when it is passed by more than kRise: P stays below 2^12
+                            alpha[n][e] = 1.0f;
+                            if (top > m[n][e] + kRise) {
+                                alpha[n][e] = ex2(m[n][e] - top);
+                                l[n][e] *= alpha[n][e];
+                                m[n][e] = top;
+                                moved = true;
+                            }
+                            off[e] = m[n][e] == kNone ? kNone : bias + lv - m[n][e];
+                        }
                     }
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
@@ -599,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
                     const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
                     *(uint2*) ((uint16_t*) A.out + at * D + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
                 }
-                if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total);
+                if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total, kBias<F32>);
             }
             fence_proxy_async();                                                 // the next copies write where this was read
             if (A.direct) break;
@@ -698,7 +714,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const Ba
     const size_t at = out_row(A, T, h, r);
 #pragma unroll
     for (int e = 0; e < V; ++e) st_act<!F32>(A.out, at * D + lane * V + e, acc[e] * inv);
-    if (A.lse != nullptr && lane == 0) A.lse[at] = lse_of(mm, total);
+    if (A.lse != nullptr && lane == 0) A.lse[at] = lse_of(mm, total, kBias<F32>);
 }
 
 template<int D, bool F32, int NT, int RW>

@@ -12,7 +12,7 @@
 
 namespace maya {
 
-constexpr float kPBias = 12.0f;                  // P is kept as 2^12 p
+constexpr float kRise = 8.0f;                    // how far a maximum may pass m (base 2) before m is raised to it
 constexpr float kNone = -INFINITY;
 
 struct AttnView {

@@ -27,7 +27,7 @@ constexpr int kPThreads = 16 * 32;
 constexpr int kExpandWarps = 7, kIssueWarp = 15;
 // Registers a thread of each part, out of the 128 a thread that 512 threads are launched with: 256 * 168 + 256 * 88 = 65536.
 constexpr int kRegsSoftmax = 168, kRegsOther = 88;
-constexpr float kRise = 8.0f, kUp = 4.0f;
+constexpr float kUp = 4.0f;
 constexpr int kMetaRing = 4;                     // (a step's numbers are written while the softmax may be three steps behind)
 
 struct StepMeta {                                // of the two cache blocks of a step
