@@ -27,7 +27,7 @@
 namespace maya {
 namespace {
 
-constexpr int kThreads = 128, kWarps = 4;
+constexpr int kJoinWarps = 4;
 template<bool F32> constexpr float kBias = F32 ? 12.0f : 4.0f;                  // P is kept as 2^bias p
 constexpr int kMeta = 128;                        // cache blocks looked up at a time
 constexpr int kPiece = 4096;                      // bytes of a ring's slot: 64 tokens x 64 values of K or of V
@@ -64,14 +64,14 @@ __device__ __forceinline__ uint32_t pack_rest(uint32_t hi, float a, float b) {
     return pack_half(a - f.x, b - f.y);
 }
 
-template<int D, bool F32, int NT, int RW> struct Cfg {
-    static constexpr int BW = kWarps / RW;
+template<int D, bool F32, int NT, int RW, int NW> struct Cfg {
+    static constexpr int BW = NW / RW;
     static constexpr int rows = 8 * NT * RW;
-    static constexpr int ctas = D == 64 ? (F32 && NT == 2 ? 2 : 3) : D == 128 ? (F32 || NT == 2 ? 2 : 3) : F32 ? 1 : 2;   // thread blocks an SM
-    static constexpr int room = ctas == 3 ? 71680 : ctas == 2 ? 108544 : 212992; // and shared memory of each
+    static constexpr int ctas = NW == 1 ? (D == 64 ? 14 : D == 128 ? (F32 ? 8 : 12) : 7) : D == 64 ? (F32 && NT == 2 ? 2 : 3) : D == 128 ? (F32 || NT == 2 ? 2 : 3) : F32 ? 1 : 2;   // thread blocks an SM
+    static constexpr int room = NW == 1 ? 228 * 1024 / ctas - 4800 : ctas == 3 ? 71680 : ctas == 2 ? 108544 : 212992; // and shared memory of each
     static constexpr int frag = RW * NT * (D / 64) * 2 * 512;                    // queries as fragments
     static constexpr int wide = D + 4;                                           // floats of a row where the rings' outputs meet, over the rings
-    static constexpr int merge = kWarps * 8 * NT * wide * 4;
+    static constexpr int merge = NW * 8 * NT * wide * 4;
     static constexpr int desk = (F32 ? 2 : 1) * frag;
     static constexpr int slots = (room - desk) / kPiece / BW;                    // of a ring
     static constexpr int body = BW * slots * kPiece;
@@ -107,26 +107,27 @@ __device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int 
 // O is P V, l the sum of P (V's scale taken out again)
 __device__ __forceinline__ float lse_of(float m, float l, float bias) { return l > 0.0f ? (m + log2f(l) - bias) * 0.69314718055994531f : kNone; }
 
-// A (tile, head)'s cache blocks are cut into pieces of about `q`, of which a thread block works on one at a time: about six a thread block where there are
+// A (tile, head)'s cache blocks are cut into pieces of about `q`, of which a thread block works on one at a time: about four a thread block where there are
 // many blocks (the SMs are not equally fast: with even shares fixed beforehand the last of 444 thread blocks ended at 147 us, the middle one at 113), none
-// below a round of 16, or more than there is room for parts of.
+// below 24 blocks for that, or more than there is room for parts of.
 __device__ __forceinline__ unsigned piece_of(const AttnView& A, unsigned blocks, int bw) {
-    const unsigned turns = max(1u, min(6u, blocks / A.grid / 16)), share = A.grid * turns;
+    const unsigned turns = max(1u, min(4u, blocks / A.grid / 24)), share = A.grid * turns;
     const unsigned q = max((blocks + share - 1) / share, blocks / (A.parts_most - A.pairs) + 1);
     return (q + bw - 1) / bw * bw;
 }
 __device__ __forceinline__ unsigned pieces_of(unsigned nb, unsigned q) { return (nb + q - 1) / q; }
 
-template<int D, bool F32, int NT, int RW>
-__global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
-    using K = Cfg<D, F32, NT, RW>;
+template<int D, bool F32, int NT, int RW, int NW>
+__global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_kernel(const KvView C, const BatchView B, const AttnView A) {
+    using K = Cfg<D, F32, NT, RW, NW>;
+    constexpr int kWarps = NW, kThreads = 32 * NW;
     constexpr int BW = K::BW, P = D / 64, V = D / 32, TF = F32 ? 2 : 1;
     constexpr float bias = kBias<F32>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Meta meta[kMeta];
     __shared__ __align__(8) uint64_t full[BW][K::slots], empty[BW][K::slots];
     __shared__ float qinv[K::rows], sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT], sm_vr[kWarps];
-    __shared__ int pre[kTilesMost + 1];
+    __shared__ int pre[NW == 1 ? 1 : kTilesMost + 1];
     __shared__ unsigned sums[kWarps], upcoming;
     __shared__ int lost;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -151,45 +152,47 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
 
     // ---- the pieces in front of each tile (of one head)
     unsigned units = 0;
-    if (A.direct) {
+    if (NW == 1 || A.direct) {
         __syncthreads();
     } else if (A.sel != nullptr) {
         units = (unsigned) A.tiles * pieces_of((unsigned) A.n_sel, piece_of(A, (unsigned) A.tiles * (unsigned) C.n_kv * (unsigned) A.n_sel, BW));
         __syncthreads();
     } else {
-        const int each = (A.tiles + kThreads - 1) / kThreads;
-        unsigned nb[kTilesMost / kThreads], sum = 0;
+        if constexpr (NW > 1) {
+            const int each = (A.tiles + kThreads - 1) / kThreads;
+            unsigned nb[kTilesMost / kThreads], sum = 0;
 #pragma unroll
-        for (int i = 0; i < kTilesMost / kThreads; ++i) {
-            nb[i] = i < each && tid * each + i < A.tiles ? (unsigned) tile_of(B, A, tid * each + i, K::rows).n_blocks : 0u;
-            sum += nb[i];
+            for (int i = 0; i < kTilesMost / kThreads; ++i) {
+                nb[i] = i < each && tid * each + i < A.tiles ? (unsigned) tile_of(B, A, tid * each + i, K::rows).n_blocks : 0u;
+                sum += nb[i];
+            }
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) sums[warp] = sum;
+            __syncthreads();
+            unsigned all = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) all += sums[w];
+            const unsigned q = piece_of(A, all * (unsigned) C.n_kv, BW);
+            sum = 0;
+#pragma unroll
+            for (int i = 0; i < kTilesMost / kThreads; ++i) sum += pieces_of(nb[i], q);
+            unsigned up = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) { const unsigned y = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += y; }
+            __syncthreads();
+            if (lane == 31) sums[warp] = up;
+            __syncthreads();
+            unsigned before = up - sum;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sums[w]; units += sums[w]; }
+#pragma unroll
+            for (int i = 0; i < kTilesMost / kThreads; ++i)
+                if (i < each && tid * each + i < A.tiles) { pre[tid * each + i] = (int) before; before += pieces_of(nb[i], q); }
+            if (tid == 0) pre[A.tiles] = (int) units;
+            __syncthreads();
+            if (blockIdx.x == 0)                                                     // for the join
+                for (int i = tid; i <= A.tiles; i += kThreads) A.pre[i] = pre[i];
         }
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0) sums[warp] = sum;
-        __syncthreads();
-        unsigned all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all += sums[w];
-        const unsigned q = piece_of(A, all * (unsigned) C.n_kv, BW);
-        sum = 0;
-#pragma unroll
-        for (int i = 0; i < kTilesMost / kThreads; ++i) sum += pieces_of(nb[i], q);
-        unsigned up = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) { const unsigned y = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += y; }
-        __syncthreads();
-        if (lane == 31) sums[warp] = up;
-        __syncthreads();
-        unsigned before = up - sum;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sums[w]; units += sums[w]; }
-#pragma unroll
-        for (int i = 0; i < kTilesMost / kThreads; ++i)
-            if (i < each && tid * each + i < A.tiles) { pre[tid * each + i] = (int) before; before += pieces_of(nb[i], q); }
-        if (tid == 0) pre[A.tiles] = (int) units;
-        __syncthreads();
-        if (blockIdx.x == 0)                                                     // for the join
-            for (int i = tid; i <= A.tiles; i += kThreads) A.pre[i] = pre[i];
     }
     units *= (unsigned) C.n_kv;
 
@@ -638,11 +641,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F32, NT, RW>::ctas) attn_kern
 // The rows of (tile, head)s that were cut into pieces, from their parts in order: a thread block a row (WIDE: few rows, each of many
 // parts), or a warp.
 template<int D, bool F32, bool WIDE>
-__global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows, int bw) {
-    constexpr int V = D / 32, W = WIDE ? kWarps : 1;
-    __shared__ float acc_of[WIDE ? kWarps : 1][D], l_of[kWarps];
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const KvView C, const BatchView B, const AttnView A, int rows, int bw) {
+    constexpr int V = D / 32, W = WIDE ? kJoinWarps : 1;
+    __shared__ float acc_of[WIDE ? kJoinWarps : 1][D], l_of[kJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = WIDE ? warp : 0;
-    const long long id = WIDE ? (long long) blockIdx.x : (long long) blockIdx.x * kWarps + warp;
+    const long long id = WIDE ? (long long) blockIdx.x : (long long) blockIdx.x * kJoinWarps + warp;
     const int r = (int) (id % rows), h = (int) (id / rows % C.n_kv), tile = (int) (id / rows / C.n_kv);
     grid_launch_dependents();
     grid_dependency_wait();
@@ -702,12 +705,12 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const Ba
         if (warp != 0) return;
         total = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kWarps; ++x) total += l_of[x];
+        for (int x = 0; x < kJoinWarps; ++x) total += l_of[x];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             acc[e] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < kWarps; ++x) acc[e] += acc_of[x][lane * V + e];
+            for (int x = 0; x < kJoinWarps; ++x) acc[e] += acc_of[x][lane * V + e];
         }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -717,9 +720,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvView C, const Ba
     if (A.lse != nullptr && lane == 0) A.lse[at] = lse_of(mm, total, kBias<F32>);
 }
 
-template<int D, bool F32, int NT, int RW>
+template<int D, bool F32, int NT, int RW, int NW = 4>
 int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, cudaStream_t s) {
-    using K = Cfg<D, F32, NT, RW>;
+    using K = Cfg<D, F32, NT, RW, NW>;
     static_assert(K::slots >= 2, "a ring holds a piece in use and one on its way");
     const long long rows = a.sel ? A.group : (long long) b.max_new * A.group;
     A.row_tiles = (int) ((rows + K::rows - 1) / K::rows);
@@ -746,7 +749,9 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
     A.pairs = (unsigned) (tiles * c.n_kv);
     A.parts_most = (unsigned) (kPartRows / K::rows);
     if (A.pairs >= A.parts_most / 2) A.direct = true;                            // many (tile, head)s: whole ones, as many thread blocks
+    if (NW == 1) A.direct = true;
     if (A.direct) grid = tiles * c.n_kv;
+    if (grid > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
     const long long q_bytes = ((long long) (b.n_tokens - 1) * a.ld_q + (long long) a.n_q * D) * (F32 ? 4 : 2), table_bytes = (long long) b.n_seq * c.table_ld * 4;
     A.warm_q = (unsigned) ((q_bytes < kWarm ? q_bytes : kWarm) / 128);
     A.warm_table = (unsigned) ((table_bytes < kWarm ? table_bytes : kWarm) / 128);
@@ -755,21 +760,24 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
     A.part_ml = (float2*) (scratch + kAttnHead + kAttnPre);
     A.part_o = (float*) (A.part_ml + kPartRows);
     static SmemLimit limit;
-    if (!limit.raise((const void*) attn_kernel<D, F32, NT, RW>, K::smem)) return note_launch("kv attention smem attribute");
-    launch_dependent(attn_kernel<D, F32, NT, RW>, dim3((unsigned) grid), dim3(kThreads), K::smem, s, kv_view(c), batch_view(b), A);
+    if (!limit.raise((const void*) attn_kernel<D, F32, NT, RW, NW>, K::smem)) return note_launch("kv attention smem attribute");
+    launch_dependent(attn_kernel<D, F32, NT, RW, NW>, dim3((unsigned) grid), dim3(32 * NW), K::smem, s, kv_view(c), batch_view(b), A);
     const int st = note_launch("attn_q8");
     if (st != MAYA_OK || A.direct || grid == 1) return st;
     const long long all_rows = tiles * c.n_kv * K::rows;
     if (all_rows <= 4 * sm_count())
-        launch_dependent(join_kernel<D, F32, true>, dim3((unsigned) all_rows), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
+        launch_dependent(join_kernel<D, F32, true>, dim3((unsigned) all_rows), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
     else
-        launch_dependent(join_kernel<D, F32, false>, dim3((unsigned) ((all_rows + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
+        launch_dependent(join_kernel<D, F32, false>, dim3((unsigned) ((all_rows + kJoinWarps - 1) / kJoinWarps)), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
     return note_launch("attn_q8 join");
 }
 
 template<int D, bool F32>
 int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, uint8_t* scratch, cudaStream_t s) {
     const long long rows = (long long) (a.sel ? 1 : b.max_new) * (a.n_q / c.n_kv);
+    // Lists of many tokens, 8 heads a group or fewer: a warp a (token, head), by itself - no barrier, nothing to meet - once there are enough of them to
+    // fill the chip several times (a chunk of 4096 tokens, 4 key/value heads, 16 blocks each: four warps a list 608 us, one 515).
+    if (a.sel && rows <= 8 && (long long) b.n_tokens * c.n_kv >= 48ll * sm_count()) return launch_attn<D, F32, 1, 1, 1>(c, b, a, A, scratch, s);
     if (rows <= 8) return launch_attn<D, F32, 1, 1>(c, b, a, A, scratch, s);
     if constexpr (D <= 128) {
         if (rows <= 16) return launch_attn<D, F32, 2, 1>(c, b, a, A, scratch, s);

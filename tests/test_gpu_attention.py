@@ -267,6 +267,27 @@ def test_selected_blocks(cuda, group, dim, bf16):
     check(out, lse, want, bf16)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group,dim", [(8, 128), (3, 64), (1, 256), (5, 192)])
+def test_selected_blocks_of_many_tokens(cuda, group, dim, bf16):
+    """A prompt's lists, a warp each: the first tokens, some in the middle, the last."""
+    import torch as T
+    rng = np.random.default_rng(20 + group)
+    n, n_kv, n_sel = 1900, 4, 6
+    cache, host = make_cache(T, rng, [n], n_kv, dim)
+    own = np.arange(n) // BLOCK
+    sel = np.sort(np.where(rng.random((n, n_kv, n_sel)) < 0.8, np.floor(rng.random((n, n_kv, n_sel)) * (own[:, None, None] + 1)), -1).astype(np.int32), -1)
+    sel[:, :, 1:][sel[:, :, 1:] == sel[:, :, :-1]] = -1                      # each block once
+    sel[7] = -1                                                              # a row that sees nothing
+    q = T.from_numpy(rng.standard_normal((n, n_kv * group, dim)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32).cuda()
+    s = T.from_numpy(sel).cuda()
+    out, lse = attend(T, cache, [n], [n], q, sel=s)
+    assert (out[7] == 0).all()
+    for a in (0, 640, 1860):
+        want = plain_attention(host, [40], [a + 40], q[a:a + 40].double().cpu().numpy(), n_kv, dim ** -0.5, sel=sel[a:a + 40])
+        check(out[a:a + 40], lse[a:a + 40], want, bf16)
+
+
 def test_blocks_the_table_does_not_have(cuda):
     import torch as T
     rng = np.random.default_rng(9)
