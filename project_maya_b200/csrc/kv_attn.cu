@@ -2,13 +2,14 @@
 //
 // What bounds it is the cache's bytes: 2 * head_dim bytes a token and key/value head, read once for the group of query heads
 // that shares them.  So everything is made to keep copies in flight: a thread block is four warps with rings of 4 KB pieces (64 tokens of 64 key
-// values, or 64 values of 64 tokens: contiguous in the cache, one bulk copy each), three thread blocks an SM.
+// values, or 64 values of 64 tokens: contiguous in the cache, one bulk copy each), three thread blocks an SM.  Measured, one B200: 64
+// tokens at 1k..16k, 64 heads over 8 of 128: 150 us, 5.15 TB/s of cache (the copies alone 135 us); one at 131071 57 us, 4.7 TB/s.
 //   RW warps share a ring and take 8 NT rows each; BW = 4 / RW rings take every BW-th cache block.  One token of up to 8 (16) heads a
 //   group: RW = 1, NT = 1 (2), every warp on its own; 17..32 rows: 2 x 2; more: one ring, 64 rows.
 //
 // The codes are the first operand of both products, the queries and P the second: S^T = K Q^T and O^T = V^T P^T.  Rows are then tokens (values), of which
 // there are always enough, and columns come in eights, so that a group of 8 heads wastes nothing (with queries as rows of 16 it took twice the
-// products, exponentials and registers: 1165 warp instructions a block against ...).  Between HBM and the tensor cores a code costs a byte permute and half
+// products, exponentials and registers; the products of a batch of 64 at up to 16k alone 131 us, so 100).  Between HBM and the tensor cores a code costs a byte permute and half
 // a subtraction (codes_to_half).
 //
 // Fragments.  The contraction index of m16n8k16 may be permuted as long as both operands agree, and the cache's layout is chosen for

@@ -9,7 +9,8 @@
 //                      ahead (codes come straight to registers: staging them would cost shared-memory bandwidth the products need).
 //   warp 15            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory).
 // The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
-// tensor pipe (D = 128) and 2048 of the exponential's pipe.
+// tensor pipe (D = 128) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096 and 2923 tokens, 32 heads over 8, 427 us, 786 TFLOP/s; what
+// bounds it is the chain of a softmax warp, 2500 cycles a block of 64 tokens (half of them exponentials that two warps share a pipe for).
 //
 // Numbers.  A query row is scaled by a power of two into f16 (exact for bf16).  With vs the block's scale of V,
 //   P = 2^(s + log2 vs - m + 4),  O = sum P code,  l = sum P / vs:
