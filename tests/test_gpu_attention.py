@@ -207,6 +207,59 @@ def test_prompt_with_large_scores_and_scales_far_apart(cuda):
     check(out, lse, plain_attention(host, new, lens, q.double().cpu().numpy(), 1, 128 ** -0.5, absent=((0, 3), (0, 8), (0, 9))), True)
 
 
+@pytest.mark.parametrize("bf16,dim,group", [(True, 128, 4), (False, 64, 9), (True, 256, 2), (False, 128, 8)])
+def test_many_sequences(cuda, bf16, dim, group):
+    """More sequences than a thread block adds up: one a thread block, in one piece, the long one over several look-ups of its blocks."""
+    import torch as T
+    rng = np.random.default_rng(30 + group)
+    lens = [int(n) for n in rng.integers(0, 200, 300)]
+    lens[5], lens[17], lens[299] = 0, 9000, 64
+    new = [1] * 300
+    cache, host = make_cache(T, rng, lens, 1, dim)
+    q = T.from_numpy(rng.standard_normal((300, group, dim)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32)
+    out, lse = attend(T, cache, new, lens, q.cuda())
+    check(out, lse, plain_attention(host, new, lens, q.double().numpy(), 1, dim ** -0.5), bf16)
+
+
+def test_many_heads_and_sequences(cuda):
+    """So many (sequence, head)s that there is no room for parts of them: none is cut."""
+    import torch as T
+    rng = np.random.default_rng(40)
+    lens, n_kv = [int(n) for n in rng.integers(1, 300, 240)], 16
+    cache, host = make_cache(T, rng, lens, n_kv, 64)
+    q = T.from_numpy(rng.standard_normal((240, n_kv, 64)).astype(np.float32)).bfloat16()
+    out, lse = attend(T, cache, [1] * 240, lens, q.cuda())
+    check(out, lse, plain_attention(host, [1] * 240, lens, q.double().numpy(), n_kv, 0.125), True)
+
+
+def test_long_f32_prompt(cuda):
+    """Rows that fill more than 256 tiles: first, middle and last tokens."""
+    import torch as T
+    rng = np.random.default_rng(41)
+    n, group, dim = 2200, 8, 64
+    cache, host = make_cache(T, rng, [n], 1, dim)
+    q = T.from_numpy(rng.standard_normal((n, group, dim)).astype(np.float32)).cuda()
+    out, lse = attend(T, cache, [n], [n], q)
+    for a in (0, 1000, n - 8):
+        want = plain_attention(host, [8], [a + 8], q[a:a + 8].double().cpu().numpy(), 1, dim ** -0.5)
+        check(out[a:a + 8], lse[a:a + 8], want, False)
+
+
+def test_long_lists_of_many_tokens(cuda):
+    """Lists longer than one look-up of their blocks, a warp each."""
+    import torch as T
+    rng = np.random.default_rng(42)
+    n, new, n_kv, n_sel = 13000, 1800, 4, 150
+    cache, host = make_cache(T, rng, [n], n_kv, 64)
+    sel = np.sort(np.argsort(rng.random((new, n_kv, (n - new) // BLOCK)), -1)[..., :n_sel], -1).astype(np.int32)
+    q = T.from_numpy(rng.standard_normal((new, n_kv * 2, 64)).astype(np.float32)).cuda()
+    out, lse = attend(T, cache, [new], [n], q, sel=T.from_numpy(sel).cuda())
+    for a in (0, new - 5):
+        end = n - new + a + 5
+        want = plain_attention(host, [5], [end], q[a:a + 5].double().cpu().numpy(), n_kv, 0.125, sel=sel[a:a + 5])
+        check(out[a:a + 5], lse[a:a + 5], want, False)
+
+
 def test_strided_and_unaligned_queries(cuda):
     import torch as T
     rng = np.random.default_rng(6)
