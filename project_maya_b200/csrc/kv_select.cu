@@ -162,7 +162,7 @@ __device__ __forceinline__ void list_of(int n_sel, int n_first, int n_last, cons
 
 template<int D, bool BF16>
 __global__ void __launch_bounds__(kSelThreads, D <= 128 ? 2 : 1) select_kernel(const KvView C, const BatchView B, const SelView S) {
-    constexpr int V = D / 32, ST = D / 16;
+    constexpr int ST = D / 16;
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t* keys = (uint32_t*) smem;                                    // [tokens the tiles have room for][ld_keys]
     uint8_t* frag = smem + (size_t) S.room * S.ld_keys * 4;             // [tiles][ST / 2][kFrag]: f16
@@ -354,6 +354,8 @@ int launch_select(const maya_kv_cache& c, const maya_attn_batch& b, const maya_s
     int tokens = rows_per_token >= 128 ? 1 : 128 / rows_per_token;
     if (tokens > b.max_new) tokens = b.max_new;
     while (tokens > 1 && need(tokens) > kSmemMost) tokens = (tokens + 1) / 2;
+    // (fewer while that leaves the chip's two thread blocks an SM unfilled: 100 tokens of two sequences at 26k, 3 key/value heads of 2: 70 us, so 27)
+    while (tokens > 1 && (long long) b.n_seq * ((b.max_new + tokens - 1) / tokens) * c.n_kv < 2ll * sm_count()) tokens = (tokens + 1) / 2;
     if (need(tokens) > kSmemMost) return refuse(MAYA_ERR_LIMIT);
     S.tokens = tokens;
     S.tiles = tiles_of(tokens);
