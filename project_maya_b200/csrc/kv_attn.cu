@@ -198,13 +198,12 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
     units *= (unsigned) C.n_kv;
 
     float o[NT][D / 16][4], m[NT][2], l[NT][2], vr = F32 ? 0.0f : 1.0f;          // columns 2 t, 2 t + 1
-    int pos[NT][2], wpos_lo = 0, wpos_hi = 0;
+    int pos[NT][2];
     unsigned u_put = 0, put_phase = 0, get_phase = 0;                            // pieces this ring has asked for; the phases of
     int put_slot = 0, get_slot = 0;                                              // the slots that the next one goes into, and is taken from
     bool ok = true;
     Tile T;
     int tile = 0, h = 0;
-    unsigned seg0 = 0, seg1 = 0;                                                 // the (tile, head) at hand: its triples
     constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
     float qx[U][V];
     auto ask_rows = [&](int r4) {
@@ -652,7 +651,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const KvView C, c
     grid_dependency_wait();
     if (tile >= A.tiles) return;
     unsigned pieces, s0;
-    if (A.sel != nullptr) {
+    if (A.fixed > 0) {
+        pieces = A.fixed;
+        s0 = ((unsigned) tile * (unsigned) C.n_kv + h) * pieces;
+    } else if (A.sel != nullptr) {
         pieces = pieces_of((unsigned) A.n_sel, piece_of(A, (unsigned) A.tiles * (unsigned) C.n_kv * (unsigned) A.n_sel, bw));
         s0 = ((unsigned) tile * (unsigned) C.n_kv + h) * pieces;
     } else {
@@ -721,6 +723,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const KvView C, c
     if (A.lse != nullptr && lane == 0) A.lse[at] = lse_of(mm, total, kBias<F32>);
 }
 
+template<int D, bool F32>
+int launch_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, int rows, int bw, cudaStream_t s) {
+    const long long all = (long long) A.tiles * c.n_kv * rows;
+    if (all <= 4 * sm_count()) launch_dependent(join_kernel<D, F32, true>, dim3((unsigned) all), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, rows, bw);
+    else launch_dependent(join_kernel<D, F32, false>, dim3((unsigned) ((all + kJoinWarps - 1) / kJoinWarps)), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, rows, bw);
+    return note_launch("attn_q8 join");
+}
+
 template<int D, bool F32, int NT, int RW, int NW = 4>
 int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, cudaStream_t s) {
     using K = Cfg<D, F32, NT, RW, NW>;
@@ -756,21 +766,12 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
     const long long q_bytes = ((long long) (b.n_tokens - 1) * a.ld_q + (long long) a.n_q * D) * (F32 ? 4 : 2), table_bytes = (long long) b.n_seq * c.table_ld * 4;
     A.warm_q = (unsigned) ((q_bytes < kWarm ? q_bytes : kWarm) / 128);
     A.warm_table = (unsigned) ((table_bytes < kWarm ? table_bytes : kWarm) / 128);
-    A.taken = (unsigned*) (scratch + 16);
-    A.pre = (int*) (scratch + kAttnHead);
-    A.part_ml = (float2*) (scratch + kAttnHead + kAttnPre);
-    A.part_o = (float*) (A.part_ml + kPartRows);
     static SmemLimit limit;
     if (!limit.raise((const void*) attn_kernel<D, F32, NT, RW, NW>, K::smem)) return note_launch("kv attention smem attribute");
     launch_dependent(attn_kernel<D, F32, NT, RW, NW>, dim3((unsigned) grid), dim3(32 * NW), K::smem, s, kv_view(c), batch_view(b), A);
     const int st = note_launch("attn_q8");
     if (st != MAYA_OK || A.direct || grid == 1) return st;
-    const long long all_rows = tiles * c.n_kv * K::rows;
-    if (all_rows <= 4 * sm_count())
-        launch_dependent(join_kernel<D, F32, true>, dim3((unsigned) all_rows), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
-    else
-        launch_dependent(join_kernel<D, F32, false>, dim3((unsigned) ((all_rows + kJoinWarps - 1) / kJoinWarps)), dim3(32 * kJoinWarps), 0, s, kv_view(c), batch_view(b), A, K::rows, K::BW);
-    return note_launch("attn_q8 join");
+    return launch_join<D, F32>(c, b, A, K::rows, K::BW, s);
 }
 
 template<int D, bool F32>
@@ -791,6 +792,12 @@ int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_ar
 }
 
 }  // namespace
+
+int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, int rows, cudaStream_t s) {
+    if (!bf16) return refuse(MAYA_ERR_ARG);
+    return c.head_dim == 64 ? launch_join<64, false>(c, b, A, rows, 1, s) : launch_join<128, false>(c, b, A, rows, 1, s);
+}
+
 }  // namespace maya
 
 using namespace maya;
@@ -819,6 +826,10 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     A.wide_q = rows_wide(a->q, a->ld_q, a->is_bf16 ? 2 : 4);
     A.scale_log2 = a->scale * 1.4426950408889634f;
     A.error = (unsigned*) scratch;
+    A.taken = (unsigned*) ((uint8_t*) scratch + 16);
+    A.pre = (int*) ((uint8_t*) scratch + kAttnHead);
+    A.part_ml = (float2*) ((uint8_t*) scratch + kAttnHead + kAttnPre);
+    A.part_o = (float*) (A.part_ml + kPartRows);
     st = attn_prompt(*c, *b, A, a->is_bf16 != 0, s);
     if (st != kNotTaken) return st;
 #define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, (uint8_t*) scratch, s) : by_rows<D, true>(*c, *b, *a, A, (uint8_t*) scratch, s)

@@ -27,6 +27,7 @@ struct AttnView {
     int tiles;                                   // of all sequences (tokens)
     bool direct;                                 // a thread block a (tile, head), in one piece
     unsigned* error;
+    unsigned fixed;                              // > 0: every (tile, head) is cut into so many pieces (prompts)
     unsigned grid, pairs, parts_most;            // thread blocks; (tile, head)s; parts there is room for
     unsigned warm_q, warm_table;                 // lines of 128 bytes
     unsigned* taken;                             // pieces taken beyond each thread block's first; thread blocks that have left
@@ -40,6 +41,8 @@ constexpr size_t kAttnHead = 256, kAttnPre = 2048;
 constexpr int kCtasMost = 448;                   // thread blocks that share out the work: three an SM
 constexpr int kPartRows = 2 * kCtasMost * 64;      // rows of parts
 constexpr float kVsLeast = 1e-30f;               // a value scale of 0 is this in P's exponent: P is 0 in f16 and right in l
+// The join of the pieces' parts (kv_attn.cu), `rows` rows a tile.
+int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, int rows, cudaStream_t s);
 constexpr int kNotTaken = 1;
 // Attention of a prompt's rows on tcgen05 (kv_attn_prompt.cu); kNotTaken: not that kernel's call, nothing launched.
 int attn_prompt(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, cudaStream_t s);

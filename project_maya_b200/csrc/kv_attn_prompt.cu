@@ -129,8 +129,10 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     const bool here = r0 < n_rows;
     const int last_row = min(r0 + 256, n_rows) - 1;
     const int pos_lo = first + r0 / A.group, pos_hi = here ? first + last_row / A.group : -1;
-    const int b_lo = A.window > 0 ? max(0, pos_lo - A.window + 1) / kKvBlock : 0;
-    const int n_blocks = pos_hi < 0 ? 0 : max(0, pos_hi / kKvBlock + 1 - b_lo);
+    const int b_first = A.window > 0 ? max(0, pos_lo - A.window + 1) / kKvBlock : 0;
+    // (few tiles over a long context: a tile's blocks in A.fixed pieces, whose parts the join puts together)
+    const int all_blocks = pos_hi < 0 ? 0 : max(0, pos_hi / kKvBlock + 1 - b_first), cuts = max(1u, A.fixed), each = (all_blocks + cuts - 1) / cuts;
+    const int b_lo = b_first + (int) blockIdx.z * each, n_blocks = max(0, min(each, all_blocks - (int) blockIdx.z * each));
     const int steps = (n_blocks + 1) / 2;
     const int tiles = here && n_rows - r0 > 128 ? 2 : 1;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -403,6 +405,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             if (ok) {                                                       // (warp-uniform: a wait runs out for a whole warp)
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 const int n = s.row + row / A.group, hq = h * A.group + row % A.group;
+                const size_t part = (((size_t) blockIdx.x * C.n_kv + h) * A.fixed + blockIdx.z) * 256 + tid;
+                const bool cut = A.fixed > 1;
                 uint16_t* dst = (uint16_t*) A.out + ((size_t) n * A.n_q + hq) * D;
 #pragma unroll
                 for (int d = 0; d < D; d += 16) {
@@ -411,7 +415,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                     else
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = 0.0f;
-                    if (row < n_rows) {
+                    if (cut) {
+                        if (row < n_rows)
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *(float4*) (A.part_o + part * D + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    } else if (row < n_rows) {
                         uint32_t w[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -422,7 +430,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         ((uint4*) (dst + d))[1] = make_uint4(w[4], w[5], w[6], w[7]);
                     }
                 }
-                if (A.lse != nullptr && row < n_rows)
+                if (cut && row < n_rows) A.part_ml[part] = make_float2(m, l);
+                else if (A.lse != nullptr && row < n_rows)
                     A.lse[(size_t) n * A.n_q + hq] = l > 0.0f ? (m + log2f(l) - kUp) * 0.69314718055994531f : kNone;
             }
         }
@@ -438,10 +447,23 @@ template<int D> int launch_prompt(const maya_kv_cache& c, const maya_attn_batch&
     A.row_tiles = (int) ((rows + 255) / 256);
     const long long tiles = (long long) A.row_tiles * b.n_seq;
     if (tiles > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
+    // Pieces: as many as fill the SMs, of 16 blocks at least, as far as there is room for parts (61 tokens of four sequences at up to 34k, 12 heads over 4: in
+    // one piece each 643 us, so 90).
+    const long long pairs = tiles * c.n_kv;
+    long long most = (b.max_len + kKvBlock - 1) / kKvBlock;
+    if (A.window > 0 && most > (A.window + 255ll / A.group) / kKvBlock + 2) most = (A.window + 255ll / A.group) / kKvBlock + 2;
+    long long cuts = sm_count() / pairs;
+    if (cuts > most / 16) cuts = most / 16;
+    if (cuts > kPartRows / (256 * pairs)) cuts = kPartRows / (256 * pairs);
+    if (cuts < 1) cuts = 1;
+    A.tiles = (int) tiles;
+    A.fixed = cuts > 1 ? (unsigned) cuts : 0u;
     static SmemLimit limit;
     if (!limit.raise((const void*) prompt_kernel<D>, PCfg<D>::smem)) return note_launch("kv prompt attention smem attribute");
-    launch_dependent(prompt_kernel<D>, dim3((unsigned) tiles, (unsigned) c.n_kv), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
-    return note_launch("attn_q8 prompt");
+    launch_dependent(prompt_kernel<D>, dim3((unsigned) tiles, (unsigned) c.n_kv, (unsigned) cuts), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
+    const int st = note_launch("attn_q8 prompt");
+    if (st != MAYA_OK || cuts == 1) return st;
+    return attn_join(c, b, A, true, 256, s);
 }
 
 }  // namespace

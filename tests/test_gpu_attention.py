@@ -185,6 +185,20 @@ def test_prompts(cuda, case, bf16):
     assert T.equal(out, again)
 
 
+@pytest.mark.parametrize("dim,window", [(128, 0), (64, 0), (128, 2500)])
+def test_few_prompt_rows_over_a_long_context(cuda, dim, window):
+    """A tile or two a head over many blocks: cut into pieces that are joined; a sequence so short that some of its pieces are empty, one of no tokens."""
+    import torch as T
+    rng = np.random.default_rng(50 + dim)
+    new, lens, n_kv, group = [50, 50, 0, 60], [7000, 90, 300, 40], 2, 3                # (the last: 20 rows before the sequence)
+    cache, host = make_cache(T, rng, lens, n_kv, dim)
+    q = T.from_numpy(rng.standard_normal((160, n_kv * group, dim)).astype(np.float32)).bfloat16()
+    out, lse = attend(T, cache, new, lens, q.cuda(), window)
+    check(out, lse, plain_attention(host, new, lens, q.double().numpy(), n_kv, dim ** -0.5, window), True)
+    again, _ = attend(T, cache, new, lens, q.cuda(), window, lse=False)
+    assert T.equal(out, again)
+
+
 def test_prompt_with_large_scores_and_scales_far_apart(cuda):
     """Rows whose maximum rises late and by much, value scales 1e-20 .. 1 and 0, blocks the table does not have, unaligned queries."""
     import torch as T
