@@ -7,9 +7,10 @@
 //                      to tensor memory as f16 over the scores it came from.
 //   warps 8..14        expand the codes of K and V to f16 into the swizzled shared-memory tiles that the tensor cores read, one step
 //                      ahead (codes come straight to registers: staging them would cost shared-memory bandwidth the products need).
-//   warp 15            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory).
+//   warp 15            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory), with few
+//                      instructions and few barriers: what it takes to issue them shows in the whole call's time.
 // The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
-// tensor pipe (D = 128) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096 and 2923 tokens, 32 heads over 8, 427 us, 786 TFLOP/s; what
+// tensor pipe (D = 128) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096 and 2923 tokens, 32 heads over 8, 411 us, 816 TFLOP/s; what
 // bounds it is the chain of a softmax warp, 2500 cycles a block of 64 tokens (half of them exponentials that two warps share a pipe for).
 //
 // Numbers.  A query row is scaled by a power of two into f16 (exact for bf16).  With vs the block's scale of V,
@@ -85,16 +86,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// One K = 16 product, operands in shared memory (SS) or A in tensor memory (TS); `acc` = 0 overwrites.  By one elected lane of a converged warp.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Four K = 16 products one behind the other (32 bytes of a 128-byte row on each), operands in shared memory (SS) or A in tensor memory (TS); `acc` = 0: the first
+// overwrites.  By one elected lane of a converged warp.  (In one piece, so that the issuing warp keeps ahead of the tensor cores.)
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred e, p;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b64 a1, a2, a3;\n\tadd.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n\t"
+        "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred e, p;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\tadd.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
+        "}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 
 template<int D>
@@ -102,7 +116,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     using K = PCfg<D>;
     constexpr int P = K::panels;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2], q_ready[2];
+    __shared__ __align__(8) uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_ready[2][2], pv_done, o_done[2], q_ready[2];
     __shared__ StepMeta meta[kMetaRing];
     __shared__ uint32_t tmem_base;
     __shared__ int lost;
@@ -112,9 +126,10 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], kExpandWarps); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], kExpandWarps); mbar_init(&v_free[i], 1);
-            mbar_init(&s_full[i][0], 1); mbar_init(&s_full[i][1], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4);
-            mbar_init(&pv_done[i], 1); mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
+            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4);
+            mbar_init(&o_done[i], 1); mbar_init(&q_ready[i], 4);
         }
+        mbar_init(&pv_done, 1);
         lost = 0;
         mbar_fence_init();
     }
@@ -123,7 +138,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     grid_dependency_wait();
 
     // ---- the rows, and the cache blocks they see
-    const int h = blockIdx.y, si = blockIdx.x / A.row_tiles, r0 = (A.row_tiles - 1 - blockIdx.x % A.row_tiles) * 256;   // the longest rows first
+    const int h = blockIdx.x % C.n_kv, tile = blockIdx.x / C.n_kv, si = tile % B.n_seq, r0 = (A.row_tiles - 1 - tile / B.n_seq) * 256;   // every sequence's last rows first
     const Seq s = seq_of(B, si);
     const int n_rows = s.n_new * A.group, first = s.len - s.n_new;
     const bool here = r0 < n_rows;
@@ -240,16 +255,15 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 const uint32_t qa = base + K::q + x * K::tile, ka = base + K::k + ((k >> 1) & 1) * K::tile + (k & 1) * (64 * 128);
 #pragma unroll
                 for (int p = 0; p < P; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + K::col_s + 128 * x + 64 * (k & 1), smem_desc_sw128(qa + p * (128 * 128) + i * 32), smem_desc_sw128(ka + p * (128 * 128) + i * 32),
-                               K::idesc_s, p + i > 0);
-                mma_commit_elect(smem_u32(&s_full[x][k & 1]));
+                    mma4_ss(tmem + K::col_s + 128 * x + 64 * (k & 1), smem_desc_sw128(qa + p * (128 * 128)), smem_desc_sw128(ka + p * (128 * 128)), K::idesc_s, p);
             };
             bool ok = steps == 0 || (wait(&k_full[0], 0) && wait(&q_ready[0], 0) && (tiles == 1 || wait(&q_ready[1], 0)));
             tc_fence_after();
             if (ok && steps > 0)
+            {
                 for (int x = 0; x < tiles; ++x) scores(x, 0);
+                mma_commit_elect(smem_u32(&s_full[0]));
+            }
             for (int k = 0; k < blocks && ok; ++k) {
                 const int j = k >> 1;
                 if (k + 1 < blocks) {
@@ -257,22 +271,24 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                     if (j1 != j) ok = wait(&k_full[j1 & 1], (j1 >> 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int x = 0; x < tiles; ++x) scores(x, k + 1);
+                    scores(0, k + 1);
+                    if (tiles > 1) scores(1, k + 1);
+                    mma_commit_elect(smem_u32(&s_full[(k + 1) & 1]));
                     if (j1 == j) mma_commit_elect(smem_u32(&k_free[j & 1]));
                 }
                 if ((k & 1) == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
                 const uint32_t va = base + K::v + (j & 1) * K::tile + (k & 1) * (D * 128);
-                for (int x = 0; x < tiles && ok; ++x) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (x >= tiles || !ok) break;
                     ok = wait(&p_ready[x][k & 1], j & 1);
                     if (!ok) break;
                     tc_fence_after();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mma_ts(tmem + K::col_o + D * x, tmem + K::col_s + 128 * x + 64 * (k & 1) + 8 * i, smem_desc_sw128(va + i * 32), K::idesc_o, k + i > 0);
-                    mma_commit_elect(smem_u32(&pv_done[x]));
+                    mma4_ts(tmem + K::col_o + D * x, tmem + K::col_s + 128 * x + 64 * (k & 1), smem_desc_sw128(va), K::idesc_o, k);
                     if (k + 1 == blocks) mma_commit_elect(smem_u32(&o_done[x]));
                 }
                 if (ok && (k & 1)) mma_commit_elect(smem_u32(&v_free[j & 1]));
+                if (ok && k + 2 == blocks) mma_commit_elect(smem_u32(&pv_done));
             }
             if (!ok && steps > 0) {                                         // what has been issued ends before the memory is given back
                 mma_commit_elect(smem_u32(&o_done[1]));
@@ -329,7 +345,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             bool ok = true;
 #pragma unroll 1
             for (int k = 0; k < 2 * steps; ++k) {                       // (not unrolled: the parts' code side by side is more than the instruction cache holds)
-                    if (!wait(&s_full[x][k & 1], (k >> 1) & 1)) { ok = false; break; }
+                    if (!wait(&s_full[k & 1], (k >> 1) & 1)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t at_k = at_s + 64 * (k & 1);
                     const StepMeta& sm = meta[(k >> 1) % kMetaRing];
@@ -362,7 +378,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         m = up;
                         l *= alpha;
                         if (k > 0) {
-                            if (!wait(&pv_done[x], (k - 1) & 1)) { ok = false; break; }       // (the one before it ended in front of these scores)
+                            // O up to the block before is there when the next scores are, which are issued behind it; at the last block it has a barrier of its own.
+                            if (!(k + 1 < 2 * steps ? wait(&s_full[(k + 1) & 1], ((k + 1) >> 1) & 1) : wait(&pv_done, 0))) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < D; d += 16) {
@@ -405,7 +422,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             if (ok) {                                                       // (warp-uniform: a wait runs out for a whole warp)
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 const int n = s.row + row / A.group, hq = h * A.group + row % A.group;
-                const size_t part = (((size_t) blockIdx.x * C.n_kv + h) * A.fixed + blockIdx.z) * 256 + tid;
+                const size_t part = (((size_t) (si * A.row_tiles + A.row_tiles - 1 - r0 / 256) * C.n_kv + h) * A.fixed + blockIdx.z) * 256 + tid;
                 const bool cut = A.fixed > 1;
                 uint16_t* dst = (uint16_t*) A.out + ((size_t) n * A.n_q + hq) * D;
 #pragma unroll
@@ -446,10 +463,10 @@ template<int D> int launch_prompt(const maya_kv_cache& c, const maya_attn_batch&
     const long long rows = (long long) b.max_new * A.group;
     A.row_tiles = (int) ((rows + 255) / 256);
     const long long tiles = (long long) A.row_tiles * b.n_seq;
-    if (tiles > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
     // Pieces: as many as fill the SMs, of 16 blocks at least, as far as there is room for parts (61 tokens of four sequences at up to 34k, 12 heads over 4: in
     // one piece each 643 us, so 90).
     const long long pairs = tiles * c.n_kv;
+    if (pairs > 0x7fffffffll) return refuse(MAYA_ERR_LIMIT);
     long long most = (b.max_len + kKvBlock - 1) / kKvBlock;
     if (A.window > 0 && most > (A.window + 255ll / A.group) / kKvBlock + 2) most = (A.window + 255ll / A.group) / kKvBlock + 2;
     long long cuts = sm_count() / pairs;
@@ -460,7 +477,7 @@ template<int D> int launch_prompt(const maya_kv_cache& c, const maya_attn_batch&
     A.fixed = cuts > 1 ? (unsigned) cuts : 0u;
     static SmemLimit limit;
     if (!limit.raise((const void*) prompt_kernel<D>, PCfg<D>::smem)) return note_launch("kv prompt attention smem attribute");
-    launch_dependent(prompt_kernel<D>, dim3((unsigned) tiles, (unsigned) c.n_kv, (unsigned) cuts), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
+    launch_dependent(prompt_kernel<D>, dim3((unsigned) pairs, 1, (unsigned) cuts), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
     const int st = note_launch("attn_q8 prompt");
     if (st != MAYA_OK || cuts == 1) return st;
     return attn_join(c, b, A, true, 256, s);
