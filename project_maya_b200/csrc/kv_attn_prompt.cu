@@ -6,12 +6,14 @@
 //   warps 0..3, 4..7   softmax of tile 0, 1: a thread a row.  64 scores at a time (a cache block: one scale) from tensor memory, 2^x, P back
 //                      to tensor memory as f16 over the scores it came from.
 //   warps 8..14        expand the codes of K and V to f16 into the swizzled shared-memory tiles that the tensor cores read, one step
-//                      ahead (codes come straight to registers: staging them would cost shared-memory bandwidth the products need).
+//                      ahead (codes come straight to registers).
 //   warp 15            issues the products: S = Q K^T (both operands in shared memory), O += P V (P from tensor memory), with few
 //                      instructions and few barriers: what it takes to issue them shows in the whole call's time.
 // The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
-// tensor pipe (D = 128) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096 and 2923 tokens, 32 heads over 8, 411 us, 816 TFLOP/s; what
-// bounds it is the chain of a softmax warp, 2500 cycles a block of 64 tokens (half of them exponentials that two warps share a pipe for).
+// tensor pipe (D = 128) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096 and 2923 tokens, 32 heads over 8, 411 us, 816 TFLOP/s.
+// What bounds it is the chain from part to part with the products in it, 5200 cycles a step, and 62 us of starts: without the exponentials, the loads or the
+// stores of codes it takes as long, without the softmax 378, without the products 357 (of 428 then).  Dropped: the softmax of a row over two threads (486), codes
+// staged by bulk copies (446), thread blocks that stay (460).
 //
 // Numbers.  A query row is scaled by a power of two into f16 (exact for bf16).  With vs the block's scale of V,
 //   P = 2^(s + log2 vs - m + 4),  O = sum P code,  l = sum P / vs:
