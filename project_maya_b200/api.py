@@ -671,6 +671,7 @@ class KvCache:
         if mean is None and self.k_sum is not None:
             mean = torch.empty((n, self.n_kv, self.head_dim), dtype=dtype, device=dev)
         assert k.dtype == v.dtype and (mean is None or mean.dtype == k.dtype) and k.dtype in (torch.float32, torch.bfloat16)
+        assert k.shape == v.shape == (n, KV_BLOCK, self.n_kv, self.head_dim) and (mean is None or mean.shape == (n, self.n_kv, self.head_dim))
         assert blocks.dtype == torch.int32 and (counts is None or (counts.dtype == torch.int32 and counts.numel() == n))
         _check("kv_read", _lib.load().maya_kv_read(self._ref, _ptr(blocks), _ptr(counts), n, int(k.dtype == torch.bfloat16), _ptr(k), _ptr(v),
                                                    _ptr(mean), _stream(stream)))
