@@ -710,6 +710,7 @@ class Rope:
         assert (cos is None) == (sin is None) and (cos is None or cos.shape == sin.shape)
         n_pos, rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
         self._keep = cos, sin, q_w, k_w
+        self.weight_shapes = tuple(t.shape for t in (q_w, k_w) if t is not None)
         self.args = RopeArgs(q_w=_ptr(q_w), k_w=_ptr(k_w), eps=eps, cos=_ptr(cos), sin=_ptr(sin), n_pos=n_pos, rot_dim=rot_dim, pairs=int(pairs))
         self._ref = C.byref(self.args)
 
@@ -755,6 +756,7 @@ class KvAttention:
         """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
         (None: the tokens' positions)."""
         a, c, n = rope.args, self.cache, batch.n_tokens
+        assert all(shape == (c.head_dim,) for shape in rope.weight_shapes), "norm weights [head_dim] expected"
         dtype = self._queries(a, batch, q)
         a.n_q = self.n_q
         if k is not None:

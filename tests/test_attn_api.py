@@ -24,3 +24,12 @@ def test_read_refuses_outputs_of_another_size(api, cache):
             out = {n: T.empty(shape if n == name else s, dtype=T.bfloat16) for n, s in right.items()}
             with pytest.raises(AssertionError):
                 cache.read(blocks, **out)
+
+
+def test_append_refuses_norm_weights_of_another_size(api, cache):
+    """Shorter ones would be read beyond their end, longer ones be taken for their first head's."""
+    batch, attn = api.AttnBatch.of([1], [3], device="cpu"), api.KvAttention(cache, 2)
+    q, k, v = (T.zeros((1, 2, 128)) for _ in range(3))
+    for kw in (dict(q_w=T.ones(64)), dict(k_w=T.ones(64)), dict(q_w=T.ones(256)), dict(q_w=T.ones(128), k_w=T.ones(127)), dict(q_w=T.ones((2, 128)))):
+        with pytest.raises(AssertionError, match="weights"):
+            attn.append(batch, q, k, v, api.Rope(**kw))
