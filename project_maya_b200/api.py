@@ -702,7 +702,7 @@ class AttnBatch:
 class Rope:
     """What stands between a layer's projections and its attention: cos and sin f32 [positions, rot_dim / 2] (None: no rotation), the
     weights f32 [head_dim] of the queries' and keys' RMS norms (None: no norm).  pairs: value 2 i turns with 2 i + 1, else i with
-    i + rot_dim / 2."""
+    i + rot_dim / 2.  Never written after this: layers and threads may share one."""
 
     def __init__(self, cos=None, sin=None, q_w=None, k_w=None, eps: float = 1e-6, pairs: bool = False):
         for t in (cos, sin, q_w, k_w):
@@ -712,7 +712,6 @@ class Rope:
         self._keep = cos, sin, q_w, k_w
         self.weight_shapes = tuple(t.shape for t in (q_w, k_w) if t is not None)
         self.args = RopeArgs(q_w=_ptr(q_w), k_w=_ptr(k_w), eps=eps, cos=_ptr(cos), sin=_ptr(sin), n_pos=n_pos, rot_dim=rot_dim, pairs=int(pairs))
-        self._ref = C.byref(self.args)
 
 
 def _rows(x, n: int, heads: int, head_dim: int):
@@ -728,8 +727,8 @@ class KvAttention:
     append(batch, q, k, v, rope) normalises and rotates the new tokens' queries and keys and puts keys and values into the cache;
     forward(batch, q) attends over it; select(batch, q) chooses the n_sel blocks each token reads and forward(batch, q, sel=...) attends over those
     alone.  f32 or bf16; q, k, v [n_tokens, heads, head_dim], views into rows of projections among them.  scale: of the scores
-    (head_dim ** -0.5); window > 0: a token sees the last `window` positions.  The scratch belongs to this object: one stream at a
-    time."""
+    (head_dim ** -0.5); window > 0: a token sees the last `window` positions.  The scratch and the arguments of a call belong to this object: one
+    thread and one stream at a time."""
 
     def __init__(self, cache: KvCache, n_q: int, scale: float | None = None, window: int = 0, n_sel: int = 0, n_first: int = 1,
                  n_last: int = 2, max_tokens: int = 65536):
@@ -741,7 +740,8 @@ class KvAttention:
         self.scratch[:1 << 12].zero_()                      # the error word and the counters
         self._attn = AttnArgs(None, 0, 0, n_q, cache.head_dim ** -0.5 if scale is None else scale, window, None, 0, None, None)
         self._select = SelectArgs(None, 0, 0, n_q, n_first, n_last, n_sel, None)
-        self._refs = C.byref(self._attn), C.byref(self._select)
+        self._rope = RopeArgs()
+        self._refs = C.byref(self._attn), C.byref(self._select), C.byref(self._rope)
 
     def _queries(self, a, batch, q):
         """The queries of a call into its arguments; returns their type."""
@@ -755,21 +755,20 @@ class KvAttention:
     def append(self, batch: AttnBatch, q, k, v, rope: Rope, pos=None, q_out=None, stream=None):
         """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
         (None: the tokens' positions)."""
-        a, c, n = rope.args, self.cache, batch.n_tokens
+        a, c, n = self._rope, self.cache, batch.n_tokens
         assert all(shape == (c.head_dim,) for shape in rope.weight_shapes), "norm weights [head_dim] expected"
+        C.memmove(self._refs[2], C.byref(rope.args), C.sizeof(RopeArgs))
         dtype = self._queries(a, batch, q)
         a.n_q = self.n_q
         if k is not None:
             assert k.dtype is dtype and v.dtype is dtype
             a.k, a.ld_k = _rows(k, n, c.n_kv, c.head_dim)
             a.v, a.ld_v = _rows(v, n, c.n_kv, c.head_dim)
-        else:
-            a.k = a.v = None
         if q_out is None:
             q_out = torch.empty((n, self.n_q, c.head_dim), dtype=dtype, device=q.device)
         assert q_out.dtype is dtype and q_out.shape == (n, self.n_q, c.head_dim) and (pos is None or (pos.dtype == torch.int32 and pos.numel() == n))
         a.pos, a.q_out = _ptr(pos), _ptr(q_out)
-        _check("qk_norm_rope_append", _lib.load().maya_qk_norm_rope_append(c._ref, batch._ref, rope._ref, _stream(stream)))
+        _check("qk_norm_rope_append", _lib.load().maya_qk_norm_rope_append(c._ref, batch._ref, self._refs[2], _stream(stream)))
         return q_out
 
     def forward(self, batch: AttnBatch, q, sel=None, out=None, lse=None, stream=None):
