@@ -710,7 +710,7 @@ class Rope:
         assert (cos is None) == (sin is None) and (cos is None or cos.shape == sin.shape)
         n_pos, rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
         self._keep = cos, sin, q_w, k_w
-        self.weight_shapes = tuple(t.shape for t in (q_w, k_w) if t is not None)
+        self.weight_sizes = tuple(t.numel() for t in (q_w, k_w) if t is not None)
         self.args = RopeArgs(q_w=_ptr(q_w), k_w=_ptr(k_w), eps=eps, cos=_ptr(cos), sin=_ptr(sin), n_pos=n_pos, rot_dim=rot_dim, pairs=int(pairs))
 
 
@@ -756,7 +756,7 @@ class KvAttention:
         """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
         (None: the tokens' positions)."""
         a, c, n = self._rope, self.cache, batch.n_tokens
-        assert all(shape == (c.head_dim,) for shape in rope.weight_shapes), "norm weights [head_dim] expected"
+        assert all(size == c.head_dim for size in rope.weight_sizes), "norm weights [head_dim] expected"
         C.memmove(self._refs[2], C.byref(rope.args), C.sizeof(RopeArgs))
         dtype = self._queries(a, batch, q)
         a.n_q = self.n_q
