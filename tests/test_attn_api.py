@@ -61,3 +61,24 @@ def test_attention_objects_that_share_a_rotation_keep_their_own_arguments(api, c
         assert (q_ptr, k_ptr, out, n_q) == (q.data_ptr(), None if keys is None else k.data_ptr(), o.data_ptr(), q.shape[1])
         assert cos == rope._keep[0].data_ptr() and rot == 128
     assert rope.args.q is None and rope.args.k is None and rope.args.q_out is None and rope.args.n_q == 0
+
+
+def test_error_sets_the_scratch_back(api, cache, monkeypatch):
+    """A launch that gave up leaves its counters somewhere in between: the next ones would start from there."""
+    real, code = api._lib.load(), [1]
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def maya_attn_error(self, scratch, stream):
+            return code[0]
+
+    monkeypatch.setattr(api._lib, "load", Library)
+    monkeypatch.setattr(api, "_stream", lambda stream: 0)
+    attn = api.KvAttention(cache, 2)
+    attn.scratch[:256] = 7
+    assert attn.error() == 1 and not attn.scratch[:256].any()
+    code[0] = 0
+    attn.scratch[:256] = 7                                                     # (nothing wrong: nothing written)
+    assert attn.error() == 0 and (attn.scratch[:256] == 7).all()
