@@ -802,7 +802,7 @@ class KvAttention:
         """1 after a call whose bounded wait ran out (its outputs are not valid, and neither are those of the calls since); synchronises the
         stream.  The error word and the counters are zeroed then, so that the calls after this are sound again."""
         code = int(_lib.load().maya_attn_error(self.scratch.data_ptr(), _stream(stream)))
-        if code:
+        if code > 0:
             self.scratch[:1 << 12].zero_()
             if self.scratch.is_cuda:
                 torch.cuda.current_stream(self.scratch.device).synchronize()      # (the next call may be on another stream)
