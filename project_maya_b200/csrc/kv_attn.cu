@@ -105,8 +105,6 @@ __device__ __forceinline__ size_t out_row(const AttnView& A, const Tile& T, int 
     const int row = T.r0 + r;
     return (size_t) (T.s.row + T.i0 + row / A.group) * A.n_q + h * A.group + row % A.group;
 }
-// O is P V, l the sum of P (V's scale taken out again)
-__device__ __forceinline__ float lse_of(float m, float l, float bias) { return l > 0.0f ? (m + log2f(l) - bias) * 0.69314718055994531f : kNone; }
 
 // A (tile, head)'s cache blocks are cut into pieces of about `q`, of which a thread block works on one at a time: about four a thread block where there are
 // many blocks (the SMs are not equally fast: with even shares fixed beforehand the last of 444 thread blocks ended at 147 us, the middle one at 113), none
@@ -342,7 +340,7 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
                     amax = warp_max(amax);
                     const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
                     const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
-                    if (lane == 0) qinv[r] = __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2;
+                    if (lane == 0) qinv[r] = scale_of_row(amax, __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2);
 #pragma unroll
                     for (int e = 0; e < V; e += 2) {
                         const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;

@@ -14,6 +14,11 @@ namespace maya {
 
 constexpr float kRise = 8.0f;                    // how far a maximum may pass m (base 2) before m is raised to it
 constexpr float kNone = -INFINITY;
+// What multiplies the scores of a query row whose largest value is amax: NaN for a row with an infinity, whose products may be anything (0 times it among
+// them).  A row with a NaN has NaN scores by itself.  Such rows are NaN wherever they see a token, so that what went wrong in front stays visible.
+__device__ __forceinline__ float scale_of_row(float amax, float scale) { return amax < INFINITY ? scale : __uint_as_float(0x7fc00000u); }
+// ln of a row's sum of exp(scores) from m and l, the sum of P (V's scale taken out again); -inf for a row that saw nothing.
+__device__ __forceinline__ float lse_of(float m, float l, float bias) { return l == 0.0f ? kNone : (m + log2f(l) - bias) * 0.69314718055994531f; }
 
 struct AttnView {
     const void* q;

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 for (int i = 0; i < D / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
                 const int e2 = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;    // amax * 2^e2 in [2^11, 2^12)
                 const float up = __uint_as_float((uint32_t) (127 + e2) << 23);
-                qinv = __uint_as_float((uint32_t) (127 - e2) << 23) * A.scale_log2;
+                qinv = scale_of_row(amax, __uint_as_float((uint32_t) (127 - e2) << 23) * A.scale_log2);
         #pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
                     uint4 o;
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             if (ok && steps > 0) ok = wait(&o_done[x], 0);
             tc_fence_after();
             if (ok) {                                                       // (warp-uniform: a wait runs out for a whole warp)
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;                  // (a row that saw nothing; a NaN stays one)
                 const int n = s.row + row / A.group, hq = h * A.group + row % A.group;
                 const size_t part = (((size_t) (si * A.row_tiles + A.row_tiles - 1 - r0 / 256) * C.n_kv + h) * A.fixed + blockIdx.z) * 256 + tid;
                 const bool cut = A.fixed > 1;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                         uint32_t w[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(l > 0.0f ? o[2 * i] * inv : 0.0f, l > 0.0f ? o[2 * i + 1] * inv : 0.0f);
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(l == 0.0f ? 0.0f : o[2 * i] * inv, l == 0.0f ? 0.0f : o[2 * i + 1] * inv);
                             w[i] = *(const uint32_t*) &b;
                         }
                         ((uint4*) (dst + d))[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 }
                 if (cut && row < n_rows) A.part_ml[part] = make_float2(m, l);
                 else if (A.lse != nullptr && row < n_rows)
-                    A.lse[(size_t) n * A.n_q + hq] = l > 0.0f ? (m + log2f(l) - kUp) * 0.69314718055994531f : kNone;
+                    A.lse[(size_t) n * A.n_q + hq] = lse_of(m, l, kUp);
             }
         }
     }

@@ -1,0 +1,54 @@
+"""Attention over the 8-bit cache, its append and its selection where they can go wrong: numbers that are not finite, very large and very small ones,
+bounds of the arguments, long contexts.  Helpers and plain forms are those of test_gpu_attention.py, and so are the tolerances where nothing else is said."""
+import numpy as np
+import pytest
+
+from test_gpu_attention import BLOCK, attend, check, make_cache, plain_attention, plain_rows, plain_select, unpack
+
+pytestmark = pytest.mark.gpu
+
+
+FORMS = [
+    # new tokens, lengths, key/value heads, group, head size, bf16, lists
+    ([1, 1, 4], [3000, 70, 2], 2, 4, 128, False, 0),     # tokens; two rows before their sequence
+    ([1, 1, 4], [3000, 70, 2], 2, 4, 128, True, 0),
+    ([9, 3], [400, 90], 1, 6, 64, False, 0),             # windows
+    ([2], [100], 1, 16, 256, True, 0),
+    ([150, 40], [150, 20], 2, 2, 128, True, 0),          # prompts, whole; twenty tokens before their sequence
+    ([300], [500], 1, 1, 64, True, 0),
+    ([50, 50], [7000, 40], 2, 3, 128, True, 0),          # cut into pieces and joined
+    ([90], [200], 1, 2, 128, False, 0),                  # in f32
+    ([1, 2], [1500, 90], 2, 8, 128, True, 5),            # lists
+    ([1800], [1900], 4, 2, 64, True, 4),                 # a warp a list
+]
+
+
+@pytest.mark.parametrize("case", range(len(FORMS)))
+def test_queries_that_are_not_finite(cuda, case):
+    """One NaN or infinity in a query: that row alone is not finite, in the output and in lse, whichever kernel has it; a row that sees nothing is 0 all the
+    same; every other row keeps its bits."""
+    import torch as T
+    new, lens, n_kv, group, dim, bf16, n_sel = FORMS[case]
+    rng = np.random.default_rng(600 + case)
+    cache, _ = make_cache(T, rng, lens, n_kv, dim)
+    N, H = sum(new), n_kv * group
+    q = T.from_numpy(rng.standard_normal((N, H, dim)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32).cuda()
+    sel = None
+    if n_sel:
+        own = np.concatenate([(n - m + np.arange(m)) // BLOCK for m, n in zip(new, lens)])
+        sel = T.from_numpy(np.sort(np.where(np.arange(n_sel) <= own[:, None, None], own[:, None, None] - np.arange(n_sel), -1).repeat(n_kv, 1).astype(np.int32), -1)).cuda()
+    pos = np.concatenate([n - m + np.arange(m) for m, n in zip(new, lens)])
+    bad = T.zeros((N, H), dtype=T.bool, device="cuda")
+    clean = q.clone()
+    for i, x in enumerate((float("nan"), float("inf"), -float("inf"))):
+        for row in (i * 7 % N, N - 1 - i * 5 % N):
+            bad[row, i % H] = True
+            q[row, i % H, (11 * i + 3) % dim] = x
+            clean[row, i % H] = 0
+    out, lse = attend(T, cache, new, lens, q, sel=sel)
+    want, want_lse = attend(T, cache, new, lens, clean, sel=sel)
+    seen = T.from_numpy(pos >= 0).cuda()
+    lost = bad & seen[:, None]
+    assert lost.any() and not T.isfinite(out[lost]).any() and T.isnan(lse[lost]).all()
+    assert (out[~seen] == 0).all() and T.isneginf(lse[~seen]).all()
+    assert T.equal(out[~lost], want[~lost]) and T.equal(lse[~lost], want_lse[~lost])
