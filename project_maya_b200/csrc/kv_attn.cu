@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
 #pragma unroll
                     for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
                     amax = warp_max(amax);
-                    const int exp2_ = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;   // amax * 2^e in [2^11, 2^12)
+                    const int exp2_ = up_of_row(amax);   // amax * 2^e in [2^11, 2^12)
                     const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
                     if (lane == 0) qinv[r] = scale_of_row(amax, __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2);
 #pragma unroll

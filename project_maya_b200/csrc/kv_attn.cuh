@@ -14,6 +14,9 @@ namespace maya {
 
 constexpr float kRise = 8.0f;                    // how far a maximum may pass m (base 2) before m is raised to it
 constexpr float kNone = -INFINITY;
+// The power of two that brings a query row's largest value to 2^11 .. 2^12: -116 for the largest numbers there are, 126 at most (2^-126 is the smallest normal
+// number), so that it and its reciprocal are normal numbers.
+__device__ __forceinline__ int up_of_row(float amax) { return amax > 0.0f ? min(126, 138 - (int) (__float_as_uint(amax) >> 23)) : 0; }
 // What multiplies the scores of a query row whose largest value is amax: NaN for a row with an infinity, whose products may be anything (0 times it among
 // them).  A row with a NaN has NaN scores by itself.  Such rows are NaN wherever they see a token, so that what went wrong in front stays visible.
 __device__ __forceinline__ float scale_of_row(float amax, float scale) { return amax < INFINITY ? scale : __uint_as_float(0x7fc00000u); }

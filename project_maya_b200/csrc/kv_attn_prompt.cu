@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 float amax = 0.0f;
         #pragma unroll
                 for (int i = 0; i < D / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
-                const int e2 = amax > 0.0f ? max(-100, min(100, 138 - (int) (__float_as_uint(amax) >> 23))) : 0;    // amax * 2^e2 in [2^11, 2^12)
+                const int e2 = up_of_row(amax);    // amax * 2^e2 in [2^11, 2^12)
                 const float up = __uint_as_float((uint32_t) (127 + e2) << 23);
                 qinv = scale_of_row(amax, __uint_as_float((uint32_t) (127 - e2) << 23) * A.scale_log2);
         #pragma unroll

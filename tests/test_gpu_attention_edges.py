@@ -52,3 +52,17 @@ def test_queries_that_are_not_finite(cuda, case):
     assert lost.any() and not T.isfinite(out[lost]).any() and T.isnan(lse[lost]).all()
     assert (out[~seen] == 0).all() and T.isneginf(lse[~seen]).all()
     assert T.equal(out[~lost], want[~lost]) and T.equal(lse[~lost], want_lse[~lost])
+
+
+@pytest.mark.parametrize("bf16,new,length", [(False, 3, 300), (True, 3, 300), (True, 140, 300)])
+def test_queries_of_any_finite_size(cuda, bf16, new, length):
+    """Rows near the largest and the smallest normal number, with a scale that brings their scores back."""
+    import torch as T
+    rng = np.random.default_rng(61)
+    cache, host = make_cache(T, rng, [length], 1, 64)
+    x = rng.standard_normal((new, 1, 64))
+    for size, scale in ((2.0 ** 126 / np.abs(x).max(), 0.125 * 2.0 ** -123), (2.0 ** -124 / np.abs(x).max(), 0.125 * 2.0 ** 122)):
+        q = T.from_numpy((x * size).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32)
+        want = plain_attention(host, [new], [length], q.double().numpy(), 1, float(np.float32(scale)))
+        out, lse = attend(T, cache, [new], [length], q.cuda(), scale=scale)
+        check(out, lse, want, bf16)
