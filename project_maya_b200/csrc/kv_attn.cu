@@ -737,8 +737,8 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
     A.row_tiles = (int) ((rows + K::rows - 1) / K::rows);
     const long long tiles = (long long) A.row_tiles * (a.sel ? b.n_tokens : b.n_seq);
     long long most = a.sel ? a.n_sel : (b.max_len + kKvBlock - 1) / kKvBlock;    // cache blocks of the longest tile
-    if (!a.sel && a.window > 0) {
-        const long long reach = (a.window + (K::rows + A.group - 1) / A.group + 2 * kKvBlock) / kKvBlock;
+    if (!a.sel && A.window > 0) {
+        const long long reach = (A.window + (K::rows + A.group - 1) / A.group + 2 * kKvBlock) / kKvBlock;
         if (reach < most) most = reach;
     }
     if (most < 1) most = 1;
@@ -820,7 +820,7 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     cudaStream_t s = as_stream(stream);
     AttnView A{};
     A.q = a->q; A.ld_q = a->ld_q; A.out = a->out; A.lse = a->lse; A.sel = a->sel; A.n_sel = a->n_sel; A.n_q = a->n_q; A.group = a->n_q / c->n_kv;
-    A.window = a->window;
+    A.window = a->window < b->max_len ? a->window : 0;                           // (wider than any sequence: none; what is left keeps int arithmetic in range)
     A.wide_q = rows_wide(a->q, a->ld_q, a->is_bf16 ? 2 : 4);
     A.scale_log2 = a->scale * 1.4426950408889634f;
     A.error = (unsigned*) scratch;

@@ -66,3 +66,16 @@ def test_queries_of_any_finite_size(cuda, bf16, new, length):
         want = plain_attention(host, [new], [length], q.double().numpy(), 1, float(np.float32(scale)))
         out, lse = attend(T, cache, [new], [length], q.cuda(), scale=scale)
         check(out, lse, want, bf16)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 70, 40000])
+@pytest.mark.parametrize("new,length,group,bf16", [(1, 30000, 1, False), (4, 30000, 2, True), (5, 3, 1, False), (140, 9000, 1, True), (200, 130, 1, True)])
+def test_windows_wider_than_the_context(cuda, window, new, length, group, bf16):
+    """The same as no window, up to the largest number there is."""
+    import torch as T
+    rng = np.random.default_rng(62)
+    cache, _ = make_cache(T, rng, [length], 1, 64)
+    q = T.from_numpy(rng.standard_normal((new, group, 64)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32).cuda()
+    want, want_lse = attend(T, cache, [new], [length], q)
+    out, lse = attend(T, cache, [new], [length], q, window=window)
+    assert T.equal(out, want) and T.equal(lse, want_lse)
