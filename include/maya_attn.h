@@ -34,7 +34,7 @@ extern "C" {
 
 #define MAYA_KV_BLOCK 64
 #define MAYA_MAX_SELECTED 512      /* list entries of maya_block_select / maya_attn_q8 */
-#define MAYA_MAX_KV_BLOCKS 16384   /* blocks of one sequence maya_block_select takes (1M tokens) */
+#define MAYA_MAX_KV_BLOCKS 16384   /* blocks of one sequence maya_block_select takes (1M tokens; so many for groups of up to 248 heads) */
 
 typedef struct maya_kv_cache {
     void* k;

@@ -79,3 +79,44 @@ def test_windows_wider_than_the_context(cuda, window, new, length, group, bf16):
     want, want_lse = attend(T, cache, [new], [length], q)
     out, lse = attend(T, cache, [new], [length], q, window=window)
     assert T.equal(out, want) and T.equal(lse, want_lse)
+
+
+LONG = [
+    # new tokens, tokens, group, head size, selected, first, last
+    (1, 1 << 20, 1, 64, 40, 1, 1),               # the longest context that the header names, for every size of group: one list by a whole thread block
+    (1, 1 << 20, 2, 64, 7, 0, 1),
+    (2, (1 << 20) - 30, 4, 64, 16, 1, 2),        # a warp a list
+    (1, 1 << 20, 8, 64, 512, 2, 3),
+    (3, 1 << 20, 1, 64, 33, 0, 2),
+    (2, 300000, 16, 128, 20, 1, 2),
+    (30, 40000, 8, 128, 16, 1, 2),
+    (40, 70001, 3, 64, 100, 1, 1),
+    (9, 140000, 40, 64, 12, 1, 1),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_select_over_long_contexts(cuda, case):
+    """Lists over more blocks than a warp's (256) or a thread block's (2048) registers hold, up to 16384 blocks; many places share a block of the cache."""
+    import torch as T
+    from project_maya_b200 import api
+    new, n, group, dim, n_sel, n_first, n_last = LONG[case]
+    rng = np.random.default_rng(630 + case)
+    cache, host = make_cache(T, rng, [90 * BLOCK], 1, dim)
+    host["table"] = rng.integers(0, cache.n_blocks, (1, -(-n // BLOCK))).astype(np.int32)
+    cache = api.KvCache(cache.k, cache.v, cache.k_scale, cache.v_scale, T.from_numpy(host["table"]).cuda(), cache.k_sum)
+    q = T.from_numpy(rng.standard_normal((new, group, dim)).astype(np.float32))
+    attn = api.KvAttention(cache, group, n_sel=n_sel, n_first=n_first, n_last=n_last)
+    sel = attn.select(api.AttnBatch.of([new], [n]), q.cuda(), sel=T.full((new, 1, n_sel), -5, dtype=T.int32, device="cuda"))
+    assert np.array_equal(sel.cpu().numpy(), plain_select(host, [new], [n], q.numpy(), 1, n_sel, n_first, n_last))
+
+
+def test_select_beyond_the_longest_context_is_refused(cuda):
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(64)
+    cache, _ = make_cache(T, rng, [90], 1, 64, wide=16385)
+    q = T.zeros((1, 1, 64), device="cuda")
+    with pytest.raises(api.MayaError) as e:
+        api.KvAttention(cache, 1, n_sel=4).select(api.AttnBatch.of([1], [(1 << 20) + 1]), q)
+    assert e.value.status == -4
