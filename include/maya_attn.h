@@ -127,7 +127,7 @@ typedef struct maya_select_args {
 /* For each new token and key/value head the n_sel blocks it reads: the forced ones, and of those between them the ones with the
  * highest score, max over the group's query heads g of (f32(q8_g . k_sum_b) * s_g) * k_scale_b, where q8_g = round(q_g / s_g) and
  * s_g = amax(q_g) * f32(1 / 127).  The dot is of whole numbers and exact, so a list does not depend on the order of any sum; equal
- * scores go to the lower block. */
+ * scores go to the lower block.  A block that the table does not have stands behind all that it has. */
 MAYA_API int maya_block_select(const maya_kv_cache* cache, const maya_attn_batch* batch, const maya_select_args* a, void* stream);
 
 #ifdef __cplusplus

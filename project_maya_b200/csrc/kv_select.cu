@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kSelThreads, D <= 128 ? 2 : 1) select_kernel(c
             const uint4* src = (const uint4*) (C.k_sum + bh * D) + t;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) raw[x][i] = phys[x] >= 0 ? src[i * 4] : make_uint4(0u, 0u, 0u, 0u);
-            raw_ks[x] = phys[x] >= 0 ? C.k_scale[bh] : 0.0f;
+            raw_ks[x] = phys[x] >= 0 ? C.k_scale[bh] : -INFINITY;         // (a block that is not there: 0 times this, a NaN, below every score)
         }
     };
     look_up(b16);

@@ -120,3 +120,27 @@ def test_select_beyond_the_longest_context_is_refused(cuda):
     with pytest.raises(api.MayaError) as e:
         api.KvAttention(cache, 1, n_sel=4).select(api.AttnBatch.of([1], [(1 << 20) + 1]), q)
     assert e.value.status == -4
+
+
+@pytest.mark.parametrize("new,n,group", [(1, 5000, 4), (20, 5000, 1), (1, 5000, 12)])
+def test_select_passes_over_blocks_the_table_does_not_have(cuda, new, n, group):
+    """Keys that all point away from the queries: every real block scores below 0, and still stands before one that is not there."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(65)
+    cache, host = make_cache(T, rng, [n], 1, 64)
+    q = T.from_numpy(rng.uniform(0.5, 1, (new, group, 64)).astype(np.float32))
+    host["sums"][:] = rng.integers(-4000, -1000, host["sums"].shape)
+    cache.k_sum.copy_(T.from_numpy(host["sums"]))
+    gone = rng.permutation(np.arange(1, n // BLOCK - 5))[:30]
+    cache.table[0, T.from_numpy(gone).cuda()] = T.from_numpy(np.where(np.arange(30) % 2, -1, cache.n_blocks).astype(np.int32)).cuda()
+    attn, batch = api.KvAttention(cache, group, n_sel=12, n_first=1, n_last=2), api.AttnBatch.of([new], [n])
+    sel = attn.select(batch, q.cuda()).cpu().numpy()
+    assert not np.isin(sel, gone).any() and (sel >= 0).all()
+    # the same list as with scores below every real one in their places
+    host["ks"][host["table"][0, gone]] = 1e6
+    assert np.array_equal(sel, plain_select(host, [new], [n], q.numpy(), 1, 12, 1, 2))
+    # fewer real ones than entries: they are all there
+    few = api.KvAttention(cache, group, n_sel=60, n_first=1, n_last=2).select(batch, q.cuda()).cpu().numpy()
+    real = np.setdiff1d(np.arange((n - new) // BLOCK + 1), gone)
+    assert all(np.isin(real, few[i]).all() for i in range(new))
