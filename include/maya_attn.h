@@ -75,7 +75,8 @@ typedef struct maya_rope_args {
 /* For each new token: q_out = rotate(rms(q) * q_w); rotate(rms(k) * k_w) and v into the cache.  rms(x) = x / sqrt(mean(x^2) + eps)
  * over a head's values; rotate: (a, b) -> (a cos - b sin, b cos + a sin).  In f32; q_out rounded once.
  * A block takes the pass's tokens together: its new scale is max(the old one if it holds tokens from before, amax of the new
- * tokens / 127); when that grows, the codes it holds become round(code * old / new), so a code is rounded once more at each
+ * tokens / 127, or 2^-126 where that is less and amax is not 0); a code is value / scale rounded to nearest, by the scale's reciprocal
+ * (within 2^-15 of a step); when the scale grows, the codes it holds become round(code * old / new), so a code is rounded once more at each
  * growth; k_sum is made from the codes.  A pass may start at an earlier length than the last one ended (tokens taken back).  Not finite: a NaN is stored as 0, an infinity as 127 times a scale of 1e30.
  * No two sequences of a batch may append to the same block. */
 MAYA_API int maya_qk_norm_rope_append(const maya_kv_cache* cache, const maya_attn_batch* batch, const maya_rope_args* a, void* stream);

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(Form<FEW>::threads, Form<FEW>::blocks(D)) appe
     if (phys < 0) return;
 #pragma unroll
     for (int i = 0; i < kAppendWarps; ++i) amax = fmaxf(amax, swarp[i]);
-    const float s1 = fmaxf(s0, fminf(amax * kInv127, kScaleMost)), inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
+    const float s1 = fmaxf(s0, amax > 0.0f ? fmaxf(kScaleLeast, fminf(amax * kInv127, kScaleMost)) : 0.0f), inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
     const bool grew = t0 > 0 && s1 > s0;
     const float ratio = grew ? __fdiv_rn(s0, s1) : 1.0f;
 

@@ -10,6 +10,7 @@ namespace maya {
 
 constexpr int kKvBlock = MAYA_KV_BLOCK;
 constexpr float kInv127 = 1.0f / 127.0f;
+constexpr float kScaleLeast = 0x1p-126f;  // of a block with a value that is not 0: its reciprocal is finite
 constexpr float kScaleMost = 1e30f;       // of a block that was given an infinity: 127 * kScaleMost is finite
 
 // The cache and the batch as the kernels take them.

@@ -144,3 +144,25 @@ def test_select_passes_over_blocks_the_table_does_not_have(cuda, new, n, group):
     few = api.KvAttention(cache, group, n_sel=60, n_first=1, n_last=2).select(batch, q.cuda()).cpu().numpy()
     real = np.setdiff1d(np.arange((n - new) // BLOCK + 1), gone)
     assert all(np.isin(real, few[i]).all() for i in range(new))
+
+
+@pytest.mark.parametrize("size", [1e-36, 3e-37, 1e-38, 1e-40, 1e-44])
+def test_append_of_the_smallest_values(cuda, size):
+    """Values whose 127th is no normal number: a scale is 2^-126 at least, and a code is off by half of it at most."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(66)
+    for new, dim in ((1, 64), (40, 128)):
+        cache = api.KvCache.empty(1, 1, dim, T.zeros((1, 1), dtype=T.int32, device="cuda"))
+        x = (size * rng.uniform(-1, 1, (new, 1, dim))).astype(np.float32)
+        d = T.from_numpy(x).cuda()
+        api.KvAttention(cache, 1).append(api.AttnBatch.of([new], [new]), d, d, d, api.Rope())
+        k, v = unpack(cache)
+        for codes, scale in ((k, cache.k_scale), (v, cache.v_scale)):
+            s = float(scale.double()[0, 0])
+            assert s == max(2.0 ** -126, float(np.float32(np.abs(x).max()) * np.float32(1 / 127)))
+            assert (np.abs(codes[0, 0, :new] * s - x[:, 0].astype(np.float64)) <= s * (0.5 + 2.0 ** -15)).all()
+        assert np.array_equal(cache.k_sum[0, 0].cpu().numpy(), k[0, 0, :new].sum(0))
+        zero = api.KvCache.empty(1, 1, dim, T.zeros((1, 1), dtype=T.int32, device="cuda"))
+        api.KvAttention(zero, 1).append(api.AttnBatch.of([new], [new]), d, 0 * d, 0 * d, api.Rope())
+        assert float(zero.v_scale) == 0 and (unpack(zero)[1][0, 0, :new] == 0).all()
