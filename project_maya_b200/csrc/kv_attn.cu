@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Meta meta[kMeta];
     __shared__ __align__(8) uint64_t full[BW][K::slots], empty[BW][K::slots];
-    __shared__ float qinv[K::rows], sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT], sm_vr[kWarps];
+    __shared__ float qinv[K::rows], sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT];
     __shared__ int pre[NW == 1 ? 1 : kTilesMost + 1];
     __shared__ unsigned sums[kWarps], upcoming;
     __shared__ int lost;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
     }
     units *= (unsigned) C.n_kv;
 
-    float o[NT][D / 16][4], m[NT][2], l[NT][2], vr = F32 ? 0.0f : 1.0f;          // columns 2 t, 2 t + 1
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];                                  // columns 2 t, 2 t + 1
     int pos[NT][2];
     unsigned u_put = 0, put_phase = 0, get_phase = 0;                            // pieces this ring has asked for; the phases of
     int put_slot = 0, get_slot = 0;                                              // the slots that the next one goes into, and is taken from
@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
             pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
         }
     }
-    vr = F32 ? 0.0f : 1.0f;
     int low = min(pos[0][0], pos[0][1]);
     if constexpr (NT == 2) low = min(low, min(pos[NT - 1][0], pos[NT - 1][1]));
     const int wpos_lo = __reduce_min_sync(0xffffffffu, low);                     // over the warp's rows
@@ -427,12 +426,14 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
                 // ---- running maximum, P^T
                 const int tb = x.lb * kKvBlock;
                 const bool cut = tb + kKvBlock - 1 > wpos_lo || (A.window > 0 && tb <= wpos_hi - A.window);      // not visible to every row in whole
-                // V's scale: bf16: in P's exponent (m is then of s + log2 vs, and l takes it out again); f32, where that would cost bits: a factor
-                // against the largest one so far
-                float beta = 1.0f, wv = 1.0f, lv = 0.0f, ivs = 1.0f;
+                // V's scale is in P's exponent (m is then of s + log2 vs, and l takes it out again): bf16: all of it; f32, where a logarithm would cost
+                // bits: its power of two, the rest (1 .. 2) a factor
+                float wv = 1.0f, lv, ivs;
                 if constexpr (F32) {
-                    if (x.vs > vr) { beta = __fdividef(vr, x.vs); vr = x.vs; }
-                    wv = vr > 0.0f ? x.vs == vr ? 1.0f : __fdiv_rn(x.vs, vr) : 0.0f;
+                    const uint32_t e = min(max(__float_as_uint(x.vs) >> 23, kVsExpLeast), 253u);
+                    lv = (float) ((int) e - 127);
+                    ivs = __uint_as_float((254u - e) << 23);
+                    wv = x.vs * ivs;
                 } else {
                     const float vs = fmaxf(x.vs, kVsLeast);
                     lv = __log2f(vs);
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
                             off[e] = bias + lv - use;
                             m[n][e] = mn;
                             l[n][e] *= al;
-                            alpha[n][e] = al * beta;
+                            alpha[n][e] = al;
                         } else {                                                 // m is raised only when it is passed by more than kRise: P stays below 2^12
                             alpha[n][e] = 1.0f;
                             if (top > m[n][e] + kRise) {
@@ -573,7 +574,6 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
-                if (t == 0) sm_vr[warp] = vr;
             }
             __syncthreads();                                                     // every ring is empty
             float* buf = (float*) smem;                                          // [warp][8 NT][wide]
@@ -598,10 +598,10 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
 #pragma unroll
                 for (int b = 0; b < BW; ++b) {
                     const int x = x0 + RW * b;
-                    const float f = ex2(sm_m[x][rr] - use), fv = F32 ? f * sm_vr[x] : f;
+                    const float f = ex2(sm_m[x][rr] - use);
                     total += sm_l[x][rr] * f;
                     const float4 z = *(const float4*) (buf + (x * 8 * NT + rr) * K::wide + d);
-                    y.x += z.x * fv; y.y += z.y * fv; y.z += z.z * fv; y.w += z.w * fv;
+                    y.x += z.x * f; y.y += z.y * f; y.z += z.z * f; y.w += z.w * f;
                 }
                 if (!whole) {
                     *(float4*) (A.part_o + (part_at + r) * D + d) = y;

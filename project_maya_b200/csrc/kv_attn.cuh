@@ -4,7 +4,7 @@
 //   s_j = (q . k_j) * scale * k_scale[block] * log2(e)          p_j = 2^(s_j - m)          O = sum p_j v_j,  l = sum p_j
 // The codes of K and V become f16 exactly (|code| <= 127); a query row is multiplied by a power of two that brings its largest
 // value to 2^11 .. 2^12 and rounded to f16, or for f32 activations split in two f16 terms (22 bits); P likewise, as 2^12 p
-// with v_scale[block] in its exponent or as a factor against the largest one so far, which keeps it in f16's range whatever the scales.  Products are summed in f32.
+// (bf16: 2^4 p) with v_scale[block] in its exponent, so that m is a maximum of p v_scale and P in f16's range whatever the scales.  Products are summed in f32.
 #pragma once
 
 #include "maya_kv.cuh"
@@ -48,7 +48,8 @@ struct AttnView {
 constexpr size_t kAttnHead = 256, kAttnPre = 2048;
 constexpr int kCtasMost = 448;                   // thread blocks that share out the work: three an SM
 constexpr int kPartRows = 2 * kCtasMost * 64;      // rows of parts
-constexpr float kVsLeast = 1e-30f;               // a value scale of 0 is this in P's exponent: P is 0 in f16 and right in l
+constexpr float kVsLeast = 1e-30f;               // bf16: a value scale of 0 is this in P's exponent, and so is one below it (off by 127e-30 at most): l stays in f32's range
+constexpr uint32_t kVsExpLeast = 127 - 64;       // f32: 2^-64, the exponent alone; what is below it is in the factor, in full for scales down to 2^-79
 // The join of the pieces' parts (kv_attn.cu), `rows` rows a tile.
 int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, int rows, cudaStream_t s);
 constexpr int kNotTaken = 1;

@@ -166,3 +166,46 @@ def test_append_of_the_smallest_values(cuda, size):
         zero = api.KvCache.empty(1, 1, dim, T.zeros((1, 1), dtype=T.int32, device="cuda"))
         api.KvAttention(zero, 1).append(api.AttnBatch.of([new], [new]), d, 0 * d, 0 * d, api.Rope())
         assert float(zero.v_scale) == 0 and (unpack(zero)[1][0, 0, :new] == 0).all()
+
+
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("bf16,seqs,new,length", [(False, 1, 1, 4 * BLOCK), (False, 300, 1, 40 * BLOCK), (False, 300, 20, 40 * BLOCK), (True, 300, 1, 40 * BLOCK), (True, 1, 130, 40 * BLOCK)])
+def test_value_scales_far_apart(cuda, bf16, seqs, new, length, order):
+    """Rows whose weight lies on blocks of small values, beside blocks of values up to 1e15 times as large that they hardly see: off by what P's bits (22 or 11) and
+    the scores' error make of sum p |v|, and by what f16 drops of a P 2^-36 (f32; 2^-28 in bf16) of the largest p * value scale - not by a part of the largest value."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(67)
+    cache, host = make_cache(T, rng, [length], 1, 64)
+    x = rng.standard_normal((1, 1, 64)).repeat(seqs * new, 0)
+    x *= rng.uniform(0.9, 1.1, (seqs * new, 1, 1))
+    q = T.from_numpy(x.astype(np.float32)).to(T.bfloat16 if bf16 else T.float32)
+    x = q.double().numpy()
+    blocks = host["table"][0, :length // BLOCK]
+    toward = np.where(x[0, 0] > 0, 1, -1)
+    lift = np.linspace(0, 1, len(blocks))[::order]                            # scores from 0 to 60, value scales from 1 down to 1e-15
+    for b, f in zip(blocks, lift):
+        host["k"][b, 0] = 128 + np.round(toward * rng.uniform(60, 127, (BLOCK, 64)))
+        host["ks"][b] = 60 * f / (0.125 * np.abs(x[0, 0]).sum() * 94)
+        host["vs"][b] = 10.0 ** (-15 * f)
+    raw = host["k"].reshape(*host["k"].shape[:3], 1, 64).transpose(0, 1, 3, 2, 4)
+    cache.k.copy_(T.from_numpy(np.ascontiguousarray(raw).astype(np.uint8)))
+    cache.k_scale.copy_(T.from_numpy(host["ks"]))
+    cache.v_scale.copy_(T.from_numpy(host["vs"]))
+    cache = api.KvCache(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table.repeat(seqs, 1), cache.k_sum)      # (every sequence reads the same blocks)
+    out, lse = attend(T, cache, [new] * seqs, [length] * seqs, q.cuda())
+    vs = host["vs"][blocks].astype(np.float64).repeat(BLOCK)
+    k = ((host["k"][blocks, 0] - 128) * host["ks"][blocks].astype(np.float64)[..., None]).reshape(-1, 64)
+    v = ((host["v"][blocks, 0] - 128) * host["vs"][blocks].astype(np.float64)[..., None]).reshape(-1, 64)
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    for i in range(0, seqs * new, 1 + seqs * new // 100):
+        n = length - new + i % new + 1
+        z = 0.125 * (k[:n] @ x[i, 0])
+        p = np.exp(z - z.max())
+        ref_lse = z.max() + np.log(p.sum())
+        p /= p.sum()
+        want, A = p @ v[:n], 0.125 * (np.abs(k[:n]) @ np.abs(x[i, 0])).max()
+        tol = (2 * 2.0 ** -20 * A + 2.0 ** -19 + (2.0 ** -11 if bf16 else 0)) * (p @ np.abs(v[:n]))
+        tol = tol + (2.0 ** -28 if bf16 else 2.0 ** -36) * (p * vs[:n]).max() * 127 * n + (2.0 ** -8 * np.abs(want) if bf16 else 0)
+        assert (np.abs(got[i, 0] - want) <= tol).all(), (i, (np.abs(got[i, 0] - want) / tol).max())
+        assert abs(got_lse[i, 0] - ref_lse) <= 2 * 2.0 ** -20 * A + 2.0 ** -19 + 2.0 ** -22 * abs(ref_lse)
