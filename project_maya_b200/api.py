@@ -647,6 +647,7 @@ class KvCache:
         assert k_sum is None or k_sum.dtype == torch.int16
         self.k, self.v, self.k_scale, self.v_scale, self.table, self.k_sum = k, v, k_scale, v_scale, table, k_sum
         self.n_blocks, self.n_kv, self.head_dim, self.n_seq = n_blocks, n_kv, head_dim, table.shape[0]
+        self.block_values = KV_BLOCK * n_kv * head_dim
         self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), _ptr(k_sum), _ptr(table), table.shape[1], n_blocks, n_kv,
                                 head_dim)
         self._ref = C.byref(self.desc)
@@ -671,7 +672,7 @@ class KvCache:
         if mean is None and self.k_sum is not None:
             mean = torch.empty((n, self.n_kv, self.head_dim), dtype=dtype, device=dev)
         assert k.dtype == v.dtype and (mean is None or mean.dtype == k.dtype) and k.dtype in (torch.float32, torch.bfloat16)
-        assert k.shape == v.shape == (n, KV_BLOCK, self.n_kv, self.head_dim) and (mean is None or mean.shape == (n, self.n_kv, self.head_dim))
+        assert k.numel() == v.numel() == n * self.block_values and (mean is None or mean.numel() == n * self.block_values // KV_BLOCK)
         assert blocks.dtype == torch.int32 and (counts is None or (counts.dtype == torch.int32 and counts.numel() == n))
         _check("kv_read", _lib.load().maya_kv_read(self._ref, _ptr(blocks), _ptr(counts), n, int(k.dtype == torch.bfloat16), _ptr(k), _ptr(v),
                                                    _ptr(mean), _stream(stream)))
@@ -710,8 +711,11 @@ class Rope:
         assert (cos is None) == (sin is None) and (cos is None or cos.shape == sin.shape)
         n_pos, rot_dim = (cos.shape[0], 2 * cos.shape[1]) if cos is not None else (0, 0)
         self._keep = cos, sin, q_w, k_w
-        self.weight_sizes = tuple(t.numel() for t in (q_w, k_w) if t is not None)
+        sizes = {t.numel() for t in (q_w, k_w) if t is not None}
+        assert len(sizes) < 2, "norm weights of two head sizes"
+        self.head_dim = sizes.pop() if sizes else None       # that the weights are for
         self.args = RopeArgs(q_w=_ptr(q_w), k_w=_ptr(k_w), eps=eps, cos=_ptr(cos), sin=_ptr(sin), n_pos=n_pos, rot_dim=rot_dim, pairs=int(pairs))
+        self.image = bytes(self.args)                       # what a call starts from
 
 
 def _rows(x, n: int, heads: int, head_dim: int):
@@ -741,6 +745,7 @@ class KvAttention:
         self._attn = AttnArgs(None, 0, 0, n_q, cache.head_dim ** -0.5 if scale is None else scale, window, None, 0, None, None)
         self._select = SelectArgs(None, 0, 0, n_q, n_first, n_last, n_sel, None)
         self._rope = RopeArgs()
+        self._rope_bytes = memoryview(self._rope).cast("B")
         self._refs = C.byref(self._attn), C.byref(self._select), C.byref(self._rope)
 
     def _queries(self, a, batch, q):
@@ -756,8 +761,8 @@ class KvAttention:
         """Returns the normalised and rotated queries.  k and v None: queries only.  pos i32 [n_tokens]: rows of cos and sin to turn by
         (None: the tokens' positions)."""
         a, c, n = self._rope, self.cache, batch.n_tokens
-        assert all(size == c.head_dim for size in rope.weight_sizes), "norm weights [head_dim] expected"
-        C.memmove(self._refs[2], C.byref(rope.args), C.sizeof(RopeArgs))
+        assert rope.head_dim is None or rope.head_dim == c.head_dim, "norm weights [head_dim] expected"
+        self._rope_bytes[:] = rope.image
         dtype = self._queries(a, batch, q)
         a.n_q = self.n_q
         if k is not None:

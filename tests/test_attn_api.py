@@ -18,7 +18,7 @@ def cache(api):
 def test_read_refuses_outputs_of_another_size(api, cache):
     """They are written in full: one too short would be written beyond its end."""
     blocks, right = T.arange(3, dtype=T.int32), dict(k=(3, 64, 2, 128), v=(3, 64, 2, 128), mean=(3, 2, 128))
-    for name, shapes in (("k", ((2, 64, 2, 128), (3, 64, 1, 128), (3, 64, 2, 64), (3 * 64 * 2 * 128,))), ("v", ((2, 64, 2, 128), (3, 32, 2, 128))),
+    for name, shapes in (("k", ((2, 64, 2, 128), (3, 64, 1, 128), (3, 64, 2, 64))), ("v", ((2, 64, 2, 128), (3, 32, 2, 128))),
                          ("mean", ((2, 2, 128), (3, 128), (3, 2, 64)))):
         for shape in shapes:
             out = {n: T.empty(shape if n == name else s, dtype=T.bfloat16) for n, s in right.items()}
