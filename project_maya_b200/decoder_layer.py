@@ -30,6 +30,10 @@ class AttentionConfig:
     eps: float = 1e-6
     n_sel: int = 0                       # blocks a token reads in a long context; 0: all of them always
     sparse_from: int = 8192              # tokens of context from which on single tokens read selected blocks
+    rows: torch.dtype = torch.float32    # of queries, keys, values and outputs between the products: f32 (P in 22 bits), or bf16 (P in 11; prompts on tcgen05)
+
+    def __post_init__(self):
+        assert self.rows in (torch.float32, torch.bfloat16)
 
     @property
     def qkv_rows(self) -> int:
@@ -73,9 +77,7 @@ class DecoderLayer:
         afterwards."""
         c, T = self.cfg, h.shape[0]
         rows = self._product(self.w_qkv, self._rms(h, self.norms["in"]), c.qkv_rows).view(T, -1, c.head_dim)
-        if T > api.MAX_COLS:                 # a prompt's rows: 16 bits and the tensor cores' rate (f32 rows keep 22 bits of P, at a quarter of it)
-            rows = rows.bfloat16()
-        q, k, v = rows.split((c.n_q, c.n_kv, c.n_kv), 1)
+        q, k, v = rows.to(c.rows).split((c.n_q, c.n_kv, c.n_kv), 1)
         q = self.attn.append(batch, q, k, v, self.rope)
         sparse = c.n_sel > 0 and batch.desc.max_new == 1 and batch.desc.max_len >= c.sparse_from
         out = self.attn.forward(batch, q, sel=self.attn.select(batch, q) if sparse else None)
@@ -119,7 +121,7 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=64, help="tokens decoded after it")
     ap.add_argument("--long", action="store_true", help="tokens read 32 selected blocks from 2048 tokens of context on")
     a = ap.parse_args()
-    cfg = AttentionConfig(4096, 32, 8, 128, n_sel=32 if a.long else 0, sparse_from=2048)
+    cfg = AttentionConfig(4096, 32, 8, 128, n_sel=32 if a.long else 0, sparse_from=2048, rows=torch.bfloat16)
     moe = api.MoeLayerConfig(4096, 1536, 64, 8, api.Q4_K, api.Q4_K)
     layer = synthetic_layer(cfg, moe, a.tokens + a.steps, max(a.tokens, 32))
     h = torch.randn((a.tokens + a.steps, cfg.n_embd), device="cuda")
