@@ -209,3 +209,65 @@ def test_value_scales_far_apart(cuda, bf16, seqs, new, length, order):
         tol = tol + (2.0 ** -28 if bf16 else 2.0 ** -36) * (p * vs[:n]).max() * 127 * n + (2.0 ** -8 * np.abs(want) if bf16 else 0)
         assert (np.abs(got[i, 0] - want) <= tol).all(), (i, (np.abs(got[i, 0] - want) / tol).max())
         assert abs(got_lse[i, 0] - ref_lse) <= 2 * 2.0 ** -20 * A + 2.0 ** -19 + 2.0 ** -22 * abs(ref_lse)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("new,lens,pairs", [([1, 1], [30, 70], False), ([9, 70], [9, 200], True)])
+def test_append_with_positions_of_its_own(cuda, new, lens, pairs, bf16):
+    """Rows of cos and sin by `pos`, in any order; those outside the table take the nearest."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(68)
+    N, H, n_kv, dim = sum(new), 4, 2, 128
+    cache, _ = make_cache(T, rng, lens, n_kv, dim)
+    pos = rng.permutation(300)[:N].astype(np.int32) - 40
+    pos[0], pos[-1] = 10 ** 9, -10 ** 9
+    angle = np.arange(200)[:, None] * 100.0 ** (-np.arange(32) / 32)
+    cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+    q, k, v = (T.from_numpy(rng.standard_normal((N, heads, dim)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32) for heads in (H, n_kv, n_kv))
+    got = api.KvAttention(cache, H).append(api.AttnBatch.of(new, lens), q.cuda(), k.cuda(), v.cuda(), api.Rope(T.from_numpy(cos).cuda(), T.from_numpy(sin).cuda(), pairs=pairs),
+                                           pos=T.from_numpy(pos).cuda()).double().cpu().numpy()
+    turn = np.clip(pos, 0, 199)
+    want = plain_rows(q.double().numpy(), None, cos, sin, turn, 0, pairs)
+    assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want).max(-1, keepdims=True) + (2.0 ** -8 * np.abs(want) if bf16 else 0)).all()
+    keys = plain_rows(k.double().numpy(), None, cos, sin, turn, 0, pairs)
+    codes, scale = unpack(cache)[0], cache.k_scale.double().cpu().numpy()
+    table, row = cache.table.cpu().numpy(), 0
+    for s, (m, n) in enumerate(zip(new, lens)):
+        for i in range(m):
+            at = n - m + i
+            b = table[s, at // BLOCK]
+            assert (np.abs(codes[b, :, at % BLOCK] * scale[b][:, None] - keys[row + i]) <= scale[b][:, None] * (0.5 + 127 * 2.0 ** -19)).all()
+        row += m
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_append_of_queries_alone_and_in_place(cuda, bf16):
+    """Without keys and values the cache keeps every byte; queries may be turned where they lie."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(69)
+    for new, lens in (([3, 1], [40, 130]), ([200, 9], [200, 70])):
+        cache, _ = make_cache(T, rng, lens, 2, 64)
+        N, H = sum(new), 6
+        held = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_sum)]
+        q = T.from_numpy(rng.standard_normal((N, H, 64)).astype(np.float32)).to(T.bfloat16 if bf16 else T.float32).cuda()
+        angle = T.arange(300, device="cuda")[:, None] * 100.0 ** (-T.arange(32, device="cuda") / 32)
+        rope = api.Rope(angle.cos(), angle.sin(), q_w=T.rand(64, device="cuda"))
+        attn, batch = api.KvAttention(cache, H), api.AttnBatch.of(new, lens)
+        out = attn.append(batch, q, None, None, rope)
+        assert attn.append(batch, q, None, None, rope, q_out=q) is q and T.equal(q, out)
+        assert all(T.equal(a, b) for a, b in zip(held, (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_sum)))
+
+
+def test_calls_after_an_error_are_sound(cuda):
+    """The error word and counters as a launch that gave up would leave them (set here by the host)."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(70)
+    cache, _ = make_cache(T, rng, [20000], 1, 64)
+    q, attn, batch = T.randn((1, 2, 64), device="cuda"), api.KvAttention(cache, 2), api.AttnBatch.of([1], [20000])
+    want = attn.forward(batch, q)
+    attn.scratch[:32].view(T.int32).copy_(T.tensor([1, 0, 0, 0, 3, 5, 0, 0]))
+    assert attn.error() == 1 and attn.error() == 0
+    assert T.equal(attn.forward(batch, q), want) and attn.error() == 0
