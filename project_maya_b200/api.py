@@ -682,11 +682,11 @@ class KvCache:
 class AttnBatch:
     """The new tokens of a pass: those of sequence s are rows start[s] .. start[s + 1] - 1 (i32 [n_seq + 1]) and the last of its
     kv_len[s] tokens (i32 [n_seq]; it counts them).  n_tokens = start[n_seq]; max_new and max_len: upper bounds of the new tokens and
-    of kv_len of any sequence, which size the launches."""
+    of kv_len of any sequence, which size the launches; min_len: a lower bound of kv_len of those that have new tokens."""
 
-    def __init__(self, start, kv_len, n_tokens: int, max_new: int, max_len: int):
+    def __init__(self, start, kv_len, n_tokens: int, max_new: int, max_len: int, min_len: int = 0):
         assert start.dtype == kv_len.dtype == torch.int32 and start.numel() == kv_len.numel() + 1
-        self.start, self.kv_len, self.n_tokens, self.n_seq = start, kv_len, n_tokens, kv_len.numel()
+        self.start, self.kv_len, self.n_tokens, self.n_seq, self.min_len = start, kv_len, n_tokens, kv_len.numel(), min_len
         self.desc = AttnBatchDesc(_ptr(start), _ptr(kv_len), kv_len.numel(), n_tokens, max_new, max_len)
         self._ref = C.byref(self.desc)
 
@@ -697,7 +697,7 @@ class AttnBatch:
         for n in new:
             start.append(start[-1] + n)
         return cls(torch.tensor(start, dtype=torch.int32, device=device), torch.tensor(list(kv_len), dtype=torch.int32, device=device),
-                   start[-1], max(new, default=0), max(kv_len, default=0))
+                   start[-1], max(new, default=0), max(kv_len, default=0), min((n for m, n in zip(new, kv_len) if m), default=0))
 
 
 class Rope:

@@ -5,7 +5,7 @@
 runs one layer of random weights over a prompt and then token by token, and prints what each half takes.
 
     h -> RMS norm -> q8_1 -> [q | k | v] rows (GGUF product) -> norms of the heads, rotation, cache append
-      -> attention (over the blocks that select() chooses, for single tokens of contexts beyond `sparse_from`) -> output rows (GGUF product)
+      -> attention (over the blocks that select() chooses, for single tokens of contexts of `sparse_from` tokens and more) -> output rows (GGUF product)
     h + attention -> RMS norm, router logits -> experts -> h
 """
 from __future__ import annotations
@@ -29,7 +29,7 @@ class AttentionConfig:
     theta: float = 10000.0
     eps: float = 1e-6
     n_sel: int = 0                       # blocks a token reads in a long context; 0: all of them always
-    sparse_from: int = 8192              # tokens of context from which on single tokens read selected blocks
+    sparse_from: int = 8192              # tokens of its own context from which on a sequence's single token reads selected blocks
     rows: torch.dtype = torch.float32    # of queries, keys, values and outputs between the products: f32 (P in 22 bits), or bf16 (P in 11; prompts on tcgen05)
 
     def __post_init__(self):
@@ -78,10 +78,21 @@ class DecoderLayer:
         c, T = self.cfg, h.shape[0]
         rows = self._product(self.w_qkv, self._rms(h, self.norms["in"]), c.qkv_rows).view(T, -1, c.head_dim)
         q, k, v = rows.to(c.rows).split((c.n_q, c.n_kv, c.n_kv), 1)
-        q = self.attn.append(batch, q, k, v, self.rope)
-        sparse = c.n_sel > 0 and batch.desc.max_new == 1 and batch.desc.max_len >= c.sparse_from
-        out = self.attn.forward(batch, q, sel=self.attn.select(batch, q) if sparse else None)
+        out = self._attend(batch, self.attn.append(batch, q, k, v, self.rope))
         return self._product(self.w_o, out.view(T, -1).float(), c.n_embd)
+
+    def _attend(self, batch: api.AttnBatch, q):
+        """Attention over every block, or over selected ones for the single tokens of contexts of `sparse_from` tokens and more."""
+        c, b = self.cfg, batch.desc
+        if c.n_sel == 0 or b.max_new > 1 or b.max_len < c.sparse_from:
+            return self.attn.forward(batch, q)
+        if batch.min_len >= c.sparse_from:
+            return self.attn.forward(batch, q, sel=self.attn.select(batch, q))
+        # Lengths on both sides, or not known here: a pass for each side in which the other's sequences have no tokens, whose rows are zeros then.
+        long = batch.kv_len >= c.sparse_from
+        far = api.AttnBatch(batch.start, torch.where(long, batch.kv_len, 0), b.n_tokens, 1, b.max_len)
+        near = api.AttnBatch(batch.start, torch.where(long, 0, batch.kv_len), b.n_tokens, 1, c.sparse_from - 1)
+        return self.attn.forward(far, q, sel=self.attn.select(far, q)) + self.attn.forward(near, q)
 
     def forward(self, h, batch: api.AttnBatch):
         a = self.attention(h, batch)

@@ -90,3 +90,29 @@ def test_layer_with_selected_blocks(cuda):
         outs.append(layer.attention(h[399:], api.AttnBatch.of([1], [400])).double().cpu().numpy())
     assert rel(outs[1], outs[0]) < 1e-3                                        # (sums in another order, rounded to 8 bits once more)
     assert 1e-3 < rel(outs[2], outs[0]) < 1.0
+
+
+def test_short_contexts_beside_long_ones_read_every_block(cuda):
+    """A batch of a context beyond `sparse_from` and one below it: the short one's token is what it is without selection, the long one's what it is alone."""
+    import torch as T
+    from project_maya_b200 import api, decoder_layer as L
+    T.manual_seed(8)
+    lens = (400, 330)
+    h = [T.randn((n, 512), device="cuda") for n in lens]
+
+    def run(n_sel, which, batch_of=api.AttnBatch.of):
+        cfg = L.AttentionConfig(512, 8, 2, 64, n_sel=n_sel, sparse_from=350)
+        layer = L.synthetic_layer(cfg, api.MoeLayerConfig(512, 256, 8, 2, api.Q8_0, api.Q8_0), 400, 512, n_seq=2)
+        layer.attention(T.cat([x[:-1] for x in h]), api.AttnBatch.of([n - 1 for n in lens], [n - 1 for n in lens]))
+        out = layer.attention(T.cat([h[i][-1:] for i in which]), batch_of([int(i in which) for i in (0, 1)], lens))
+        assert layer.attn.error() == 0
+        return out.double().cpu().numpy()
+
+    def bounds_alone(new, kv_len):                                             # as a graph's batch: lengths on the device, a bound on the host
+        b = api.AttnBatch.of(new, kv_len)
+        return api.AttnBatch(b.start, b.kv_len, b.n_tokens, 1, 400)
+
+    both, dense, alone = run(4, (0, 1)), run(0, (0, 1)), run(4, (0,))
+    assert rel(both[1], dense[1]) < 1e-3 and rel(both[0], alone[0]) < 1e-3     # (sums in another order, rounded to 8 bits once more)
+    assert rel(both[0], dense[0]) > 1e-3
+    assert rel(run(4, (0, 1), bounds_alone), both) < 1e-3
