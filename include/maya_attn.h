@@ -105,7 +105,7 @@ typedef struct maya_attn_args {
 /* out = sum_j softmax(scale * q . k_j)_j v_j over the tokens j of the sequence that stand at or before the query's own position,
  * within `window` and within the selected blocks; a row that sees nothing is 0.  A query with a NaN or an infinity gives a row of NaN
  * (and NaN in lse) wherever it sees a token.  bf16: value scales below 1e-30 count as 1e-30.  The cache holds the new tokens' keys and values already.
- * scratch: maya_attn_scratch_bytes(...) bytes, 256-byte aligned, zeroed before the first use and after a call that left its
+ * scratch: maya_attn_scratch_bytes(...) bytes (the same for any max_tokens > 0: parts have room of their own), 256-byte aligned, zeroed before the first use and after a call that left its
  * error word set; one buffer serves one stream at a time. */
 MAYA_API size_t maya_attn_scratch_bytes(const maya_kv_cache* cache, int n_q, int max_tokens);
 MAYA_API int maya_attn_q8(const maya_kv_cache* cache, const maya_attn_batch* batch, const maya_attn_args* a, void* scratch,

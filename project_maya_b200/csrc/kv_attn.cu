@@ -200,158 +200,144 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
     unsigned u_put = 0, put_phase = 0, get_phase = 0;                            // pieces this ring has asked for; the phases of
     int put_slot = 0, get_slot = 0;                                              // the slots that the next one goes into, and is taken from
     bool ok = true;
-    Tile T;
-    int tile = 0, h = 0;
-    constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
-    float qx[U][V];
-    auto ask_rows = [&](int r4) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int row = T.r0 + r4 + u * kWarps;
-#pragma unroll
-            for (int e = 0; e < V; ++e) qx[u][e] = 0.0f;
-            if (row < T.n_rows)
-                ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
-        }
-    };
     // ---- one piece after the other: the thread block's own number first, then whichever is next
     for (unsigned unit = blockIdx.x;;) {
-    if (!A.direct && unit >= units) break;
-    unsigned next = 0xffffffffu, pieces = 1, piece = 0;
-    if (tid == 0 && !A.direct) next = gridDim.x + atomicAdd(A.taken, 1u);        // (its number arrives meanwhile)
-    int tile, h;
-    if (A.direct) {
-        tile = (int) (unit / (unsigned) C.n_kv);
-        h = (int) (unit % (unsigned) C.n_kv);
-    } else {
-        unsigned in;
-        if (A.sel != nullptr) {
-            pieces = units / ((unsigned) A.tiles * (unsigned) C.n_kv);
-            tile = (int) (unit / (pieces * (unsigned) C.n_kv));
-            in = unit % (pieces * (unsigned) C.n_kv);
+        if (!A.direct && unit >= units) break;
+        unsigned next = 0xffffffffu, pieces = 1, piece = 0;
+        if (tid == 0 && !A.direct) next = gridDim.x + atomicAdd(A.taken, 1u);        // (its number arrives meanwhile)
+        int tile, h;
+        if (A.direct) {
+            tile = (int) (unit / (unsigned) C.n_kv);
+            h = (int) (unit % (unsigned) C.n_kv);
         } else {
-            int lo = 0, hi = A.tiles - 1;                                        // the last tile whose first piece is not behind it
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if ((unsigned) pre[mid] * (unsigned) C.n_kv <= unit) lo = mid; else hi = mid - 1;
+            unsigned in;
+            if (A.sel != nullptr) {
+                pieces = units / ((unsigned) A.tiles * (unsigned) C.n_kv);
+                tile = (int) (unit / (pieces * (unsigned) C.n_kv));
+                in = unit % (pieces * (unsigned) C.n_kv);
+            } else {
+                int lo = 0, hi = A.tiles - 1;                                        // the last tile whose first piece is not behind it
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if ((unsigned) pre[mid] * (unsigned) C.n_kv <= unit) lo = mid; else hi = mid - 1;
+                }
+                tile = lo;
+                pieces = (unsigned) (pre[lo + 1] - pre[lo]);
+                in = unit - (unsigned) pre[lo] * (unsigned) C.n_kv;
             }
-            tile = lo;
-            pieces = (unsigned) (pre[lo + 1] - pre[lo]);
-            in = unit - (unsigned) pre[lo] * (unsigned) C.n_kv;
+            h = (int) (in / pieces);
+            piece = in % pieces;
         }
-        h = (int) (in / pieces);
-        piece = in % pieces;
-    }
-    const Tile T = tile_of(B, A, tile, K::rows);
-    const unsigned base = (unsigned) T.n_blocks / pieces, rest = (unsigned) T.n_blocks % pieces;
-    const int w0 = (int) (piece * base + min(piece, rest)), w1 = w0 + (int) (base + (piece < rest ? 1u : 0u));
-    constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
-    float qx[U][V];
-    auto ask_rows = [&](int r4) {
+        const Tile T = tile_of(B, A, tile, K::rows);
+        const unsigned base = (unsigned) T.n_blocks / pieces, rest = (unsigned) T.n_blocks % pieces;
+        const int w0 = (int) (piece * base + min(piece, rest)), w1 = w0 + (int) (base + (piece < rest ? 1u : 0u));
+        constexpr int U = K::rows / kWarps < 4 ? K::rows / kWarps : 4;               // query rows of a warp in flight
+        float qx[U][V];
+        auto ask_rows = [&](int r4) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int row = T.r0 + r4 + u * kWarps;
+            for (int u = 0; u < U; ++u) {
+                const int row = T.r0 + r4 + u * kWarps;
 #pragma unroll
-            for (int e = 0; e < V; ++e) qx[u][e] = 0.0f;
-            if (row < T.n_rows)
-                ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
+                for (int e = 0; e < V; ++e) qx[u][e] = 0.0f;
+                if (row < T.n_rows)
+                    ld_acts<!F32, V>(A.q, (size_t) (T.s.row + T.i0 + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D + lane * V, A.wide_q, qx[u]);
+            }
+        };
+        ask_rows(warp);                                                              // (in front of the copies, behind which they would have to wait)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[n][e] = kNone;
+                l[n][e] = 0.0f;
+                const int row = T.r0 + (rw * NT + n) * 8 + 2 * t + e;                // last visible position (rows beyond the tile's: all, not kept)
+                pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
+            }
         }
-    };
-    ask_rows(warp);                                                              // (in front of the copies, behind which they would have to wait)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            m[n][e] = kNone;
-            l[n][e] = 0.0f;
-            const int row = T.r0 + (rw * NT + n) * 8 + 2 * t + e;                // last visible position (rows beyond the tile's: all, not kept)
-            pos[n][e] = row < T.n_rows ? T.first + T.i0 + row / A.group : 0x3fffffff;
-        }
-    }
-    int low = min(pos[0][0], pos[0][1]);
-    if constexpr (NT == 2) low = min(low, min(pos[NT - 1][0], pos[NT - 1][1]));
-    const int wpos_lo = __reduce_min_sync(0xffffffffu, low);                     // over the warp's rows
-    const int wpos_hi = T.first + T.i0 + min(min(T.r0 + K::rows, T.n_rows) - 1, T.r0 + (rw + 1) * NT * 8 - 1) / A.group;
+        int low = min(pos[0][0], pos[0][1]);
+        if constexpr (NT == 2) low = min(low, min(pos[NT - 1][0], pos[NT - 1][1]));
+        const int wpos_lo = __reduce_min_sync(0xffffffffu, low);                     // over the warp's rows
+        const int wpos_hi = T.first + T.i0 + min(min(T.r0 + K::rows, T.n_rows) - 1, T.r0 + (rw + 1) * NT * 8 - 1) / A.group;
 
-    for (int c0 = w0; c0 < w1; c0 += kMeta) {
-        const int nc = min(kMeta, w1 - c0);
-        if (c0 > w0) __syncthreads();                                            // everybody is done with meta
-        if (lost) break;
-        for (int i = tid; i < nc; i += kThreads) {
-            const int lb = A.sel != nullptr ? T.n_rows > 0 ? A.sel[((size_t) (tile / A.row_tiles) * C.n_kv + h) * A.n_sel + c0 + i] : -1 : T.b_lo + c0 + i;
-            const int phys = lb >= 0 && T.pos_hi >= 0 && lb <= T.pos_hi / kKvBlock ? block_of(C, T.si, lb) : -1;
-            meta[i].lb = lb;
-            meta[i].bh = phys >= 0 ? phys * C.n_kv + h : -1;
-        }
-        __syncthreads();
+        for (int c0 = w0; c0 < w1; c0 += kMeta) {
+            const int nc = min(kMeta, w1 - c0);
+            if (c0 > w0) __syncthreads();                                            // everybody is done with meta
+            if (lost) break;
+            for (int i = tid; i < nc; i += kThreads) {
+                const int lb = A.sel != nullptr ? T.n_rows > 0 ? A.sel[((size_t) (tile / A.row_tiles) * C.n_kv + h) * A.n_sel + c0 + i] : -1 : T.b_lo + c0 + i;
+                const int phys = lb >= 0 && T.pos_hi >= 0 && lb <= T.pos_hi / kKvBlock ? block_of(C, T.si, lb) : -1;
+                meta[i].lb = lb;
+                meta[i].bh = phys >= 0 ? phys * C.n_kv + h : -1;
+            }
+            __syncthreads();
 
-        // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots
-        int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
-        const uint8_t* src = nullptr;                                            // the piece
-        auto ask = [&]() {                                                       // one piece, by the ring's first warp
-            if (put_at == 0) {
-                while (put < nc && meta[put].bh < 0) put += BW;
-                if (put < nc) src = C.k + (size_t) meta[put].bh * (P * kPiece);
+            // copies of this ring's blocks: the pieces of a block's keys, then of its values, as many ahead as there are slots
+            int put = bw, put_at = 0;                                                // next block to ask for, and its next piece
+            const uint8_t* src = nullptr;                                            // the piece
+            auto ask = [&]() {                                                       // one piece, by the ring's first warp
+                if (put_at == 0) {
+                    while (put < nc && meta[put].bh < 0) put += BW;
+                    if (put < nc) src = C.k + (size_t) meta[put].bh * (P * kPiece);
+                }
+                if (put >= nc) return;
+                if (RW > 1 && u_put >= K::slots && !mbar_wait(&empty[bw][put_slot], put_phase ^ 1u)) { ok = false; return; }
+                if (lane == 0) {
+                    mbar_expect_tx(&full[bw][put_slot], kPiece);
+                    bulk_load(ring + put_slot * kPiece, src, kPiece, &full[bw][put_slot]);
+                }
+                ++u_put;
+                if (++put_slot == K::slots) { put_slot = 0; put_phase ^= 1u; }
+                src += kPiece;
+                if (++put_at == P) src += C.v - C.k - P * kPiece;
+                if (put_at == 2 * P) { put_at = 0; put += BW; }
+            };
+            auto take = [&]() -> const uint8_t* {                                    // the ring's next piece, once it is there
+                if (!mbar_wait(&full[bw][get_slot], get_phase)) { ok = false; return nullptr; }
+                return ring + get_slot * kPiece;
+            };
+            auto leave = [&]() {                                                     // and its room for another
+                __syncwarp();
+                if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][get_slot]);
+                if (++get_slot == K::slots) { get_slot = 0; get_phase ^= 1u; }
+                if (rw == 0) ask();
+            };
+            if (rw == 0)
+                for (int i = 0; i < K::slots && ok; ++i) ask();
+            for (int i = tid; i < nc; i += kThreads) {                               // the scales, behind the first copies
+                const int bh = meta[i].bh;
+                meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
+                meta[i].vs = bh >= 0 ? C.v_scale[bh] : 0.0f;
             }
-            if (put >= nc) return;
-            if (RW > 1 && u_put >= K::slots && !mbar_wait(&empty[bw][put_slot], put_phase ^ 1u)) { ok = false; return; }
-            if (lane == 0) {
-                mbar_expect_tx(&full[bw][put_slot], kPiece);
-                bulk_load(ring + put_slot * kPiece, src, kPiece, &full[bw][put_slot]);
-            }
-            ++u_put;
-            if (++put_slot == K::slots) { put_slot = 0; put_phase ^= 1u; }
-            src += kPiece;
-            if (++put_at == P) src += C.v - C.k - P * kPiece;
-            if (put_at == 2 * P) { put_at = 0; put += BW; }
-        };
-        auto take = [&]() -> const uint8_t* {                                    // the ring's next piece, once it is there
-            if (!mbar_wait(&full[bw][get_slot], get_phase)) { ok = false; return nullptr; }
-            return ring + get_slot * kPiece;
-        };
-        auto leave = [&]() {                                                     // and its room for another
-            __syncwarp();
-            if (RW > 1 && lane == 0) mbar_arrive_one(&empty[bw][get_slot]);
-            if (++get_slot == K::slots) { get_slot = 0; get_phase ^= 1u; }
-            if (rw == 0) ask();
-        };
-        if (rw == 0)
-            for (int i = 0; i < K::slots && ok; ++i) ask();
-        for (int i = tid; i < nc; i += kThreads) {                               // the scales, behind the first copies
-            const int bh = meta[i].bh;
-            meta[i].ks = bh >= 0 ? C.k_scale[bh] : 0.0f;
-            meta[i].vs = bh >= 0 ? C.v_scale[bh] : 0.0f;
-        }
-        if (c0 == w0) {
-            // scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
-            for (int r4 = warp; r4 < K::rows; r4 += kWarps * U) {
-                if (r4 != warp) ask_rows(r4);
+            if (c0 == w0) {
+                // scaled by a power of two, rounded to f16 (f32: two terms), laid out as fragments
+                for (int r4 = warp; r4 < K::rows; r4 += kWarps * U) {
+                    if (r4 != warp) ask_rows(r4);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int r = r4 + u * kWarps;
-                    float amax = 0.0f;
+                    for (int u = 0; u < U; ++u) {
+                        const int r = r4 + u * kWarps;
+                        float amax = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
-                    amax = warp_max(amax);
-                    const int exp2_ = up_of_row(amax);   // amax * 2^e in [2^11, 2^12)
-                    const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
-                    if (lane == 0) qinv[r] = scale_of_row(amax, __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2);
+                        for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(qx[u][e]));
+                        amax = warp_max(amax);
+                        const int exp2_ = up_of_row(amax);   // amax * 2^e in [2^11, 2^12)
+                        const float up = __uint_as_float((uint32_t) (127 + exp2_) << 23);
+                        if (lane == 0) qinv[r] = scale_of_row(amax, __uint_as_float((uint32_t) (127 - exp2_) << 23) * A.scale_log2);
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
-                        uint8_t* f = desk + ((((r >> 3) * P + (d >> 6)) * 2 + (st >> 1)) * 32 + (r & 7) * 4 + tt) * 16 + ((st & 1) * 2 + (w >> 1)) * 4;
-                        const uint32_t hi = pack_half(qx[u][e] * up, qx[u][e + 1] * up);
-                        *(uint32_t*) f = hi;
-                        if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, qx[u][e] * up, qx[u][e + 1] * up);
+                        for (int e = 0; e < V; e += 2) {
+                            const int d = lane * V + e, dd = d & 63, tt = dd >> 4, st = (dd >> 2) & 3, w = dd & 3;
+                            uint8_t* f = desk + ((((r >> 3) * P + (d >> 6)) * 2 + (st >> 1)) * 32 + (r & 7) * 4 + tt) * 16 + ((st & 1) * 2 + (w >> 1)) * 4;
+                            const uint32_t hi = pack_half(qx[u][e] * up, qx[u][e + 1] * up);
+                            *(uint32_t*) f = hi;
+                            if constexpr (F32) *(uint32_t*) (f + K::frag) = pack_rest(hi, qx[u][e] * up, qx[u][e + 1] * up);
+                        }
                     }
                 }
             }
-        }
-        __syncthreads();
+            __syncthreads();
 
             for (int b = bw; b < nc && ok; b += BW) {
                 const Meta x = meta[b];
@@ -560,69 +546,69 @@ __global__ void __launch_bounds__(32 * NW, Cfg<D, F32, NT, RW, NW>::ctas) attn_k
                 if (!ok) break;
             }
             if (!ok) lost = 1;
-    }
+        }
 
-            // ---- the rings' results meet in the rings' memory (nothing is on its way into it), a thread four values of a row
+        // ---- the rings' results meet in the rings' memory (nothing is on its way into it), a thread four values of a row
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+        if (g == 0) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
+        }
+        __syncthreads();                                                     // every ring is empty
+        float* buf = (float*) smem;                                          // [warp][8 NT][wide]
 #pragma unroll
-                    for (int x = 4; x < 32; x *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-            if (g == 0) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) { sm_m[warp][n * 8 + 2 * t + e] = m[n][e]; sm_l[warp][n * 8 + 2 * t + e] = l[n][e]; }
+                for (int e = 0; e < 4; ++e) buf[((warp * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][i][e];
+        __syncthreads();
+        if (lost) break;
+        const bool whole = pieces == 1;
+        const size_t part_at = (size_t) unit * K::rows;
+        for (int i = tid; i < K::rows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = r % (8 * NT), x0 = r / (8 * NT);      // the row's warps: x0 + RW * b
+            if (T.r0 + r >= T.n_rows) break;
+            float mm = kNone, total = 0.0f;
+#pragma unroll
+            for (int b = 0; b < BW; ++b) mm = fmaxf(mm, sm_m[x0 + RW * b][rr]);
+            const float use = mm == kNone ? 0.0f : mm;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int b = 0; b < BW; ++b) {
+                const int x = x0 + RW * b;
+                const float f = ex2(sm_m[x][rr] - use);
+                total += sm_l[x][rr] * f;
+                const float4 z = *(const float4*) (buf + (x * 8 * NT + rr) * K::wide + d);
+                y.x += z.x * f; y.y += z.y * f; y.z += z.z * f; y.w += z.w * f;
             }
-            __syncthreads();                                                     // every ring is empty
-            float* buf = (float*) smem;                                          // [warp][8 NT][wide]
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) buf[((warp * NT + n) * 8 + 2 * t + (e & 1)) * K::wide + 16 * i + g + (e & 2) * 4] = o[n][i][e];
-            __syncthreads();
-            if (lost) break;
-            const bool whole = pieces == 1;
-            const size_t part_at = (size_t) unit * K::rows;
-            for (int i = tid; i < K::rows * (D / 4); i += kThreads) {
-                const int r = i / (D / 4), d = (i % (D / 4)) * 4, rr = r % (8 * NT), x0 = r / (8 * NT);      // the row's warps: x0 + RW * b
-                if (T.r0 + r >= T.n_rows) break;
-                float mm = kNone, total = 0.0f;
-#pragma unroll
-                for (int b = 0; b < BW; ++b) mm = fmaxf(mm, sm_m[x0 + RW * b][rr]);
-                const float use = mm == kNone ? 0.0f : mm;
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int b = 0; b < BW; ++b) {
-                    const int x = x0 + RW * b;
-                    const float f = ex2(sm_m[x][rr] - use);
-                    total += sm_l[x][rr] * f;
-                    const float4 z = *(const float4*) (buf + (x * 8 * NT + rr) * K::wide + d);
-                    y.x += z.x * f; y.y += z.y * f; y.z += z.z * f; y.w += z.w * f;
-                }
-                if (!whole) {
-                    *(float4*) (A.part_o + (part_at + r) * D + d) = y;
-                    if (d == 0) A.part_ml[part_at + r] = make_float2(mm, total);
-                    continue;
-                }
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
-                const size_t at = out_row(A, T, h, r);
-                if constexpr (F32) *(float4*) ((float*) A.out + at * D + d) = y;
-                else {
-                    const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-                    *(uint2*) ((uint16_t*) A.out + at * D + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
-                }
-                if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total, kBias<F32>);
+            if (!whole) {
+                *(float4*) (A.part_o + (part_at + r) * D + d) = y;
+                if (d == 0) A.part_ml[part_at + r] = make_float2(mm, total);
+                continue;
             }
-            fence_proxy_async();                                                 // the next copies write where this was read
-            if (A.direct) break;
-            if (tid == 0) upcoming = next;
-            __syncthreads();
-            unit = upcoming;
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+            const size_t at = out_row(A, T, h, r);
+            if constexpr (F32) *(float4*) ((float*) A.out + at * D + d) = y;
+            else {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+                *(uint2*) ((uint16_t*) A.out + at * D + d) = make_uint2(*(const uint32_t*) &a, *(const uint32_t*) &b);
+            }
+            if (d == 0 && A.lse != nullptr) A.lse[at] = lse_of(mm, total, kBias<F32>);
+        }
+        fence_proxy_async();                                                 // the next copies write where this was read
+        if (A.direct) break;
+        if (tid == 0) upcoming = next;
+        __syncthreads();
+        unit = upcoming;
     }
     if (!ok && rw == 0)                                                          // a copy that did not land in time: none may land after the end
         for (unsigned u = u_put > K::slots ? u_put - K::slots : 0; u < u_put; ++u) mbar_wait(&full[bw][u % K::slots], (u / K::slots) & 1);
@@ -730,7 +716,7 @@ int launch_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView
 }
 
 template<int D, bool F32, int NT, int RW, int NW = 4>
-int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, uint8_t* scratch, cudaStream_t s) {
+int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, AttnView A, cudaStream_t s) {
     using K = Cfg<D, F32, NT, RW, NW>;
     static_assert(K::slots >= 2, "a ring holds a piece in use and one on its way");
     const long long rows = a.sel ? A.group : (long long) b.max_new * A.group;
@@ -773,26 +759,25 @@ int launch_attn(const maya_kv_cache& c, const maya_attn_batch& b, const maya_att
 }
 
 template<int D, bool F32>
-int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, uint8_t* scratch, cudaStream_t s) {
+int by_rows(const maya_kv_cache& c, const maya_attn_batch& b, const maya_attn_args& a, const AttnView& A, cudaStream_t s) {
     const long long rows = (long long) (a.sel ? 1 : b.max_new) * (a.n_q / c.n_kv);
     // Lists of many tokens, 8 heads a group or fewer: a warp a (token, head), by itself - no barrier, nothing to meet - once there are enough of them to
     // fill the chip several times (a chunk of 4096 tokens, 4 key/value heads, 16 blocks each: four warps a list 608 us, one 515).
-    if (a.sel && rows <= 8 && (long long) b.n_tokens * c.n_kv >= 48ll * sm_count()) return launch_attn<D, F32, 1, 1, 1>(c, b, a, A, scratch, s);
-    if (rows <= 8) return launch_attn<D, F32, 1, 1>(c, b, a, A, scratch, s);
+    if (a.sel && rows <= 8 && (long long) b.n_tokens * c.n_kv >= 48ll * sm_count()) return launch_attn<D, F32, 1, 1, 1>(c, b, a, A, s);
+    if (rows <= 8) return launch_attn<D, F32, 1, 1>(c, b, a, A, s);
     if constexpr (D <= 128) {
-        if (rows <= 16) return launch_attn<D, F32, 2, 1>(c, b, a, A, scratch, s);
-        if (rows <= 32) return launch_attn<D, F32, 2, 2>(c, b, a, A, scratch, s);
-        return launch_attn<D, F32, 2, 4>(c, b, a, A, scratch, s);
+        if (rows <= 16) return launch_attn<D, F32, 2, 1>(c, b, a, A, s);
+        if (rows <= 32) return launch_attn<D, F32, 2, 2>(c, b, a, A, s);
+        return launch_attn<D, F32, 2, 4>(c, b, a, A, s);
     } else {                                                                     // (two columns of outputs of these sizes do not fit the registers)
-        if (rows <= 16) return launch_attn<D, F32, 1, 2>(c, b, a, A, scratch, s);
-        return launch_attn<D, F32, 1, 4>(c, b, a, A, scratch, s);
+        if (rows <= 16) return launch_attn<D, F32, 1, 2>(c, b, a, A, s);
+        return launch_attn<D, F32, 1, 4>(c, b, a, A, s);
     }
 }
 
 }  // namespace
 
-int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, int rows, cudaStream_t s) {
-    if (!bf16) return refuse(MAYA_ERR_ARG);
+int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, int rows, cudaStream_t s) {
     return c.head_dim == 64 ? launch_join<64, false>(c, b, A, rows, 1, s) : launch_join<128, false>(c, b, A, rows, 1, s);
 }
 
@@ -830,7 +815,7 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     A.part_o = (float*) (A.part_ml + kPartRows);
     st = attn_prompt(*c, *b, A, a->is_bf16 != 0, s);
     if (st != kNotTaken) return st;
-#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, (uint8_t*) scratch, s) : by_rows<D, true>(*c, *b, *a, A, (uint8_t*) scratch, s)
+#define ATTN(D) a->is_bf16 ? by_rows<D, false>(*c, *b, *a, A, s) : by_rows<D, true>(*c, *b, *a, A, s)
     switch (c->head_dim) {
         case 64: return ATTN(64);
         case 128: return ATTN(128);

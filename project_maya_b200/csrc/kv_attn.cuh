@@ -50,8 +50,8 @@ constexpr int kCtasMost = 448;                   // thread blocks that share out
 constexpr int kPartRows = 2 * kCtasMost * 64;      // rows of parts
 constexpr float kVsLeast = 1e-30f;               // bf16: a value scale of 0 is this in P's exponent, and so is one below it (off by 127e-30 at most): l stays in f32's range
 constexpr uint32_t kVsExpLeast = 127 - 64;       // f32: 2^-64, the exponent alone; what is below it is in the factor, in full for scales down to 2^-79
-// The join of the pieces' parts (kv_attn.cu), `rows` rows a tile.
-int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, int rows, cudaStream_t s);
+// The join of the prompt kernel's pieces (kv_attn.cu), `rows` rows a tile.
+int attn_join(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, int rows, cudaStream_t s);
 constexpr int kNotTaken = 1;
 // Attention of a prompt's rows on tcgen05 (kv_attn_prompt.cu); kNotTaken: not that kernel's call, nothing launched.
 int attn_prompt(const maya_kv_cache& c, const maya_attn_batch& b, const AttnView& A, bool bf16, cudaStream_t s);

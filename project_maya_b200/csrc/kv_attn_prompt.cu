@@ -167,86 +167,86 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp != kIssueWarp) {
-        // ================================================================ codes -> f16 operands
-        // A warp takes every seventh group of eight rows of a tile, a lane 16 codes of it: group u lies 1024 u bytes into the f16 tile, for keys
-        // (panel, block, tokens) and for values (block, values) alike.
-        constexpr int groups = 128 * D / 512, pieces = (groups + kExpandWarps - 1) / kExpandWarps;
-        const int cw = warp - 8, r8 = lane >> 2, c4 = lane & 3;
-        const uint32_t to0 = r8 * 128 + (((2 * c4) ^ r8) << 4), to1 = r8 * 128 + (((2 * c4 + 1) ^ r8) << 4);
-        int batch = -1;
-        int my_bh = -1, my_lb = -1;
-        float my_ks = 0.0f, my_vs = 0.0f;
-        auto look_up = [&](int b) {                                     // cache block b_lo + b of this range: 32 at a time, a lane each
-            if ((b >> 5) != batch) {
-                batch = b >> 5;
-                const int x = (batch << 5) + lane;
-                my_lb = x < n_blocks ? b_lo + x : -1;
-                const int phys = my_lb >= 0 ? block_of(C, si, my_lb) : -1;
-                my_bh = phys >= 0 ? phys * C.n_kv + h : -1;
-                my_ks = my_bh >= 0 ? C.k_scale[my_bh] : 0.0f;
-                my_vs = my_bh >= 0 ? C.v_scale[my_bh] : 0.0f;
-            }
-        };
-        uint4 cur[pieces], nxt[pieces];
-        int bh[2];                                                      // the step's blocks and head in the cache, -1: none
-        auto load = [&](uint4 (&w)[pieces], const uint8_t* cache, bool val) {
-            const uint8_t* src[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) src[x] = cache + (size_t) max(bh[x], 0) * (kKvBlock * D) + lane * 16;
-#pragma unroll
-            for (int i = 0; i < pieces; ++i) {
-                const int u = cw + i * kExpandWarps, x = val ? u / (D / 8) : (u >> 3) & 1;
-                const int at = val ? u % (D / 8) : (u >> 4) * 8 + (u & 7);                             // group of the block's 512-byte groups
-                w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (u < groups && (x == 0 ? bh[0] : bh[1]) >= 0) w[i] = *(const uint4*) ((x == 0 ? src[0] : src[1]) + at * 512);
-            }
-        };
-        auto store = [&](const uint4 (&w)[pieces], uint8_t* dst) {
-#pragma unroll
-            for (int i = 0; i < pieces; ++i) {
-                const int u = cw + i * kExpandWarps;
-                if (u >= groups) break;
-                uint32_t o[8];
-                codes_to_half(w[i].x, o[0], o[1]); codes_to_half(w[i].y, o[2], o[3]);
-                codes_to_half(w[i].z, o[4], o[5]); codes_to_half(w[i].w, o[6], o[7]);
-                *(uint4*) (dst + u * 1024 + to0) = make_uint4(o[0], o[1], o[2], o[3]);
-                *(uint4*) (dst + u * 1024 + to1) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-            fence_proxy_async();
-            __syncwarp();
-        };
-        auto find = [&](int j) {                                        // the step's two blocks
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                look_up(2 * j + x);
-                bh[x] = __shfl_sync(0xffffffffu, my_bh, (2 * j + x) & 31);
-            }
-            if (warp == 8 && ((2 * j) & 31) == (lane & 30)) {           // their numbers, from the two lanes that have them
-                StepMeta& m = meta[j % kMetaRing];
-                const float vs = fmaxf(my_vs, kVsLeast);
-                m.lb[lane & 1] = my_bh >= 0 ? my_lb : -1;
-                m.ks[lane & 1] = my_ks;
-                m.lv[lane & 1] = __log2f(vs);
-                m.ivs[lane & 1] = __fdividef(1.0f, vs);
-            }
-        };
-        if (here && steps > 0) {
-            find(0);
-            load(cur, C.k, false);
-            for (int j = 0; j < steps; ++j) {
-                load(nxt, C.v, true);                                         // this step's values, under the conversion of its keys
-                if (j >= 2 && !wait(&k_free[j & 1], ((j >> 1) - 1) & 1)) break;
-                store(cur, smem + K::k + (j & 1) * K::tile);
-                if (lane == 0) mbar_arrive_one(&k_full[j & 1]);
-                if (j + 1 < steps) {
-                    find(j + 1);
-                    load(cur, C.k, false);
+            // ================================================================ codes -> f16 operands
+            // A warp takes every seventh group of eight rows of a tile, a lane 16 codes of it: group u lies 1024 u bytes into the f16 tile, for keys
+            // (panel, block, tokens) and for values (block, values) alike.
+            constexpr int groups = 128 * D / 512, pieces = (groups + kExpandWarps - 1) / kExpandWarps;
+            const int cw = warp - 8, r8 = lane >> 2, c4 = lane & 3;
+            const uint32_t to0 = r8 * 128 + (((2 * c4) ^ r8) << 4), to1 = r8 * 128 + (((2 * c4 + 1) ^ r8) << 4);
+            int batch = -1;
+            int my_bh = -1, my_lb = -1;
+            float my_ks = 0.0f, my_vs = 0.0f;
+            auto look_up = [&](int b) {                                     // cache block b_lo + b of this range: 32 at a time, a lane each
+                if ((b >> 5) != batch) {
+                    batch = b >> 5;
+                    const int x = (batch << 5) + lane;
+                    my_lb = x < n_blocks ? b_lo + x : -1;
+                    const int phys = my_lb >= 0 ? block_of(C, si, my_lb) : -1;
+                    my_bh = phys >= 0 ? phys * C.n_kv + h : -1;
+                    my_ks = my_bh >= 0 ? C.k_scale[my_bh] : 0.0f;
+                    my_vs = my_bh >= 0 ? C.v_scale[my_bh] : 0.0f;
                 }
-                if (j >= 2 && !wait(&v_free[j & 1], ((j >> 1) - 1) & 1)) break;
-                store(nxt, smem + K::v + (j & 1) * K::tile);
-                if (lane == 0) mbar_arrive_one(&v_full[j & 1]);
+            };
+            uint4 cur[pieces], nxt[pieces];
+            int bh[2];                                                      // the step's blocks and head in the cache, -1: none
+            auto load = [&](uint4 (&w)[pieces], const uint8_t* cache, bool val) {
+                const uint8_t* src[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) src[x] = cache + (size_t) max(bh[x], 0) * (kKvBlock * D) + lane * 16;
+#pragma unroll
+                for (int i = 0; i < pieces; ++i) {
+                    const int u = cw + i * kExpandWarps, x = val ? u / (D / 8) : (u >> 3) & 1;
+                    const int at = val ? u % (D / 8) : (u >> 4) * 8 + (u & 7);                             // group of the block's 512-byte groups
+                    w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                    if (u < groups && (x == 0 ? bh[0] : bh[1]) >= 0) w[i] = *(const uint4*) ((x == 0 ? src[0] : src[1]) + at * 512);
+                }
+            };
+            auto store = [&](const uint4 (&w)[pieces], uint8_t* dst) {
+#pragma unroll
+                for (int i = 0; i < pieces; ++i) {
+                    const int u = cw + i * kExpandWarps;
+                    if (u >= groups) break;
+                    uint32_t o[8];
+                    codes_to_half(w[i].x, o[0], o[1]); codes_to_half(w[i].y, o[2], o[3]);
+                    codes_to_half(w[i].z, o[4], o[5]); codes_to_half(w[i].w, o[6], o[7]);
+                    *(uint4*) (dst + u * 1024 + to0) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *(uint4*) (dst + u * 1024 + to1) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+                fence_proxy_async();
+                __syncwarp();
+            };
+            auto find = [&](int j) {                                        // the step's two blocks
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    look_up(2 * j + x);
+                    bh[x] = __shfl_sync(0xffffffffu, my_bh, (2 * j + x) & 31);
+                }
+                if (warp == 8 && ((2 * j) & 31) == (lane & 30)) {           // their numbers, from the two lanes that have them
+                    StepMeta& m = meta[j % kMetaRing];
+                    const float vs = fmaxf(my_vs, kVsLeast);
+                    m.lb[lane & 1] = my_bh >= 0 ? my_lb : -1;
+                    m.ks[lane & 1] = my_ks;
+                    m.lv[lane & 1] = __log2f(vs);
+                    m.ivs[lane & 1] = __fdividef(1.0f, vs);
+                }
+            };
+            if (here && steps > 0) {
+                find(0);
+                load(cur, C.k, false);
+                for (int j = 0; j < steps; ++j) {
+                    load(nxt, C.v, true);                                         // this step's values, under the conversion of its keys
+                    if (j >= 2 && !wait(&k_free[j & 1], ((j >> 1) - 1) & 1)) break;
+                    store(cur, smem + K::k + (j & 1) * K::tile);
+                    if (lane == 0) mbar_arrive_one(&k_full[j & 1]);
+                    if (j + 1 < steps) {
+                        find(j + 1);
+                        load(cur, C.k, false);
+                    }
+                    if (j >= 2 && !wait(&v_free[j & 1], ((j >> 1) - 1) & 1)) break;
+                    store(nxt, smem + K::v + (j & 1) * K::tile);
+                    if (lane == 0) mbar_arrive_one(&v_full[j & 1]);
+                }
             }
-        }
         } else if (here) {
             // ================================================================ products
             const uint32_t base = smem_u32(smem);
@@ -261,8 +261,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
             };
             bool ok = steps == 0 || (wait(&k_full[0], 0) && wait(&q_ready[0], 0) && (tiles == 1 || wait(&q_ready[1], 0)));
             tc_fence_after();
-            if (ok && steps > 0)
-            {
+            if (ok && steps > 0) {
                 for (int x = 0; x < tiles; ++x) scores(x, 0);
                 mma_commit_elect(smem_u32(&s_full[0]));
             }
@@ -311,27 +310,27 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
                 if (row < n_rows) {
                     const uint16_t* src = (const uint16_t*) A.q + (size_t) (s.row + row / A.group) * A.ld_q + (size_t) (h * A.group + row % A.group) * D;
                     if (A.wide_q) {
-        #pragma unroll
+#pragma unroll
                         for (int i = 0; i < D / 8; ++i) *(uint4*) &w[4 * i] = ((const uint4*) src)[i];
                     } else {
-        #pragma unroll
+#pragma unroll
                         for (int i = 0; i < D / 2; ++i) w[i] = src[2 * i] | (uint32_t) src[2 * i + 1] << 16;
                     }
                 } else {
-        #pragma unroll
+#pragma unroll
                     for (int i = 0; i < D / 2; ++i) w[i] = 0u;
                 }
                 float amax = 0.0f;
-        #pragma unroll
+#pragma unroll
                 for (int i = 0; i < D / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
                 const int e2 = up_of_row(amax);    // amax * 2^e2 in [2^11, 2^12)
                 const float up = __uint_as_float((uint32_t) (127 + e2) << 23);
                 qinv = scale_of_row(amax, __uint_as_float((uint32_t) (127 - e2) << 23) * A.scale_log2);
-        #pragma unroll
+#pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
                     uint4 o;
                     uint32_t* ow = (uint32_t*) &o;
-        #pragma unroll
+#pragma unroll
                     for (int i = 0; i < 4; ++i) ow[i] = half2_of(__uint_as_float(w[4 * c + i] << 16) * up, __uint_as_float(w[4 * c + i] & 0xFFFF0000u) * up);
                     *(uint4*) (dst + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = o;
                 }
@@ -482,7 +481,7 @@ template<int D> int launch_prompt(const maya_kv_cache& c, const maya_attn_batch&
     launch_dependent(prompt_kernel<D>, dim3((unsigned) pairs, 1, (unsigned) cuts), dim3(kPThreads), PCfg<D>::smem, s, kv_view(c), batch_view(b), A);
     const int st = note_launch("attn_q8 prompt");
     if (st != MAYA_OK || cuts == 1) return st;
-    return attn_join(c, b, A, true, 256, s);
+    return attn_join(c, b, A, 256, s);
 }
 
 }  // namespace
