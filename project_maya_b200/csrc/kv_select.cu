@@ -32,7 +32,7 @@ struct SelView {
     int64_t ld_q;
     int n_q, group;
     int span_log2, tiles_per_token;              // heads of a tile of eight that are one token's: 1 .. 8; tiles of a token of more than 8 heads, else 1
-    int tokens, tiles;                           // of a thread block; tiles of eight heads they fill
+    int tokens, tiles, room;                     // of a thread block; tiles of eight heads they fill; tokens those have room for
     int token_tiles;                             // thread blocks (clusters) of a sequence
     int n_first, n_last, n_sel, ld_keys, wide_q;
     int* sel;
@@ -164,8 +164,8 @@ template<int D, bool BF16>
 __global__ void __launch_bounds__(kSelThreads, D <= 128 ? 2 : 1) select_kernel(const KvView C, const BatchView B, const SelView S) {
     constexpr int ST = D / 16;
     extern __shared__ __align__(16) uint8_t smem[];
-    uint32_t* keys = (uint32_t*) smem;                                    // [tokens][ld_keys]
-    uint8_t* frag = smem + (size_t) S.tokens * S.ld_keys * 4;           // [tiles][ST / 2][kFrag]: f16
+    uint32_t* keys = (uint32_t*) smem;                                    // [tokens the tiles have room for][ld_keys]
+    uint8_t* frag = smem + (size_t) S.room * S.ld_keys * 4;             // [tiles][ST / 2][kFrag]: f16
     float* qs = (float*) (frag + (size_t) S.tiles * (ST / 2) * kFrag);            // [tiles * 8]; NaN: no row
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
@@ -269,7 +269,6 @@ __global__ void __launch_bounds__(kSelThreads, D <= 128 ? 2 : 1) select_kernel(c
             look_up(b16 + stride);
             int part = 0;                                                 // the tile among its token's
             float m0 = -INFINITY, m1 = -INFINITY;                         // the maxima over a token's tiles so far
-            int left = n_tok - (span == 4 ? t1 : span == 2 ? t : 2 * t);  // tokens from the lane's own on (the last tile may have none for some lanes)
 #pragma unroll 2
             for (int tile = 0; tile < S.tiles; ++tile) {
                 float ch[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cl[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -300,27 +299,18 @@ __global__ void __launch_bounds__(kSelThreads, D <= 128 ? 2 : 1) select_kernel(c
                     }
                 } else if constexpr (span == 4) {
                     const float v0 = fmaxf(s00, s01), v1 = fmaxf(s10, s11), v = meet(t0 ? v1 : v0, t0 ? v0 : v1, 1);
-                    if (left > 0) row[t1 * S.ld_keys + 8 * t0] = key_of(__fmul_rn(v, t0 ? ks1 : ks0));
+                    row[t1 * S.ld_keys + 8 * t0] = key_of(__fmul_rn(v, t0 ? ks1 : ks0));
                     row += 2 * S.ld_keys;
-                    left -= 2;
                 } else if constexpr (span == 2) {
-                    if (left > 0) {
-                        row[t * S.ld_keys] = key_of(__fmul_rn(fmaxf(s00, s01), ks0));
-                        row[t * S.ld_keys + 8] = key_of(__fmul_rn(fmaxf(s10, s11), ks1));
-                    }
+                    row[t * S.ld_keys] = key_of(__fmul_rn(fmaxf(s00, s01), ks0));
+                    row[t * S.ld_keys + 8] = key_of(__fmul_rn(fmaxf(s10, s11), ks1));
                     row += 4 * S.ld_keys;
-                    left -= 4;
                 } else {
-                    if (left > 0) {
-                        row[2 * t * S.ld_keys] = key_of(__fmul_rn(s00, ks0));
-                        row[2 * t * S.ld_keys + 8] = key_of(__fmul_rn(s10, ks1));
-                    }
-                    if (left > 1) {
-                        row[(2 * t + 1) * S.ld_keys] = key_of(__fmul_rn(s01, ks0));
-                        row[(2 * t + 1) * S.ld_keys + 8] = key_of(__fmul_rn(s11, ks1));
-                    }
+                    row[2 * t * S.ld_keys] = key_of(__fmul_rn(s00, ks0));
+                    row[(2 * t + 1) * S.ld_keys] = key_of(__fmul_rn(s01, ks0));
+                    row[2 * t * S.ld_keys + 8] = key_of(__fmul_rn(s10, ks1));
+                    row[(2 * t + 1) * S.ld_keys + 8] = key_of(__fmul_rn(s11, ks1));
                     row += 8 * S.ld_keys;
-                    left -= 8;
                 }
             }
             ask();                                                        // (in registers that the fragments have left: two thread blocks an SM)
@@ -354,13 +344,18 @@ int launch_select(const maya_kv_cache& c, const maya_attn_batch& b, const maya_s
     S.wide_q = rows_wide(a.q, a.ld_q, BF16 ? 2 : 4);
     while ((1 << S.span_log2) < S.group && S.span_log2 < 3) ++S.span_log2;
     S.tiles_per_token = (S.group + 7) / 8;
-    const int rows_per_token = S.group > 8 ? S.tiles_per_token * 8 : 1 << S.span_log2;
     S.ld_keys = ((b.max_len + kKvBlock - 1) / kKvBlock + 15) / 16 * 16 + 4;      // whole groups of 16 blocks; + 4: the tokens' keys in other banks
     if (S.ld_keys < 20) S.ld_keys = 20;
     // Tokens a thread block: 16 tiles of heads, as far as the tokens reach and their keys fit shared memory (128 heads).
-    auto tiles_of = [&](int n) { return (n * rows_per_token + 7) / 8; };
-    auto need = [&](int n) { return (size_t) n * S.ld_keys * 4 + (size_t) tiles_of(n) * (D / 32 * kFrag + 32); };
-    int tokens = rows_per_token >= 128 ? 1 : 128 / rows_per_token;
+    auto rows_of = [&]() { return S.group > 8 ? S.tiles_per_token * 8 : 1 << S.span_log2; };      // of a token
+    auto tiles_of = [&](int n) { return (n * rows_of() + 7) / 8; };
+    auto room_of = [&](int n) { return S.tiles_per_token > 1 ? n : tiles_of(n) << (3 - S.span_log2); };
+    auto need = [&](int n) { return (size_t) room_of(n) * S.ld_keys * 4 + (size_t) tiles_of(n) * (D / 32 * kFrag + 32); };
+    // (tiles are whole, and every token they have room for gets keys: one token of a group of one head has eight times its own.  Where that is beyond shared
+    // memory, from 404k tokens on, a token takes more rows than it has heads, a tile by itself in the end.  Guards at the stores instead cost every call
+    // registers: 16.1 us where this takes 15.7, 16 tokens at up to 64k.)
+    while (S.span_log2 < 3 && need(1) > kSmemMost) ++S.span_log2;
+    int tokens = rows_of() >= 128 ? 1 : 128 / rows_of();
     if (tokens > b.max_new) tokens = b.max_new;
     while (tokens > 1 && need(tokens) > kSmemMost) tokens = (tokens + 1) / 2;
     // (fewer while that leaves the chip's two thread blocks an SM unfilled: 100 tokens of two sequences at 26k, 3 key/value heads of 2: 70 us, so 27)
@@ -368,6 +363,7 @@ int launch_select(const maya_kv_cache& c, const maya_attn_batch& b, const maya_s
     if (need(tokens) > kSmemMost) return refuse(MAYA_ERR_LIMIT);
     S.tokens = tokens;
     S.tiles = tiles_of(tokens);
+    S.room = room_of(tokens);
     S.token_tiles = (b.max_new + tokens - 1) / tokens;
     const size_t smem = need(tokens);
     // A sequence's blocks are shared out over a cluster while all thread blocks are on the chip at once (two an SM) and each of their
