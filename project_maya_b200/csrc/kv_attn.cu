@@ -801,6 +801,7 @@ extern "C" int maya_attn_q8(const maya_kv_cache* c, const maya_attn_batch* b, co
     if (a->ld_q < (int64_t) a->n_q * c->head_dim || !aligned16(a->out)) return refuse(MAYA_ERR_ARG);
     if (a->sel && a->n_sel <= 0) return refuse(MAYA_ERR_ARG);
     if ((a->sel && a->n_sel > MAYA_MAX_SELECTED) || c->n_kv > 65535) return refuse(MAYA_ERR_LIMIT);
+    if ((long long) b->max_new * (a->n_q / c->n_kv) > 0x7fffff00ll) return refuse(MAYA_ERR_LIMIT);      // (rows of a sequence are ints)
     if (!scratch || ((uintptr_t) scratch & 255u) || scratch_bytes < maya_attn_scratch_bytes(c, a->n_q, 1)) return refuse(MAYA_ERR_ARG);
     cudaStream_t s = as_stream(stream);
     AttnView A{};

@@ -85,3 +85,13 @@ def test_other_refusals(made):
     assert all(calls(*made)[name]() == 0 for name in ("append", "attn", "select"))
     for name in ("maya_qk_norm_rope_append", "maya_block_select"):
         assert getattr(lib, name)(None, C.byref(batch), None, None) == -1
+
+
+def test_rows_of_a_sequence_beyond_32_bits_are_refused(made):
+    """Kernels count the rows (tokens * heads of a group) of a sequence in 32 bits."""
+    lib, cache, batch, rope, attn, sel = made
+    cache.n_kv = 1
+    batch.n_tokens = batch.max_new = 1 << 24
+    for n_q in (128, 200):
+        attn.n_q, attn.ld_q = n_q, n_q * cache.head_dim
+        assert calls(*made)["attn"]() == -4
