@@ -43,14 +43,15 @@ class AttentionConfig:
 class DecoderLayer:
     """w_qkv uint8: qkv_rows GGUF rows of n_embd values, [q | k | v]; w_o: n_embd rows of n_q * head_dim values; norms f32 (in, post: [n_embd];
     q, k: [head_dim]); router_w [n_expert, n_embd] f32; experts as for api.MoeLayer.  `table` i32 [n_seq, blocks of a sequence] hands out the
-    cache's blocks; max_tokens: the longest context (rotation table) and, with max_chunk, the longest prompt chunk."""
+    cache's blocks; max_tokens: the longest context; max_chunk: the longest prompt chunk."""
 
     def __init__(self, cfg: AttentionConfig, moe_cfg: api.MoeLayerConfig, w_qkv, w_o, norms: dict, router_w, experts, table, n_blocks: int,
                  max_tokens: int, max_chunk: int = 1024):
         c, dev = cfg, w_qkv.device
         self.cfg, self.moe_cfg, self.w_qkv, self.w_o, self.norms, self.router_w = cfg, moe_cfg, w_qkv, w_o, norms, router_w
         half = (c.rot_dim or c.head_dim) // 2
-        angle = torch.arange(max_tokens, device=dev, dtype=torch.float64)[:, None] * c.theta ** (-torch.arange(half, device=dev, dtype=torch.float64) / half)
+        positions = max(max_tokens, table.shape[1] * api.KV_BLOCK)             # all that the table's blocks hold
+        angle = torch.arange(positions, device=dev, dtype=torch.float64)[:, None] * c.theta ** (-torch.arange(half, device=dev, dtype=torch.float64) / half)
         self.rope = api.Rope(angle.cos().float(), angle.sin().float(), q_w=norms["q"], k_w=norms["k"], eps=c.eps)
         self.cache = api.KvCache.empty(n_blocks, c.n_kv, c.head_dim, table, sums=c.n_sel > 0)
         self.attn = api.KvAttention(self.cache, c.n_q, n_sel=c.n_sel)

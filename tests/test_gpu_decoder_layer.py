@@ -116,3 +116,15 @@ def test_short_contexts_beside_long_ones_read_every_block(cuda):
     assert rel(both[1], dense[1]) < 1e-3 and rel(both[0], alone[0]) < 1e-3     # (sums in another order, rounded to 8 bits once more)
     assert rel(both[0], dense[0]) > 1e-3
     assert rel(run(4, (0, 1), bounds_alone), both) < 1e-3
+
+
+def test_the_last_block_of_the_table_has_positions_of_its_own(cuda):
+    """A table of whole blocks holds up to 63 tokens more than max_tokens: each turns by its own angle."""
+    import torch as T
+    from project_maya_b200 import api
+    T.manual_seed(9)
+    layer, n = layer_of(tokens=200), 256
+    h = T.randn((n, 512), device="cuda")
+    want = plain_attention(layer, h.double().cpu().numpy())
+    got = T.cat([layer.attention(h[:190], api.AttnBatch.of([190], [190])), layer.attention(h[190:], api.AttnBatch.of([66], [256]))]).double().cpu().numpy()
+    assert rel(got, want) < 0.04 and max(rel(got[i], want[i]) for i in range(n)) < 0.15
