@@ -105,6 +105,10 @@ typedef struct maya_attn_args {
 /* out = sum_j softmax(scale * q . k_j)_j v_j over the tokens j of the sequence that stand at or before the query's own position,
  * within `window` and within the selected blocks; a row that sees nothing is 0.  A query with a NaN or an infinity gives a row of NaN
  * (and NaN in lse) wherever it sees a token.  bf16: value scales below 1e-30 count as 1e-30.  The cache holds the new tokens' keys and values already.
+ * One kernel serves a call's sequences: those of a few rows (new tokens times heads of a group) are cut along their contexts, from 128 rows
+ * of any sequence on (bf16, heads of 64 and 128) all go through the prompt kernel, and beyond 256 sequences (fewer, of windows) none is cut.  So pass prompt chunks
+ * and single tokens at long contexts as two calls (196 + 912 us where one call takes 3843: 4096 tokens, and 64 at up to 131k), and sequences
+ * far longer than the rest in calls of at most 256.
  * scratch: maya_attn_scratch_bytes(...) bytes (the same for any max_tokens > 0: parts have room of their own), 256-byte aligned, zeroed before the first use and after a call that left its
  * error word set; one buffer serves one stream at a time. */
 MAYA_API size_t maya_attn_scratch_bytes(const maya_kv_cache* cache, int n_q, int max_tokens);

@@ -3,7 +3,7 @@
 // What bounds it is the cache's bytes: 2 * head_dim bytes a token and key/value head, read once for the group of query heads
 // that shares them.  So everything is made to keep copies in flight: a thread block is four warps with rings of 4 KB pieces (64 tokens of 64 key
 // values, or 64 values of 64 tokens: contiguous in the cache, one bulk copy each), three thread blocks an SM.  Measured, one B200: 64
-// tokens at 1k..16k, 64 heads over 8 of 128: 150 us, 5.15 TB/s of cache (the copies alone 135 us); one at 131071 57 us, 4.7 TB/s.
+// tokens at 1k..16k, 64 heads over 8 of 128: 145 to 151 us, 5.1 to 5.3 TB/s of cache (the copies alone 135 us; f32 154); one at 131071 56 us, 4.8 TB/s (f32 63).
 //   RW warps share a ring and take 8 NT rows each; BW = 4 / RW rings take every BW-th cache block.  One token of up to 8 (16) heads a
 //   group: RW = 1, NT = 1 (2), every warp on its own; 17..32 rows: 2 x 2; more: one ring, 64 rows.
 //
@@ -20,7 +20,8 @@
 //
 // Long sequences are cut into pieces of a few dozen blocks, and the resident thread blocks take one after the other, whatever the sequences' lengths (they
 // are known on the device only).  The pieces of a (tile, head) leave (m, l, O) parts, which a second launch joins in order, a warp or a thread block a
-// row, so that the bits do not depend on who worked on what.
+// row, so that the bits do not depend on who worked on what.  With more than kTilesMost tiles, or more (tile, head)s than there is room for parts of, none is cut: a
+// call then ends with its longest sequence (257 tokens, one at 131k, one key/value head: 968 us, 256 of them 33).
 #include <cuda_fp16.h>
 
 #include "kv_attn.cuh"
