@@ -732,7 +732,7 @@ class KvAttention:
     forward(batch, q) attends over it; select(batch, q) chooses the n_sel blocks each token reads and forward(batch, q, sel=...) attends over those
     alone.  f32 or bf16; q, k, v [n_tokens, heads, head_dim], views into rows of projections among them.  scale: of the scores
     (head_dim ** -0.5); window > 0: a token sees the last `window` positions.  Prompt chunks and single tokens at long contexts are better passed as
-    two batches (include/maya_attn.h says why).  The scratch and the arguments of a call belong to this object: one
+    two batches (include/maya_attn.h says why).  max_tokens > 0 does not size anything: the scratch is the same for any batch.  The scratch and the arguments of a call belong to this object: one
     thread and one stream at a time."""
 
     def __init__(self, cache: KvCache, n_q: int, scale: float | None = None, window: int = 0, n_sel: int = 0, n_first: int = 1,

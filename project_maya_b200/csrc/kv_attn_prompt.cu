@@ -11,7 +11,7 @@
 //                      instructions and few barriers: what it takes to issue them shows in the whole call's time.
 // The two tiles take turns: while one is in its softmax the tensor cores work on the other.  Both bounds are close: a step is 2048 cycles of
 // tensor pipe (D = 128; what the operands' way out of shared memory adds is not counted) and 2048 of the exponential's pipe.  Measured, one B200: chunks of 4096
-// and 2923 tokens, 32 heads over 8, 421 us, 797 TFLOP/s (418 to 426 from box to box).
+// and 2923 tokens, 32 heads over 8, 421 us, 797 TFLOP/s (418 to 426 from one B200 to another).
 // Sequences with fewer rows in the same call come here too, one thread block a head and uncut: a chunk beside single tokens at long contexts is better as two calls.
 // What bounds it is the chain from part to part with the products in it, 5200 cycles a step, and 62 us of starts: without the exponentials, the loads or the
 // stores of codes it takes as long, without the softmax 378, without the products 357 (of 428 then).  Dropped: the softmax of a row over two threads (486), codes
