@@ -297,6 +297,32 @@ MAYA_API size_t maya_mmq_chain_bytes(int64_t total_rows, int n_matrices, int n_p
 MAYA_API int maya_mmq_run_chain(const maya_mmq_product* gate_up, const maya_mmq_product* down, int n_pairs, float limit,
                                 void* counters, size_t counter_bytes, void* stream);
 
+/* The producer in front of a product: glmf::rms_q8 (glm_fast.hpp:534) for any number of rows, with either 8-bit form:
+ *   t = h + add (f32; add NULL: h); h_out = t; x = t / sqrt(mean(t^2) + eps) * w over a row, in f32 of the unrounded t; x_out = x;
+ *   xq = x as maya_quantize_q8_1 (MAYA_XQ_Q8_1: n_rows * n / 32 blocks of 36 bytes) or maya_mmq_quantize (MAYA_XQ_MMQ:
+ *   maya_mmq_q8_bytes(n_rows, n) bytes) rounds it, byte for byte.
+ * Rows of h, add, h_out and x_out are ld_* elements apart (>= n).  h_out, x_out, xq: NULL where not wanted, one at least is.  h_out may be h or add, x_out
+ * may be h or add when h_out is not, of the same type and stride; otherwise the outputs overlap nothing.  n <= 32768, with xq n % 32 == 0; any
+ * alignment and n are taken, 16-byte aligned rows with n % 8 == 0 are fast.  n_rows <= 0: no-op. */
+enum maya_xq_image { MAYA_XQ_NONE = 0, MAYA_XQ_Q8_1 = 1, MAYA_XQ_MMQ = 2 };
+typedef struct maya_rms_args {
+    const void* h;
+    const void* add;
+    const float* w;              /* [n] */
+    void* h_out;                 /* of h's type */
+    void* x_out;
+    void* xq;                    /* 16-byte aligned; given exactly when image is not MAYA_XQ_NONE */
+    int64_t ld_h, ld_add, ld_h_out, ld_x, n_rows;
+    int n;
+    float eps;
+    int h_is_bf16, add_is_bf16, x_is_bf16;      /* else f32 */
+    int image;                   /* enum maya_xq_image */
+} maya_rms_args;
+MAYA_API int maya_rms_q8(const maya_rms_args* a, void* stream);
+/* No counterpart in the reference: `rows` rows of n values of either 8-bit form as the values they stand for, values [rows][n] (bf16 or f32) and the f16
+ * sums of their groups of 32 before rounding, sums [rows][n / 32] (for the image: of what it keeps, rounded once more).  Either may be NULL. */
+MAYA_API int maya_q8_read(const void* xq, int image, int64_t rows, int n, int out_is_bf16, void* values, uint16_t* sums, void* stream);
+
 /* The producer in front of the layer: glmf::rms_q8 (glm_fast.hpp:534: h += add; x = rms(h) * norm_w, eps inside the
  * square root) and the router job of the GEMV batch Glm5Model::fast_moe issues next (glm_fast_path.cu:6925:
  * logits = router_w . x, router_w [n_expert][n_embd] F32 or BF16 bits) in ONE launch, so that a decode layer is this call

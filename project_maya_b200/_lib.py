@@ -66,6 +66,12 @@ class HcPostArgs(C.Structure):
     _fields_ = [("R_old", c_void_p), ("post", c_void_p), ("comb", c_void_p), ("R_new", c_void_p)]
 
 
+class RmsArgs(C.Structure):
+    _fields_ = [("h", c_void_p), ("add", c_void_p), ("w", c_void_p), ("h_out", c_void_p), ("x_out", c_void_p), ("xq", c_void_p),
+                ("ld_h", c_int64), ("ld_add", c_int64), ("ld_h_out", c_int64), ("ld_x", c_int64), ("n_rows", c_int64), ("n", c_int),
+                ("eps", c_float), ("h_is_bf16", c_int), ("add_is_bf16", c_int), ("x_is_bf16", c_int), ("image", c_int)]
+
+
 class KvCacheDesc(C.Structure):
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_sum", c_void_p),
                 ("table", c_void_p), ("table_ld", c_int), ("n_blocks", c_int), ("n_kv", c_int), ("head_dim", c_int)]
@@ -131,6 +137,8 @@ _SIGNATURES = {
     "maya_moe_combine_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "maya_rms_router": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p]),
+    "maya_rms_q8": (c_int, [C.POINTER(RmsArgs), c_void_p]),
+    "maya_q8_read": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "maya_mmq_supported": (c_int, [c_int]),
     "maya_mmq_q8_bytes": (c_size_t, [c_int64, c_int64]),
     "maya_mmq_quantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p]),

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RopeArgs, SelectArgs
+from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, SelectArgs
 
 Q8_0, Q4_K, IQ3_S, IQ2_S = 8, 12, 21, 22
 Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ1_S, IQ4_XS = 13, 14, 16, 18, 19, 23      # decode paths only (see maya_ggml_type in the header)
@@ -25,6 +25,7 @@ TYPE_NAMES = {Q8_0: "Q8_0", Q4_K: "Q4_K", IQ3_S: "IQ3_S", IQ2_S: "IQ2_S", Q5_K: 
 STATUS = {0: "ok", -1: "bad argument", -2: "unsupported ggml type", -3: "CUDA launch failed", -4: "beyond a limit",
           -5: "no sm_100 device"}
 LAYER_CHOICE, LAYER_FUSED, LAYER_TOKEN, LAYER_STAGED = 0, 1, 2, 3        # maya_layer_kernel
+XQ_Q8_1, XQ_MMQ = 1, 2        # 8-bit rows: q8_1 blocks (native_mmvq reads them), the prompt path's image (mmq_run) - enum maya_xq_image
 INF = float("inf")
 MAX_COLS = 8                 # activation columns of native_mmvq (MAYA_MAX_COLS)
 
@@ -247,6 +248,64 @@ def rms_router(h, add, norm_w, eps: float, router_w, h_out=None, stream=None):
                                                     int(router_w.dtype == torch.bfloat16), n_expert, _ptr(h_out), _ptr(x),
                                                     _ptr(logits), _stream(stream)))
     return x, logits
+
+
+def _here(what: str, *tensors) -> None:
+    """Tensors of a call: all on the current device, whose stream the call goes to."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise MayaError(f"{what}: tensors of the current device expected", -1)
+
+
+def _matrix(t, shape):
+    """(address, elements between rows) of a matrix of that shape (one row: [n] too) whose rows are contiguous."""
+    strides = t.stride()
+    assert t.shape == shape or (shape[0] == 1 and t.shape == shape[1:]), "rows of another shape"
+    assert t.dtype is torch.float32 or t.dtype is torch.bfloat16
+    assert strides[-1] == 1 or shape[1] <= 1
+    return t.data_ptr(), strides[0] if shape[0] > 1 else shape[1]
+
+
+def xq_bytes(image: int, rows: int, n: int) -> int:
+    """Bytes of `rows` 8-bit rows of n values."""
+    return (rows * n >> 5) * 36 if image == XQ_Q8_1 else mmq_q8_bytes(rows, n)
+
+
+def rms_q8(h, add, norm_w, eps: float, image: int | None = XQ_Q8_1, xq=None, h_out=None, x=None, stream=None):
+    """glmf::rms_q8 (glm_fast.hpp:534) for any number of rows: t = h + add (add None: h), x = rms(t) * norm_w, and x in 8 bits.  h and add [T, n] f32 or
+    bf16 (one row: [n] too), rows may lie apart.  image: XQ_Q8_1 or XQ_MMQ, what native_quantize_q8_1(x) or mmq_quantize(x) would write, returned as
+    uint8 - in `xq` where it is given; None: no 8-bit rows.  h_out (h's type; may be h): receives t; x (f32 or bf16): the normed rows."""
+    _here("rms_q8", h, add, norm_w, h_out, x, xq)
+    shape = h.shape if h.dim() == 2 else h[None].shape
+    T, n = shape
+    assert norm_w.dtype is torch.float32 and norm_w.shape == shape[1:] and (h_out is None or h_out.dtype is h.dtype)
+    if image is not None:
+        need = xq_bytes(image, T, n)
+        if xq is None:
+            xq = torch.empty(max(need, 16), dtype=torch.uint8, device=h.device)
+        assert xq.numel() * xq.element_size() >= need, "xq is too small"
+    else:
+        assert xq is None
+    hp, ld_h = _matrix(h, shape)
+    ap, ld_add = (None, n) if add is None else _matrix(add, shape)
+    op, ld_out = (None, n) if h_out is None else _matrix(h_out, shape)
+    rows, ld_x = (None, n) if x is None else _matrix(x, shape)
+    bf16 = torch.bfloat16
+    a = RmsArgs(hp, ap, _ptr(norm_w), op, rows, _ptr(xq), ld_h, ld_add, ld_out, ld_x, T, n, eps, h.dtype is bf16,
+                add is not None and add.dtype is bf16, x is not None and x.dtype is bf16, image or 0)
+    _check("rms_q8", _lib.load().maya_rms_q8(C.byref(a), _stream(stream)))
+    return xq
+
+
+def q8_read(xq, rows: int, n: int, image: int = XQ_Q8_1, dtype=torch.bfloat16, stream=None):
+    """8-bit rows as the values they stand for: (values [rows, n] of dtype bf16 or f32, sums f16 [rows, n / 32] of their groups before rounding)."""
+    _here("q8_read", xq)
+    assert dtype in (torch.float32, torch.bfloat16) and xq.numel() * xq.element_size() >= xq_bytes(image, rows, n)
+    values = torch.empty((rows, n), dtype=dtype, device=xq.device)
+    sums = torch.empty((rows, n // 32), dtype=torch.float16, device=xq.device)
+    _check("q8_read", _lib.load().maya_q8_read(_ptr(xq), image, rows, n, int(dtype is torch.bfloat16), _ptr(values), _ptr(sums), _stream(stream)))
+    return values, sums
 
 
 # ---------------------------------------------------------------- prompt-path grouped GEMM (tensor cores)

@@ -50,6 +50,7 @@
 #include <utility>
 
 #include "maya_internal.cuh"
+#include "maya_mmq_image.cuh"
 #include "maya_rows.cuh"
 #include "maya_tcgen05.cuh"
 
@@ -97,18 +98,11 @@ template<int T> constexpr size_t kSmemBytes = (size_t) kTabOff<T> + kTabBytes<T>
 template<int T> constexpr bool kUnitsFit = kUnits<T> <= kMaxUnits && kUnits<T> % (kIq<T> ? 8 : 4) == 0 && kSmemBytes<T> <= 227 * 1024 - 1024;
 static_assert(kUnitsFit<MAYA_Q4_K> && kUnitsFit<MAYA_Q8_0> && kUnitsFit<MAYA_IQ2_S> && kUnitsFit<MAYA_IQ3_S>, "the ring of raw units");
 
-// The activation image: a row is its w_cols f16 values d * q, then one f16 per 32 values - the group's SUM CORRECTION
-// xa = f16(sum of the unquantized values) - sum of the row's stored d * q values - padded with zeros to a multiple of 64.  llama.cpp's
-// MMQ keeps that unquantized sum beside the block (the "ds4" q8_1 layout) and a type with a constant term per group
-// (Q4_K: -dmin * m) multiplies the term by it, not by the sum of the rounded values; here the same result comes from
-// extra K steps inside a Q4_K product: A = -dmin * m of a row's groups, B = xa.  Other types do not read the tail.
 // Optional clock stamps of a tile's phases (built only with -DMAYA_MMQ_STAMPS, see build.py --stamps and
 // mmq_tile_phases.py): 16 slots per tile for the first 4096 tiles of each of the four (type class, fused) kernels.
 #ifdef MAYA_MMQ_STAMPS
 __device__ long long g_stamps[4 * 4096 * 16];
 #endif
-__host__ __device__ constexpr int64_t xq_tail(int64_t cols) { return ((cols / 32) + 63) & ~(int64_t) 63; }
-__host__ __device__ constexpr int64_t xq_ld(int64_t cols) { return cols + xq_tail(cols); }
 
 struct MmqArgs {
     int w_rows, w_cols;          // rows of one output (n_ff for the fused form: gate rows, then up rows), K
@@ -130,47 +124,10 @@ struct MmqArgs {
     int alone;                   // not behind another product of its chain: everything in front has to be done first
 };
 
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *(uint32_t*) &h; }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *(__half2*) &u; }
 // bytes (lo, hi) of x -> the half2 (1024 + lo, 1024 + hi): 0x64 is the high byte of 1024.0 in f16
 __device__ __forceinline__ __half2 bytes01_plus1024(uint32_t x) { return bits_h2(__byte_perm(x, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ __half2 bytes23_plus1024(uint32_t x) { return bits_h2(__byte_perm(x, 0x64646464u, 0x4342)); }
-
-// The q8_1 rounding of maya_mmq_quantize for a thread that holds 8 consecutive values of a 32-value group (the group's
-// four threads are four consecutive lanes; every lane of the warp must call): llama.cpp's quantize_mmq_q8_1 as the
-// reference's host model states it - d_inv = 127 / amax, q = round(v * d_inv) clamped to +-127, d = min(1 / d_inv, 65504)
-// kept as f16, stored f16(d) * q.  o = the 8 stored values; the return value is the group's sum correction
-// f16(S) - sum of the stored values, with S added in quantize_mmq_q8_1's order: four consecutive values left to right
-// (this thread holds partial sums 2j and 2j + 1 of the group's eight), then the tree at distances 4, 2, 1.
-__device__ __forceinline__ __half q8_1_round8(const float (&v)[8], uint32_t (&o)[4]) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-    const float d_inv = __fdiv_rn(127.0f, amax);
-    const float dh = amax == 0.0f ? 0.0f : __half2float(__float2half_rn(fminf(__fdiv_rn(1.0f, d_inv), 65504.0f)));
-    float bsum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float q0 = 0.0f, q1 = 0.0f;
-        if (amax != 0.0f) {
-            q0 = fmaxf(-127.0f, fminf(127.0f, roundf(__fmul_rn(v[2 * i], d_inv))));
-            q1 = fmaxf(-127.0f, fminf(127.0f, roundf(__fmul_rn(v[2 * i + 1], d_inv))));
-        }
-        const __half2 r = __floats2half2_rn(dh * q0, dh * q1);
-        o[i] = h2_bits(r);
-        bsum += __low2float(r) + __high2float(r);     // the stored values: multiples of one power of two, 24 bits in all - exact
-    }
-    float s0 = __fadd_rn(__fadd_rn(__fadd_rn(v[0], v[1]), v[2]), v[3]), s1 = __fadd_rn(__fadd_rn(__fadd_rn(v[4], v[5]), v[6]), v[7]);
-    s0 = __fadd_rn(s0, __shfl_xor_sync(0xFFFFFFFFu, s0, 2));
-    s1 = __fadd_rn(s1, __shfl_xor_sync(0xFFFFFFFFu, s1, 2));
-    s0 = __fadd_rn(s0, __shfl_xor_sync(0xFFFFFFFFu, s0, 1));
-    s1 = __fadd_rn(s1, __shfl_xor_sync(0xFFFFFFFFu, s1, 1));
-    bsum += __shfl_xor_sync(0xFFFFFFFFu, bsum, 1);
-    bsum += __shfl_xor_sync(0xFFFFFFFFu, bsum, 2);
-    return __float2half_rn(__half2float(__float2half_rn(__fadd_rn(s0, s1))) - bsum);
-}
 
 // ---- Q4_K: of a 144-byte block's 16-byte header, d * sc and -(dmin * m) of sub-blocks 2 (2 i + t) and 2 (2 i + t) + 1, i = 0 or 1, as a half2
 // each.  y, z, w: the header's scale words, shifted so that their low 16 bits are columns 2 t and 2 t + 1.  (Two sub-blocks at a time and only those a
