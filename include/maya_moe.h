@@ -93,6 +93,23 @@ MAYA_API int maya_router_top10(const float* logits, int n_tokens, int n_expert, 
 MAYA_API int maya_router_sigmoid(const float* logits, const float* bias, int n_tokens, int n_expert, int k,
                                  float w_scale, int norm_w, int* ids, float* weights, void* stream);
 
+/* No counterpart in the reference: routing over groups of neighbouring experts, softmax or sigmoid.
+ *   s = softmax(logits) or 1 / (1 + exp(-logit)); c = s + bias (bias NULL: s); a group of n_expert / n_group experts scores its highest c, or with top2
+ *   the sum of its two highest; the n_keep best groups are kept (ties: the lower group), of their experts the k highest c are chosen (ties: the lower
+ *   expert), in that order; weights = s, divided by max(their sum, 2^-14) when norm_w, times w_scale.  In 64 bits, the weights rounded once.
+ * A score that is no number (a NaN logit; any logit of a softmax row with a NaN or +inf) ranks behind every other; a softmax row of nothing but -inf has
+ * scores of 0.  n_group = n_keep = 1: no groups.  n_expert <= 2048, k <= 64, n_group <= 32 and a divisor of n_expert, k <= n_keep * n_expert / n_group. */
+typedef struct maya_route_args {
+    const float* logits;         /* [n_tokens][n_expert] */
+    const float* bias;           /* [n_expert] or NULL */
+    int n_tokens, n_expert, k, n_group, n_keep;
+    int sigmoid, top2, norm_w;
+    float w_scale;
+    int* ids;                    /* [n_tokens][k] */
+    float* weights;              /* [n_tokens][k] */
+} maya_route_args;
+MAYA_API int maya_router_groups(const maya_route_args* a, void* stream);
+
 /* Activations ------------------------------------------------------------------------------------- */
 /* native_quantize_q8_1 (native_mmvq.hpp:38) / quantize_q8_1_rows (iq_kernels.hpp:21): x [ncols, n_in] f32 ->
  * ncols * n_in/32 q8_1 blocks {f16 d, f16 sum(x), i8 q[32]}.  n_in % 32 == 0. */
@@ -398,6 +415,12 @@ struct maya_hc_post_args;
 MAYA_API int maya_moe_layer_decode_checked(const maya_moe_layer* L, const float* logits, const void* x, int x_is_bf16, int* ids,
                                            float* weights, float* out, void* scratch, size_t scratch_bytes, int kernel,
                                            unsigned polls, const struct maya_hc_post_args* hc, void* stream);
+/* No counterpart in the reference: the layer for tokens that are routed already, by maya_router_groups or by the caller: ids and weights
+ * [n_tokens][k] on the device (L->router and its fields are not read; an id outside 0 .. n_expert - 1 contributes nothing).  1 .. 16 tokens, through the
+ * window kernels: a token's output equals maya_moe_layer_decode's with `staged` for the same ids and weights, bit for bit.  A slice of the shared expert is refused. */
+MAYA_API int maya_moe_layer_decode_routed(const maya_moe_layer* L, const int* ids, const float* weights, const void* x, int x_is_bf16,
+                                          int n_tokens, float* out, void* scratch, size_t scratch_bytes, void* stream);
+
 
 /* Cross-GPU sum of expert partials -------------------------------------------------------------- */
 #define MAYA_PEER_AR_MAX_RANKS 8

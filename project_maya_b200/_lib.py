@@ -66,6 +66,12 @@ class HcPostArgs(C.Structure):
     _fields_ = [("R_old", c_void_p), ("post", c_void_p), ("comb", c_void_p), ("R_new", c_void_p)]
 
 
+class RouteArgs(C.Structure):
+    _fields_ = [("logits", c_void_p), ("bias", c_void_p), ("n_tokens", c_int), ("n_expert", c_int), ("k", c_int), ("n_group", c_int),
+                ("n_keep", c_int), ("sigmoid", c_int), ("top2", c_int), ("norm_w", c_int), ("w_scale", c_float), ("ids", c_void_p),
+                ("weights", c_void_p)]
+
+
 class RmsArgs(C.Structure):
     _fields_ = [("h", c_void_p), ("add", c_void_p), ("w", c_void_p), ("h_out", c_void_p), ("x_out", c_void_p), ("xq", c_void_p),
                 ("ld_h", c_int64), ("ld_add", c_int64), ("ld_h_out", c_int64), ("ld_x", c_int64), ("n_rows", c_int64), ("n", c_int),
@@ -137,6 +143,8 @@ _SIGNATURES = {
     "maya_moe_combine_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "maya_rms_router": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p]),
+    "maya_router_groups": (c_int, [C.POINTER(RouteArgs), c_void_p]),
+    "maya_moe_layer_decode_routed": (c_int, [C.POINTER(MoeLayerDesc), c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "maya_rms_q8": (c_int, [C.POINTER(RmsArgs), c_void_p]),
     "maya_q8_read": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "maya_mmq_supported": (c_int, [c_int]),

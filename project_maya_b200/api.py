@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, SelectArgs
+from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, RouteArgs, SelectArgs
 
 Q8_0, Q4_K, IQ3_S, IQ2_S = 8, 12, 21, 22
 Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ1_S, IQ4_XS = 13, 14, 16, 18, 19, 23      # decode paths only (see maya_ggml_type in the header)
@@ -54,6 +54,14 @@ def _stream(stream=None) -> int:
     if stream is None:           # the current stream's handle, without the Stream object (0.2 us instead of 3.1: a small layer's token takes 18)
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _here(what: str, *tensors) -> None:
+    """Tensors of a call: all on the current device, whose stream the call goes to."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise MayaError(f"{what}: tensors of the current device expected", -1)
 
 
 # ---------------------------------------------------------------- formats (host only: usable without a GPU)
@@ -107,6 +115,40 @@ def router_sigmoid(logits, bias, k: int, w_scale: float = 1.0, norm_w: bool = Tr
     weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
     _check("router_sigmoid", _lib.load().maya_router_sigmoid(_ptr(logits), _ptr(bias), T, E, k, w_scale, int(norm_w),
                                                              _ptr(ids), _ptr(weights), _stream(stream)))
+    return ids, weights
+
+
+@dataclass
+class GroupRouting:
+    """How router_groups chooses: n_group groups of neighbouring experts of which the n_keep best are kept (1, 1: no groups), bias f32 [n_expert] or
+    None, sigmoid or softmax scores, top2: a group scores the sum of its two highest (else its highest), norm_w and w_scale of the weights."""
+    n_group: int = 1
+    n_keep: int = 1
+    bias: "torch.Tensor | None" = None
+    sigmoid: bool = True
+    top2: bool = True
+    norm_w: bool = True
+    w_scale: float = 1.0
+
+    def route(self, logits, k: int, ids=None, weights=None, stream=None):
+        return router_groups(logits, k, self.n_group, self.n_keep, self.bias, self.sigmoid, self.top2, self.norm_w, self.w_scale, ids, weights, stream)
+
+
+def router_groups(logits, k: int, n_group: int = 1, n_keep: int = 1, bias=None, sigmoid: bool = True, top2: bool = True, norm_w: bool = True,
+                  w_scale: float = 1.0, ids=None, weights=None, stream=None):
+    """No counterpart in the reference.  logits [T, n_expert] f32 -> ids i32, weights f32 [T, k]: scores s = sigmoid or softmax of the logits, choice by
+    s + bias - the n_keep best of n_group groups, then the k best of their experts - and weights s / max(their sum, 2^-14) * w_scale (norm_w False:
+    s * w_scale).  include/maya_moe.h states it in full (maya_router_groups)."""
+    T, E = logits.shape
+    _here("router_groups", logits, bias, ids, weights)
+    assert logits.dtype is torch.float32 and (bias is None or (bias.dtype is torch.float32 and bias.numel() == E))
+    if ids is None:
+        ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
+    if weights is None:
+        weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+    assert ids.dtype is torch.int32 and weights.dtype is torch.float32 and ids.numel() == weights.numel() == T * k
+    a = RouteArgs(_ptr(logits), _ptr(bias), T, E, k, n_group, n_keep, sigmoid, top2, norm_w, w_scale, _ptr(ids), _ptr(weights))
+    _check("router_groups", _lib.load().maya_router_groups(C.byref(a), _stream(stream)))
     return ids, weights
 
 
@@ -248,14 +290,6 @@ def rms_router(h, add, norm_w, eps: float, router_w, h_out=None, stream=None):
                                                     int(router_w.dtype == torch.bfloat16), n_expert, _ptr(h_out), _ptr(x),
                                                     _ptr(logits), _stream(stream)))
     return x, logits
-
-
-def _here(what: str, *tensors) -> None:
-    """Tensors of a call: all on the current device, whose stream the call goes to."""
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise MayaError(f"{what}: tensors of the current device expected", -1)
 
 
 def _matrix(t, shape):
@@ -451,11 +485,14 @@ class MoeLayer:
     left out of `out` (another rank adds them).  shared_range = (lo, hi) gives this rank a slice of the shared expert's
     FFN width instead of all of it (single-token calls only).  sigmoid = (bias [n_expert] or None, w_scale, norm_w):
     sigmoid routing with a selection bias instead of softmax.  cpu_part [T, n_embd] f32 / cpu_flag [T] i32: a host lane's
-    contribution, added to token t's output when cpu_flag[t] != 0 (the tier hooks of the reference's MoeDev)."""
+    contribution, added to token t's output when cpu_flag[t] != 0 (the tier hooks of the reference's MoeDev).  routing (a GroupRouting): routing over
+    groups of experts, a launch of its own in front of the window kernels (no peer, no hc)."""
 
     def __init__(self, cfg: MoeLayerConfig, experts, shared=None, expert_range=None, shared_here=True, max_tokens: int = 16,
-                 staged: bool = False, shared_range=None, sigmoid=None, cpu_part=None, cpu_flag=None):
-        self.cfg = cfg
+                 staged: bool = False, shared_range=None, sigmoid=None, cpu_part=None, cpu_flag=None, routing: GroupRouting | None = None):
+        if routing is not None and (sigmoid is not None or shared_range is not None):
+            raise MayaError("moe_layer: routing over groups beside sigmoid or shared_range", -1)
+        self.cfg, self.routing = cfg, routing
         self.experts = experts
         self.shared = shared
         lo, hi = expert_range if expert_range is not None else (0, cfg.n_expert)
@@ -499,6 +536,12 @@ class MoeLayer:
             weights = weights if weights is not None else torch.empty_like(like[1], memory_format=torch.contiguous_format)
             out = out if out is not None else torch.empty_like(like[2], memory_format=torch.contiguous_format)
         assert x.dtype in (torch.float32, torch.bfloat16)
+        if self.routing is not None:
+            if peer is not None or hc is not None:
+                raise MayaError("moe_layer: routing over groups with peer or hc", -1)
+            assert logits.shape[1] == self.cfg.n_expert and x.shape == (T, self.cfg.n_embd)
+            self.routing.route(logits, self.cfg.k, ids, weights, stream)
+            return ids, weights, self.forward_routed(ids, weights, x, out, stream)
         if hc is not None:
             args = HcPostArgs(*[_ptr(t) for t in hc])
             seq = 0
@@ -524,9 +567,24 @@ class MoeLayer:
                                                  self.scratch.numel(), _stream(stream)))
         return ids, weights, out
 
+    def forward_routed(self, ids, weights, x, out=None, stream=None):
+        """The layer for up to 16 tokens that are routed already: ids i32 and weights f32 [T, k] (an id outside 0 .. n_expert - 1 contributes nothing)."""
+        T, k = ids.shape
+        assert k == self.cfg.k and ids.dtype is torch.int32 and weights.dtype is torch.float32 and weights.shape == ids.shape
+        assert x.dtype in (torch.float32, torch.bfloat16) and x.shape == (T, self.cfg.n_embd)
+        if out is None:
+            out = torch.empty((T, self.cfg.n_embd), dtype=torch.float32, device=ids.device)
+        assert out.dtype is torch.float32 and out.numel() == T * self.cfg.n_embd
+        _check("moe_layer_decode_routed",
+               _lib.load().maya_moe_layer_decode_routed(C.byref(self.desc), _ptr(ids), _ptr(weights), _ptr(x), int(x.dtype == torch.bfloat16), T,
+                                                        _ptr(out), _ptr(self.scratch), self.scratch.numel(), _stream(stream)))
+        return out
+
     def forward_checked(self, logits, x, kernel: int, polls: int = 1 << 22, out=None, hc=None, stream=None):
-        """forward of one token with the caller's choice of kernel (LAYER_CHOICE, LAYER_FUSED, LAYER_TOKEN, LAYER_STAGED; a kernel that
+        """forward of one token (not of a layer with routing over groups) with the caller's choice of kernel (LAYER_CHOICE, LAYER_FUSED, LAYER_TOKEN, LAYER_STAGED; a kernel that
         does not take the layer raises) and bound on its waits for weight rows."""
+        if self.routing is not None:
+            raise MayaError("moe_layer: routing over groups runs the window kernels", -1)
         dev = logits.device
         ids = torch.empty((1, self.cfg.k), dtype=torch.int32, device=dev)
         weights = torch.empty((1, self.cfg.k), dtype=torch.float32, device=dev)
@@ -566,9 +624,13 @@ class MoePrefill:
     `experts` is uint8 [n_expert, blob_bytes] of one type (cfg.gu_type == cfg.d_type is not required), or None with
     `pools` = [(ggml_type, blobs uint8 [n_i, blob_bytes of that type], expert ids of the n_i blobs), ...] for a layer whose
     experts are stored in different types: one product per pool, each matrix finding its rows through the pool's
-    expert map (the reference's staged groups, moe_mmq.hpp:41-53 with bounds per group)."""
+    expert map (the reference's staged groups, moe_mmq.hpp:41-53 with bounds per group).
 
-    def __init__(self, cfg: MoeLayerConfig, experts, shared=None, max_tokens: int = 4096, pools=None, expert_range=None):
+    routing (a GroupRouting): routing over groups of experts instead of the softmax top-k."""
+
+    def __init__(self, cfg: MoeLayerConfig, experts, shared=None, max_tokens: int = 4096, pools=None, expert_range=None,
+                 routing: GroupRouting | None = None):
+        self.routing = routing
         H, FF = cfg.n_embd, cfg.n_ff
         self.expert_range = expert_range         # (lo, hi): an expert-parallel rank's experts; ffn is then its partial sum
         if pools is None:
@@ -630,7 +692,11 @@ class MoePrefill:
         quant = lib.maya_mmq_quantize_bf16 if x.dtype == torch.bfloat16 else lib.maya_mmq_quantize
         quant_routed = lib.maya_mmq_quantize_routed_bf16 if x.dtype == torch.bfloat16 else lib.maya_mmq_quantize_routed
         ids, w = self.ids[:T], self.weights[:T]
-        _check("router_top10", lib.maya_router_top10(_ptr(logits), T, E, k, _ptr(ids), _ptr(w), s))
+        if self.routing is None:
+            _check("router_top10", lib.maya_router_top10(_ptr(logits), T, E, k, _ptr(ids), _ptr(w), s))
+        else:
+            assert logits.shape == (T, E)
+            self.routing.route(logits, k, ids, w, s)
         if n <= 4096 and E <= 1024:  # one block does it all: 20 tokens of top 8 109.6 / 107.0 us a layer, 300 135.9 / 134.3; 2000 over 512 experts 457 / 466
             _check("expert_group", lib.maya_expert_group_counts(_ptr(ids), n, k, E, _ptr(self.counts), _ptr(self.rank), _ptr(self.bounds),
                                                                 _ptr(self.row_tok), _ptr(self.pos), s))

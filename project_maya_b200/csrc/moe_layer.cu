@@ -76,6 +76,8 @@ Scratch carve(const maya_moe_layer& L, int T, uint8_t* base) {
 struct PrepArgs {
     const float* logits;
     const float* bias;           // sigmoid router
+    const int* given_ids;        // routed already (RT 2): ids and weights [T][k]
+    const float* given_w;
     float w_scale;
     int norm_w;
     int n_expert, k;
@@ -120,7 +122,12 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs P) {
         return;
     }
     const float* logits = P.logits + (size_t) t * P.n_expert;
-    if constexpr (RT == 1) route_sigmoid<PER, BlockSync>(logits, P.bias, P.n_expert, P.k, P.w_scale, P.norm_w, tid, 256, s_ex, route);
+    if constexpr (RT == 2) {
+        if (tid < P.k) {
+            route.ids[tid] = P.given_ids[(size_t) t * P.k + tid];
+            route.val[tid] = P.given_w[(size_t) t * P.k + tid];
+        }
+    } else if constexpr (RT == 1) route_sigmoid<PER, BlockSync>(logits, P.bias, P.n_expert, P.k, P.w_scale, P.norm_w, tid, 256, s_ex, route);
     else route_softmax<PER, BlockSync>(logits, P.n_expert, P.k, tid, 256, s_ex, route);
     if (tid < 8) {
         unsigned long long p = 0ull;
@@ -129,8 +136,10 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs P) {
             const int e = route.ids[tid];
             w = route.val[tid];
             if (e >= P.lo && e < P.hi) p = (unsigned long long) (P.experts + (size_t) e * P.stride);
-            P.ids[(size_t) t * P.k + tid] = e;
-            P.weights[(size_t) t * P.k + tid] = w;
+            if constexpr (RT != 2) {
+                P.ids[(size_t) t * P.k + tid] = e;
+                P.weights[(size_t) t * P.k + tid] = w;
+            }
         }
         P.plan_ptr[t * 8 + tid] = p;
         P.plan_w[t * 8 + tid] = w;
@@ -150,6 +159,10 @@ template<int RT> int launch_prep(const PrepArgs& P, int T, cudaStream_t s) {
     const int per = (P.n_expert + 255) / 256, nblk = P.n_embd / 32;
     const dim3 grid((unsigned) T, (unsigned) (1 + (nblk >= 256 ? 8 : (nblk + 31) / 32)));
     const size_t smem = (size_t) P.n_expert * sizeof(double);
+    if constexpr (RT == 2) {
+        launch_dependent(prep_kernel<RT, 1>, grid, dim3(256), 0, s, P);
+        return note_launch("moe_prep");
+    }
     if (per <= 1) launch_dependent(prep_kernel<RT, 1>, grid, dim3(256), smem, s, P);
     else if (per <= 2) launch_dependent(prep_kernel<RT, 2>, grid, dim3(256), smem, s, P);
     else if (per <= 4) launch_dependent(prep_kernel<RT, 4>, grid, dim3(256), smem, s, P);
@@ -209,7 +222,7 @@ extern "C" int maya_moe_layer_phase_ns(const maya_moe_layer* L, const void* scra
 static int layer_decode(const maya_moe_layer* L, const float* logits, const void* x, int x_is_bf16, int n_tokens, int* ids,
                         float* weights, float* out, void* scratch, size_t scratch_bytes, const maya_peer_ar* ar, int mi,
                         unsigned seq, void* stream, const maya_hc_post_args* hc = nullptr, int kernel = MAYA_LAYER_CHOICE,
-                        unsigned polls = kMbarPolls);
+                        unsigned polls = kMbarPolls, bool routed = false);
 static int ar_args_ok(const maya_moe_layer* L, int n_tokens, float* out, const maya_peer_ar* a, int mi, unsigned seq);
 
 extern "C" int maya_moe_layer_decode(const maya_moe_layer* L, const float* logits, const void* x, int x_is_bf16,
@@ -259,6 +272,13 @@ extern "C" int maya_moe_layer_decode_checked(const maya_moe_layer* L, const floa
     return layer_decode(L, logits, x, x_is_bf16, 1, ids, weights, out, scratch, scratch_bytes, nullptr, 0, 0, stream, hc, kernel, polls);
 }
 
+extern "C" int maya_moe_layer_decode_routed(const maya_moe_layer* L, const int* ids, const float* weights, const void* x, int x_is_bf16,
+                                            int n_tokens, float* out, void* scratch, size_t scratch_bytes, void* stream) {
+    if (!ids || !weights) return refuse(MAYA_ERR_ARG);
+    return layer_decode(L, nullptr, x, x_is_bf16, n_tokens, (int*) ids, (float*) weights, out, scratch, scratch_bytes, nullptr, 0, 0, stream,
+                        nullptr, MAYA_LAYER_STAGED, kMbarPolls, true);
+}
+
 // The staged paths' consumer: one hc_post launch per token, after `out` is complete.
 static int hc_post_tokens(const maya_hc_post_args* hc, const float* out, int T, int n_embd, void* stream) {
     if (hc == nullptr) return MAYA_OK;
@@ -272,18 +292,18 @@ static int hc_post_tokens(const maya_hc_post_args* hc, const float* out, int T, 
 
 static int layer_decode(const maya_moe_layer* L, const float* logits, const void* x, int x_is_bf16, int n_tokens, int* ids,
                         float* weights, float* out, void* scratch, size_t scratch_bytes, const maya_peer_ar* ar, int mi,
-                        unsigned seq, void* stream, const maya_hc_post_args* hc, int kernel, unsigned polls) {
+                        unsigned seq, void* stream, const maya_hc_post_args* hc, int kernel, unsigned polls, bool routed) {
     int st = check_layer(L);
     if (st != MAYA_OK) return refuse(st);
     if (n_tokens < 1 || n_tokens > MAYA_MAX_WIN_TOKENS) return refuse(MAYA_ERR_LIMIT);
-    if (!logits || !x || !out || !scratch || (((uintptr_t) scratch) & 255u)) return refuse(MAYA_ERR_ARG);
+    if ((!logits && !routed) || !x || !out || !scratch || (((uintptr_t) scratch) & 255u)) return refuse(MAYA_ERR_ARG);
     const int T = n_tokens;
     const Scratch S = carve(*L, T, (uint8_t*) scratch);
     if (S.bytes > scratch_bytes) return refuse(MAYA_ERR_LIMIT);
     cudaStream_t s = as_stream(stream);
     int* d_ids = ids ? ids : S.ids;
     float* d_w = weights ? weights : S.weights;
-    if (T == 1 && (kernel == MAYA_LAYER_CHOICE ? !L->staged : kernel != MAYA_LAYER_STAGED)) {
+    if (T == 1 && !routed && (kernel == MAYA_LAYER_CHOICE ? !L->staged : kernel != MAYA_LAYER_STAGED)) {
         st = fused_t1(*L, logits, x, x_is_bf16, d_ids, d_w, out, S.h, S.unit_count, S.sync, ar, mi, seq, hc, kernel, polls, s);
         if (st != kNotHere) return st;
         if (kernel != MAYA_LAYER_CHOICE) return refuse(MAYA_ERR_LIMIT);
@@ -293,13 +313,14 @@ static int layer_decode(const maya_moe_layer* L, const float* logits, const void
 
     if (L->k > 64 || L->n_expert > 256 * kRouterMaxPerThread) return refuse(MAYA_ERR_LIMIT);
     PrepArgs P{};
+    P.given_ids = ids; P.given_w = weights;
     P.logits = logits; P.bias = L->router_bias; P.w_scale = L->router_w_scale; P.norm_w = L->router_norm_w;
     P.n_expert = L->n_expert; P.k = L->k; P.x = x; P.x_is_bf16 = x_is_bf16; P.n_embd = L->n_embd; P.xq = S.xq;
     P.experts = (const uint8_t*) L->experts; P.stride = L->expert_stride; P.lo = L->expert_lo; P.hi = L->expert_hi;
     P.ids = d_ids; P.weights = d_w; P.plan_ptr = S.plan_ptr; P.plan_w = S.plan_w;
     P.group = GroupOut{S.grp_ptr, S.grp_start, S.grp_ent, S.n_groups};
     P.ticket = S.sync + 3;
-    st = L->router == 1 ? launch_prep<1>(P, T, s) : launch_prep<0>(P, T, s);
+    st = routed ? launch_prep<2>(P, T, s) : L->router == 1 ? launch_prep<1>(P, T, s) : launch_prep<0>(P, T, s);
     if (st != MAYA_OK) return st;
 
     const bool shared = L->n_ff_sh > 0 && L->shared_here;
