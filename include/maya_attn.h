@@ -52,6 +52,49 @@ typedef struct maya_attn_batch {
     int n_seq, n_tokens, max_new, max_len;
 } maya_attn_batch;
 
+/* Pages --------------------------------------------------------------------------------------------- */
+/* The blocks of the caches of n_layers layers that share one table, handed out and taken back on the device.  refs[b] says how many entries of the
+ * table hold block b (0 or less: free); table entries of -1 hold none.  A call that needs blocks gets the free ones of the lowest numbers in the order of
+ * asking: of those that are free when it begins, so that what a call frees can be had by the next.  When there are too few, the entries left without are -1 and
+ * the scratch's error word is set (sticky).  Nothing here reads or writes a block or sequence outside what the descriptor says: such numbers in device
+ * memory are passed over.  One scratch serves one stream at a time. */
+#define MAYA_MAX_PAGES (1 << 20)   /* blocks of a descriptor */
+typedef struct maya_kv_layer {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int16_t* k_sum;
+} maya_kv_layer;
+typedef struct maya_kv_pages {
+    const maya_kv_layer* layers;   /* [n_layers], in device memory: buffers laid out as maya_kv_cache's */
+    int32_t* table;                /* [n_seq][table_ld] */
+    int32_t* refs;                 /* [n_blocks], 16-byte aligned */
+    void* scratch;                 /* maya_pages_scratch_bytes bytes, 256-byte aligned, its first 256 zeroed before the first use: words [0] error, [1]
+                                      blocks that the last call had to move, [2] live blocks as the last compaction found them */
+    size_t scratch_bytes;
+    int n_seq, table_ld, n_blocks, n_layers, n_kv, head_dim;
+    int has_sums;                  /* the layers keep k_sum */
+} maya_kv_pages;
+MAYA_API size_t maya_pages_scratch_bytes(const maya_kv_pages* p);          /* 0 for a descriptor that is refused */
+/* Room for a batch's new tokens: every table entry that they fall into and that holds no block gets one.  An entry whose block others hold too gets a
+ * block of its own, with a copy of what it held if that has tokens from before (others of the same batch that share it each get one).  The sequences
+ * are the table's first; batch->max_len <= 64 * table_ld. */
+MAYA_API int maya_pages_reserve(const maya_kv_pages* p, const maya_attn_batch* batch, void* stream);
+/* For each i < n (n <= n_seq), all at once: sequence children[i] gives up its blocks and becomes the first lens[i] tokens of sequence parents[i] as it was
+ * before the call: full blocks are shared, the last one, where it is not full, is copied to a block of its own.  children[i] == parents[i]: left as it is.
+ * Of several pairs with one child the first counts. */
+MAYA_API int maya_pages_fork(const maya_kv_pages* p, const int32_t* parents, const int32_t* children, const int32_t* lens, int n, void* stream);
+/* Sequences seqs[0 .. n) give up their blocks. */
+MAYA_API int maya_pages_free(const maya_kv_pages* p, const int32_t* seqs, int n, void* stream);
+/* The live blocks move to the lowest numbers, 0 .. live - 1: the i-th live one from `live` on goes to the i-th hole in front, for
+ * the first `most` of them (>= 0; n_blocks: all), so that a call's time can be bounded and the next goes on.  The table and refs follow. */
+MAYA_API int maya_pages_compact(const maya_kv_pages* p, int most, void* stream);
+/* Blocks src[i] to blocks dst[i], i < n <= n_blocks, in all layers; refs and table are not looked at.  No block may be in dst twice, nor in both. */
+MAYA_API int maya_pages_copy(const maya_kv_pages* p, const int32_t* src, const int32_t* dst, int n, void* stream);
+/* The sticky error word: 0, or 1 after a call that found too few free blocks.  Synchronises the stream. */
+MAYA_API int maya_pages_error(const maya_kv_pages* p, void* stream);
+
 /* Norm, rotation, append ---------------------------------------------------------------------------- */
 typedef struct maya_rope_args {
     const void* q;            /* [n_tokens][n_q][head_dim], rows ld_q elements apart */

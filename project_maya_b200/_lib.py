@@ -87,6 +87,12 @@ class AttnBatchDesc(C.Structure):
     _fields_ = [("start", c_void_p), ("kv_len", c_void_p), ("n_seq", c_int), ("n_tokens", c_int), ("max_new", c_int), ("max_len", c_int)]
 
 
+class KvPagesDesc(C.Structure):
+    _fields_ = [("layers", c_void_p), ("table", c_void_p), ("refs", c_void_p), ("scratch", c_void_p), ("scratch_bytes", c_size_t),
+                ("n_seq", c_int), ("table_ld", c_int), ("n_blocks", c_int), ("n_layers", c_int), ("n_kv", c_int), ("head_dim", c_int),
+                ("has_sums", c_int)]
+
+
 class RopeArgs(C.Structure):
     _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("ld_q", c_int64), ("ld_k", c_int64), ("ld_v", c_int64),
                 ("is_bf16", c_int), ("n_q", c_int), ("q_w", c_void_p), ("k_w", c_void_p), ("eps", c_float), ("cos", c_void_p),
@@ -145,6 +151,13 @@ _SIGNATURES = {
                                 c_void_p]),
     "maya_router_groups": (c_int, [C.POINTER(RouteArgs), c_void_p]),
     "maya_moe_layer_decode_routed": (c_int, [C.POINTER(MoeLayerDesc), c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "maya_pages_scratch_bytes": (c_size_t, [C.POINTER(KvPagesDesc)]),
+    "maya_pages_reserve": (c_int, [C.POINTER(KvPagesDesc), C.POINTER(AttnBatchDesc), c_void_p]),
+    "maya_pages_fork": (c_int, [C.POINTER(KvPagesDesc), c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "maya_pages_free": (c_int, [C.POINTER(KvPagesDesc), c_void_p, c_int, c_void_p]),
+    "maya_pages_compact": (c_int, [C.POINTER(KvPagesDesc), c_int, c_void_p]),
+    "maya_pages_copy": (c_int, [C.POINTER(KvPagesDesc), c_void_p, c_void_p, c_int, c_void_p]),
+    "maya_pages_error": (c_int, [C.POINTER(KvPagesDesc), c_void_p]),
     "maya_rms_q8": (c_int, [C.POINTER(RmsArgs), c_void_p]),
     "maya_q8_read": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "maya_mmq_supported": (c_int, [c_int]),

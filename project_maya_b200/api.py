@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, RouteArgs, SelectArgs
+from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, KvPagesDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, RouteArgs, SelectArgs
 
 Q8_0, Q4_K, IQ3_S, IQ2_S = 8, 12, 21, 22
 Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ1_S, IQ4_XS = 13, 14, 16, 18, 19, 23      # decode paths only (see maya_ggml_type in the header)
@@ -823,6 +823,81 @@ class AttnBatch:
             start.append(start[-1] + n)
         return cls(torch.tensor(start, dtype=torch.int32, device=device), torch.tensor(list(kv_len), dtype=torch.int32, device=device),
                    start[-1], max(new, default=0), max(kv_len, default=0), min((n for m, n in zip(new, kv_len) if m), default=0))
+
+
+class KvPages:
+    """The blocks of one or more layers' caches (KvCaches over one table, of one shape), handed out, shared and taken back on the device: nothing here
+    waits for the GPU, and captured calls do in a replay what they would then do.  refs i32 [n_blocks]: how many entries of the table hold a block (0: free; None:
+    counted from the table here).  Table entries without a block are -1.  A call that needs blocks gets the free ones of the lowest numbers, of those that are
+    free when it begins; too few leave -1 behind, and error() says so.  One thread and one stream at a time (include/maya_attn.h)."""
+
+    def __init__(self, caches, refs=None):
+        first = caches[0]
+        shape = lambda c: (c.table.data_ptr(), c.table.shape, c.n_blocks, c.n_kv, c.head_dim, c.k_sum is None, c.k.device)   # noqa: E731
+        assert all(shape(c) == shape(first) for c in caches), "caches of one table and one shape expected"
+        dev, table = first.k.device, first.table
+        if refs is None:
+            held = table[(table >= 0) & (table < first.n_blocks)].long()
+            refs = torch.bincount(held, minlength=first.n_blocks).to(torch.int32)
+        assert refs.dtype is torch.int32 and refs.shape == (first.n_blocks,) and refs.device == dev and table.device == dev
+        self.caches, self.table, self.refs = list(caches), table, refs
+        self.n_blocks, self.n_seq = first.n_blocks, table.shape[0]
+        self._layers = torch.tensor([[0 if t is None else t.data_ptr() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_sum)] for c in caches],
+                                    dtype=torch.int64).to(dev)
+        self.desc = KvPagesDesc(_ptr(self._layers), _ptr(table), _ptr(refs), None, 0, table.shape[0], table.shape[1], first.n_blocks, len(caches), first.n_kv,
+                                first.head_dim, int(first.k_sum is not None))
+        nbytes = int(_lib.load().maya_pages_scratch_bytes(C.byref(self.desc)))
+        if nbytes == 0:
+            raise MayaError("pages_scratch_bytes", -1)
+        self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self.scratch[:256].zero_()
+        self.desc.scratch, self.desc.scratch_bytes = self.scratch.data_ptr(), nbytes
+        self.live = self.scratch[8:12].view(torch.int32)     # i32 [1]: live blocks as the last compact() found them
+        self._ref = C.byref(self.desc)
+
+    def _list(self, what, *lists):
+        _here(what, self.scratch, *lists)
+        n = lists[0].numel()
+        assert all(t.dtype is torch.int32 and t.numel() == n for t in lists)
+        return n, *(_ptr(t) for t in lists)
+
+    def reserve(self, batch: AttnBatch, stream=None) -> None:
+        """Blocks for the batch's new tokens, in front of append(): entries without one get one, a block that other sequences hold too is replaced by a
+        block of the sequence's own (with a copy of the tokens from before in it)."""
+        _here("pages_reserve", self.scratch, batch.start, batch.kv_len)
+        _check("pages_reserve", _lib.load().maya_pages_reserve(self._ref, batch._ref, _stream(stream)))
+
+    def fork(self, parents, children, lens, stream=None) -> None:
+        """i32 [n] each: sequence children[i] becomes the first lens[i] tokens of sequence parents[i], all at once (a beam search's step).  Full blocks are
+        shared, one that is not full is copied; what the children held is given up.  A child that is its own parent is left as it is."""
+        n, p, c, k = self._list("pages_fork", parents, children, lens)
+        _check("pages_fork", _lib.load().maya_pages_fork(self._ref, p, c, k, n, _stream(stream)))
+
+    def free(self, seqs, stream=None) -> None:
+        """Sequences seqs (i32 [n]) give up their blocks; their table rows are -1."""
+        n, s = self._list("pages_free", seqs)
+        _check("pages_free", _lib.load().maya_pages_free(self._ref, s, n, _stream(stream)))
+
+    def compact(self, most: int | None = None, stream=None) -> None:
+        """The live blocks move to the lowest numbers, tables and counts with them: all that lie too high, or the `most` lowest of these (the next call
+        goes on).  `live` says how many blocks are live."""
+        _here("pages_compact", self.scratch)
+        _check("pages_compact", _lib.load().maya_pages_compact(self._ref, self.n_blocks if most is None else most, _stream(stream)))
+
+    def copy(self, src, dst, stream=None) -> None:
+        """Blocks src[i] to blocks dst[i] (i32 [n]) in all layers.  No block twice in dst, none in both."""
+        n, s, d = self._list("pages_copy", src, dst)
+        _check("pages_copy", _lib.load().maya_pages_copy(self._ref, s, d, n, _stream(stream)))
+
+    def error(self, stream=None) -> int:
+        """1 after a call that found too few free blocks (synchronises the stream); the word is zeroed then."""
+        code = int(_lib.load().maya_pages_error(self._ref, _stream(stream)))
+        if code < 0:
+            raise MayaError("pages_error", code)
+        if code > 0:
+            self.scratch[:4].zero_()
+            torch.cuda.current_stream(self.scratch.device).synchronize()      # (the next call may be on another stream)
+        return code
 
 
 class Rope:
