@@ -416,7 +416,7 @@ def _own_pages(st):
         r = st["round"]
         st["round"] = (r + 1) % len(st["leave"])
         pages.free(st["leave"][r])
-        pages.compact()
+        pages.compact(c["some"] * _blocks(c["len"]))
         pages.reserve(st["batches"][r])
     return _pages_out(st)
 
