@@ -127,6 +127,33 @@ MAYA_API int maya_swiglu_q8_1(const float* gate, const float* up, float limit, i
 MAYA_API int maya_mmvq(int ggml_type, const void* weights, const void* x_q8_1, float* y, int n_in, int n_out,
                        int ncols, void* stream);
 
+/* Low-rank adapters ------------------------------------------------------------------------------- */
+/* No counterpart in the reference: what adapters of many requests add beside a projection that all share,
+ *   out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t], and out[t] = y[t] where idx[t] is outside 0 .. n_adapters - 1,
+ * in f32 (prompts: matrix instructions over operands in two parts, 22 bits at least, sums in f32).  Which kernel serves a call goes by its sizes, so a token's
+ * bits may differ between calls of other numbers of tokens; the same call gives the same bits.
+ * x, out and y (NULL: zeros) are [n_tokens] rows ld_* elements apart; out may be y (the same ld), otherwise they overlap nothing.  x, a and b are 16-byte
+ * aligned, ld_x a multiple of 16 bytes; n_in % 32 == 0; rank a multiple of 16 (smaller ranks are padded with zeros).
+ * scratch: maya_lora_scratch_bytes(n_in, rank, n_adapters, at least n_tokens) bytes, 256-byte aligned; nothing needs clearing; one stream at a time. */
+#define MAYA_MAX_LORA_RANK 256
+#define MAYA_MAX_LORA_TOKENS 65535
+typedef struct maya_lora_args {
+    const void* x;               /* [n_tokens][n_in] f32 or bf16 */
+    const float* y;              /* [n_tokens][n_out] or NULL */
+    float* out;                  /* [n_tokens][n_out] */
+    const void* a;               /* [n_adapters][rank][n_in] bf16 or f16 */
+    const void* b;               /* [n_adapters][n_out][rank] */
+    const float* scale;          /* [n_adapters] or NULL: 1 */
+    const int* idx;              /* [n_tokens] */
+    void* scratch;
+    size_t scratch_bytes;
+    int64_t ld_x, ld_y, ld_out;
+    int n_tokens, n_in, n_out, rank, n_adapters;
+    int x_is_bf16, w_is_f16;
+} maya_lora_args;
+MAYA_API size_t maya_lora_scratch_bytes(int n_in, int rank, int n_adapters, int max_tokens);     /* 0 for sizes that are refused */
+MAYA_API int maya_lora(const maya_lora_args* a, void* stream);
+
 /* Decode experts (plan form) ---------------------------------------------------------------------- */
 /* The part of MoeDev the expert kernels read (glm_fast.hpp:293-300): k blob addresses (0 = entry skipped),
  * k router weights, optional CPU-lane partial and flag, optional skip flag (non-zero = do nothing). */

@@ -66,6 +66,12 @@ class HcPostArgs(C.Structure):
     _fields_ = [("R_old", c_void_p), ("post", c_void_p), ("comb", c_void_p), ("R_new", c_void_p)]
 
 
+class LoraArgs(C.Structure):
+    _fields_ = [("x", c_void_p), ("y", c_void_p), ("out", c_void_p), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p), ("idx", c_void_p),
+                ("scratch", c_void_p), ("scratch_bytes", c_size_t), ("ld_x", c_int64), ("ld_y", c_int64), ("ld_out", c_int64), ("n_tokens", c_int),
+                ("n_in", c_int), ("n_out", c_int), ("rank", c_int), ("n_adapters", c_int), ("x_is_bf16", c_int), ("w_is_f16", c_int)]
+
+
 class RouteArgs(C.Structure):
     _fields_ = [("logits", c_void_p), ("bias", c_void_p), ("n_tokens", c_int), ("n_expert", c_int), ("k", c_int), ("n_group", c_int),
                 ("n_keep", c_int), ("sigmoid", c_int), ("top2", c_int), ("norm_w", c_int), ("w_scale", c_float), ("ids", c_void_p),
@@ -158,6 +164,8 @@ _SIGNATURES = {
     "maya_pages_compact": (c_int, [C.POINTER(KvPagesDesc), c_int, c_void_p]),
     "maya_pages_copy": (c_int, [C.POINTER(KvPagesDesc), c_void_p, c_void_p, c_int, c_void_p]),
     "maya_pages_error": (c_int, [C.POINTER(KvPagesDesc), c_void_p]),
+    "maya_lora_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "maya_lora": (c_int, [C.POINTER(LoraArgs), c_void_p]),
     "maya_rms_q8": (c_int, [C.POINTER(RmsArgs), c_void_p]),
     "maya_q8_read": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "maya_mmq_supported": (c_int, [c_int]),

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, KvPagesDesc, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, RouteArgs, SelectArgs
+from ._lib import AttnArgs, AttnBatchDesc, ExpertLayout, HcPostArgs, KvCacheDesc, KvPagesDesc, LoraArgs, MmqProduct, MoeLayerDesc, MoePlan, MoeWin, RmsArgs, RopeArgs, RouteArgs, SelectArgs
 
 Q8_0, Q4_K, IQ3_S, IQ2_S = 8, 12, 21, 22
 Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ1_S, IQ4_XS = 13, 14, 16, 18, 19, 23      # decode paths only (see maya_ggml_type in the header)
@@ -181,6 +181,47 @@ def native_mmvq(ggml_type: int, weights, x_q8_1, n_in: int, n_out: int, ncols: i
     _check("native_mmvq", _lib.load().maya_mmvq(ggml_type, _ptr(weights), _ptr(x_q8_1), _ptr(y), n_in, n_out, ncols,
                                                _stream(stream)))
     return y
+
+
+# ---------------------------------------------------------------- low-rank adapters
+class LoraAdapters:
+    """Low-rank adapters of one projection, of which every token uses its own or none: out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t].
+
+    a [n, rank, n_in] and b [n, n_out, rank] bf16 or f16, scale f32 [n] or None (1); they are kept as they are, or - where the rank is not a multiple
+    of 16 - as copies padded with zeros.  n_in % 32 == 0, rank <= 256.  max_tokens sizes the scratch, which belongs to this object: one thread and one
+    stream at a time."""
+
+    def __init__(self, a, b, scale=None, max_tokens: int = 4096):
+        n, rank, n_in = a.shape
+        n_out = b.shape[1]
+        assert b.shape == (n, n_out, rank) and a.dtype is b.dtype and a.dtype in (torch.bfloat16, torch.float16)
+        assert scale is None or (scale.dtype is torch.float32 and scale.shape == (n,))
+        wide = -(-rank // 16) * 16
+        if wide != rank:
+            a, b = torch.nn.functional.pad(a, (0, 0, 0, wide - rank)), torch.nn.functional.pad(b, (0, wide - rank))
+        self.a, self.b, self.scale, self.rank, self.n_in, self.n_out, self.max_tokens = a, b, scale, wide, n_in, n_out, max_tokens
+        nbytes = int(_lib.load().maya_lora_scratch_bytes(n_in, wide, n, max_tokens))
+        if nbytes == 0:
+            raise MayaError("lora_scratch_bytes", -1)
+        self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+        self._fixed = _ptr(a), _ptr(b), _ptr(scale)
+        self._sizes = n_in, n_out, wide, n
+
+    def forward(self, x, idx, y=None, out=None, stream=None):
+        """x [T, n_in] f32 or bf16, idx i32 [T] (outside 0 .. n - 1: no adapter), y f32 [T, n_out] (None: zeros) -> out f32 [T, n_out], which may be y."""
+        _here("lora", self.scratch, x, idx, y, out)
+        T = x.shape[0]
+        if out is None:
+            out = torch.empty((T, self.n_out), dtype=torch.float32, device=x.device)
+        assert idx.dtype is torch.int32 and idx.shape == (T,) and out.dtype is torch.float32 and (y is None or y.dtype is torch.float32)
+        xp, ld_x = _matrix(x, (T, self.n_in))
+        op, ld_out = _matrix(out, (T, self.n_out))
+        yp, ld_y = (None, self.n_out) if y is None else _matrix(y, (T, self.n_out))
+        a, b, scale = self._fixed
+        args = LoraArgs(xp, yp, op, a, b, scale, _ptr(idx), self.scratch.data_ptr(), self.scratch.numel(), ld_x, ld_y, ld_out, T, *self._sizes,
+                        x.dtype is torch.bfloat16, self.a.dtype is torch.float16)
+        _check("lora", _lib.load().maya_lora(C.byref(args), _stream(stream)))
+        return out
 
 
 # ---------------------------------------------------------------- decode experts

@@ -1,0 +1,153 @@
+"""Low-rank adapters of many tokens beside a shared projection, against the formula in 64 bits.
+
+Tolerance, from the arithmetic: with m = sum_k |A_rk x_k| of a rank's sum and M = |scale| sum_r |B_nr| m_r, z is off by at most u m where u = 2^-16: sums of up to 8192 products in f32 whose
+partial sums are rounded (each at most 128 in a row, then a tree or pieces: 160 * 2^-24 < 2^-16) or cut (matrix instructions) and operands of 22 bits (2^-21 in
+all); the second product, up to 256 ranks, likewise, and the addition to y rounds once: |error| <= 2^-15 M + 2^-23 (|y| + M).
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale=True, seed=0, lead=0, gap=0, adapters=None, in_place=False):
+    from project_maya_b200 import api
+    g = T.Generator(device="cuda").manual_seed(seed + tokens + n_in)
+    randn = lambda *s: T.randn(s, generator=g, device="cuda")   # noqa: E731
+    a, b = (randn(n, rank, n_in) / n_in ** 0.5).to(weights), (randn(n, n_out, rank) / rank ** 0.5).to(weights)
+    sc = 0.1 + randn(n).abs() if scale else None
+    x = randn(tokens, lead + n_in + gap).to(act)[:, lead:lead + n_in]
+    yy = randn(tokens, n_out + gap)[:, :n_out] if y else None
+    if idx is None:
+        idx = T.randint(-1, n, (tokens,), generator=g, device="cuda", dtype=T.int32)
+    ad = adapters or api.LoraAdapters(a, b, sc, max_tokens=tokens)
+    want, big = (yy.double().clone() if y else T.zeros((tokens, n_out), device="cuda", dtype=T.float64)), T.zeros((tokens, n_out), device="cuda", dtype=T.float64)
+    for i in range(n):
+        rows = (idx == i).nonzero().flatten()
+        if len(rows):
+            s = float(sc[i]) if scale else 1.0
+            xd, ad64, bd = x[rows].double(), a[i].double(), b[i].double()
+            want[rows] += s * (xd @ ad64.T @ bd.T)
+            big[rows] = abs(s) * (xd.abs() @ ad64.abs().T @ bd.abs().T)
+    base = yy.clone() if y else None
+    if in_place:
+        out = ad.forward(x, idx, yy, out=yy)
+        assert out is yy
+    else:
+        out = ad.forward(x, idx, yy)
+        assert not y or T.equal(yy, base)
+    err = (out.double() - want).abs()
+    size = base.double().abs() if y else 0.0
+    assert bool((err <= 2.0 ** -15 * big + 2.0 ** -23 * (size + big) + 1e-37).all()), float((err - 2.0 ** -15 * big).max())
+    none = (idx < 0) | (idx >= n)
+    assert T.equal(out[none], base[none] if y else T.zeros_like(out[none]))
+    return ad, x, idx, yy, out
+
+
+TYPES = [("float32", "bfloat16"), ("float32", "float16"), ("bfloat16", "bfloat16"), ("bfloat16", "float16")]
+
+
+@pytest.mark.parametrize("act,weights", TYPES)
+@pytest.mark.parametrize("tokens,n_in,n_out,rank,n", [(1, 32, 1, 1, 1), (1, 4096, 6144, 16, 8), (3, 544, 257, 8, 2), (16, 2048, 1000, 64, 5), (64, 4096, 512, 16, 24),
+                                                      (33, 1024, 333, 24, 40), (2, 8192, 130, 256, 3), (100, 512, 96, 100, 7)])
+def test_tokens(cuda, act, weights, tokens, n_in, n_out, rank, n):
+    import torch as T
+    check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights))
+
+
+@pytest.mark.parametrize("act,weights", TYPES)
+@pytest.mark.parametrize("tokens,n_in,n_out,rank,n", [(200, 1024, 640, 16, 3), (257, 2080, 1001, 64, 2), (1000, 512, 300, 8, 50), (700, 4096, 264, 32, 1),
+                                                      (300, 96, 6144, 48, 5), (513, 1024, 200, 128, 4), (300, 1024, 72, 256, 2), (2500, 640, 129, 16, 300)])
+def test_prompts(cuda, act, weights, tokens, n_in, n_out, rank, n):
+    import torch as T
+    check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights))
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 300, 900])
+def test_who_uses_which(cuda, tokens):
+    """Everyone the same, everyone none, numbers outside, runs of requests."""
+    import torch as T
+    i32 = lambda v: T.tensor(v, dtype=T.int32, device="cuda")   # noqa: E731
+    for idx in ([1] * tokens, [-1] * tokens, [(7, -9, 3, 1 << 30)[t % 4] for t in range(tokens)], [t * 5 // tokens - 1 for t in range(tokens)],
+                [0] * (tokens - 1) + [3]):
+        check(T, tokens, 512, 320, 16, 4, T.float32, T.bfloat16, idx=i32(idx))
+
+
+@pytest.mark.parametrize("tokens", [5, 300])
+def test_without_y_or_scale_in_place_and_rows_apart(cuda, tokens):
+    import torch as T
+    for n_out in (256, 301):
+        check(T, tokens, 512, n_out, 16, 3, T.float32, T.bfloat16, y=False)
+        check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, scale=False)
+        check(T, tokens, 512, n_out, 16, 3, T.float32, T.bfloat16, in_place=True)
+        check(T, tokens, 512, n_out, 16, 3, T.bfloat16, T.bfloat16, lead=8, gap=24)
+        check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, lead=4, gap=12, in_place=True)
+
+
+@pytest.mark.parametrize("tokens", [3, 400])
+def test_large_and_small_values(cuda, tokens):
+    """Rows of 1e30 beside rows of 1e-30: each token by itself."""
+    import torch as T
+    from project_maya_b200 import api
+    a, b = (T.randn((2, 16, 512), device="cuda") / 22).bfloat16(), (T.randn((2, 256, 16), device="cuda") / 4).bfloat16()
+    ad = api.LoraAdapters(a, b, max_tokens=tokens)
+    x = T.randn((tokens, 512), device="cuda")
+    idx = (T.arange(tokens, device="cuda") % 2).int()
+    out = ad.forward(x, idx)
+    up = 2.0 ** ((T.arange(tokens, device="cuda") % 3 - 1) * 90).float()[:, None]
+    got = ad.forward(x * up, idx)
+    assert bool(((got / up - out).abs() <= 2.0 ** -20 * out.abs().amax(1, keepdim=True)).all())
+    x[1, 5] = float("nan")
+    x[2, 7] = float("inf")
+    bad = ad.forward(x, idx)
+    assert bool(bad[1].isnan().all()) and not bool(bad[2].isfinite().any())
+    keep = [t for t in range(tokens) if t not in (1, 2)]
+    assert T.equal(bad[keep], out[keep])
+
+
+@pytest.mark.parametrize("tokens", [4, 500])
+def test_the_same_call_again_another_stream_and_captured(cuda, tokens):
+    import torch as T
+    ad, x, idx, y, out = check(T, tokens, 1024, 520, 32, 6, T.float32, T.bfloat16)
+    assert T.equal(ad.forward(x, idx, y), out)
+    s = T.cuda.Stream()
+    s.wait_stream(T.cuda.current_stream())
+    with T.cuda.stream(s):
+        other = ad.forward(x, idx, y)
+    s.synchronize()
+    assert T.equal(other, out)
+    g, got = T.cuda.CUDAGraph(), T.empty_like(out)
+    with T.cuda.graph(g, stream=s):
+        ad.forward(x, idx, y, out=got)
+    x2, idx2 = x.flip(0).clone(), idx.flip(0).clone()
+    want = ad.forward(x2, idx2, y)
+    x.copy_(x2)
+    idx.copy_(idx2)
+    g.replay()
+    assert T.equal(got, want)
+
+
+def test_beside_a_product(cuda):
+    """The shared projection (GGUF rows), then the adapters onto its output."""
+    import torch as T
+    from project_maya_b200 import api
+    w = api.synth_weights(api.Q8_0, 1, 0.02, 256, 512)
+    for tokens in (1, 8):
+        x = T.randn((tokens, 512), device="cuda")
+        a, b = (T.randn((3, 16, 512), device="cuda") / 22).half(), (T.randn((3, 256, 16), device="cuda") / 4).half()
+        ad, idx = api.LoraAdapters(a, b), T.tensor([t % 4 - 1 for t in range(tokens)], dtype=T.int32, device="cuda")
+        y = api.native_mmvq(api.Q8_0, w, api.native_quantize_q8_1(x), 512, 256, tokens)
+        delta = ad.forward(x, idx)
+        both = ad.forward(x, idx, y)
+        assert bool(((both - (y + delta)).abs() <= 2.0 ** -22 * (y.abs() + delta.abs())).all())
+        assert T.equal(ad.forward(x, idx, y, out=y), both)
+
+
+def test_more_tokens_than_the_scratch_is_for(cuda):
+    import torch as T
+    from project_maya_b200 import api
+    ad = api.LoraAdapters(T.zeros((1, 16, 64), device="cuda").half(), T.zeros((1, 64, 16), device="cuda").half(), max_tokens=4)
+    with pytest.raises(api.MayaError) as e:
+        ad.forward(T.zeros((5, 64), device="cuda"), T.zeros(5, dtype=T.int32, device="cuda"))
+    assert e.value.status == -4
+    assert ad.forward(T.zeros((0, 64), device="cuda"), T.zeros(0, dtype=T.int32, device="cuda")).shape == (0, 64)
