@@ -130,11 +130,12 @@ MAYA_API int maya_mmvq(int ggml_type, const void* weights, const void* x_q8_1, f
 /* Low-rank adapters ------------------------------------------------------------------------------- */
 /* No counterpart in the reference: what adapters of many requests add beside a projection that all share,
  *   out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t], and out[t] = y[t] where idx[t] is outside 0 .. n_adapters - 1,
- * in f32 (prompts: matrix instructions over operands in two parts, 22 bits at least, sums in f32).  Which kernel serves a call goes by its sizes, so a token's
+ * in f32 (prompts: matrix instructions over operands in as many parts as hold all their bits, sums in f32).  Which kernel serves a call goes by its sizes, so a token's
  * bits may differ between calls of other numbers of tokens; the same call gives the same bits.
  * x, out and y (NULL: zeros) are [n_tokens] rows ld_* elements apart; out may be y (the same ld), otherwise they overlap nothing.  x, a and b are 16-byte
  * aligned, ld_x a multiple of 16 bytes; n_in % 32 == 0; rank a multiple of 16 (smaller ranks are padded with zeros).
- * scratch: maya_lora_scratch_bytes(n_in, rank, n_adapters, at least n_tokens) bytes, 256-byte aligned; nothing needs clearing; one stream at a time. */
+ * scratch: maya_lora_scratch_bytes(n_in, rank, n_adapters, at least n_tokens) bytes, 256-byte aligned, its first 256 zeroed before the first use; one stream
+ * at a time.  Waits are bounded: one that ran out sets its first word (sticky; the call's out is not valid), which maya_lora_error answers. */
 #define MAYA_MAX_LORA_RANK 256
 #define MAYA_MAX_LORA_TOKENS 65535
 typedef struct maya_lora_args {
@@ -153,6 +154,7 @@ typedef struct maya_lora_args {
 } maya_lora_args;
 MAYA_API size_t maya_lora_scratch_bytes(int n_in, int rank, int n_adapters, int max_tokens);     /* 0 for sizes that are refused */
 MAYA_API int maya_lora(const maya_lora_args* a, void* stream);
+MAYA_API int maya_lora_error(const void* scratch, void* stream);       /* synchronises the stream */
 
 /* Decode experts (plan form) ---------------------------------------------------------------------- */
 /* The part of MoeDev the expert kernels read (glm_fast.hpp:293-300): k blob addresses (0 = entry skipped),

@@ -165,6 +165,7 @@ _SIGNATURES = {
     "maya_pages_copy": (c_int, [C.POINTER(KvPagesDesc), c_void_p, c_void_p, c_int, c_void_p]),
     "maya_pages_error": (c_int, [C.POINTER(KvPagesDesc), c_void_p]),
     "maya_lora_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "maya_lora_error": (c_int, [c_void_p, c_void_p]),
     "maya_lora": (c_int, [C.POINTER(LoraArgs), c_void_p]),
     "maya_rms_q8": (c_int, [C.POINTER(RmsArgs), c_void_p]),
     "maya_q8_read": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),

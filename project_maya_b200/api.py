@@ -204,6 +204,7 @@ class LoraAdapters:
         if nbytes == 0:
             raise MayaError("lora_scratch_bytes", -1)
         self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+        self.scratch[:256].zero_()
         self._fixed = _ptr(a), _ptr(b), _ptr(scale)
         self._sizes = n_in, n_out, wide, n
 
@@ -222,6 +223,16 @@ class LoraAdapters:
                         x.dtype is torch.bfloat16, self.a.dtype is torch.float16)
         _check("lora", _lib.load().maya_lora(C.byref(args), _stream(stream)))
         return out
+
+    def error(self, stream=None) -> int:
+        """1 after a call whose bounded wait ran out (its output is not valid); synchronises the stream.  The word is zeroed then."""
+        code = int(_lib.load().maya_lora_error(self.scratch.data_ptr(), _stream(stream)))
+        if code < 0:
+            raise MayaError("lora_error", code)
+        if code > 0:
+            self.scratch[:4].zero_()
+            torch.cuda.current_stream(self.scratch.device).synchronize()
+        return code
 
 
 # ---------------------------------------------------------------- decode experts

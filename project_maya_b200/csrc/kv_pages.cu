@@ -13,11 +13,11 @@
 // in the scratch.  Sources and destinations are disjoint: blocks are handed out that were free when the call began, and a compaction moves across its
 // border.  Reference counts change by atomic additions of whole numbers alone, in any order the same.
 #include "maya_kv.cuh"
+#include "maya_scan.cuh"
 
 namespace maya {
 namespace {
 
-constexpr int kPlan = 1024;                    // threads that count and rank
 constexpr int kRefsEach = 16;                  // blocks a thread looks at in a round
 constexpr int kPieceBytes = 16384;             // of keys or values that a thread block copies at a time
 constexpr int kCopyThreads = 256;
@@ -65,39 +65,6 @@ int pages_ready(const maya_kv_pages* p, Pages* v) {
 }
 
 // ---------------------------------------------------------------- counting and ranking, by one thread block
-struct PlanShared {
-    int part[kPlan / 32];
-    int total;
-};
-// The sum of v over the threads in front of this one; total: over all.
-__device__ __forceinline__ int rank_of(int v, PlanShared& sh, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int incl = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
-    }
-    if (lane == 31) sh.part[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-        const int mine = sh.part[lane];
-        int in = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, in, o);
-            if (lane >= o) in += u;
-        }
-        sh.part[lane] = in - mine;
-        if (lane == 31) sh.total = in;
-    }
-    __syncthreads();
-    const int r = sh.part[warp] + incl - v;
-    total = sh.total;
-    __syncthreads();                                      // (the next call writes part)
-    return r;
-}
-
 // Bit i: block b0 + i is held by the table (blocks from n on: `beyond`).
 __device__ __forceinline__ unsigned live_bits(const Pages& P, int b0, bool beyond) {
     unsigned m = 0u;

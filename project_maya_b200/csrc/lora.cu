@@ -10,41 +10,15 @@
 //
 // Few tokens (lora_z_kernel, lora_out_kernel): each token reads its adapter's matrices, out of L2 where tokens share one.  What bounds a step of decode
 // is latency: two launches, two round trips each.
-#include "maya_common.cuh"
+#include "maya_lora.cuh"
 
 namespace maya {
 namespace {
 
-struct Lora {
-    const void* x;
-    const float* y;
-    float* out;
-    const void* a;
-    const void* b;
-    const float* scale;
-    const int* idx;
-    float* z;                    // [pieces][n_tokens][rank]
-    int64_t ld_x, ld_y, ld_out;
-    int n_adapters, n_in, n_out, rank, n_tokens, pieces;
-};
-
 constexpr int kLoraRows = 4;                   // rows of A a warp multiplies: x is read once for them
 constexpr int kLoraPiece = 512;                // values of n_in a warp takes: two 16-byte loads of each row a lane
 constexpr int kLoraWarps = 8;
-
-// 8 weights of 16 bits as f32.
-template<bool F16> __device__ __forceinline__ void weights8(const uint4 u, float (&w)[8]) {
-    const uint32_t p[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (F16) {
-            const float2 f = __half22float2(*(const __half2*) &p[i]);
-            w[2 * i] = f.x; w[2 * i + 1] = f.y;
-        } else {
-            w[2 * i] = __uint_as_float(p[i] << 16); w[2 * i + 1] = __uint_as_float(p[i] & 0xFFFF0000u);
-        }
-    }
-}
+constexpr size_t kLoraWords = 256;             // bytes of the scratch in front of z: the error word of the prompts' kernels
 
 // z of one token: a warp takes four rows of A over one piece of n_in.  blockIdx.y: the token.
 template<bool XB, bool F16>
@@ -161,7 +135,17 @@ using namespace maya;
 
 extern "C" size_t maya_lora_scratch_bytes(int n_in, int rank, int n_adapters, int max_tokens) {
     if (n_in <= 0 || n_in % 32 || rank <= 0 || rank % 16 || rank > MAYA_MAX_LORA_RANK || n_adapters <= 0 || max_tokens <= 0 || max_tokens > MAYA_MAX_LORA_TOKENS) return 0;
-    return (size_t) lora_pieces(n_in) * max_tokens * rank * sizeof(float);
+    const size_t few = kLoraWords + (size_t) lora_pieces(n_in) * max_tokens * rank * sizeof(float);
+    const size_t many = lora_takes_prompt(max_tokens, n_adapters) ? lora_prompt_bytes(max_tokens, n_adapters, rank) : 0;
+    return few > many ? few : many;
+}
+
+extern "C" int maya_lora_error(const void* scratch, void* stream) {
+    if (!scratch) return refuse(MAYA_ERR_ARG);
+    int word = 0;
+    cudaStream_t s = as_stream(stream);
+    if (cudaMemcpyAsync(&word, scratch, sizeof(word), cudaMemcpyDeviceToHost, s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess) return note_launch("lora error");
+    return word;
 }
 
 extern "C" int maya_lora(const maya_lora_args* a, void* stream) {
@@ -174,7 +158,8 @@ extern "C" int maya_lora(const maya_lora_args* a, void* stream) {
     if (a->y == a->out && a->ld_y != a->ld_out) return refuse(MAYA_ERR_ARG);
     if (!aligned16(a->x) || !aligned16(a->a) || !aligned16(a->b) || (((uintptr_t) a->scratch) & 255u) || a->ld_x % (a->x_is_bf16 ? 8 : 4)) return refuse(MAYA_ERR_ARG);
     if (a->scratch_bytes < maya_lora_scratch_bytes(a->n_in, a->rank, a->n_adapters, a->n_tokens)) return refuse(MAYA_ERR_LIMIT);
-    const Lora A{a->x, a->y, a->out, a->a, a->b, a->scale, a->idx, (float*) a->scratch, a->ld_x, a->ld_y, a->ld_out, a->n_adapters, a->n_in, a->n_out,
+    const Lora A{a->x, a->y, a->out, a->a, a->b, a->scale, a->idx, (float*) ((uint8_t*) a->scratch + kLoraWords), a->ld_x, a->ld_y, a->ld_out, a->n_adapters, a->n_in, a->n_out,
                  a->rank, a->n_tokens, lora_pieces(a->n_in)};
+    if (lora_takes_prompt(a->n_tokens, a->n_adapters)) return lora_prompt(A, a->x_is_bf16, a->w_is_f16, a->scratch, as_stream(stream));
     return a->w_is_f16 ? lora_launch<true>(A, a->x_is_bf16, as_stream(stream)) : lora_launch<false>(A, a->x_is_bf16, as_stream(stream));
 }

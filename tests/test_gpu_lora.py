@@ -39,6 +39,7 @@ def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale
     err = (out.double() - want).abs()
     size = base.double().abs() if y else 0.0
     assert bool((err <= 2.0 ** -15 * big + 2.0 ** -23 * (size + big) + 1e-37).all()), float((err - 2.0 ** -15 * big).max())
+    assert ad.error() == 0
     none = (idx < 0) | (idx >= n)
     assert T.equal(out[none], base[none] if y else T.zeros_like(out[none]))
     return ad, x, idx, yy, out
