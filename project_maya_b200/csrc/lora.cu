@@ -69,23 +69,24 @@ __global__ void __launch_bounds__(32 * kLoraWarps) lora_z_kernel(const Lora A) {
     if (lane == 0) *(float4*) (A.z + ((size_t) piece * A.n_tokens + t) * A.rank + r0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
 }
 
-// out of one token: a thread an output.  The first 32 values of its row of B and its y are asked for ahead of z.
+// out of one token: a thread an output.  The first 32 values of its row of B and its y are asked for ahead of z (out of L2: L1 may hold what an earlier call
+// left there).
 template<bool F16>
 __global__ void __launch_bounds__(256) lora_out_kernel(const Lora A) {
     extern __shared__ __align__(16) float zs[];
     const int tid = threadIdx.x, n = blockIdx.x * 256 + tid, t = blockIdx.y;
-    const int i = A.idx[t];
+    const int i = __ldcg(A.idx + t);
     const bool has = i >= 0 && i < A.n_adapters, live = n < A.n_out;
     const uint4* row = (const uint4*) ((const uint16_t*) A.b + ((size_t) (has ? i : 0) * A.n_out + (live ? n : 0)) * A.rank);
     const int eights = A.rank >> 3;
     uint4 w[4];
     float y = 0.0f, s = 1.0f;
-    if (live && A.y != nullptr) y = A.y[t * A.ld_y + n];
+    if (live && A.y != nullptr) y = __ldcg(A.y + t * A.ld_y + n);
     if (has) {
-        if (A.scale != nullptr) s = A.scale[i];
+        if (A.scale != nullptr) s = __ldcg(A.scale + i);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (q < eights) w[q] = __ldg(row + q);
+            if (q < eights) w[q] = __ldcg(row + q);
     }
     grid_launch_dependents();
     grid_dependency_wait();
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(256) lora_out_kernel(const Lora A) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         if (q < eights) add(w[q], q);
-    for (int q = 4; q < eights; ++q) add(__ldg(row + q), q);
+    for (int q = 4; q < eights; ++q) add(__ldcg(row + q), q);
     if (live) A.out[t * A.ld_out + n] = __fmaf_rn(s, acc, y);
 }
 

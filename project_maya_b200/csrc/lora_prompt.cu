@@ -4,7 +4,7 @@
 //   lora_tiles_kernel  one thread block sorts the tokens by adapter into tiles of 128 rows of one adapter (tokens without one last: copied)
 //   lora_down_kernel   z = A x of a tile: a cluster of up to eight thread blocks takes a tile, each a part of n_in; their partial sums meet over
 //                      distributed shared memory, in the order of the parts, so that no partial sum leaves the chip and none depends on who is first
-//   lora_up_kernel     out = y + B z: a thread block takes a tile and 128 outputs.  Its 64 KB of y are asked for, straight into registers, before z is there.
+//   lora_up_kernel     out = y + B z: a thread block takes a tile and some groups of 64 outputs.  The first groups' y is asked for before z is there.
 // What bounds it is memory: x once, y and out once; the adapters' matrices come out of L2.
 //
 // Numbers.  The products run on bf16 matrix instructions.  An f32 is three bf16 terms cut off its mantissa, 8 bits each, exactly; an f16 weight
@@ -18,10 +18,9 @@
 namespace maya {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kDownThreads = 512;
 constexpr int kChunk = 64;                     // values of a contraction in a stage: 128 bytes of bf16 a row
 constexpr int kTileBytes = kLoraTile * kChunk * 2;
-constexpr int kOutCols = 128;                  // outputs of a thread block of lora_up_kernel
 constexpr uint32_t kBf16 = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t) (128 >> 4) << 24);       // instruction: f32 sums of bf16, 128 rows; + columns / 8 << 17
 
 struct Tiles {
@@ -53,8 +52,26 @@ __global__ void __launch_bounds__(kPlan) lora_tiles_kernel(const Lora A, const T
     grid_dependency_wait();
     for (int a = tid; a <= n; a += kPlan) count[a] = 0;
     __syncthreads();
-    auto group_of = [&](int t) { const int i = A.idx[t]; return i >= 0 && i < n ? i : n; };
-    for (int t = tid; t < A.n_tokens; t += kPlan) atomicAdd(&count[group_of(t)], 1);
+    // A place among a group's tokens for each token: one addition a group and warp (prompts are runs of one adapter), four tokens of a thread on their
+    // way at a time.  Places wait for the second pass where z will be.
+    const int lane = tid & 31;
+    int* places = (int*) G.z;
+    auto group_of = [&](int i) { return i >= 0 && i < n ? i : n; };
+    for (int t0 = 0; t0 < A.n_tokens; t0 += 4 * kPlan) {
+        int i[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) i[q] = t0 + q * kPlan + tid < A.n_tokens ? A.idx[t0 + q * kPlan + tid] : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int t = t0 + q * kPlan + tid, g = t < A.n_tokens ? group_of(i[q]) : n + 1;
+            const unsigned same = __match_any_sync(0xffffffffu, g);
+            const int first = __ffs(same) - 1;
+            int at = 0;
+            if (lane == first && g <= n) at = atomicAdd(&count[g], __popc(same));
+            at = __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1u));
+            if (t < A.n_tokens) places[t] = at;
+        }
+    }
     __syncthreads();
     int tiles = 0;
     for (int a0 = 0; a0 <= n; a0 += kPlan) {
@@ -68,7 +85,20 @@ __global__ void __launch_bounds__(kPlan) lora_tiles_kernel(const Lora A, const T
     }
     __syncthreads();
     // (which row of its tiles a token gets changes nothing that is computed for it)
-    for (int t = tid; t < A.n_tokens; t += kPlan) G.token[atomicAdd(&count[group_of(t)], 1)] = t;
+    for (int t0 = 0; t0 < A.n_tokens; t0 += 4 * kPlan) {
+        int i[4], at[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int t = t0 + q * kPlan + tid;
+            i[q] = t < A.n_tokens ? A.idx[t] : 0;
+            at[q] = t < A.n_tokens ? places[t] : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int t = t0 + q * kPlan + tid;
+            if (t < A.n_tokens) G.token[count[group_of(i[q])] + at[q]] = t;
+        }
+    }
     if (tid == 0) G.words[1] = tiles;
 }
 
@@ -111,23 +141,31 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Shared memory of lora_down_kernel: two stages of x's terms and the weights', over which the partial sums lie at the end.
+// Shared memory of lora_down_kernel: a stage of x's terms and the weights' for each set of warps, over which the partial sums lie at the end.
 __host__ __device__ constexpr int x_terms(bool x_bf16) { return x_bf16 ? 1 : 3; }
 __host__ __device__ constexpr int w_terms(bool f16) { return f16 ? 2 : 1; }
 __host__ __device__ inline int stage_bytes(bool x_bf16, bool f16, int rank) { return x_terms(x_bf16) * kTileBytes + w_terms(f16) * rank * 128; }
 __host__ __device__ inline int z_stride(int rank) { return rank + 4; }           // floats: rows of a quarter warp in different banks
-__host__ __device__ inline int down_cols(int rank) { return (3 * rank <= 256 ? 3 : 2) * rank; }       // tensor memory: the leading sums (two of them or one), the rest
+__host__ __device__ inline int down_body(bool x_bf16, bool f16, int rank) {
+    const int stages = 2 * stage_bytes(x_bf16, f16, rank), sums = kLoraTile * z_stride(rank) * 4;
+    return stages > sums ? stages : sums;
+}
+// Tensor memory: each set's leading sums and, where there is room, the rest apart.
+__host__ __device__ inline bool rest_apart(int rank) { return rank <= 128; }
+__host__ __device__ inline int set_cols(int rank) { return rest_apart(rank) ? 2 * rank : rank; }
 __host__ __device__ inline int pow2_cols(int c) { int p = 32; while (p < c) p *= 2; return p; }
 
 // ---------------------------------------------------------------- z of a tile
 // XB: x is bf16.  F16: weights are.  WI: 16-byte pieces of a weight stage a thread brings (rank * 8 / 256, rounded up).
+// Two sets of eight warps take chunks of 64 values in turn, so that one's fence, barrier and products run under the other's cutting of x into terms:
+// with one set a chunk took 1.3 us, most of it waiting (whole kernel 31 us of the case in lora.cu, two sets REPLACED_FIGURE).
 template<bool XB, bool F16, int WI>
-__global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const Tiles G, int parts) {
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t done[2];
+__global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A, const Tiles G, int parts) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t done[2];                 // of a set: its stage has been read
     __shared__ uint32_t tmem_base;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), set = warp >> 3, st = tid & 255;
     const int part = blockIdx.x % parts, tile = blockIdx.x / parts;
     grid_dependency_wait();
     grid_launch_dependents();                  // (behind the wait: what the next launch reads ahead of its own is finished)
@@ -137,8 +175,8 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int rank = A.rank, chunks = (A.n_in + kChunk - 1) / kChunk;
     const int c_first = (int) ((int64_t) chunks * part / parts), c_end = (int) ((int64_t) chunks * (part + 1) / parts);
-    const uint32_t stage = (uint32_t) stage_bytes(XB, F16, rank), w_at = x_terms(XB) * kTileBytes, w_next = (uint32_t) rank * 128;
-    const int cols = pow2_cols(down_cols(rank)), mains = down_cols(rank) / rank - 1;
+    const uint32_t stage = (uint32_t) stage_bytes(XB, F16, rank), at = smem + set * stage, w_at = at + x_terms(XB) * kTileBytes, w_next = (uint32_t) rank * 128;
+    const int cols = pow2_cols(2 * set_cols(rank));
     if (tid == 0) {
         mbar_init(&done[0], 1);
         mbar_init(&done[1], 1);
@@ -148,14 +186,16 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base, rest = tmem + (uint32_t) (mains * rank), idesc = kBf16 | ((uint32_t) (rank >> 3) << 17);
+    const bool apart = rest_apart(rank);
+    const uint32_t tmem = tmem_base, lead = tmem + (uint32_t) (set * set_cols(rank)), rest = lead + (apart ? (uint32_t) rank : 0u);
+    const uint32_t idesc = kBf16 | ((uint32_t) (rank >> 3) << 17);
 
     // this thread's pieces: 8 values of a row, four rows of x (32 apart) and WI rows of A
-    const int c8 = tid & 7;
-    const uint16_t* wrow = (const uint16_t*) A.a + ((size_t) adapter * rank + (tid >> 3)) * A.n_in + c8 * 8;
+    const int c8 = tid & 7, r0 = st >> 3;
+    const uint16_t* wrow = (const uint16_t*) A.a + ((size_t) adapter * rank + r0) * A.n_in + c8 * 8;
     int tok[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tok[i] = G.token[(size_t) tile * kLoraTile + (tid >> 3) + 32 * i];
+    for (int i = 0; i < 4; ++i) tok[i] = G.token[(size_t) tile * kLoraTile + r0 + 32 * i];
     uint4 xr[4][XB ? 1 : 2], wr[WI];
     auto load = [&](int c) {
         const int k = c * kChunk + c8 * 8;
@@ -178,20 +218,18 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
 #pragma unroll
         for (int j = 0; j < WI; ++j) {
             wr[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (in && (tid >> 3) + 32 * j < rank) wr[j] = __ldg((const uint4*) (wrow + (size_t) (32 * j) * A.n_in + c * kChunk));
+            if (in && r0 + 32 * j < rank) wr[j] = __ldg((const uint4*) (wrow + (size_t) (32 * j) * A.n_in + c * kChunk));
         }
     };
     bool lost = false;
     int issued = 0;
-    load(c_first);
-    for (int c = c_first; c < c_end; ++c, ++issued) {
-        const int it = c - c_first, s = it & 1;
-        const uint32_t at = smem + s * stage;
-        if (it >= 2) lost |= !mbar_wait(&done[s], ((it >> 1) - 1) & 1);
+    if (c_first + set < c_end) load(c_first + set);
+    for (int c = c_first + set; c < c_end; c += 2) {
+        if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
         if (!lost) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t off = sw128((tid >> 3) + 32 * i, c8);
+                const uint32_t off = sw128(r0 + 32 * i, c8);
                 if constexpr (XB) {
                     const uint32_t o[4] = {xr[i][0].x, xr[i][0].y, xr[i][0].z, xr[i][0].w};
                     st16(at + off, o);
@@ -207,20 +245,19 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
                 }
             }
 #pragma unroll
-            for (int j = 0; j < WI; ++j) {
-                const int r = (tid >> 3) + 32 * j;
-                if (r < rank) weights_to(at + w_at, sw128(r, c8), wr[j], F16, w_next);
-            }
+            for (int j = 0; j < WI; ++j)
+                if (r0 + 32 * j < rank) weights_to(w_at, sw128(r0 + 32 * j, c8), wr[j], F16, w_next);
         }
+        if (c + 2 < c_end) load(c + 2);
         fence_proxy_async();
-        if (c + 1 < c_end) load(c + 1);
-        lost = __syncthreads_or(lost);
+        lost = named_bar_or(1 + set, 256, lost);
         if (lost) break;
-        if (warp == 0) {
+        if ((warp & 7) == 0) {
             tc_fence_after();
-            const uint64_t w0 = smem_desc_sw128(at + w_at), w1 = smem_desc_sw128(at + w_at + w_next);
-            mma4_ss(tmem + (uint32_t) ((it % mains) * rank), smem_desc_sw128(at), w0, idesc, it >= mains);
-            uint32_t more = it > 0;            // the terms that are less
+            const uint64_t w0 = smem_desc_sw128(w_at), w1 = smem_desc_sw128(w_at + w_next);
+            uint32_t more = issued > 0;
+            mma4_ss(lead, smem_desc_sw128(at), w0, idesc, more);
+            if (!apart) more = 1u;             // the terms that are less
             if constexpr (!XB) {
                 mma4_ss(rest, smem_desc_sw128(at + 2 * kTileBytes), w0, idesc, more);
                 mma4_ss(rest, smem_desc_sw128(at + kTileBytes), w0, idesc, 1u);
@@ -230,32 +267,31 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
                 mma4_ss(rest, smem_desc_sw128(at), w1, idesc, more);
                 if constexpr (!XB) mma4_ss(rest, smem_desc_sw128(at + kTileBytes), w1, idesc, 1u);
             }
-            mma_commit_elect(smem_u32(&done[s]));
+            mma_commit_elect(smem_u32(&done[set]));
         }
+        ++issued;
     }
-    // the last commit stands for every product in front of it
-    const int n = c_end - c_first;
-    if (issued > 0) lost |= !mbar_wait(&done[(issued - 1) & 1], ((issued - 1) >> 1) & 1);
+    // the last commit of a set stands for every product of its in front
+    if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
     lost = __syncthreads_or(lost);
     if (lost && tid == 0) G.words[0] = 1;
     tc_fence_after();
     const int stride = z_stride(rank);
     {
-        const int row = 32 * (warp & 3) + lane, half = rank >> 1, first = (warp >> 2) * half;
-        const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16, dst = smem + (uint32_t) (row * stride) * 4u;
-        for (int c = first; c < first + half; c += 8) {
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t from = tmem + ((uint32_t) (32 * (warp & 3)) << 16), dst = smem + (uint32_t) (row * stride) * 4u, next = (uint32_t) set_cols(rank);
+        const bool both = c_end - c_first > 1, small = apart && (!XB || F16);
+        for (int c = (warp >> 2) * 8; c < rank; c += 32) {
             float v[8], u[8];
-            tmem_ld8(tmem + lanes + (uint32_t) c, v);
-            if (mains == 2 && n > 1) {
-                tmem_ld8(tmem + lanes + (uint32_t) (rank + c), u);
+            auto add = [&](uint32_t addr) {
+                tmem_ld8(addr, u);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] += u[i];
-            }
-            if constexpr (!XB || F16) {
-                tmem_ld8(rest + lanes + (uint32_t) c, u);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += u[i];
-            }
+            };
+            tmem_ld8(from + (uint32_t) c, v);
+            if (both) add(from + next + (uint32_t) c);
+            if (small) add(from + (uint32_t) (rank + c));
+            if (small && both) add(from + next + (uint32_t) (rank + c));
 #pragma unroll
             for (int i = 0; i < 8; i += 4)
                 asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t) (c + i) * 4u), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
@@ -268,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
     cluster_wait();
     const float scale = A.scale != nullptr ? A.scale[adapter] : 1.0f;
     const int quads = rank >> 2, rows = kLoraTile / parts;
-    for (int i = tid; i < rows * quads; i += kThreads) {
+    for (int i = tid; i < rows * quads; i += kDownThreads) {
         const int row = part * rows + i / quads, c = (i % quads) * 4;
         const uint32_t from = smem + (uint32_t) (row * stride + c) * 4u;
         float4 v = ld_peer(from, 0);
@@ -296,147 +332,198 @@ __global__ void __launch_bounds__(kThreads) lora_down_kernel(const Lora A, const
 }
 
 // ---------------------------------------------------------------- out of a tile
-constexpr int kStage = 32 * 33;                // floats a warp turns its rows around in
-__host__ __device__ constexpr int up_bytes(bool f16) {
-    const int operands = (3 + w_terms(f16)) * kTileBytes, turn = (kThreads / 32) * kStage * 4;
-    return (operands > turn ? operands : turn) + 1024;
-}
+// A thread block takes 128 tokens and `per` groups of 64 outputs; z's three terms stay in shared memory.  Two sets of eight warps take the groups in turn, one
+// in its products while the other writes.  y comes by asynchronous copies into places of each warp's own, two groups ahead, and a warp turns its 32 x 32
+// sums around where its y lay, so that a lane has four neighbours of a row: 16 bytes a load and store.
+constexpr int kUpThreads = 512;
+constexpr int kOutCols = 64;
+constexpr int kAhead = 2;
+constexpr int kOutBytes = kOutCols * kChunk * 2;              // a group's weights, one term
+constexpr int kWarpBytes = 32 * 32 * 4;                       // a warp's part of a group
+__host__ __device__ constexpr int up_bytes(bool f16) { return 3 * kTileBytes + 2 * w_terms(f16) * kOutBytes + 16 * kAhead * kWarpBytes + 1024; }
 
-template<bool F16>
-__global__ void __launch_bounds__(kThreads, 2) lora_up_kernel(const Lora A, const Tiles G) {
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template<int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// VEC: y and out in whole 16 bytes.  k0: the first of the up to 64 ranks that this launch adds; y is then what the launch in front left.
+template<bool F16, bool VEC>
+__global__ void __launch_bounds__(kUpThreads, 1) lora_up_kernel(const Lora A, const Tiles G, int per, int k0) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t done;
+    __shared__ __align__(8) uint64_t ready[2];                // a set's sums are there
     __shared__ uint32_t tmem_base;
-    __shared__ int tok[kLoraTile];
-    const int tid = threadIdx.x, lane = tid & 31, tile = blockIdx.y, n0 = blockIdx.x * kOutCols;
-    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    if (tile >= G.words[1]) return;
-    const int adapter = G.adapter[tile];
-    if (tid < kLoraTile) tok[tid] = G.token[(size_t) tile * kLoraTile + tid];
+    __shared__ int64_t y_at[kLoraTile], out_at[kLoraTile];    // -1: no token
+    const int tid = threadIdx.x, lane = tid & 31, tile = blockIdx.y;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), set = warp >> 3, st = tid & 255;
+    // What is read ahead of the wait was written at least two launches ago, and is read out of L2: L1 may hold what an earlier call left there.
+    if (k0 > 0 || !VEC) grid_dependency_wait();               // (y is the launch in front's out; copies of 4 bytes go through L1)
+    if (tile >= __ldcg(G.words + 1)) return;
+    const int adapter = __ldcg(G.adapter + tile);
+    if (adapter < 0 && (A.y == A.out || k0 > 0)) return;
+    if (tid < kLoraTile) {
+        const int t = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
+        y_at[tid] = t >= 0 ? t * A.ld_y : -1;
+        out_at[tid] = t >= 0 ? t * A.ld_out : -1;
+    }
     if (tid == 0) {
-        mbar_init(&done, 1);
+        mbar_init(&ready[0], 1);
+        mbar_init(&ready[1], 1);
         mbar_fence_init();
     }
     __syncthreads();
-    // a warp's part of the tile: 32 rows, 64 outputs; a lane has outputs col and col + 32 of every row
-    const int row0 = 32 * (warp & 3), col = n0 + (warp >> 2) * 64 + lane;
-    float y[32][2];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t wt = smem + 3 * kTileBytes + (uint32_t) (set * w_terms(F16) * kOutBytes);
+    const uint32_t mine = smem + 3 * kTileBytes + 2 * w_terms(F16) * kOutBytes + (uint32_t) (warp * kAhead * kWarpBytes);      // this warp's y, then its sums
+    uint8_t* mine_p = smem_raw + (mine - smem_u32(smem_raw));
+    // a lane's four outputs of rows row0, row0 + 4, ... of a group
+    const int tile_row = 32 * (warp & 3), row0 = lane >> 3, col0 = ((warp >> 2) & 1) * 32 + (lane & 7) * 4, rank = A.rank, c8 = tid & 7;
+    const int g_first = blockIdx.x * per, g_end = min(g_first + per, (A.n_out + kOutCols - 1) / kOutCols);
+    auto group = [&](int i) { return g_first + 2 * i + set; };
+    auto fetch = [&](int i) {                                 // (always closes a group of copies, so that they can be counted)
+        const int n = group(i) * kOutCols + col0;
+        if (group(i) < g_end && A.y != nullptr && n < A.n_out) {
+            const uint32_t dst = mine + (uint32_t) (i % kAhead * kWarpBytes) + 16u * lane;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) {
-        const int t = tok[row0 + r];
+            for (int r = 0; r < 8; ++r) {
+                const int64_t at = y_at[tile_row + row0 + 4 * r];
+                if (at < 0) continue;
+                if constexpr (VEC) {
+                    copy16(dst + 512u * r, A.y + at + n);
+                } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            y[r][j] = 0.0f;
-            if (A.y != nullptr && t >= 0 && col + 32 * j < A.n_out) y[r][j] = __ldcs(A.y + (int64_t) t * A.ld_y + col + 32 * j);
+                    for (int q = 0; q < 4; ++q)
+                        if (n + q < A.n_out) copy4(dst + 512u * r + 4u * q, A.y + at + n + q);
+                }
+            }
         }
-    }
-    auto store = [&](int r, int j, float v) {
-        const int t = tok[row0 + r];
-        if (t >= 0 && col + 32 * j < A.n_out) __stcs(A.out + (int64_t) t * A.ld_out + col + 32 * j, v);
+        copies_close();
     };
+    // out of group i: the sums of the warp's rows (columns of the group's half from tensor memory), turned around, and y
+    auto write = [&](int i, uint32_t sums, bool has) {
+        const int n = group(i) * kOutCols + col0;
+        float4* place = (float4*) (mine_p + i % kAhead * kWarpBytes);
+        float4 y[8];
+        copies_wait<kAhead - 1>();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) y[r] = A.y != nullptr ? place[32 * r + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (has) {
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[16];
+                tmem_ld16(sums + 16u * h, v);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)                   // (16 bytes of a row at a place that the row's number turns)
+                    place[lane * 8 + ((4 * h + c) ^ (lane & 7))] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int row = row0 + 4 * r;
+                const float4 d = place[row * 8 + ((lane & 7) ^ (row & 7))];
+                y[r].x += d.x; y[r].y += d.y; y[r].z += d.z; y[r].w += d.w;
+            }
+            __syncwarp();
+        }
+        if (n >= A.n_out) return;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int64_t at = out_at[tile_row + row0 + 4 * r];
+            if (at < 0) continue;
+            float* p = A.out + at + n;
+            if constexpr (VEC) {
+                __stcs((float4*) p, y[r]);
+            } else {
+                __stcs(p, y[r].x);
+                if (n + 1 < A.n_out) __stcs(p + 1, y[r].y);
+                if (n + 2 < A.n_out) __stcs(p + 2, y[r].z);
+                if (n + 3 < A.n_out) __stcs(p + 3, y[r].w);
+            }
+        }
+    };
+    uint4 wr[2];
+    auto weights = [&](int i) {                               // 64 rows of B, 8 pieces each, by a set's 256 threads
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int o = group(i) * kOutCols + (st >> 3) + 32 * q, k = k0 + c8 * 8;
+            wr[q] = make_uint4(0u, 0u, 0u, 0u);
+            if (k < rank && o < A.n_out && group(i) < g_end) wr[q] = __ldcg((const uint4*) ((const uint16_t*) A.b + ((size_t) adapter * A.n_out + o) * rank + k));
+        }
+    };
+    for (int i = 0; i < kAhead; ++i) fetch(i);
+    if (adapter >= 0) weights(0);
+    if (k0 == 0 && VEC) grid_dependency_wait();
     grid_launch_dependents();
-    grid_dependency_wait();
     if (adapter < 0) {
-#pragma unroll
-        for (int r = 0; r < 32; ++r)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) store(r, j, y[r][j]);
+        for (int i = 0; group(i) < g_end; ++i) {
+            write(i, 0u, false);
+            fetch(i + kAhead);
+        }
+        copies_wait<0>();
         return;
     }
-    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* base = smem_raw + (smem - smem_u32(smem_raw));
-    if (warp == 0) tmem_alloc(&tmem_base, kOutCols);         // (behind the wait: the launch in front needs tensor memory to get there)
+    if (warp == 0) tmem_alloc(&tmem_base, 2 * kOutCols);      // (behind the wait: the launch in front needs tensor memory to get there)
+    for (int i = tid; i < 3 * kLoraTile * 8; i += kUpThreads) {
+        const int c = i & 7, r = (i >> 3) & (kLoraTile - 1), q = i / (8 * kLoraTile), k = k0 + c * 8;
+        uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        if (k < rank) z = __ldcg((const uint4*) (G.z + (((size_t) tile * kLoraTile + r) * 3 + q) * rank + k));
+        const uint32_t o[4] = {z.x, z.y, z.z, z.w};
+        st16(smem + (uint32_t) (q * kTileBytes) + sw128(r, c), o);
+    }
+    fence_proxy_async();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base, idesc = kBf16 | ((uint32_t) (kOutCols >> 3) << 17);
-    const int rank = A.rank, c8 = tid & 7;
+    const uint32_t tmem = tmem_base + (uint32_t) (set * kOutCols), idesc = kBf16 | ((uint32_t) (kOutCols >> 3) << 17);
+    const uint32_t sums = tmem + ((uint32_t) tile_row << 16) + (uint32_t) (((warp >> 2) & 1) * 32);
     bool lost = false;
-    int n = 0;
-    for (int k0 = 0; k0 < rank; k0 += kChunk, ++n) {
-        if (n > 0) {                                          // one stage: ranks beyond 64 are rare
-            lost |= !mbar_wait(&done, (n - 1) & 1);
-            lost = __syncthreads_or(lost);
-            if (lost) break;
-        }
-        const bool in = k0 + c8 * 8 < rank;
-        uint4 wr[4], zr[4];
+    for (int i = 0; group(i) < g_end; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int o = n0 + (tid >> 3) + 32 * i;
-            wr[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (in && o < A.n_out) wr[i] = __ldg((const uint4*) ((const uint16_t*) A.b + ((size_t) adapter * A.n_out + o) * rank + k0 + c8 * 8));
-        }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = (tid >> 3) + 32 * i;
-                zr[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (in) zr[i] = __ldcg((const uint4*) (G.z + (((size_t) tile * kLoraTile + r) * 3 + q) * rank + k0 + c8 * 8));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t o[4] = {zr[i].x, zr[i].y, zr[i].z, zr[i].w};
-                st16(smem + q * kTileBytes + sw128((tid >> 3) + 32 * i, c8), o);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) weights_to(smem + 3 * kTileBytes, sw128((tid >> 3) + 32 * i, c8), wr[i], F16, kTileBytes);
+        for (int q = 0; q < 2; ++q) weights_to(wt, sw128((st >> 3) + 32 * q, c8), wr[q], F16, kOutBytes);
         fence_proxy_async();
-        __syncthreads();
-        if (warp == 0) {                                      // the smallest terms first: a sum is cut by less while it is small
+        weights(i + 1);
+        named_bar_sync(1 + set, 256);
+        if ((warp & 7) == 0) {                                // the smallest terms first: a sum is cut by less while it is small
             tc_fence_after();
-            const uint64_t w0 = smem_desc_sw128(smem + 3 * kTileBytes), w1 = smem_desc_sw128(smem + 4 * kTileBytes);
+            const uint64_t w0 = smem_desc_sw128(wt), w1 = smem_desc_sw128(wt + kOutBytes);
             const uint64_t z0 = smem_desc_sw128(smem), z1 = smem_desc_sw128(smem + kTileBytes), z2 = smem_desc_sw128(smem + 2 * kTileBytes);
-            mma4_ss(tmem, z2, w0, idesc, n > 0);
+            mma4_ss(tmem, z2, w0, idesc, 0u);
             if constexpr (F16) mma4_ss(tmem, z1, w1, idesc, 1u);
             mma4_ss(tmem, z1, w0, idesc, 1u);
             if constexpr (F16) mma4_ss(tmem, z0, w1, idesc, 1u);
             mma4_ss(tmem, z0, w0, idesc, 1u);
-            mma_commit_elect(smem_u32(&done));
+            mma_commit_elect(smem_u32(&ready[set]));
         }
+        lost = !mbar_wait(&ready[set], i & 1);
+        lost = named_bar_or(1 + set, 256, lost);
+        if (lost) break;                                      // nothing more is asked for or written
+        tc_fence_after();
+        write(i, sums, true);
+        fetch(i + kAhead);
+        tc_fence_before();                                    // (the sums are read, ahead of the barrier that the next products come behind)
     }
-    if (n > 0) lost |= !mbar_wait(&done, (n - 1) & 1);
-    lost = __syncthreads_or(lost);
-    if (lost && tid == 0) G.words[0] = 1;
-    tc_fence_after();
-    float* turn = (float*) base + warp * kStage;              // (every product is done: the operands' room is free)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        uint32_t v[32];
-        tmem_ld32(tmem + ((uint32_t) row0 << 16) + (uint32_t) ((warp >> 2) * 64 + 32 * j), v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) turn[lane * 33 + c] = __uint_as_float(v[c]);
-        __syncwarp();
-        if (!lost) {
-#pragma unroll
-            for (int r = 0; r < 32; ++r) store(r, j, y[r][j] + turn[r * 33 + lane]);
-        }
-        __syncwarp();
+    copies_wait<0>();
+    if (lost && st == 0) {
+        G.words[0] = 1;
+        for (unsigned i = 0; i < kMbarPolls && !mbar_try_wait(&ready[set], 0) && !mbar_try_wait(&ready[set], 1); ++i) {}
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, kOutCols);
+    if (warp == 0) tmem_dealloc(tmem_base, 2 * kOutCols);
 }
+
+constexpr int kDownMost = 226 * 1024;          // (1 KB is static)
 
 template<class K> bool raise(SmemLimit& limit, K kernel, size_t bytes) { return limit.raise((const void*) kernel, bytes); }
 
 template<bool XB, bool F16, int WI> int launch_down(const Lora& A, const Tiles& G, int parts, cudaStream_t s) {
     static SmemLimit limit;
-    // never so little that more thread blocks fit an SM than its 512 columns of tensor memory serve
-    const int cols = pow2_cols(down_cols(A.rank)), least = 227 * 1024 / (512 / cols + 1);
-    int bytes = 2 * stage_bytes(XB, F16, A.rank);
-    const int sums = kLoraTile * z_stride(A.rank) * 4;
-    if (bytes < sums) bytes = sums;
-    if (bytes < least) bytes = least;
-    bytes += 1024;
-    if (bytes > 227 * 1024 - 64) return refuse(MAYA_ERR_LIMIT);
-    if (!raise(limit, lora_down_kernel<XB, F16, WI>, 227 * 1024 - 64)) return note_launch("lora smem attribute");
+    const int bytes = down_body(XB, F16, A.rank) + 1024;
+    if (!raise(limit, lora_down_kernel<XB, F16, WI>, kDownMost)) return note_launch("lora smem attribute");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned) (G.most * parts));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kDownThreads);
     cfg.dynamicSmemBytes = (size_t) bytes;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -450,21 +537,37 @@ template<bool XB, bool F16, int WI> int launch_down(const Lora& A, const Tiles& 
     cudaLaunchKernelEx(&cfg, lora_down_kernel<XB, F16, WI>, A, G, parts);
     return note_launch("lora down");
 }
+template<bool F16, bool VEC> int launch_up(const Lora& A, const Tiles& G, int k0, cudaStream_t s) {
+    static SmemLimit limit;
+    if (!raise(limit, lora_up_kernel<F16, VEC>, up_bytes(F16))) return note_launch("lora smem attribute");
+    // groups of outputs a thread block: as many as leave one thread block an SM, an even number (each set as many)
+    const int groups = (A.n_out + kOutCols - 1) / kOutCols;
+    int per = (int) (((int64_t) groups * G.most + sm_count() - 1) / sm_count());
+    per = (per + 1) & ~1;
+    if (per > groups) per = groups;
+    launch_dependent(lora_up_kernel<F16, VEC>, dim3((unsigned) ((groups + per - 1) / per), (unsigned) G.most), dim3(kUpThreads), (size_t) up_bytes(F16), s, A, G, per, k0);
+    return note_launch("lora up");
+}
 template<bool XB, bool F16> int launch_prompt(const Lora& A, const Tiles& G, cudaStream_t s) {
     launch_dependent(lora_tiles_kernel, dim3(1), dim3(kPlan), 0, s, A, G);
     int st = note_launch("lora tiles");
     if (st != MAYA_OK) return st;
-    // the fewest parts of n_in that give every SM two thread blocks, a chunk each at least
+    // as many parts of n_in as the SMs have thread blocks for, a quarter more at most, a chunk for each at least
     const int chunks = (A.n_in + kChunk - 1) / kChunk, tiles = (A.n_tokens + kLoraTile - 1) / kLoraTile;
     int parts = 1;
-    while (parts < 8 && 2 * parts <= chunks && tiles * parts < 2 * sm_count()) parts *= 2;
+    while (parts < 8 && 2 * parts <= chunks && tiles * parts * 2 <= sm_count() + sm_count() / 4) parts *= 2;
     st = A.rank <= 32 ? launch_down<XB, F16, 1>(A, G, parts, s) : A.rank <= 64 ? launch_down<XB, F16, 2>(A, G, parts, s)
        : A.rank <= 128 ? launch_down<XB, F16, 4>(A, G, parts, s) : launch_down<XB, F16, 8>(A, G, parts, s);
     if (st != MAYA_OK) return st;
-    static SmemLimit limit;
-    if (!raise(limit, lora_up_kernel<F16>, up_bytes(F16))) return note_launch("lora smem attribute");
-    launch_dependent(lora_up_kernel<F16>, dim3((unsigned) ((A.n_out + kOutCols - 1) / kOutCols), (unsigned) G.most), dim3(kThreads), up_bytes(F16), s, A, G);
-    return note_launch("lora up");
+    const bool vec = A.n_out % 4 == 0 && aligned16(A.out) && A.ld_out % 4 == 0 && (A.y == nullptr || (aligned16(A.y) && A.ld_y % 4 == 0));
+    Lora U = A;
+    for (int k0 = 0; k0 < A.rank; k0 += kChunk) {             // ranks beyond 64: a launch for every 64 adds to what the one in front left
+        st = vec ? launch_up<F16, true>(U, G, k0, s) : launch_up<F16, false>(U, G, k0, s);
+        if (st != MAYA_OK) return st;
+        U.y = A.out;
+        U.ld_y = A.ld_out;
+    }
+    return MAYA_OK;
 }
 
 }  // namespace
