@@ -4,7 +4,7 @@
 //   lora_tiles_kernel  one thread block sorts the tokens by adapter into tiles of 128 rows of one adapter (tokens without one last: copied)
 //   lora_down_kernel   z = A x of a tile: a cluster of up to eight thread blocks takes a tile, each a part of n_in; their partial sums meet over
 //                      distributed shared memory, in the order of the parts, so that no partial sum leaves the chip and none depends on who is first
-//   lora_up_kernel     out = y + B z: a thread block takes a tile and some groups of 64 outputs.  The first groups' y is asked for before z is there.
+//   lora_up_kernel     out = y + B z: a thread block takes a run of groups of 64 outputs of a tile.  The first one's y is asked for before z is there.
 // What bounds it is memory: x once, y and out once; the adapters' matrices come out of L2.
 //
 // Numbers.  The products run on bf16 matrix instructions.  An f32 is three bf16 terms cut off its mantissa, 8 bits each, exactly; an f16 weight
@@ -332,104 +332,79 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
 }
 
 // ---------------------------------------------------------------- out of a tile
-// A thread block takes 128 tokens and `per` groups of 64 outputs; z's three terms stay in shared memory.  Two sets of eight warps take the groups in turn, one
-// in its products while the other writes.  y comes by asynchronous copies into places of each warp's own, two groups ahead, and a warp turns its 32 x 32
-// sums around where its y lay, so that a lane has four neighbours of a row: 16 bytes a load and store.
-constexpr int kUpThreads = 512;
+// The pairs of a tile and a group of 64 outputs are shared out evenly, one run of them a thread block.  z's three terms lie in tensor memory; a group's products run
+// under the write-back of the one in front.  A warp turns its 32 x 32 sums around in shared memory, so that a lane has four neighbours of a row: 16
+// bytes a load of y and a store of out.  y is on its way in registers from the last group's write-back on.
+// Ways to this (the kernel alone, case in lora.cu, us): a thread block a tile and 128 outputs, 4 bytes a lane 53; several groups a thread block with the
+// loads of y between the uses of the last ones, each of which then waits for the loads in front of it, 145; outputs as the product's rows, so
+// that nothing has to be turned, 124 and, with fewer instructions, 83; z in shared memory, y by asynchronous copies two groups ahead, two sets of warps a thread block 51: four
+// ways through shared memory for every value beside the products' operands.
+constexpr int kUpThreads = 256;
 constexpr int kOutCols = 64;
-constexpr int kAhead = 2;
 constexpr int kOutBytes = kOutCols * kChunk * 2;              // a group's weights, one term
-constexpr int kWarpBytes = 32 * 32 * 4;                       // a warp's part of a group
-__host__ __device__ constexpr int up_bytes(bool f16) { return 3 * kTileBytes + 2 * w_terms(f16) * kOutBytes + 16 * kAhead * kWarpBytes + 1024; }
+constexpr int kTurnBytes = 32 * 32 * 4;                       // a warp's part of a group
+constexpr int kUpCols = 256;                                  // tensor memory: two groups' sums, then z: 3 * 32 columns
+__host__ __device__ constexpr int up_bytes(bool f16) { return 2 * w_terms(f16) * kOutBytes + 8 * kTurnBytes + 1024; }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const float* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copy4(uint32_t dst, const float* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template<int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// (each time anew: kept in registers over the groups, the rows' places leave too few for y)
+__device__ __forceinline__ int64_t look_up(const int64_t* p) {
+    int64_t v;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
 
 // VEC: y and out in whole 16 bytes.  k0: the first of the up to 64 ranks that this launch adds; y is then what the launch in front left.
 template<bool F16, bool VEC>
-__global__ void __launch_bounds__(kUpThreads, 1) lora_up_kernel(const Lora A, const Tiles G, int per, int k0) {
+__global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, const Tiles G, int k0) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t ready[2];                // a set's sums are there
+    __shared__ __align__(8) uint64_t ready[2];                // a group's sums are there
     __shared__ uint32_t tmem_base;
     __shared__ int64_t y_at[kLoraTile], out_at[kLoraTile];    // -1: no token
-    const int tid = threadIdx.x, lane = tid & 31, tile = blockIdx.y;
-    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), set = warp >> 3, st = tid & 255;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     // What is read ahead of the wait was written at least two launches ago, and is read out of L2: L1 may hold what an earlier call left there.
-    if (k0 > 0 || !VEC) grid_dependency_wait();               // (y is the launch in front's out; copies of 4 bytes go through L1)
-    if (tile >= __ldcg(G.words + 1)) return;
-    const int adapter = __ldcg(G.adapter + tile);
-    if (adapter < 0 && (A.y == A.out || k0 > 0)) return;
-    if (tid < kLoraTile) {
-        const int t = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
-        y_at[tid] = t >= 0 ? t * A.ld_y : -1;
-        out_at[tid] = t >= 0 ? t * A.ld_out : -1;
-    }
+    if (k0 > 0) grid_dependency_wait();                       // (y is the launch in front's out)
+    const int groups = (A.n_out + kOutCols - 1) / kOutCols;
+    const int64_t units = (int64_t) __ldcg(G.words + 1) * groups;
+    const int64_t u_end = units * (blockIdx.x + 1) / gridDim.x;
+    int64_t u = units * blockIdx.x / gridDim.x;
+    if (u >= u_end) return;
     if (tid == 0) {
         mbar_init(&ready[0], 1);
         mbar_init(&ready[1], 1);
         mbar_fence_init();
     }
-    __syncthreads();
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t wt = smem + 3 * kTileBytes + (uint32_t) (set * w_terms(F16) * kOutBytes);
-    const uint32_t mine = smem + 3 * kTileBytes + 2 * w_terms(F16) * kOutBytes + (uint32_t) (warp * kAhead * kWarpBytes);      // this warp's y, then its sums
-    uint8_t* mine_p = smem_raw + (mine - smem_u32(smem_raw));
+    float4* turn = (float4*) (smem_raw + (smem - smem_u32(smem_raw)) + 2 * w_terms(F16) * kOutBytes + warp * kTurnBytes);
     // a lane's four outputs of rows row0, row0 + 4, ... of a group
-    const int tile_row = 32 * (warp & 3), row0 = lane >> 3, col0 = ((warp >> 2) & 1) * 32 + (lane & 7) * 4, rank = A.rank, c8 = tid & 7;
-    const int g_first = blockIdx.x * per, g_end = min(g_first + per, (A.n_out + kOutCols - 1) / kOutCols);
-    auto group = [&](int i) { return g_first + 2 * i + set; };
-    auto fetch = [&](int i) {                                 // (always closes a group of copies, so that they can be counted)
-        const int n = group(i) * kOutCols + col0;
-        if (group(i) < g_end && A.y != nullptr && n < A.n_out) {
-            const uint32_t dst = mine + (uint32_t) (i % kAhead * kWarpBytes) + 16u * lane;
+    const int tile_row = 32 * (warp & 3), row0 = lane >> 3, col0 = (warp >> 2) * 32 + (lane & 7) * 4, rank = A.rank, c8 = tid & 7;
+    float4 y[8];
+    uint4 wr[2];
+    int adapter = -1;
+    auto fetch = [&](int g) {
+        const int n = g * kOutCols + col0;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const int64_t at = y_at[tile_row + row0 + 4 * r];
-                if (at < 0) continue;
-                if constexpr (VEC) {
-                    copy16(dst + 512u * r, A.y + at + n);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (n + q < A.n_out) copy4(dst + 512u * r + 4u * q, A.y + at + n + q);
-                }
+        for (int r = 0; r < 8; ++r) {
+            const int64_t at = look_up(y_at + tile_row + row0 + 4 * r);
+            y[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (A.y == nullptr || at < 0 || n >= A.n_out) continue;
+            const float* p = A.y + at + n;
+            if constexpr (VEC) {
+                y[r] = __ldcg((const float4*) p);
+            } else {
+                y[r].x = __ldcg(p);
+                if (n + 1 < A.n_out) y[r].y = __ldcg(p + 1);
+                if (n + 2 < A.n_out) y[r].z = __ldcg(p + 2);
+                if (n + 3 < A.n_out) y[r].w = __ldcg(p + 3);
             }
         }
-        copies_close();
     };
-    // out of group i: the sums of the warp's rows (columns of the group's half from tensor memory), turned around, and y
-    auto write = [&](int i, uint32_t sums, bool has) {
-        const int n = group(i) * kOutCols + col0;
-        float4* place = (float4*) (mine_p + i % kAhead * kWarpBytes);
-        float4 y[8];
-        copies_wait<kAhead - 1>();
-#pragma unroll
-        for (int r = 0; r < 8; ++r) y[r] = A.y != nullptr ? place[32 * r + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (has) {
-            __syncwarp();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[16];
-                tmem_ld16(sums + 16u * h, v);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)                   // (16 bytes of a row at a place that the row's number turns)
-                    place[lane * 8 + ((4 * h + c) ^ (lane & 7))] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const int row = row0 + 4 * r;
-                const float4 d = place[row * 8 + ((lane & 7) ^ (row & 7))];
-                y[r].x += d.x; y[r].y += d.y; y[r].z += d.z; y[r].w += d.w;
-            }
-            __syncwarp();
-        }
+    auto store = [&](int g) {
+        const int n = g * kOutCols + col0;
         if (n >= A.n_out) return;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const int64_t at = out_at[tile_row + row0 + 4 * r];
+            const int64_t at = look_up(out_at + tile_row + row0 + 4 * r);
             if (at < 0) continue;
             float* p = A.out + at + n;
             if constexpr (VEC) {
@@ -442,75 +417,135 @@ __global__ void __launch_bounds__(kUpThreads, 1) lora_up_kernel(const Lora A, co
             }
         }
     };
-    uint4 wr[2];
-    auto weights = [&](int i) {                               // 64 rows of B, 8 pieces each, by a set's 256 threads
+    auto weights = [&](int g) {                               // 64 rows of B, 8 pieces each
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int o = group(i) * kOutCols + (st >> 3) + 32 * q, k = k0 + c8 * 8;
+            const int o = g * kOutCols + (tid >> 3) + 32 * q, k = k0 + c8 * 8;
             wr[q] = make_uint4(0u, 0u, 0u, 0u);
-            if (k < rank && o < A.n_out && group(i) < g_end) wr[q] = __ldcg((const uint4*) ((const uint16_t*) A.b + ((size_t) adapter * A.n_out + o) * rank + k));
+            if (k < rank && o < A.n_out) wr[q] = __ldcg((const uint4*) ((const uint16_t*) A.b + ((size_t) adapter * A.n_out + o) * rank + k));
         }
     };
-    for (int i = 0; i < kAhead; ++i) fetch(i);
-    if (adapter >= 0) weights(0);
-    if (k0 == 0 && VEC) grid_dependency_wait();
-    grid_launch_dependents();
-    if (adapter < 0) {
-        for (int i = 0; group(i) < g_end; ++i) {
-            write(i, 0u, false);
-            fetch(i + kAhead);
+    const uint32_t idesc = kBf16 | ((uint32_t) (kOutCols >> 3) << 17);
+    uint32_t tmem = 0u;
+    int made = 0;                                             // groups whose products were issued, over all tiles
+    bool lost = false, waited = k0 > 0;
+    while (u < u_end && !lost) {
+        const int tile = (int) (u / groups), g_first = (int) (u - (int64_t) tile * groups);
+        const int g_end = (int) min((int64_t) groups, (int64_t) g_first + (u_end - u));
+        u += g_end - g_first;
+        adapter = __ldcg(G.adapter + tile);
+        if (adapter < 0 && (A.y == A.out || k0 > 0)) continue;
+        __syncthreads();                                      // (the last tile's rows have been looked up)
+        if (tid < kLoraTile) {
+            const int t = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
+            y_at[tid] = t >= 0 ? t * A.ld_y : -1;
+            out_at[tid] = t >= 0 ? t * A.ld_out : -1;
         }
-        copies_wait<0>();
-        return;
-    }
-    if (warp == 0) tmem_alloc(&tmem_base, 2 * kOutCols);      // (behind the wait: the launch in front needs tensor memory to get there)
-    for (int i = tid; i < 3 * kLoraTile * 8; i += kUpThreads) {
-        const int c = i & 7, r = (i >> 3) & (kLoraTile - 1), q = i / (8 * kLoraTile), k = k0 + c * 8;
-        uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        if (k < rank) z = __ldcg((const uint4*) (G.z + (((size_t) tile * kLoraTile + r) * 3 + q) * rank + k));
-        const uint32_t o[4] = {z.x, z.y, z.z, z.w};
-        st16(smem + (uint32_t) (q * kTileBytes) + sw128(r, c), o);
-    }
-    fence_proxy_async();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_base + (uint32_t) (set * kOutCols), idesc = kBf16 | ((uint32_t) (kOutCols >> 3) << 17);
-    const uint32_t sums = tmem + ((uint32_t) tile_row << 16) + (uint32_t) (((warp >> 2) & 1) * 32);
-    bool lost = false;
-    for (int i = 0; group(i) < g_end; ++i) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) weights_to(wt, sw128((st >> 3) + 32 * q, c8), wr[q], F16, kOutBytes);
-        fence_proxy_async();
-        weights(i + 1);
-        named_bar_sync(1 + set, 256);
-        if ((warp & 7) == 0) {                                // the smallest terms first: a sum is cut by less while it is small
+        __syncthreads();
+        fetch(g_first);
+        if (adapter >= 0) weights(g_first);
+        if (!waited) { grid_launch_dependents(); grid_dependency_wait(); waited = true; }
+        if (adapter < 0) {
+            for (int g = g_first; g < g_end; ++g) {
+                store(g);
+                if (g + 1 < g_end) fetch(g + 1);
+            }
+            continue;
+        }
+        if (tmem == 0u) {                                     // (behind the wait: the launch in front needs tensor memory to get there)
+            if (warp == 0) tmem_alloc(&tmem_base, kUpCols);
+            tc_fence_before();
+            __syncthreads();
             tc_fence_after();
-            const uint64_t w0 = smem_desc_sw128(wt), w1 = smem_desc_sw128(wt + kOutBytes);
-            const uint64_t z0 = smem_desc_sw128(smem), z1 = smem_desc_sw128(smem + kTileBytes), z2 = smem_desc_sw128(smem + 2 * kTileBytes);
-            mma4_ss(tmem, z2, w0, idesc, 0u);
-            if constexpr (F16) mma4_ss(tmem, z1, w1, idesc, 1u);
-            mma4_ss(tmem, z1, w0, idesc, 1u);
-            if constexpr (F16) mma4_ss(tmem, z0, w1, idesc, 1u);
-            mma4_ss(tmem, z0, w0, idesc, 1u);
-            mma_commit_elect(smem_u32(&ready[set]));
+            tmem = tmem_base | 0x80000000u;
         }
-        lost = !mbar_wait(&ready[set], i & 1);
-        lost = named_bar_or(1 + set, 256, lost);
-        if (lost) break;                                      // nothing more is asked for or written
+        const uint32_t tm = tmem & 0x7FFFFFFFu, z_tm = tm + 2 * kOutCols;
+#pragma unroll 1
+        for (int q = warp >> 2; q < 6; q += 2) {              // half of a row's term: 32 values in 16 columns of its lane
+            uint32_t zr[16];
+            const int k = k0 + 32 * (q & 1);
+            const uint4* zp = (const uint4*) (G.z + (((size_t) tile * kLoraTile + tile_row + lane) * 3 + (q >> 1)) * rank + k);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint4 z = make_uint4(0u, 0u, 0u, 0u);
+                if (k + c * 8 < rank) z = __ldcg(zp + c);
+                zr[4 * c] = z.x; zr[4 * c + 1] = z.y; zr[4 * c + 2] = z.z; zr[4 * c + 3] = z.w;
+            }
+            tmem_st16(z_tm + ((uint32_t) tile_row << 16) + (uint32_t) (16 * q), zr);
+        }
+        tmem_wait_st();
+        tc_fence_before();                                    // (ahead of the barrier in front of the first products)
+        auto stage = [&](int m) {                             // what `weights` brought, for the m-th products
+#pragma unroll
+            for (int q = 0; q < 2; ++q) weights_to(smem + (uint32_t) ((m & 1) * w_terms(F16) * kOutBytes), sw128((tid >> 3) + 32 * q, c8), wr[q], F16, kOutBytes);
+        };
+        auto issue = [&]() {                                  // by one warp; the smallest terms first: a sum is cut by less while it is small
+            if (warp == 0) {
+                const uint32_t wt = smem + (uint32_t) ((made & 1) * w_terms(F16) * kOutBytes), d = tm + (uint32_t) ((made & 1) * kOutCols);
+                const uint64_t w0 = smem_desc_sw128(wt), w1 = smem_desc_sw128(wt + kOutBytes);
+                mma4_ts(d, z_tm + 64u, w0, idesc, 0u);
+                if constexpr (F16) mma4_ts(d, z_tm + 32u, w1, idesc, 1u);
+                mma4_ts(d, z_tm + 32u, w0, idesc, 1u);
+                if constexpr (F16) mma4_ts(d, z_tm, w1, idesc, 1u);
+                mma4_ts(d, z_tm, w0, idesc, 1u);
+                mma_commit_elect(smem_u32(&ready[made & 1]));
+            }
+            ++made;
+        };
+        int writes = made;
+        stage(made);
+        if (g_first + 1 < g_end) {
+            weights(g_first + 1);
+            stage(made + 1);
+        }
+        fence_proxy_async();
+        __syncthreads();
         tc_fence_after();
-        write(i, sums, true);
-        fetch(i + kAhead);
-        tc_fence_before();                                    // (the sums are read, ahead of the barrier that the next products come behind)
+        issue();
+        if (g_first + 1 < g_end) issue();
+        for (int g = g_first; g < g_end; ++g, ++writes) {
+            lost = !mbar_wait(&ready[writes & 1], (writes >> 1) & 1);
+            tc_fence_after();
+            if (g + 2 < g_end) weights(g + 2);                // (used below, ahead of the next loads of y: a use waits for what was asked for since, too)
+            if (!lost) {
+                const uint32_t sums = tm + ((uint32_t) tile_row << 16) + (uint32_t) ((writes & 1) * kOutCols + (warp >> 2) * 32);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[16];
+                    tmem_ld16(sums + 16u * h, v);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)               // (16 bytes of a row at a place that the row's number turns)
+                        turn[lane * 8 + ((4 * h + c) ^ (lane & 7))] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int row = row0 + 4 * r;
+                    const float4 d = turn[row * 8 + ((lane & 7) ^ (row & 7))];
+                    y[r].x += d.x; y[r].y += d.y; y[r].z += d.z; y[r].w += d.w;
+                }
+                __syncwarp();
+                store(g);
+                if (g + 2 < g_end) stage(writes);             // (these products are done: their weights' room is free)
+            }
+            if (g + 1 < g_end) fetch(g + 1);
+            fence_proxy_async();
+            tc_fence_before();                                // (the sums are read, ahead of the barrier that the next products into them come behind)
+            lost = __syncthreads_or(lost);
+            tc_fence_after();
+            if (lost) break;                                  // nothing more is asked for
+            if (g + 2 < g_end) issue();
+        }
     }
-    copies_wait<0>();
-    if (lost && st == 0) {
-        G.words[0] = 1;
-        for (unsigned i = 0; i < kMbarPolls && !mbar_try_wait(&ready[set], 0) && !mbar_try_wait(&ready[set], 1); ++i) {}
+    if (lost) {
+        if (tid == 0) G.words[0] = 1;
+        for (int m = made; m > 0 && m > made - 2; --m) mbar_wait(&ready[(m - 1) & 1], ((m - 1) >> 1) & 1);        // what is in flight gets its time
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, 2 * kOutCols);
+    if (tmem != 0u) {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 0) tmem_dealloc(tmem & 0x7FFFFFFFu, kUpCols);
+    }
 }
 
 constexpr int kDownMost = 226 * 1024;          // (1 KB is static)
@@ -540,12 +575,8 @@ template<bool XB, bool F16, int WI> int launch_down(const Lora& A, const Tiles& 
 template<bool F16, bool VEC> int launch_up(const Lora& A, const Tiles& G, int k0, cudaStream_t s) {
     static SmemLimit limit;
     if (!raise(limit, lora_up_kernel<F16, VEC>, up_bytes(F16))) return note_launch("lora smem attribute");
-    // groups of outputs a thread block: as many as leave one thread block an SM, an even number (each set as many)
-    const int groups = (A.n_out + kOutCols - 1) / kOutCols;
-    int per = (int) (((int64_t) groups * G.most + sm_count() - 1) / sm_count());
-    per = (per + 1) & ~1;
-    if (per > groups) per = groups;
-    launch_dependent(lora_up_kernel<F16, VEC>, dim3((unsigned) ((groups + per - 1) / per), (unsigned) G.most), dim3(kUpThreads), (size_t) up_bytes(F16), s, A, G, per, k0);
+    const int64_t most = (int64_t) ((A.n_out + kOutCols - 1) / kOutCols) * G.most, blocks = 2 * sm_count();
+    launch_dependent(lora_up_kernel<F16, VEC>, dim3((unsigned) (most < blocks ? most : blocks)), dim3(kUpThreads), (size_t) up_bytes(F16), s, A, G, k0);
     return note_launch("lora up");
 }
 template<bool XB, bool F16> int launch_prompt(const Lora& A, const Tiles& G, cudaStream_t s) {
