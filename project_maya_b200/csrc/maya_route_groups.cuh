@@ -4,10 +4,15 @@
 //   a group's score: its highest c, or the sum of its two highest;  the n_keep best groups are kept (ties: the lower group)
 //   the k highest c of the kept groups' experts (ties: the lower expert);  w = s / max(sum of the k s, 2^-14) * w_scale
 //
-// The choice compares neighbours - of 256 sigmoid scores two lie within 1e-6 of each other all the time - so scores, sums and comparisons are in
-// 64 bits and only the weights are rounded, once.  A score that is no number ranks behind every number.
+// The choice compares neighbours - of 256 sigmoid scores two lie within 1e-6 of each other all the time - so it is the one that scores, sums and
+// comparisons in 64 bits make, and only the weights are rounded, once.  A score that is no number ranks behind every number.
 //
-// A lane holds experts lane, lane + 32, ... in registers as 64-bit numbers that order like the scores.  A warp's maximum of them is three
+// Nearly always 32 bits can tell: scores of a known error decide every comparison that matters (the border of the kept groups, each of the k choices
+// against the next) when the values are further apart than that, and only the k weights are computed in 64 bits, a lane each (route_fast).  Where two are
+// nearer - one token in some hundreds - or a score is not finite, everything is done over in 64 bits (route_exact).  8192 tokens of 256 experts: 28 us in 64 bits
+// alone, most of it exponentials and 64-bit comparisons.
+//
+// A lane holds experts lane, lane + 32, ... in registers as whole numbers that order like the scores.  In 64 bits a warp's maximum of them is three
 // warp-wide reductions of 32 bits (high words; low words of the lanes that have the highest; the lowest expert of those that have both), where
 // a butterfly would exchange three words five times.  Groups cut across lanes: their scores are found in shared memory, a few lanes a group.
 #pragma once
@@ -62,10 +67,10 @@ __host__ __device__ inline int route_lanes(int n_group) {
 // Words between the groups in shared memory: the lanes that start on different groups find different banks.
 __host__ __device__ inline int route_stride(int size, int lanes) { return ((size + lanes - 1) / lanes) * lanes + lanes; }
 
-// One token by the calling warp.  keys: n_group * route_stride(...) words of shared memory, this warp's own (not needed when every group is kept).
-// Lane i < 32 returns in id[j], w[j] the choice number j * 32 + i and its weight (j < 2).
+// One token by the calling warp, in 64 bits.  keys: n_group * route_stride(...) words of shared memory, this warp's own (not needed when every group is
+// kept).  Lane i < 32 returns in id[j], w[j] the choice number j * 32 + i and its weight (j < 2).
 template<int PER>
-__device__ __forceinline__ void route_groups_warp(const RouteGroups& A, int64_t token, unsigned long long* keys, int lane, int (&id)[2], float (&w)[2]) {
+__device__ __noinline__ void route_exact(const RouteGroups& A, int64_t token, unsigned long long* keys, int lane, int (&id)[2], float (&w)[2]) {
     const float* l = A.logits + token * A.n_expert;
     float lv[PER];
     float top = -INFINITY;
@@ -167,6 +172,165 @@ __device__ __forceinline__ void route_groups_warp(const RouteGroups& A, int64_t 
     const double div = A.norm_w ? fmax(sum, 6.103515625e-05) : 1.0;       // 2^-14
 #pragma unroll
     for (int j = 0; j < 2; ++j) w[j] = (float) (mine[j] / div * (double) A.w_scale);
+}
+
+// Batcher's odd-even merge sort, in registers.
+template<int N> __device__ __forceinline__ void sort_descending(uint32_t (&v)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t a = v[i + j], b = v[i + j + k];
+                        v[i + j] = max(a, b);
+                        v[i + j + k] = min(a, b);
+                    }
+}
+
+// The same where 32 bits decide; false: they do not, nothing is returned.
+// Errors: expf is within 2 ulp, its argument - for a softmax a difference, rounded - within 2^-24 of itself, at most 104 before the result is 0; quotient and sums round.
+// So a score without a bias is within 2^-16 of itself (sums of up to 2048 terms among them), a sigmoid with a bias within 2^-21 and the rounding
+// of the sum, a softmax with one within 2^-16; what lies below 2^-110 of the highest is not told apart.  kApart times these, the error of a sum of two among them, has to lie between two values.
+template<int PER>
+__device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, float* keys, int lane, int (&id)[2], float (&w)[2]) {
+    const float* l = A.logits + token * A.n_expert;
+    float s[PER];
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = j * 32 + lane;
+        s[j] = e < A.n_expert ? l[e] : -INFINITY;
+        top = fmaxf(top, s[j]);
+    }
+    float all = 0.0f;
+    if (A.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) s[j] = __fdividef(1.0f, 1.0f + expf(-s[j]));       // (1 over more than 2^126: 0)
+    } else {
+        top = warp_max(top);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            s[j] = expf(s[j] - top);           // (no number beside +inf, or where nothing is above -inf)
+            all += s[j];
+        }
+        all = warp_sum(all);
+        if (A.bias != nullptr) {
+            const float inv = __fdividef(1.0f, all);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) s[j] *= inv;
+        }
+    }
+    constexpr float kApart = 8.0f;
+    constexpr float kPlaces = (float) PER * 0x1p-23f;         // (what the places in the lowest bits take from a score)
+    const float of_itself = kApart * (A.bias == nullptr ? 0x1p-16f : 0x1p-23f) + kPlaces, fixed = A.bias == nullptr ? 0x1p-110f : kApart * (A.sigmoid ? 0x1p-21f : 0x1p-16f);
+    auto near = [&](float a, float b) { return !(a - b > fixed + of_itself * fmaxf(fabsf(a), fabsf(b))); };     // a >= b
+    uint32_t o[PER];
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = j * 32 + lane;
+        o[j] = 0u;
+        if (e < A.n_expert) {
+            const float c = (A.bias != nullptr ? s[j] + A.bias[e] : s[j]) + 0.0f;
+            odd |= !(fabsf(c) < 1e30f);
+            const uint32_t u = __float_as_uint(c);
+            o[j] = u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
+        }
+    }
+    if (__any_sync(0xffffffffu, odd)) return false;
+    auto value = [](uint32_t v) { return __uint_as_float(v ^ ((v >> 31) ? 0x80000000u : 0xffffffffu)); };
+    if (A.n_keep < A.n_group) {
+        const int size = A.n_expert / A.n_group, lanes = route_lanes(A.n_group), stride = route_stride(size, lanes);
+        auto group_of = [&](int e) { return size == 1 ? e : (int) __umulhi((unsigned) e, A.group_mul); };
+        uint32_t* k32 = (uint32_t*) keys;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = j * 32 + lane;
+            if (e < A.n_expert) {
+                const int q = group_of(e);
+                k32[q * stride + e - q * size] = o[j];
+            }
+        }
+        __syncwarp();
+        const int g = lane / lanes, part = lane % lanes;
+        uint32_t a = 0u, b = 0u;
+        if (g < A.n_group)
+#pragma unroll 4
+            for (int i = part; i < size; i += lanes) {
+                const uint32_t v = k32[g * stride + i];
+                b = max(b, min(a, v));
+                a = max(a, v);
+            }
+        for (int d = 1; d < lanes; d *= 2) {
+            const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, d), ob = __shfl_xor_sync(0xffffffffu, b, d);
+            b = max(max(b, ob), min(a, oa));
+            a = max(a, oa);
+        }
+        const bool mine = part == 0 && g < A.n_group;
+        const float score = A.top2 && b != 0u ? value(a) + value(b) : value(a);
+        int rank = 0;
+        for (int q = 0; q < A.n_group; ++q) {
+            const float other = __shfl_sync(0xffffffffu, score, q * lanes);
+            rank += other > score || (other == score && q < g);
+        }
+        const unsigned last = __ballot_sync(0xffffffffu, mine && rank == A.n_keep - 1), next = __ballot_sync(0xffffffffu, mine && rank == A.n_keep);
+        const float in = __shfl_sync(0xffffffffu, score, __ffs(last) - 1), out = __shfl_sync(0xffffffffu, score, __ffs(next) - 1);
+        const unsigned kept = __ballot_sync(0xffffffffu, mine && rank < A.n_keep);
+        if (near(in, out)) return false;       // (all lanes alike)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = j * 32 + lane;
+            if (e < A.n_expert && !((kept >> (group_of(e) * lanes)) & 1u)) o[j] = 0u;
+        }
+        __syncwarp();
+    }
+    // every lane's scores in order, their places in the lowest bits; a round takes the highest of the lanes' first ones
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (o[j] != 0u) o[j] = (o[j] & ~(uint32_t) (PER - 1)) | (uint32_t) j;
+    sort_descending(o);
+    id[0] = id[1] = 0;
+    uint32_t before = 0u;
+    for (int i = 0; i <= A.k; ++i) {           // one more than is taken: the last has to be apart from it
+        const uint32_t best = __reduce_max_sync(0xffffffffu, o[0]);
+        if (i > 0 && best != 0u && near(value(before), value(best))) return false;
+        if (i == A.k) break;
+        before = best;
+        const unsigned who = __ballot_sync(0xffffffffu, o[0] == best);
+        if (__popc(who) != 1) return false;    // equal ones
+        const int from = __ffs(who) - 1;
+        if (lane == (i & 31)) id[i >> 5] = (int) (best & (uint32_t) (PER - 1)) * 32 + from;
+        if (lane == from) {
+#pragma unroll
+            for (int j = 0; j + 1 < PER; ++j) o[j] = o[j + 1];
+            o[PER - 1] = 0u;
+        }
+    }
+    double v[2] = {0.0, 0.0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (j * 32 + lane < A.k) {
+            const double x = (double) l[id[j]];
+            v[j] = A.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double) top);
+        }
+    const double sum = warp_sum64(v[0] + v[1]);
+    // a softmax's scores lack the division by the sum of all, which nothing but the least divisor asks for: far from it, or in 64 bits
+    if (!A.sigmoid && !(sum > 2.0 * 6.103515625e-05 * (double) all)) return false;
+    const double div = A.sigmoid ? (A.norm_w ? fmax(sum, 6.103515625e-05) : 1.0) : sum;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) w[j] = (float) (v[j] / div * (double) A.w_scale);
+    return true;
+}
+
+template<int PER>
+__device__ __forceinline__ void route_groups_warp(const RouteGroups& A, int64_t token, unsigned long long* keys, int lane, int (&id)[2], float (&w)[2]) {
+    const bool can = A.sigmoid || A.norm_w;    // (a softmax's own scores need the sum of all in 64 bits)
+    if (can && route_fast<PER>(A, token, (float*) keys, lane, id, w)) return;
+    route_exact<PER>(A, token, keys, lane, id, w);
 }
 
 }  // namespace maya

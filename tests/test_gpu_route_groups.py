@@ -115,6 +115,27 @@ def test_neighbours_that_f32_cannot_tell_apart(cuda):
     check(T, logits, 8)
 
 
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("spread", [0.01, 1.5, 40.0])
+def test_many_tokens(cuda, sigmoid, spread):
+    """Tens of thousands of borders, among them all degrees of nearness, with and without a bias."""
+    import torch as T
+    from project_maya_b200 import api
+    T.manual_seed(int(spread * 100))
+    logits, bias = spread * T.randn((20000, 256), device="cuda"), 0.05 * T.randn(256, device="cuda")
+    for b in (bias, None):
+        s = T.sigmoid(logits.double()) if sigmoid else T.softmax(logits.double(), -1)
+        c = s if b is None else s + b.double()
+        groups = c.view(-1, 8, 32).sort(dim=-1, descending=True).values[..., :2].sum(-1).sort(dim=-1, descending=True, stable=True).indices[:, :4]
+        seen = T.zeros((20000, 8), dtype=T.bool, device="cuda").scatter_(1, groups, True).repeat_interleave(32, 1)
+        want = c.masked_fill(~seen, -float("inf")).sort(dim=-1, descending=True, stable=True).indices[:, :8]
+        ids, w = api.router_groups(logits, 8, 8, 4, b, sigmoid)
+        assert T.equal(ids.long(), want)
+        p = s.gather(1, want)
+        p = p / p.sum(-1, keepdim=True).clamp(min=2.0 ** -14)
+        assert bool(((w.double() - p).abs() <= 2.0 ** -23 * p + 1e-44).all())
+
+
 def test_the_same_beside_others_and_captured(cuda):
     import torch as T
     from project_maya_b200 import api
