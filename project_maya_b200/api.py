@@ -142,10 +142,10 @@ def router_groups(logits, k: int, n_group: int = 1, n_keep: int = 1, bias=None, 
     T, E = logits.shape
     _here("router_groups", logits, bias, ids, weights)
     assert logits.dtype is torch.float32 and (bias is None or (bias.dtype is torch.float32 and bias.numel() == E))
-    if ids is None:
-        ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
     if weights is None:
-        weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+        weights = logits.new_empty((T, k))
+    if ids is None:
+        ids = torch.empty_like(weights, dtype=torch.int32)
     assert ids.dtype is torch.int32 and weights.dtype is torch.float32 and ids.numel() == weights.numel() == T * k
     a = RouteArgs(_ptr(logits), _ptr(bias), T, E, k, n_group, n_keep, sigmoid, top2, norm_w, w_scale, _ptr(ids), _ptr(weights))
     _check("router_groups", _lib.load().maya_router_groups(C.byref(a), _stream(stream)))
@@ -369,7 +369,7 @@ def rms_q8(h, add, norm_w, eps: float, image: int | None = XQ_Q8_1, xq=None, h_o
     if image is not None:
         need = xq_bytes(image, T, n)
         if xq is None:
-            xq = torch.empty(max(need, 16), dtype=torch.uint8, device=h.device)
+            xq = h.new_empty(need or 16, dtype=torch.uint8)
         assert xq.numel() * xq.element_size() >= need, "xq is too small"
     else:
         assert xq is None
@@ -388,8 +388,7 @@ def q8_read(xq, rows: int, n: int, image: int = XQ_Q8_1, dtype=torch.bfloat16, s
     """8-bit rows as the values they stand for: (values [rows, n] of dtype bf16 or f32, sums f16 [rows, n / 32] of their groups before rounding)."""
     _here("q8_read", xq)
     assert dtype in (torch.float32, torch.bfloat16) and xq.numel() * xq.element_size() >= xq_bytes(image, rows, n)
-    values = torch.empty((rows, n), dtype=dtype, device=xq.device)
-    sums = torch.empty((rows, n // 32), dtype=torch.float16, device=xq.device)
+    values, sums = xq.new_empty((rows, n), dtype=dtype), xq.new_empty((rows, n >> 5), dtype=torch.float16)
     _check("q8_read", _lib.load().maya_q8_read(_ptr(xq), image, rows, n, int(dtype is torch.bfloat16), _ptr(values), _ptr(sums), _stream(stream)))
     return values, sums
 

@@ -8,9 +8,9 @@
 //   compact  the live blocks take the lowest numbers: the i-th live block behind the border moves into the i-th hole in front of it, or only the first so many
 //   copy     blocks to blocks
 //
-// Two or three launches a call.  What is counted and ranked - a few thousand numbers - is one thread block's work, since every rank depends on all in front
-// of it; the rows of a fork's table take a thread block each; and what moves is copied by as many thread blocks as fit, who find the list and its length
-// in the scratch.  Sources and destinations are disjoint: blocks are handed out that were free when the call began, and a compaction moves across its
+// Two launches a call (free and copy: one).  What is counted and ranked - a few thousand numbers - is one thread block's work, since every rank depends on all in
+// front of it; its time is the latency of four to six look-ups, one behind the other.  What moves is copied by as many thread blocks as fit, who find the list
+// and its length in the scratch.  Sources and destinations are disjoint: blocks are handed out that were free when the call began, and a compaction moves across its
 // border.  Reference counts change by atomic additions of whole numbers alone, in any order the same.
 #include "maya_kv.cuh"
 #include "maya_scan.cuh"
@@ -80,12 +80,14 @@ __device__ __forceinline__ unsigned live_bits(const Pages& P, int b0, bool beyon
     }
     return m;
 }
-// list[0 .. need) = the free blocks of the lowest numbers; returns how many there are.  Ends with the block synchronised.
-__device__ __forceinline__ int take_free(const Pages& P, int need, PlanShared& sh) {
+// list[0 .. need) = the free blocks of the lowest numbers; returns how many there are.  bits: live_bits of the first round, asked for while something else was
+// waited for.  Ends with the block synchronised.
+__device__ __forceinline__ int take_free(const Pages& P, int need, unsigned bits, PlanShared& sh) {
     int found = 0;
     for (int c0 = 0; c0 < P.n_blocks && found < need; c0 += kPlan * kRefsEach) {
         const int b0 = c0 + threadIdx.x * kRefsEach;
-        unsigned open = ~live_bits(P, b0, true) & 0xffffu;
+        if (c0 > 0) bits = live_bits(P, b0, true);
+        unsigned open = ~bits & 0xffffu;
         int total, r = found + rank_of(__popc(open), sh, total);
         while (open != 0u && r < need) {
             P.list[r++] = b0 + __ffs(open) - 1;
@@ -96,18 +98,21 @@ __device__ __forceinline__ int take_free(const Pages& P, int need, PlanShared& s
     __syncthreads();
     return min(found, need);
 }
+// Numbers of sequences in shared memory where they fit (a look-up there takes a tenth of one in the scratch).
+constexpr int kSeqShared = 4096;
 __device__ __forceinline__ bool is_block(const Pages& P, int b) { return b >= 0 && b < P.n_blocks; }
 
 // ---------------------------------------------------------------- reserve
 // Items: the (sequence, block) that new tokens fall into, in that order.
 __global__ void __launch_bounds__(kPlan) pages_reserve_kernel(const Pages P, const BatchView B) {
     __shared__ PlanShared sh;
-    __shared__ int s_moves;
+    __shared__ int s_moves, s_first[kSeqShared];
     const int tid = threadIdx.x;
     grid_launch_dependents();
     grid_dependency_wait();
+    int* first = B.n_seq <= kSeqShared ? s_first : P.owner;   // items in front of every sequence
+    const unsigned bits = live_bits(P, tid * kRefsEach, true);
     if (tid == 0) s_moves = 0;
-    // items in front of every sequence
     int items = 0;
     for (int s0 = 0; s0 < B.n_seq; s0 += kPlan) {
         const int s = s0 + tid;
@@ -118,51 +123,48 @@ __global__ void __launch_bounds__(kPlan) pages_reserve_kernel(const Pages P, con
         }
         int total;
         const int r = rank_of(n, sh, total);
-        if (s < B.n_seq) P.owner[s] = items + r;
+        if (s < B.n_seq) first[s] = items + r;
         items += total;
     }
     __syncthreads();
-    auto find = [&](int i, int& s, int& b, bool& held) {      // item i: its sequence and block, and whether the block holds tokens from before
+    auto find = [&](int i, int& at, bool& held) {             // item i: its place in the table, and whether the block holds tokens from before
         int lo = 0, hi = B.n_seq - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (P.owner[mid] <= i) lo = mid; else hi = mid - 1;
+            if (first[mid] <= i) lo = mid; else hi = mid - 1;
         }
-        s = lo;
-        const Seq q = seq_of(B, s);
-        const int old = max(0, q.len - q.n_new);
-        b = old / kKvBlock + i - P.owner[s];
+        const Seq q = seq_of(B, lo);
+        const int old = max(0, q.len - q.n_new), b = old / kKvBlock + i - first[lo];
+        at = lo * P.table_ld + b;                             // (n_seq * table_ld is held below 2^28)
         held = b * kKvBlock < old;
     };
     // what each needs, by the counts as they are before anything changes
-    int need = 0;
+    int need = 0, at = 0, e = -1, r = -1;
+    bool held = false;
     for (int i0 = 0; i0 < items; i0 += kPlan) {
         const int i = i0 + tid;
         int want = 0;
-        int* at = nullptr;
         if (i < items) {
-            int s, b;
-            bool held;
-            find(i, s, b, held);
-            const int e = P.table[(size_t) s * P.table_ld + b];
-            at = P.rows + (size_t) s * P.table_ld + b;
+            find(i, at, held);
+            e = P.table[at];
             want = !is_block(P, e) || __ldcg(P.refs + e) > 1;
         }
         int total;
-        const int r = rank_of(want, sh, total);
-        if (at != nullptr) *at = want ? need + r : -1;
+        r = rank_of(want, sh, total);
+        r = want ? need + r : -1;
+        if (i < items && items > kPlan) P.rows[at] = r;       // (one round: it stays in registers)
         need += total;
     }
-    const int got = take_free(P, need, sh);
+    const int got = take_free(P, need, bits, sh);
     if (tid == 0 && got < need) P.words[0] = 1;
     for (int i = tid; i < items; i += kPlan) {
-        int s, b;
-        bool held;
-        find(i, s, b, held);
-        const int r = P.rows[(size_t) s * P.table_ld + b];
+        if (items > kPlan) {
+            find(i, at, held);
+            r = P.rows[at];
+            e = P.table[at];
+        }
         if (r < 0) continue;
-        int* entry = P.table + (size_t) s * P.table_ld + b;
-        const int e = *entry, fresh = r < got ? P.list[r] : -1;
+        const int fresh = r < got ? P.list[r] : -1;
         if (fresh >= 0) P.refs[fresh] = 1;
         if (is_block(P, e)) {
             atomicSub(P.refs + e, 1);
@@ -172,72 +174,19 @@ __global__ void __launch_bounds__(kPlan) pages_reserve_kernel(const Pages P, con
                 P.dst[m] = fresh;
             }
         }
-        *entry = fresh;
+        P.table[at] = fresh;
     }
     __syncthreads();
     if (tid == 0) P.words[1] = s_moves;
 }
 
 // ---------------------------------------------------------------- fork
-__global__ void __launch_bounds__(kPlan) pages_fork_kernel(const Pages P, const int* __restrict__ parents, const int* __restrict__ children,
-                                                           const int* __restrict__ lens, int n) {
-    __shared__ PlanShared sh;
-    const int tid = threadIdx.x;
-    grid_launch_dependents();
-    grid_dependency_wait();
-    // the first pair of a child counts
-    for (int i = tid; i < n; i += kPlan) {
-        const int c = children[i];
-        if (c >= 0 && c < P.n_seq) __stcg(P.owner + c, 0x7fffffff);
-    }
-    __syncthreads();
-    for (int i = tid; i < n; i += kPlan) {
-        const int c = children[i];
-        if (c >= 0 && c < P.n_seq) atomicMin(P.owner + c, i);
-    }
-    __syncthreads();
-    int need = 0;
-    for (int i0 = 0; i0 < n; i0 += kPlan) {
-        const int i = i0 + tid;
-        int want = 0, from = -1;
-        bool moves = false;
-        if (i < n) {
-            const int p = parents[i], c = children[i];
-            moves = p >= 0 && p < P.n_seq && c >= 0 && c < P.n_seq && p != c && __ldcg(P.owner + c) == i;
-            const int len = min(max(lens[i], 0), P.table_ld * kKvBlock);
-            if (moves && len % kKvBlock != 0) from = P.table[(size_t) p * P.table_ld + len / kKvBlock];
-            want = is_block(P, from);
-        }
-        int total;
-        const int r = need + rank_of(want, sh, total);
-        if (want) P.src[r] = from;                        // (the list of moves is the list of wants)
-        if (i < n) P.fresh[i] = want ? r : moves ? -1 : -2;
-        need += total;
-    }
-    const int got = take_free(P, need, sh);
-    for (int i = tid; i < n; i += kPlan) {
-        const int r = P.fresh[i];
-        if (r < 0) continue;
-        const int b = r < got ? P.list[r] : -1;
-        P.fresh[i] = b;
-        if (b >= 0) { P.refs[b] = 1; P.dst[r] = b; }
-    }
-    if (tid == 0) {
-        P.words[1] = got;
-        if (got < need) P.words[0] = 1;
-    }
-}
-// A pair's new row, and what it and the old one change of the counts.  The table itself stays: other pairs still read it.
-__global__ void __launch_bounds__(256) pages_fork_rows_kernel(const Pages P, const int* __restrict__ parents, const int* __restrict__ children,
-                                                              const int* __restrict__ lens) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const int i = blockIdx.x, fresh = P.fresh[i];
-    if (fresh == -2) return;
-    const int* from = P.table + (size_t) parents[i] * P.table_ld;
-    const int* old = P.table + (size_t) children[i] * P.table_ld;
-    const int full = min(max(lens[i], 0), P.table_ld * kKvBlock) / kKvBlock;
-    for (int b = threadIdx.x; b < P.table_ld; b += 256) {
+// A pair's new row, and what it and the old one change of the counts, by `nt` threads.  The table itself stays: other pairs still read it.
+__device__ __forceinline__ void fork_row(const Pages& P, int i, int parent, int child, int len, int fresh, int t, int nt) {
+    const int* from = P.table + (size_t) parent * P.table_ld;
+    const int* old = P.table + (size_t) child * P.table_ld;
+    const int full = min(max(len, 0), P.table_ld * kKvBlock) / kKvBlock;
+    for (int b = t; b < P.table_ld; b += nt) {
         const int gone = old[b];
         int e = -1;
         if (b < full) {
@@ -250,6 +199,75 @@ __global__ void __launch_bounds__(256) pages_fork_rows_kernel(const Pages P, con
         if (is_block(P, gone)) atomicSub(P.refs + gone, 1);
         P.rows[(size_t) i * P.table_ld + b] = e;
     }
+}
+__global__ void __launch_bounds__(256) pages_fork_rows_kernel(const Pages P, const int* __restrict__ parents, const int* __restrict__ children,
+                                                              const int* __restrict__ lens) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int i = blockIdx.x, fresh = P.fresh[i];
+    if (fresh != -2) fork_row(P, i, parents[i], children[i], lens[i], fresh, threadIdx.x, 256);
+}
+
+// rows_too: a warp a pair makes the rows as well and puts them into the table: few of them are done before another launch would have begun.
+__global__ void __launch_bounds__(kPlan) pages_fork_kernel(const Pages P, const int* __restrict__ parents, const int* __restrict__ children,
+                                                           const int* __restrict__ lens, int n, int rows_too) {
+    __shared__ PlanShared sh;
+    __shared__ int s_owner[kSeqShared];
+    const int tid = threadIdx.x;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    int* owner = P.n_seq <= kSeqShared ? s_owner : P.owner;
+    const unsigned bits = live_bits(P, tid * kRefsEach, true);
+    // the first pair of a child counts
+    for (int i = tid; i < n; i += kPlan) {
+        const int c = children[i];
+        if (c >= 0 && c < P.n_seq) owner[c] = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPlan) {
+        const int c = children[i];
+        if (c >= 0 && c < P.n_seq) atomicMin(owner + c, i);
+    }
+    __syncthreads();
+    int need = 0;
+    for (int i0 = 0; i0 < n; i0 += kPlan) {
+        const int i = i0 + tid;
+        int want = 0, from = -1;
+        bool moves = false;
+        if (i < n) {
+            const int p = parents[i], c = children[i];
+            moves = p >= 0 && p < P.n_seq && c >= 0 && c < P.n_seq && p != c && *(volatile int*) (owner + c) == i;
+            const int len = min(max(lens[i], 0), P.table_ld * kKvBlock);
+            if (moves && len % kKvBlock != 0) from = P.table[(size_t) p * P.table_ld + len / kKvBlock];
+            want = is_block(P, from);
+        }
+        int total;
+        const int r = need + rank_of(want, sh, total);
+        if (want) P.src[r] = from;                        // (the list of moves is the list of wants)
+        if (i < n) P.fresh[i] = want ? r : moves ? -1 : -2;
+        need += total;
+    }
+    const int got = take_free(P, need, bits, sh);
+    for (int i = tid; i < n; i += kPlan) {
+        const int r = P.fresh[i];
+        if (r < 0) continue;
+        const int b = r < got ? P.list[r] : -1;
+        P.fresh[i] = b;
+        if (b >= 0) { P.refs[b] = 1; P.dst[r] = b; }
+    }
+    if (tid == 0) {
+        P.words[1] = got;
+        if (got < need) P.words[0] = 1;
+    }
+    if (!rows_too) return;
+    __syncthreads();
+    const int lane = tid & 31;
+    for (int i = tid >> 5; i < n; i += kPlan / 32)
+        if (P.fresh[i] != -2) fork_row(P, i, parents[i], children[i], lens[i], P.fresh[i], lane, 32);
+    __syncthreads();
+    for (int i = tid >> 5; i < n; i += kPlan / 32)
+        if (P.fresh[i] != -2)
+            for (int b = lane; b < P.table_ld; b += 32) P.table[(size_t) children[i] * P.table_ld + b] = P.rows[(size_t) i * P.table_ld + b];
 }
 
 // ---------------------------------------------------------------- free
@@ -272,31 +290,14 @@ __global__ void __launch_bounds__(kPlan) pages_compact_kernel(const Pages P, int
     const int tid = threadIdx.x;
     grid_launch_dependents();
     grid_dependency_wait();
-    int mine = 0;
-    for (int c0 = 0; c0 < P.n_blocks; c0 += kPlan * kRefsEach) mine += __popc(live_bits(P, c0 + tid * kRefsEach, false));
-    int live;
-    rank_of(mine, sh, live);
-    // holes in front of the border
-    int holes = 0;
-    for (int c0 = 0; c0 < live && holes < most; c0 += kPlan * kRefsEach) {
-        const int b0 = c0 + tid * kRefsEach;
-        unsigned open = b0 < live ? ~live_bits(P, b0, true) & 0xffffu : 0u;
-        if (live - b0 < kRefsEach && b0 < live) open &= (1u << (live - b0)) - 1u;
-        int total, r = holes + rank_of(__popc(open), sh, total);
+    // holes of a thread's blocks (bits `open`), the first of which is hole number r; live ones behind the border (bits m) likewise
+    auto take_holes = [&](int b0, unsigned open, int r) {
         while (open != 0u && r < most) {
             P.dst[r++] = b0 + __ffs(open) - 1;
             open &= open - 1u;
         }
-        holes += total;
-    }
-    __syncthreads();
-    // live blocks behind it: as many
-    int tails = 0;
-    for (int c0 = live & ~(kRefsEach - 1); c0 < P.n_blocks; c0 += kPlan * kRefsEach) {
-        const int b0 = c0 + tid * kRefsEach;
-        unsigned m = b0 < P.n_blocks ? live_bits(P, b0, false) : 0u;
-        if (b0 < live) m &= ~((1u << (live - b0)) - 1u);
-        int total, r = tails + rank_of(__popc(m), sh, total);
+    };
+    auto move_tails = [&](int b0, unsigned m, int live, int r) {
         for (int i = 0; i < kRefsEach; ++i) {
             const int b = b0 + i;
             if (b < live || b >= P.n_blocks) continue;
@@ -310,7 +311,45 @@ __global__ void __launch_bounds__(kPlan) pages_compact_kernel(const Pages P, int
                 P.list[b] = b;
             }
         }
-        tails += total;
+    };
+    // bits of a thread's blocks in front of block `end`
+    auto below = [](int b0, int end) { return end <= b0 ? 0u : end - b0 >= kRefsEach ? 0xffffu : (1u << (end - b0)) - 1u; };
+    const int b0 = tid * kRefsEach;
+    const unsigned bits = live_bits(P, b0, false);
+    int live, tails;
+    if (P.n_blocks <= kPlan * kRefsEach) {                // one look: every rank follows from the live blocks in front
+        __shared__ int s_low;
+        const int front = rank_of(__popc(bits), sh, live);
+        if (tid == 0) s_low = live;                       // live blocks in front of the border
+        __syncthreads();
+        if (b0 <= live && live < b0 + kRefsEach) s_low = front + __popc(bits & below(b0, live));
+        if (b0 < live) take_holes(b0, ~bits & below(b0, live), b0 - front);
+        __syncthreads();
+        tails = live - s_low;
+        if (b0 + kRefsEach > live) move_tails(b0, bits & ~below(b0, live), live, front + __popc(bits & below(b0, live)) - s_low);
+    } else {
+        int mine = __popc(bits);
+        for (int c = b0 + kPlan * kRefsEach; c - b0 < P.n_blocks; c += kPlan * kRefsEach) mine += __popc(live_bits(P, c, false));
+        rank_of(mine, sh, live);
+        int holes = 0;
+        for (int c0 = 0; c0 < live && holes < most; c0 += kPlan * kRefsEach) {
+            const int c = c0 + b0;
+            const unsigned open = c < live ? ~live_bits(P, c, true) & below(c, live) : 0u;
+            int total;
+            const int r = holes + rank_of(__popc(open), sh, total);
+            take_holes(c, open, r);
+            holes += total;
+        }
+        __syncthreads();
+        tails = 0;
+        for (int c0 = live & ~(kRefsEach - 1); c0 < P.n_blocks; c0 += kPlan * kRefsEach) {
+            const int c = c0 + b0;
+            const unsigned m = c < P.n_blocks ? live_bits(P, c, false) & ~below(c, live) : 0u;
+            int total;
+            const int r = tails + rank_of(__popc(m), sh, total);
+            move_tails(c, m, live, r);
+            tails += total;
+        }
     }
     if (tid == 0) { P.words[1] = min(tails, most); P.words[2] = live; }
 }
@@ -382,13 +421,14 @@ __global__ void __launch_bounds__(kCopyThreads) pages_move_kernel(const Pages P,
     }
 }
 
-// As many thread blocks as the most there can be to do keeps busy, eight an SM at most.
+// A thread block a piece where the host knows how many there are (500 blocks of four layers 85 us, 96 with eight thread blocks an SM that go through the
+// pieces); where the count is in the scratch, as many as the most there can be to do, 16 an SM at most, since those that find nothing cost too.
 int launch_moves(const Pages& P, const int* src, const int* dst, int n_given, int64_t most, int mode, const int* children, int n_pairs, cudaStream_t s) {
     const int64_t pieces = ((int64_t) P.n_kv * kKvBlock * P.head_dim + kPieceBytes - 1) / kPieceBytes;
     int64_t blocks = most * P.n_layers * 2 * pieces;
     if (mode == kForkRows && blocks < n_pairs) blocks = n_pairs;
     if (mode == kRemap && blocks * kCopyThreads < (int64_t) P.n_seq * P.table_ld) blocks = ((int64_t) P.n_seq * P.table_ld + kCopyThreads - 1) / kCopyThreads;
-    const int64_t cap = (int64_t) sm_count() * 8;
+    const int64_t cap = n_given >= 0 ? 1 << 30 : (int64_t) sm_count() * 16;
     if (blocks > cap) blocks = cap;
     if (blocks < 1) blocks = 1;
     launch_dependent(pages_move_kernel, dim3((unsigned) blocks), dim3(kCopyThreads), 0, s, P, src, dst, n_given, mode, children, n_pairs);
@@ -434,13 +474,18 @@ extern "C" int maya_pages_fork(const maya_kv_pages* p, const int* parents, const
     if (n < 0 || !parents || !children || !lens) return refuse(MAYA_ERR_ARG);
     if (n > p->n_seq) return refuse(MAYA_ERR_LIMIT);              // more pairs than children there are
     cudaStream_t s = as_stream(stream);
-    launch_dependent(pages_fork_kernel, dim3(1), dim3(kPlan), 0, s, P, parents, children, lens, n);
+    // A warp makes a row of up to 2048 blocks in the plan's launch (32 rows of 26, with the step behind it: 14.6 us, 15.3 in a launch of their own), longer or more ones take a launch with a
+    // thread block each.
+    const bool rows_too = (int64_t) n * p->table_ld <= 16384;
+    launch_dependent(pages_fork_kernel, dim3(1), dim3(kPlan), 0, s, P, parents, children, lens, n, (int) rows_too);
     int launched = note_launch("kv_pages fork");
     if (launched != MAYA_OK) return launched;
-    launch_dependent(pages_fork_rows_kernel, dim3((unsigned) n), dim3(256), 0, s, P, parents, children, lens);
-    launched = note_launch("kv_pages fork rows");
-    if (launched != MAYA_OK) return launched;
-    return launch_moves(P, P.src, P.dst, -1, n, kForkRows, children, n, s);
+    if (!rows_too) {
+        launch_dependent(pages_fork_rows_kernel, dim3((unsigned) n), dim3(256), 0, s, P, parents, children, lens);
+        launched = note_launch("kv_pages fork rows");
+        if (launched != MAYA_OK) return launched;
+    }
+    return launch_moves(P, P.src, P.dst, -1, n, rows_too ? kMoves : kForkRows, children, n, s);
 }
 
 extern "C" int maya_pages_free(const maya_kv_pages* p, const int* seqs, int n, void* stream) {

@@ -274,6 +274,27 @@ def test_many_sequences(cuda):
     host.same(T, pages)
 
 
+@pytest.mark.parametrize("wide", [250, 700])
+def test_forks_of_long_rows(cuda, wide):
+    """Rows that the plan's thread block makes itself, and more of them than it does."""
+    import torch as T
+    rng = np.random.default_rng(wide)
+    S, nb = 60, 9000
+    lens = [int(n) for n in rng.integers(1, 130 * BLOCK, S)]
+    host = Host(rng, S, wide, nb, 1, 1, 64).fill(rng, lens)
+    host.layers[0]["v"][:] = (np.arange(nb) % 253).astype(np.uint8)[:, None, None, None]
+    pages = host.device(T)
+    for n in (3, 60, 25):
+        p, c = rng.integers(0, S, n).tolist(), rng.permutation(S)[:n].tolist()
+        k = [int(rng.integers(0, lens[a] + 1)) for a in p]
+        host.fork(p, c, k)
+        pages.fork(i32(T, p), i32(T, c), i32(T, k))
+        host.same(T, pages)
+        was = list(lens)
+        for a, b, m in zip(p, c, k):
+            lens[b] = m if a != b else was[b]
+
+
 def test_too_few_blocks(cuda):
     """What is left without a block is -1, the word says so once, and the others are whole."""
     import torch as T
