@@ -136,6 +136,11 @@ MAYA_API int maya_mmvq(int ggml_type, const void* weights, const void* x_q8_1, f
  * aligned, ld_x a multiple of 16 bytes; n_in % 32 == 0; rank a multiple of 16 (smaller ranks are padded with zeros).
  * scratch: maya_lora_scratch_bytes(n_in, rank, n_adapters, at least n_tokens) bytes, 256-byte aligned, its first 256 zeroed before the first use; one stream
  * at a time.  Waits are bounded: one that ran out sets its first word (sticky; the call's out is not valid), which maya_lora_error answers. */
+enum maya_lora_kernel {
+    MAYA_LORA_CHOICE = 0,        /* by the sizes */
+    MAYA_LORA_FEW = 1,           /* each token by itself */
+    MAYA_LORA_MANY = 2           /* tiles of tokens of one adapter on the tensor cores; up to 4096 adapters; MAYA_ERR_LIMIT where the scratch is too small for it */
+};
 #define MAYA_MAX_LORA_RANK 256
 #define MAYA_MAX_LORA_TOKENS 65535
 typedef struct maya_lora_args {
@@ -151,6 +156,7 @@ typedef struct maya_lora_args {
     int64_t ld_x, ld_y, ld_out;
     int n_tokens, n_in, n_out, rank, n_adapters;
     int x_is_bf16, w_is_f16;
+    int kernel;                  /* enum maya_lora_kernel */
 } maya_lora_args;
 MAYA_API size_t maya_lora_scratch_bytes(int n_in, int rank, int n_adapters, int max_tokens);     /* 0 for sizes that are refused */
 MAYA_API int maya_lora(const maya_lora_args* a, void* stream);

@@ -69,7 +69,7 @@ class HcPostArgs(C.Structure):
 class LoraArgs(C.Structure):
     _fields_ = [("x", c_void_p), ("y", c_void_p), ("out", c_void_p), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p), ("idx", c_void_p),
                 ("scratch", c_void_p), ("scratch_bytes", c_size_t), ("ld_x", c_int64), ("ld_y", c_int64), ("ld_out", c_int64), ("n_tokens", c_int),
-                ("n_in", c_int), ("n_out", c_int), ("rank", c_int), ("n_adapters", c_int), ("x_is_bf16", c_int), ("w_is_f16", c_int)]
+                ("n_in", c_int), ("n_out", c_int), ("rank", c_int), ("n_adapters", c_int), ("x_is_bf16", c_int), ("w_is_f16", c_int), ("kernel", c_int)]
 
 
 class RouteArgs(C.Structure):

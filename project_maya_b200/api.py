@@ -184,6 +184,9 @@ def native_mmvq(ggml_type: int, weights, x_q8_1, n_in: int, n_out: int, ncols: i
 
 
 # ---------------------------------------------------------------- low-rank adapters
+LORA_CHOICE, LORA_FEW, LORA_MANY = 0, 1, 2               # maya_lora_kernel
+
+
 class LoraAdapters:
     """Low-rank adapters of one projection, of which every token uses its own or none: out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t].
 
@@ -208,8 +211,9 @@ class LoraAdapters:
         self._fixed = _ptr(a), _ptr(b), _ptr(scale)
         self._sizes = n_in, n_out, wide, n
 
-    def forward(self, x, idx, y=None, out=None, stream=None):
-        """x [T, n_in] f32 or bf16, idx i32 [T] (outside 0 .. n - 1: no adapter), y f32 [T, n_out] (None: zeros) -> out f32 [T, n_out], which may be y."""
+    def forward(self, x, idx, y=None, out=None, kernel: int = LORA_CHOICE, stream=None):
+        """x [T, n_in] f32 or bf16, idx i32 [T] (outside 0 .. n - 1: no adapter), y f32 [T, n_out] (None: zeros) -> out f32 [T, n_out], which may be y.
+        kernel: LORA_FEW (each token by itself), LORA_MANY (tiles of one adapter's tokens) or the sizes' choice."""
         _here("lora", self.scratch, x, idx, y, out)
         T = x.shape[0]
         if out is None:
@@ -220,7 +224,7 @@ class LoraAdapters:
         yp, ld_y = (None, self.n_out) if y is None else _matrix(y, (T, self.n_out))
         a, b, scale = self._fixed
         args = LoraArgs(xp, yp, op, a, b, scale, _ptr(idx), self.scratch.data_ptr(), self.scratch.numel(), ld_x, ld_y, ld_out, T, *self._sizes,
-                        x.dtype is torch.bfloat16, self.a.dtype is torch.float16)
+                        x.dtype is torch.bfloat16, self.a.dtype is torch.float16, kernel)
         _check("lora", _lib.load().maya_lora(C.byref(args), _stream(stream)))
         return out
 

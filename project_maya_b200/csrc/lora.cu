@@ -137,7 +137,7 @@ using namespace maya;
 extern "C" size_t maya_lora_scratch_bytes(int n_in, int rank, int n_adapters, int max_tokens) {
     if (n_in <= 0 || n_in % 32 || rank <= 0 || rank % 16 || rank > MAYA_MAX_LORA_RANK || n_adapters <= 0 || max_tokens <= 0 || max_tokens > MAYA_MAX_LORA_TOKENS) return 0;
     const size_t few = kLoraWords + (size_t) lora_pieces(n_in) * max_tokens * rank * sizeof(float);
-    const size_t many = lora_takes_prompt(max_tokens, n_adapters) ? lora_prompt_bytes(max_tokens, n_adapters, rank) : 0;
+    const size_t many = lora_many_fits(max_tokens, n_adapters, rank) ? lora_prompt_bytes(max_tokens, n_adapters, rank) : 0;
     return few > many ? few : many;
 }
 
@@ -158,9 +158,14 @@ extern "C" int maya_lora(const maya_lora_args* a, void* stream) {
     if (a->ld_x < a->n_in || (a->y && a->ld_y < a->n_out) || a->ld_out < a->n_out) return refuse(MAYA_ERR_ARG);
     if (a->y == a->out && a->ld_y != a->ld_out) return refuse(MAYA_ERR_ARG);
     if (!aligned16(a->x) || !aligned16(a->a) || !aligned16(a->b) || (((uintptr_t) a->scratch) & 255u) || a->ld_x % (a->x_is_bf16 ? 8 : 4)) return refuse(MAYA_ERR_ARG);
-    if (a->scratch_bytes < maya_lora_scratch_bytes(a->n_in, a->rank, a->n_adapters, a->n_tokens)) return refuse(MAYA_ERR_LIMIT);
+    if (a->kernel < MAYA_LORA_CHOICE || a->kernel > MAYA_LORA_MANY) return refuse(MAYA_ERR_ARG);
+    bool many = a->kernel == MAYA_LORA_MANY;
+    if (a->kernel == MAYA_LORA_CHOICE) many = lora_many_better(a->n_tokens, a->n_adapters, a->rank, a->n_in + a->n_out);
+    if (many && a->n_adapters > kLoraAdaptersMost) return refuse(MAYA_ERR_LIMIT);
+    const size_t need = many ? lora_prompt_bytes(a->n_tokens, a->n_adapters, a->rank) : kLoraWords + (size_t) lora_pieces(a->n_in) * a->n_tokens * a->rank * sizeof(float);
+    if (a->scratch_bytes < need) return refuse(MAYA_ERR_LIMIT);
     const Lora A{a->x, a->y, a->out, a->a, a->b, a->scale, a->idx, (float*) ((uint8_t*) a->scratch + kLoraWords), a->ld_x, a->ld_y, a->ld_out, a->n_adapters, a->n_in, a->n_out,
                  a->rank, a->n_tokens, lora_pieces(a->n_in)};
-    if (lora_takes_prompt(a->n_tokens, a->n_adapters)) return lora_prompt(A, a->x_is_bf16, a->w_is_f16, a->scratch, as_stream(stream));
+    if (many) return lora_prompt(A, a->x_is_bf16, a->w_is_f16, a->scratch, as_stream(stream));
     return a->w_is_f16 ? lora_launch<true>(A, a->x_is_bf16, as_stream(stream)) : lora_launch<false>(A, a->x_is_bf16, as_stream(stream));
 }

@@ -376,26 +376,25 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
     }
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     float4* turn = (float4*) (smem_raw + (smem - smem_u32(smem_raw)) + 2 * w_terms(F16) * kOutBytes + warp * kTurnBytes);
-    // a lane's four outputs of rows row0, row0 + 4, ... of a group
-    const int tile_row = 32 * (warp & 3), row0 = lane >> 3, col0 = (warp >> 2) * 32 + (lane & 7) * 4, rank = A.rank, c8 = tid & 7;
-    float4 y[8];
+    // a lane's outputs of a group: four neighbours of rows row0, row0 + 4, ..., or (without VEC) one of each of the 32 rows, so that a warp has a line of a row
+    constexpr int kRows = VEC ? 8 : 32;
+    const int tile_row = 32 * (warp & 3), row0 = VEC ? lane >> 3 : 0, col0 = (warp >> 2) * 32 + (VEC ? (lane & 7) * 4 : lane), rank = A.rank, c8 = tid & 7;
+    float y[32];
     uint4 wr[2];
     int adapter = -1;
     auto fetch = [&](int g) {
         const int n = g * kOutCols + col0;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int64_t at = look_up(y_at + tile_row + row0 + 4 * r);
-            y[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (A.y == nullptr || at < 0 || n >= A.n_out) continue;
-            const float* p = A.y + at + n;
+        for (int r = 0; r < kRows; ++r) {
+            const int64_t at = look_up(y_at + tile_row + row0 + (VEC ? 4 : 1) * r);
+            const bool has = A.y != nullptr && at >= 0 && n < A.n_out;
             if constexpr (VEC) {
-                y[r] = __ldcg((const float4*) p);
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (has) v = __ldcg((const float4*) (A.y + at + n));
+                y[4 * r] = v.x; y[4 * r + 1] = v.y; y[4 * r + 2] = v.z; y[4 * r + 3] = v.w;
             } else {
-                y[r].x = __ldcg(p);
-                if (n + 1 < A.n_out) y[r].y = __ldcg(p + 1);
-                if (n + 2 < A.n_out) y[r].z = __ldcg(p + 2);
-                if (n + 3 < A.n_out) y[r].w = __ldcg(p + 3);
+                y[r] = 0.0f;
+                if (has) y[r] = __ldcg(A.y + at + n);
             }
         }
     };
@@ -403,18 +402,11 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         const int n = g * kOutCols + col0;
         if (n >= A.n_out) return;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int64_t at = look_up(out_at + tile_row + row0 + 4 * r);
+        for (int r = 0; r < kRows; ++r) {
+            const int64_t at = look_up(out_at + tile_row + row0 + (VEC ? 4 : 1) * r);
             if (at < 0) continue;
-            float* p = A.out + at + n;
-            if constexpr (VEC) {
-                __stcs((float4*) p, y[r]);
-            } else {
-                __stcs(p, y[r].x);
-                if (n + 1 < A.n_out) __stcs(p + 1, y[r].y);
-                if (n + 2 < A.n_out) __stcs(p + 2, y[r].z);
-                if (n + 3 < A.n_out) __stcs(p + 3, y[r].w);
-            }
+            if constexpr (VEC) __stcs((float4*) (A.out + at + n), make_float4(y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]));
+            else __stcs(A.out + at + n, y[r]);
         }
     };
     auto weights = [&](int g) {                               // 64 rows of B, 8 pieces each
@@ -519,10 +511,14 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
                 }
                 __syncwarp();
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int row = row0 + 4 * r;
-                    const float4 d = turn[row * 8 + ((lane & 7) ^ (row & 7))];
-                    y[r].x += d.x; y[r].y += d.y; y[r].z += d.z; y[r].w += d.w;
+                for (int r = 0; r < kRows; ++r) {
+                    if constexpr (VEC) {
+                        const int row = row0 + 4 * r;
+                        const float4 d = turn[row * 8 + ((lane & 7) ^ (row & 7))];
+                        y[4 * r] += d.x; y[4 * r + 1] += d.y; y[4 * r + 2] += d.z; y[4 * r + 3] += d.w;
+                    } else {
+                        y[r] += ((const float*) (turn + r * 8 + ((lane >> 2) ^ (r & 7))))[lane & 3];
+                    }
                 }
                 __syncwarp();
                 store(g);
@@ -603,7 +599,17 @@ template<bool XB, bool F16> int launch_prompt(const Lora& A, const Tiles& G, cud
 
 }  // namespace
 
-bool lora_takes_prompt(int n_tokens, int n_adapters) { return n_tokens >= 192 && n_adapters <= kLoraAdaptersMost && n_tokens >= 8 * n_adapters; }
+// Few tokens read their adapter's matrices one by one; these kernels begin with 17 us, and a tile that few tokens share costs 1 to 1.4 us.  Measured (4096 -> 6144, few /
+// many, us): rank 16, one adapter, 128 tokens 17 / 17, 192 25 / 20, 1024 120 / 29; 8 adapters 192 25 / 24, 256 32 / 24; 64 adapters 512 62 / 96, 1024
+// 121 / 102; rank 64, one adapter, 32 tokens 13 / 20, 64 24 / 20, 1024 332 / 34; 8 adapters 64 24 / 28, 96 33 / 28; 64 adapters 256 90 / 114, 384 132 / 115.
+static int64_t token_ranks(int n_tokens, int n_adapters, int rank) {
+    return (int64_t) n_tokens * rank - (190ll + (rank < 64 ? rank : 64)) * (n_adapters < n_tokens ? n_adapters : n_tokens);
+}
+bool lora_many_fits(int n_tokens, int n_adapters, int rank) { return n_adapters <= kLoraAdaptersMost && token_ranks(n_tokens, n_adapters, rank) > 0; }
+bool lora_many_better(int n_tokens, int n_adapters, int rank, int width) {
+    const int launches = (rank + kChunk - 1) / kChunk;        // (each adds 64 ranks and reads and writes out)
+    return lora_many_fits(n_tokens, n_adapters, rank) && token_ranks(n_tokens, n_adapters, rank) * width > 11250000ll * (launches + 1);
+}
 size_t lora_prompt_bytes(int n_tokens, int n_adapters, int rank) { return carve_tiles(n_tokens, n_adapters, rank, nullptr, nullptr); }
 
 int lora_prompt(const Lora& A, int x_is_bf16, int w_is_f16, void* scratch, cudaStream_t s) {

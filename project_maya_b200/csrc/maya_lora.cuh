@@ -35,7 +35,8 @@ template<bool F16> __device__ __forceinline__ void weights8(const uint4 u, float
 // ---- prompts (lora_prompt.cu): tokens of one adapter in tiles of kLoraTile rows
 constexpr int kLoraTile = 128;
 constexpr int kLoraAdaptersMost = 4096;        // whose tokens one thread block counts
-bool lora_takes_prompt(int n_tokens, int n_adapters);
+bool lora_many_fits(int n_tokens, int n_adapters, int rank);                         // the scratch has room for it
+bool lora_many_better(int n_tokens, int n_adapters, int rank, int width);            // width: n_in + n_out
 size_t lora_prompt_bytes(int n_tokens, int n_adapters, int rank);
 int lora_prompt(const Lora& A, int x_is_bf16, int w_is_f16, void* scratch, cudaStream_t s);
 

@@ -10,7 +10,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 
-def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale=True, seed=0, lead=0, gap=0, adapters=None, in_place=False):
+def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale=True, seed=0, lead=0, gap=0, in_place=False, kernel=0):
     from project_maya_b200 import api
     g = T.Generator(device="cuda").manual_seed(seed + tokens + n_in)
     randn = lambda *s: T.randn(s, generator=g, device="cuda")   # noqa: E731
@@ -20,7 +20,7 @@ def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale
     yy = randn(tokens, n_out + gap)[:, :n_out] if y else None
     if idx is None:
         idx = T.randint(-1, n, (tokens,), generator=g, device="cuda", dtype=T.int32)
-    ad = adapters or api.LoraAdapters(a, b, sc, max_tokens=tokens)
+    ad = api.LoraAdapters(a, b, sc, max_tokens=max(tokens, 32 * n) if kernel == api.LORA_MANY else tokens)
     want, big = (yy.double().clone() if y else T.zeros((tokens, n_out), device="cuda", dtype=T.float64)), T.zeros((tokens, n_out), device="cuda", dtype=T.float64)
     for i in range(n):
         rows = (idx == i).nonzero().flatten()
@@ -31,10 +31,10 @@ def check(T, tokens, n_in, n_out, rank, n, act, weights, idx=None, y=True, scale
             big[rows] = abs(s) * (xd.abs() @ ad64.abs().T @ bd.abs().T)
     base = yy.clone() if y else None
     if in_place:
-        out = ad.forward(x, idx, yy, out=yy)
+        out = ad.forward(x, idx, yy, out=yy, kernel=kernel)
         assert out is yy
     else:
-        out = ad.forward(x, idx, yy)
+        out = ad.forward(x, idx, yy, kernel=kernel)
         assert not y or T.equal(yy, base)
     err = (out.double() - want).abs()
     size = base.double().abs() if y else 0.0
@@ -53,7 +53,8 @@ TYPES = [("float32", "bfloat16"), ("float32", "float16"), ("bfloat16", "bfloat16
                                                       (33, 1024, 333, 24, 40), (2, 8192, 130, 256, 3), (100, 512, 96, 100, 7)])
 def test_tokens(cuda, act, weights, tokens, n_in, n_out, rank, n):
     import torch as T
-    check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights))
+    for kernel in (0, 1, 2):
+        check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights), kernel=kernel)
 
 
 @pytest.mark.parametrize("act,weights", TYPES)
@@ -61,7 +62,8 @@ def test_tokens(cuda, act, weights, tokens, n_in, n_out, rank, n):
                                                       (300, 96, 6144, 48, 5), (513, 1024, 200, 128, 4), (300, 1024, 72, 256, 2), (2500, 640, 129, 16, 300)])
 def test_prompts(cuda, act, weights, tokens, n_in, n_out, rank, n):
     import torch as T
-    check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights))
+    for kernel in (0, 2):
+        check(T, tokens, n_in, n_out, rank, n, getattr(T, act), getattr(T, weights), kernel=kernel)
 
 
 @pytest.mark.parametrize("tokens", [1, 40, 300, 900])
@@ -71,57 +73,62 @@ def test_who_uses_which(cuda, tokens):
     i32 = lambda v: T.tensor(v, dtype=T.int32, device="cuda")   # noqa: E731
     for idx in ([1] * tokens, [-1] * tokens, [(7, -9, 3, 1 << 30)[t % 4] for t in range(tokens)], [t * 5 // tokens - 1 for t in range(tokens)],
                 [0] * (tokens - 1) + [3]):
-        check(T, tokens, 512, 320, 16, 4, T.float32, T.bfloat16, idx=i32(idx))
+        for kernel in (1, 2):
+            check(T, tokens, 512, 320, 16, 4, T.float32, T.bfloat16, idx=i32(idx), kernel=kernel)
 
 
 @pytest.mark.parametrize("tokens", [5, 300])
 def test_without_y_or_scale_in_place_and_rows_apart(cuda, tokens):
     import torch as T
     for n_out in (256, 301):
-        check(T, tokens, 512, n_out, 16, 3, T.float32, T.bfloat16, y=False)
-        check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, scale=False)
-        check(T, tokens, 512, n_out, 16, 3, T.float32, T.bfloat16, in_place=True)
-        check(T, tokens, 512, n_out, 16, 3, T.bfloat16, T.bfloat16, lead=8, gap=24)
-        check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, lead=4, gap=12, in_place=True)
+        for kernel in (1, 2):
+            check(T, tokens, 512, n_out, 16, 3, T.float32, T.bfloat16, y=False, kernel=kernel)
+            check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, scale=False, kernel=kernel)
+            check(T, tokens, 512, n_out, 80, 3, T.float32, T.bfloat16, in_place=True, kernel=kernel)
+            check(T, tokens, 512, n_out, 16, 3, T.bfloat16, T.bfloat16, lead=8, gap=24, kernel=kernel)
+            check(T, tokens, 512, n_out, 16, 3, T.float32, T.float16, lead=4, gap=12, in_place=True, kernel=kernel)
+            check(T, tokens, 512, n_out, 200, 3, T.float32, T.float16, y=False, kernel=kernel)
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
 @pytest.mark.parametrize("tokens", [3, 400])
-def test_large_and_small_values(cuda, tokens):
-    """Rows of 1e30 beside rows of 1e-30: each token by itself."""
+def test_large_and_small_values(cuda, tokens, kernel):
+    """Rows of 1e27 beside rows of 1e-27: each token by itself."""
     import torch as T
     from project_maya_b200 import api
     a, b = (T.randn((2, 16, 512), device="cuda") / 22).bfloat16(), (T.randn((2, 256, 16), device="cuda") / 4).bfloat16()
-    ad = api.LoraAdapters(a, b, max_tokens=tokens)
+    ad = api.LoraAdapters(a, b, max_tokens=max(tokens, 64))
     x = T.randn((tokens, 512), device="cuda")
     idx = (T.arange(tokens, device="cuda") % 2).int()
-    out = ad.forward(x, idx)
+    out = ad.forward(x, idx, kernel=kernel)
     up = 2.0 ** ((T.arange(tokens, device="cuda") % 3 - 1) * 90).float()[:, None]
-    got = ad.forward(x * up, idx)
+    got = ad.forward(x * up, idx, kernel=kernel)
     assert bool(((got / up - out).abs() <= 2.0 ** -20 * out.abs().amax(1, keepdim=True)).all())
     x[1, 5] = float("nan")
     x[2, 7] = float("inf")
-    bad = ad.forward(x, idx)
+    bad = ad.forward(x, idx, kernel=kernel)
     assert bool(bad[1].isnan().all()) and not bool(bad[2].isfinite().any())
     keep = [t for t in range(tokens) if t not in (1, 2)]
     assert T.equal(bad[keep], out[keep])
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
 @pytest.mark.parametrize("tokens", [4, 500])
-def test_the_same_call_again_another_stream_and_captured(cuda, tokens):
+def test_the_same_call_again_another_stream_and_captured(cuda, tokens, kernel):
     import torch as T
-    ad, x, idx, y, out = check(T, tokens, 1024, 520, 32, 6, T.float32, T.bfloat16)
-    assert T.equal(ad.forward(x, idx, y), out)
+    ad, x, idx, y, out = check(T, tokens, 1024, 520, 32, 6, T.float32, T.bfloat16, kernel=kernel)
+    assert T.equal(ad.forward(x, idx, y, kernel=kernel), out)
     s = T.cuda.Stream()
     s.wait_stream(T.cuda.current_stream())
     with T.cuda.stream(s):
-        other = ad.forward(x, idx, y)
+        other = ad.forward(x, idx, y, kernel=kernel)
     s.synchronize()
     assert T.equal(other, out)
     g, got = T.cuda.CUDAGraph(), T.empty_like(out)
     with T.cuda.graph(g, stream=s):
-        ad.forward(x, idx, y, out=got)
+        ad.forward(x, idx, y, out=got, kernel=kernel)
     x2, idx2 = x.flip(0).clone(), idx.flip(0).clone()
-    want = ad.forward(x2, idx2, y)
+    want = ad.forward(x2, idx2, y, kernel=kernel)
     x.copy_(x2)
     idx.copy_(idx2)
     g.replay()
