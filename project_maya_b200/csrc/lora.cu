@@ -156,6 +156,7 @@ extern "C" int maya_lora(const maya_lora_args* a, void* stream) {
     if (a->n_in % 32 || a->rank <= 0 || a->rank % 16) return refuse(MAYA_ERR_ARG);
     if (a->rank > MAYA_MAX_LORA_RANK || a->n_tokens > MAYA_MAX_LORA_TOKENS) return refuse(MAYA_ERR_LIMIT);
     if (a->ld_x < a->n_in || (a->y && a->ld_y < a->n_out) || a->ld_out < a->n_out) return refuse(MAYA_ERR_ARG);
+    if (a->ld_x > 0x7FFFFFFFll || (a->y && a->ld_y > 0x7FFFFFFFll) || a->ld_out > 0x7FFFFFFFll) return refuse(MAYA_ERR_LIMIT);
     if (a->y == a->out && a->ld_y != a->ld_out) return refuse(MAYA_ERR_ARG);
     if (!aligned16(a->x) || !aligned16(a->a) || !aligned16(a->b) || (((uintptr_t) a->scratch) & 255u) || a->ld_x % (a->x_is_bf16 ? 8 : 4)) return refuse(MAYA_ERR_ARG);
     if (a->kernel < MAYA_LORA_CHOICE || a->kernel > MAYA_LORA_MANY) return refuse(MAYA_ERR_ARG);

@@ -196,8 +196,12 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     int tok[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tok[i] = G.token[(size_t) tile * kLoraTile + r0 + 32 * i];
-    uint4 xr[4][XB ? 1 : 2], wr[WI];
-    auto load = [&](int c) {
+    // two chunks of a set on their way in registers where these suffice (ranks up to 64: kernel 22 -> DEEP_FIGURE us), else one
+    constexpr int kDeep = WI <= 2 ? 2 : 1;
+    struct Ahead { uint4 x[4][XB ? 1 : 2], w[WI]; };
+    auto load = [&](int c, Ahead& R) {
+        auto& xr = R.x;
+        auto& wr = R.w;
         const int k = c * kChunk + c8 * 8;
         const bool in = k < A.n_in;
 #pragma unroll
@@ -223,8 +227,13 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     };
     bool lost = false;
     int issued = 0;
-    if (c_first + set < c_end) load(c_first + set);
-    for (int c = c_first + set; c < c_end; c += 2) {
+    Ahead ahead[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+        if (c_first + set + 2 * d < c_end) load(c_first + set + 2 * d, ahead[d]);
+    auto step = [&](int c, Ahead& R) {
+        auto& xr = R.x;
+        auto& wr = R.w;
         if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
         if (!lost) {
 #pragma unroll
@@ -248,10 +257,10 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
             for (int j = 0; j < WI; ++j)
                 if (r0 + 32 * j < rank) weights_to(w_at, sw128(r0 + 32 * j, c8), wr[j], F16, w_next);
         }
-        if (c + 2 < c_end) load(c + 2);
+        if (c + 2 * kDeep < c_end) load(c + 2 * kDeep, R);
         fence_proxy_async();
         lost = named_bar_or(1 + set, 256, lost);
-        if (lost) break;
+        if (lost) return;
         if ((warp & 7) == 0) {
             tc_fence_after();
             const uint64_t w0 = smem_desc_sw128(w_at), w1 = smem_desc_sw128(w_at + w_next);
@@ -270,6 +279,10 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
             mma_commit_elect(smem_u32(&done[set]));
         }
         ++issued;
+    };
+    for (int c = c_first + set; c < c_end && !lost; c += 2 * kDeep) {
+        step(c, ahead[0]);
+        if (kDeep == 2 && c + 2 < c_end && !lost) step(c + 2, ahead[kDeep - 1]);
     }
     // the last commit of a set stands for every product of its in front
     if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
@@ -346,10 +359,10 @@ constexpr int kTurnBytes = 32 * 32 * 4;                       // a warp's part o
 constexpr int kUpCols = 256;                                  // tensor memory: two groups' sums, then z: 3 * 32 columns
 __host__ __device__ constexpr int up_bytes(bool f16) { return 2 * w_terms(f16) * kOutBytes + 8 * kTurnBytes + 1024; }
 
-// (each time anew: kept in registers over the groups, the rows' places leave too few for y)
-__device__ __forceinline__ int64_t look_up(const int64_t* p) {
-    int64_t v;
-    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(smem_u32(p)) : "memory");
+// (each time anew: kept in registers over the groups, 32 rows' tokens leave too few for y)
+__device__ __forceinline__ int look_up(const int* p) {
+    int v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
     return v;
 }
 
@@ -359,15 +372,24 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t ready[2];                // a group's sums are there
     __shared__ uint32_t tmem_base;
-    __shared__ int64_t y_at[kLoraTile], out_at[kLoraTile];    // -1: no token
-    const int tid = threadIdx.x, lane = tid & 31;
+    __shared__ int tok[kLoraTile];                            // -1: none
+    const int tid = threadIdx.x, lane = tid & 31, ld_y = (int) A.ld_y, ld_out = (int) A.ld_out;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     // What is read ahead of the wait was written at least two launches ago, and is read out of L2: L1 may hold what an earlier call left there.
     if (k0 > 0) grid_dependency_wait();                       // (y is the launch in front's out)
     const int groups = (A.n_out + kOutCols - 1) / kOutCols;
-    const int64_t units = (int64_t) __ldcg(G.words + 1) * groups;
-    const int64_t u_end = units * (blockIdx.x + 1) / gridDim.x;
-    int64_t u = units * blockIdx.x / gridDim.x;
+    const int tiles = __ldcg(G.words + 1), split = gridDim.x / (tiles > 0 ? tiles : 1);
+    int64_t u, u_end;
+    if (split >= 4) {                                         // so many thread blocks a tile: none has to begin with another (8 us)
+        const int t = blockIdx.x / split, i = blockIdx.x - t * split;
+        if (t >= tiles) return;
+        u = (int64_t) t * groups + groups * i / split;
+        u_end = (int64_t) t * groups + groups * (i + 1) / split;
+    } else {
+        const int64_t units = (int64_t) tiles * groups;
+        u = units * blockIdx.x / gridDim.x;
+        u_end = units * (blockIdx.x + 1) / gridDim.x;
+    }
     if (u >= u_end) return;
     if (tid == 0) {
         mbar_init(&ready[0], 1);
@@ -380,14 +402,20 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
     constexpr int kRows = VEC ? 8 : 32;
     const int tile_row = 32 * (warp & 3), row0 = VEC ? lane >> 3 : 0, col0 = (warp >> 2) * 32 + (VEC ? (lane & 7) * 4 : lane), rank = A.rank, c8 = tid & 7;
     float y[32];
+    int mine[VEC ? 8 : 1];                                    // VEC: the rows' tokens
+    auto token = [&](int r) {
+        if constexpr (VEC) return mine[r];
+        else return look_up(tok + tile_row + r);
+    };
     uint4 wr[2];
     int adapter = -1;
     auto fetch = [&](int g) {
         const int n = g * kOutCols + col0;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            const int64_t at = look_up(y_at + tile_row + row0 + (VEC ? 4 : 1) * r);
-            const bool has = A.y != nullptr && at >= 0 && n < A.n_out;
+            const int t = token(r);
+            const int64_t at = (int64_t) t * ld_y;
+            const bool has = A.y != nullptr && t >= 0 && n < A.n_out;
             if constexpr (VEC) {
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (has) v = __ldcg((const float4*) (A.y + at + n));
@@ -403,8 +431,9 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         if (n >= A.n_out) return;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            const int64_t at = look_up(out_at + tile_row + row0 + (VEC ? 4 : 1) * r);
-            if (at < 0) continue;
+            const int t = token(r);
+            const int64_t at = (int64_t) t * ld_out;
+            if (t < 0) continue;
             if constexpr (VEC) __stcs((float4*) (A.out + at + n), make_float4(y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]));
             else __stcs(A.out + at + n, y[r]);
         }
@@ -428,12 +457,12 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         adapter = __ldcg(G.adapter + tile);
         if (adapter < 0 && (A.y == A.out || k0 > 0)) continue;
         __syncthreads();                                      // (the last tile's rows have been looked up)
-        if (tid < kLoraTile) {
-            const int t = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
-            y_at[tid] = t >= 0 ? t * A.ld_y : -1;
-            out_at[tid] = t >= 0 ? t * A.ld_out : -1;
-        }
+        if (tid < kLoraTile) tok[tid] = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
         __syncthreads();
+        if constexpr (VEC) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) mine[r] = look_up(tok + tile_row + row0 + 4 * r);
+        }
         fetch(g_first);
         if (adapter >= 0) weights(g_first);
         if (!waited) { grid_launch_dependents(); grid_dependency_wait(); waited = true; }
@@ -452,19 +481,20 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
             tmem = tmem_base | 0x80000000u;
         }
         const uint32_t tm = tmem & 0x7FFFFFFFu, z_tm = tm + 2 * kOutCols;
-#pragma unroll 1
-        for (int q = warp >> 2; q < 6; q += 2) {              // half of a row's term: 32 values in 16 columns of its lane
-            uint32_t zr[16];
-            const int k = k0 + 32 * (q & 1);
-            const uint4* zp = (const uint4*) (G.z + (((size_t) tile * kLoraTile + tile_row + lane) * 3 + (q >> 1)) * rank + k);
+        // half of a row's terms: 32 values in 16 columns of its lane
+        const int half = warp >> 2, k_half = k0 + 32 * half;
+        const uint4* zp = (const uint4*) (G.z + ((size_t) tile * kLoraTile + tile_row + lane) * 3 * rank + k_half);
+        uint32_t zr[3][16];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint4 z = make_uint4(0u, 0u, 0u, 0u);
-                if (k + c * 8 < rank) z = __ldcg(zp + c);
-                zr[4 * c] = z.x; zr[4 * c + 1] = z.y; zr[4 * c + 2] = z.z; zr[4 * c + 3] = z.w;
+                if (k_half + c * 8 < rank) z = __ldcg((const uint4*) ((const uint16_t*) zp + q * rank) + c);
+                zr[q][4 * c] = z.x; zr[q][4 * c + 1] = z.y; zr[q][4 * c + 2] = z.z; zr[q][4 * c + 3] = z.w;
             }
-            tmem_st16(z_tm + ((uint32_t) tile_row << 16) + (uint32_t) (16 * q), zr);
-        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) tmem_st16(z_tm + ((uint32_t) tile_row << 16) + (uint32_t) (32 * q + 16 * half), zr[q]);
         tmem_wait_st();
         tc_fence_before();                                    // (ahead of the barrier in front of the first products)
         auto stage = [&](int m) {                             // what `weights` brought, for the m-th products

@@ -14,7 +14,7 @@ P = 0x7f0000000000                       # an address that nothing reads
     (dict(x=None), ARG), (dict(out=None), ARG), (dict(a=None), ARG), (dict(b=None), ARG), (dict(idx=None), ARG), (dict(scratch=None), ARG),
     (dict(n_adapters=0), ARG), (dict(n_in=0), ARG), (dict(n_in=48, ld_x=64), ARG), (dict(n_out=0), ARG), (dict(rank=0), ARG), (dict(rank=8), ARG), (dict(rank=272), LIMIT),
     (dict(n_tokens=65536), LIMIT), (dict(ld_x=32), ARG), (dict(ld_y=32), ARG), (dict(ld_out=32), ARG), (dict(y=P, out=P, ld_out=128), ARG), (dict(x=P + 4), ARG),
-    (dict(a=P + 8), ARG), (dict(b=P + 8), ARG), (dict(scratch=P + 128), ARG), (dict(ld_x=66), ARG), (dict(ld_x=68, x_is_bf16=1), ARG), (dict(scratch_bytes=100), LIMIT), (dict(kernel=3), ARG), (dict(kernel=-1), ARG),
+    (dict(a=P + 8), ARG), (dict(b=P + 8), ARG), (dict(scratch=P + 128), ARG), (dict(ld_x=66), ARG), (dict(ld_x=68, x_is_bf16=1), ARG), (dict(scratch_bytes=100), LIMIT), (dict(ld_out=1 << 31), LIMIT), (dict(kernel=3), ARG), (dict(kernel=-1), ARG),
     (dict(kernel=2, n_adapters=4097), LIMIT), (dict(kernel=2, scratch_bytes=1000), LIMIT)])
 def test_refusals(lib, more, status):
     d = dict(x=P, y=P + 4096, out=P + 8192, a=P, b=P, scale=None, idx=P, scratch=P, scratch_bytes=1 << 30, ld_x=64, ld_y=64, ld_out=64, n_tokens=3, n_in=64, n_out=64,
