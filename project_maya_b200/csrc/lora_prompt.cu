@@ -158,7 +158,8 @@ __host__ __device__ inline int pow2_cols(int c) { int p = 32; while (p < c) p *=
 // ---------------------------------------------------------------- z of a tile
 // XB: x is bf16.  F16: weights are.  WI: 16-byte pieces of a weight stage a thread brings (rank * 8 / 256, rounded up).
 // Two sets of eight warps take chunks of 64 values in turn, so that one's fence, barrier and products run under the other's cutting of x into terms:
-// with one set a chunk took 1.3 us, most of it waiting (whole kernel 31 us of the case in lora.cu, two sets REPLACED_FIGURE).
+// with one set a chunk took 1.3 us, most of it waiting (4096 tokens, 4096 -> rank 64: kernel 31 us, two sets 24; x is 8 of them at the memory's rate).  Taken
+// back: two chunks of a set on their way instead of one (24), x as two 32-bit (tf32) terms, two operations a value instead of six (26).
 template<bool XB, bool F16, int WI>
 __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A, const Tiles G, int parts) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -196,12 +197,8 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     int tok[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tok[i] = G.token[(size_t) tile * kLoraTile + r0 + 32 * i];
-    // two chunks of a set on their way in registers where these suffice (ranks up to 64: kernel 22 -> DEEP_FIGURE us), else one
-    constexpr int kDeep = WI <= 2 ? 2 : 1;
-    struct Ahead { uint4 x[4][XB ? 1 : 2], w[WI]; };
-    auto load = [&](int c, Ahead& R) {
-        auto& xr = R.x;
-        auto& wr = R.w;
+    uint4 xr[4][XB ? 1 : 2], wr[WI];
+    auto load = [&](int c) {
         const int k = c * kChunk + c8 * 8;
         const bool in = k < A.n_in;
 #pragma unroll
@@ -227,13 +224,8 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     };
     bool lost = false;
     int issued = 0;
-    Ahead ahead[kDeep];
-#pragma unroll
-    for (int d = 0; d < kDeep; ++d)
-        if (c_first + set + 2 * d < c_end) load(c_first + set + 2 * d, ahead[d]);
-    auto step = [&](int c, Ahead& R) {
-        auto& xr = R.x;
-        auto& wr = R.w;
+    if (c_first + set < c_end) load(c_first + set);
+    for (int c = c_first + set; c < c_end; c += 2) {
         if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
         if (!lost) {
 #pragma unroll
@@ -257,10 +249,10 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
             for (int j = 0; j < WI; ++j)
                 if (r0 + 32 * j < rank) weights_to(w_at, sw128(r0 + 32 * j, c8), wr[j], F16, w_next);
         }
-        if (c + 2 * kDeep < c_end) load(c + 2 * kDeep, R);
+        if (c + 2 < c_end) load(c + 2);
         fence_proxy_async();
         lost = named_bar_or(1 + set, 256, lost);
-        if (lost) return;
+        if (lost) break;
         if ((warp & 7) == 0) {
             tc_fence_after();
             const uint64_t w0 = smem_desc_sw128(w_at), w1 = smem_desc_sw128(w_at + w_next);
@@ -279,10 +271,6 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
             mma_commit_elect(smem_u32(&done[set]));
         }
         ++issued;
-    };
-    for (int c = c_first + set; c < c_end && !lost; c += 2 * kDeep) {
-        step(c, ahead[0]);
-        if (kDeep == 2 && c + 2 < c_end && !lost) step(c + 2, ahead[kDeep - 1]);
     }
     // the last commit of a set stands for every product of its in front
     if (issued > 0) lost |= !mbar_wait(&done[set], (issued - 1) & 1);
@@ -320,11 +308,13 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     for (int i = tid; i < rows * quads; i += kDownThreads) {
         const int row = part * rows + i / quads, c = (i % quads) * 4;
         const uint32_t from = smem + (uint32_t) (row * stride + c) * 4u;
-        float4 v = ld_peer(from, 0);
-        for (int p = 1; p < parts; ++p) {
-            const float4 u = ld_peer(from, (uint32_t) p);
-            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-        }
+        float4 u[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p < parts) u[p] = ld_peer(from, (uint32_t) p);
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p < parts) { v.x += u[p].x; v.y += u[p].y; v.z += u[p].z; v.w += u[p].w; }
         float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
         uint16_t* z = G.z + ((size_t) tile * kLoraTile + row) * 3 * rank + c;
 #pragma unroll
@@ -348,10 +338,10 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
 // The pairs of a tile and a group of 64 outputs are shared out evenly, one run of them a thread block.  z's three terms lie in tensor memory; a group's products run
 // under the write-back of the one in front.  A warp turns its 32 x 32 sums around in shared memory, so that a lane has four neighbours of a row: 16
 // bytes a load of y and a store of out.  y is on its way in registers from the last group's write-back on.
-// Ways to this (the kernel alone, case in lora.cu, us): a thread block a tile and 128 outputs, 4 bytes a lane 53; several groups a thread block with the
+// Ways to this (the kernel alone, 4096 tokens, rank 64 -> 6144, us): a thread block a tile and 128 outputs, 4 bytes a lane 53; several groups a thread block with the
 // loads of y between the uses of the last ones, each of which then waits for the loads in front of it, 145; outputs as the product's rows, so
 // that nothing has to be turned, 124 and, with fewer instructions, 83; z in shared memory, y by asynchronous copies two groups ahead, two sets of warps a thread block 51: four
-// ways through shared memory for every value beside the products' operands.
+// ways through shared memory for every value beside the products' operands; as it is 44, of them 31 at the memory's rate.
 constexpr int kUpThreads = 256;
 constexpr int kOutCols = 64;
 constexpr int kOutBytes = kOutCols * kChunk * 2;              // a group's weights, one term

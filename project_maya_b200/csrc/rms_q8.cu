@@ -8,6 +8,9 @@
 //   x = t * (1 / sqrt(mean(t^2) + eps)) * w   f32, of the unrounded t; x_out rounded once
 //   xq = x as maya_quantize_q8_1 or maya_mmq_quantize rounds it, byte for byte
 //
+// Bounds: a prompt is bytes (4096 x 6144 f32 rows with add and h_out into the image: 66 us, 5.4 TB/s of the 354 MB it moves; with streaming loads and stores 65, with
+// two runs a thread instead of four 68), a token one launch with its chain of loads, reduction and stores (3 us, 2 more to read it back).
+//
 // One thread block a row.  A thread holds runs of 8 consecutive values (32 bytes of f32: two 16-byte loads) in registers across the
 // reduction, so the row is read once; four neighbouring lanes hold a 32-value group, whose amax is two shuffles away.  The group's sum keeps
 // the quantizers' order of additions - theirs is a butterfly over single values, distances 16, 8, 4, 2, 1, here the first two between lanes and the
@@ -301,7 +304,7 @@ using namespace maya;
 extern "C" int maya_rms_q8(const maya_rms_args* a, void* stream) {
     if (!a) return refuse(MAYA_ERR_ARG);
     if (a->n_rows <= 0) return MAYA_OK;
-    if (!a->h || !a->w || a->n <= 0 || (!a->h_out && !a->x_out && !a->xq)) return refuse(MAYA_ERR_ARG);
+    if (!a->h || !a->w || a->n <= 0 || !(a->eps >= 0.0f) || (!a->h_out && !a->x_out && !a->xq)) return refuse(MAYA_ERR_ARG);
     if (a->image != MAYA_XQ_NONE && a->image != MAYA_XQ_Q8_1 && a->image != MAYA_XQ_MMQ) return refuse(MAYA_ERR_ARG);
     if ((a->image != MAYA_XQ_NONE) != (a->xq != nullptr)) return refuse(MAYA_ERR_ARG);
     if (a->image != MAYA_XQ_NONE && (a->n % 32 || !aligned16(a->xq))) return refuse(MAYA_ERR_ARG);

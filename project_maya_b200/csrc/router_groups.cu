@@ -1,6 +1,7 @@
 // router_groups.cu - the router over groups of experts (maya_route_groups.cuh): a warp a token.
 //
-// What bounds it is the instructions of the 64-bit exponentials and of the selections, not the 1 KB of logits a token.
+// What bounds it is instructions, some 1650 a token of 256 experts, k = 8 (scores, groups, the lanes' sorting, nine rounds of choice, the k weights in 64 bits), not
+// the 1 KB of logits: 8192 tokens 23 us, 0.4 TB/s; issue slots are 60 % busy.  A single token is a chain of latencies, 5.7 us.
 #include "maya_route_groups.cuh"
 
 namespace maya {

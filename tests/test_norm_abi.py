@@ -18,7 +18,7 @@ def args(**more):
 
 
 @pytest.mark.parametrize("more,status", [
-    (dict(h=None), ARG), (dict(w=None), ARG), (dict(n=0), ARG), (dict(xq=None), ARG), (dict(xq=None, image=0), ARG), (dict(image=0), ARG),
+    (dict(h=None), ARG), (dict(w=None), ARG), (dict(n=0), ARG), (dict(eps=-1.0), ARG), (dict(eps=float("nan")), ARG), (dict(xq=None), ARG), (dict(xq=None, image=0), ARG), (dict(image=0), ARG),
     (dict(image=3), ARG), (dict(n=40, xq=P), ARG), (dict(xq=P + 8), ARG), (dict(n=32800, ld_h=32800), LIMIT), (dict(n_rows=1 << 31), LIMIT),
     (dict(ld_h=511), ARG), (dict(add=P, ld_add=100), ARG), (dict(h_out=P + 64, ld_h_out=500), ARG), (dict(x_out=P + 64, ld_x=500), ARG),
     (dict(h_out=P, ld_h_out=520), ARG), (dict(x_out=P, ld_x=520), ARG), (dict(x_out=P, x_is_bf16=1), ARG), (dict(x_out=P + 64, h_out=P + 64), ARG),
