@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         issue();
         if (g_first + 1 < g_end) issue();
         for (int g = g_first; g < g_end; ++g, ++writes) {
-            lost = !mbar_wait(&ready[writes & 1], (writes >> 1) & 1);
+            lost = __any_sync(0xffffffffu, !mbar_wait(&ready[writes & 1], (writes >> 1) & 1));      // (a warp reads tensor memory as one)
             tc_fence_after();
             if (g + 2 < g_end) weights(g + 2);                // (used below, ahead of the next loads of y: a use waits for what was asked for since, too)
             if (!lost) {
