@@ -56,12 +56,13 @@ def _stream(stream=None) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _here(what: str, *tensors) -> None:
-    """Tensors of a call: all on the current device, whose stream the call goes to."""
+def _here(what: str, *tensors, stream=None) -> int:
+    """Tensors of a call: all on the current device, on whose current stream (or `stream`) it goes; returns that stream's handle."""
     dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise MayaError(f"{what}: tensors of the current device expected", -1)
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)
 
 
 # ---------------------------------------------------------------- formats (host only: usable without a GPU)
@@ -140,7 +141,7 @@ def router_groups(logits, k: int, n_group: int = 1, n_keep: int = 1, bias=None, 
     s + bias - the n_keep best of n_group groups, then the k best of their experts - and weights s / max(their sum, 2^-14) * w_scale (norm_w False:
     s * w_scale).  include/maya_moe.h states it in full (maya_router_groups)."""
     T, E = logits.shape
-    _here("router_groups", logits, bias, ids, weights)
+    s = _here("router_groups", logits, bias, ids, weights, stream=stream)
     assert logits.dtype is torch.float32 and (bias is None or (bias.dtype is torch.float32 and bias.numel() == E))
     if weights is None:
         weights = logits.new_empty((T, k))
@@ -148,7 +149,7 @@ def router_groups(logits, k: int, n_group: int = 1, n_keep: int = 1, bias=None, 
         ids = torch.empty_like(weights, dtype=torch.int32)
     assert ids.dtype is torch.int32 and weights.dtype is torch.float32 and ids.numel() == weights.numel() == T * k
     a = RouteArgs(_ptr(logits), _ptr(bias), T, E, k, n_group, n_keep, sigmoid, top2, norm_w, w_scale, _ptr(ids), _ptr(weights))
-    _check("router_groups", _lib.load().maya_router_groups(C.byref(a), _stream(stream)))
+    _check("router_groups", _lib.load().maya_router_groups(C.byref(a), s))
     return ids, weights
 
 
@@ -214,7 +215,7 @@ class LoraAdapters:
     def forward(self, x, idx, y=None, out=None, kernel: int = LORA_CHOICE, stream=None):
         """x [T, n_in] f32 or bf16, idx i32 [T] (outside 0 .. n - 1: no adapter), y f32 [T, n_out] (None: zeros) -> out f32 [T, n_out], which may be y.
         kernel: LORA_FEW (each token by itself), LORA_MANY (tiles of one adapter's tokens) or the sizes' choice."""
-        _here("lora", self.scratch, x, idx, y, out)
+        s = _here("lora", self.scratch, x, idx, y, out, stream=stream)
         T = x.shape[0]
         if out is None:
             out = torch.empty((T, self.n_out), dtype=torch.float32, device=x.device)
@@ -225,7 +226,7 @@ class LoraAdapters:
         a, b, scale = self._fixed
         args = LoraArgs(xp, yp, op, a, b, scale, _ptr(idx), self.scratch.data_ptr(), self.scratch.numel(), ld_x, ld_y, ld_out, T, *self._sizes,
                         x.dtype is torch.bfloat16, self.a.dtype is torch.float16, kernel)
-        _check("lora", _lib.load().maya_lora(C.byref(args), _stream(stream)))
+        _check("lora", _lib.load().maya_lora(C.byref(args), s))
         return out
 
     def error(self, stream=None) -> int:
@@ -359,14 +360,14 @@ def _matrix(t, shape):
 
 def xq_bytes(image: int, rows: int, n: int) -> int:
     """Bytes of `rows` 8-bit rows of n values."""
-    return (rows * n >> 5) * 36 if image == XQ_Q8_1 else mmq_q8_bytes(rows, n)
+    return (rows * n >> 5) * 36 if image == XQ_Q8_1 else rows * 2 * (n + ((n >> 5) + 63 & ~63))        # (maya_mmq_q8_bytes)
 
 
 def rms_q8(h, add, norm_w, eps: float, image: int | None = XQ_Q8_1, xq=None, h_out=None, x=None, stream=None):
     """glmf::rms_q8 (glm_fast.hpp:534) for any number of rows: t = h + add (add None: h), x = rms(t) * norm_w, and x in 8 bits.  h and add [T, n] f32 or
     bf16 (one row: [n] too), rows may lie apart.  image: XQ_Q8_1 or XQ_MMQ, what native_quantize_q8_1(x) or mmq_quantize(x) would write, returned as
     uint8 - in `xq` where it is given; None: no 8-bit rows.  h_out (h's type; may be h): receives t; x (f32 or bf16): the normed rows."""
-    _here("rms_q8", h, add, norm_w, h_out, x, xq)
+    s = _here("rms_q8", h, add, norm_w, h_out, x, xq, stream=stream)
     shape = h.shape if h.dim() == 2 else h[None].shape
     T, n = shape
     assert norm_w.dtype is torch.float32 and norm_w.shape == shape[1:] and (h_out is None or h_out.dtype is h.dtype)
@@ -384,16 +385,16 @@ def rms_q8(h, add, norm_w, eps: float, image: int | None = XQ_Q8_1, xq=None, h_o
     bf16 = torch.bfloat16
     a = RmsArgs(hp, ap, _ptr(norm_w), op, rows, _ptr(xq), ld_h, ld_add, ld_out, ld_x, T, n, eps, h.dtype is bf16,
                 add is not None and add.dtype is bf16, x is not None and x.dtype is bf16, image or 0)
-    _check("rms_q8", _lib.load().maya_rms_q8(C.byref(a), _stream(stream)))
+    _check("rms_q8", _lib.load().maya_rms_q8(C.byref(a), s))
     return xq
 
 
 def q8_read(xq, rows: int, n: int, image: int = XQ_Q8_1, dtype=torch.bfloat16, stream=None):
     """8-bit rows as the values they stand for: (values [rows, n] of dtype bf16 or f32, sums f16 [rows, n / 32] of their groups before rounding)."""
-    _here("q8_read", xq)
+    s = _here("q8_read", xq, stream=stream)
     assert dtype in (torch.float32, torch.bfloat16) and xq.numel() * xq.element_size() >= xq_bytes(image, rows, n)
     values, sums = xq.new_empty((rows, n), dtype=dtype), xq.new_empty((rows, n >> 5), dtype=torch.float16)
-    _check("q8_read", _lib.load().maya_q8_read(_ptr(xq), image, rows, n, int(dtype is torch.bfloat16), _ptr(values), _ptr(sums), _stream(stream)))
+    _check("q8_read", _lib.load().maya_q8_read(_ptr(xq), image, rows, n, dtype is torch.bfloat16, values.data_ptr(), sums.data_ptr(), s))
     return values, sums
 
 
@@ -910,39 +911,40 @@ class KvPages:
         self.live = self.scratch[8:12].view(torch.int32)     # i32 [1]: live blocks as the last compact() found them
         self._ref = C.byref(self.desc)
 
-    def _list(self, what, *lists):
-        _here(what, self.scratch, *lists)
+    def _list(self, what, stream, *lists):
+        s = _here(what, self.scratch, *lists, stream=stream)
         n = lists[0].numel()
-        assert all(t.dtype is torch.int32 and t.numel() == n for t in lists)
-        return n, *(_ptr(t) for t in lists)
+        for t in lists:
+            assert t.dtype is torch.int32 and t.numel() == n
+        return n, s, *map(_ptr, lists)
 
     def reserve(self, batch: AttnBatch, stream=None) -> None:
         """Blocks for the batch's new tokens, in front of append(): entries without one get one, a block that other sequences hold too is replaced by a
         block of the sequence's own (with a copy of the tokens from before in it)."""
-        _here("pages_reserve", self.scratch, batch.start, batch.kv_len)
-        _check("pages_reserve", _lib.load().maya_pages_reserve(self._ref, batch._ref, _stream(stream)))
+        s = _here("pages_reserve", self.scratch, batch.start, batch.kv_len, stream=stream)
+        _check("pages_reserve", _lib.load().maya_pages_reserve(self._ref, batch._ref, s))
 
     def fork(self, parents, children, lens, stream=None) -> None:
         """i32 [n] each: sequence children[i] becomes the first lens[i] tokens of sequence parents[i], all at once (a beam search's step).  Full blocks are
         shared, one that is not full is copied; what the children held is given up.  A child that is its own parent is left as it is."""
-        n, p, c, k = self._list("pages_fork", parents, children, lens)
-        _check("pages_fork", _lib.load().maya_pages_fork(self._ref, p, c, k, n, _stream(stream)))
+        n, s, p, c, k = self._list("pages_fork", stream, parents, children, lens)
+        _check("pages_fork", _lib.load().maya_pages_fork(self._ref, p, c, k, n, s))
 
     def free(self, seqs, stream=None) -> None:
         """Sequences seqs (i32 [n]) give up their blocks; their table rows are -1."""
-        n, s = self._list("pages_free", seqs)
-        _check("pages_free", _lib.load().maya_pages_free(self._ref, s, n, _stream(stream)))
+        n, s, q = self._list("pages_free", stream, seqs)
+        _check("pages_free", _lib.load().maya_pages_free(self._ref, q, n, s))
 
     def compact(self, most: int | None = None, stream=None) -> None:
         """The live blocks move to the lowest numbers, tables and counts with them: all that lie too high, or the `most` lowest of these (the next call
         goes on).  `live` says how many blocks are live."""
-        _here("pages_compact", self.scratch)
-        _check("pages_compact", _lib.load().maya_pages_compact(self._ref, self.n_blocks if most is None else most, _stream(stream)))
+        s = _here("pages_compact", self.scratch, stream=stream)
+        _check("pages_compact", _lib.load().maya_pages_compact(self._ref, self.n_blocks if most is None else most, s))
 
     def copy(self, src, dst, stream=None) -> None:
         """Blocks src[i] to blocks dst[i] (i32 [n]) in all layers.  No block twice in dst, none in both."""
-        n, s, d = self._list("pages_copy", src, dst)
-        _check("pages_copy", _lib.load().maya_pages_copy(self._ref, s, d, n, _stream(stream)))
+        n, s, a, d = self._list("pages_copy", stream, src, dst)
+        _check("pages_copy", _lib.load().maya_pages_copy(self._ref, a, d, n, s))
 
     def error(self, stream=None) -> int:
         """1 after a call that found too few free blocks (synchronises the stream); the word is zeroed then."""

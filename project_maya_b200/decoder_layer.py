@@ -34,9 +34,9 @@ class AttentionConfig:
     eps: float = 1e-6
     n_sel: int = 0                       # blocks a token reads in a long context; 0: all of them always
     sparse_from: int = 8192              # tokens of its own context from which on a sequence's single token reads selected blocks
+    rows: torch.dtype = torch.float32    # of queries, keys, values and outputs between the products: f32 (P in 22 bits), or bf16 (P in 11; prompts on tcgen05)
     norm_8_bits: bool = False            # the norm in front of a product and its rounding to 8 bits in one launch (rms_q8: its sums in another order than the
                                          # separate launches', so that a code may differ where a value lies between two)
-    rows: torch.dtype = torch.float32    # of queries, keys, values and outputs between the products: f32 (P in 22 bits), or bf16 (P in 11; prompts on tcgen05)
 
     def __post_init__(self):
         assert self.rows in (torch.float32, torch.bfloat16)
