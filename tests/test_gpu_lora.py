@@ -1,8 +1,8 @@
 """Low-rank adapters of many tokens beside a shared projection, against the formula in 64 bits.
 
 Tolerance, from the arithmetic: with m = sum_k |A_rk x_k| of a rank's sum and M = |scale| sum_r |B_nr| m_r, z is off by at most u m where u = 2^-16: sums of up to 8192 products in f32 whose
-partial sums are rounded (each at most 128 in a row, then a tree or pieces: 160 * 2^-24 < 2^-16) or cut (matrix instructions) and operands of 22 bits (2^-21 in
-all); the second product, up to 256 ranks, likewise, and the addition to y rounds once: |error| <= 2^-15 M + 2^-23 (|y| + M).
+partial sums are rounded (each at most 128 in a row, then a tree or pieces: 160 * 2^-24 < 2^-16) or cut (matrix instructions over operands in parts that hold all their
+bits: at most 128 sums in a row, 2^-23 each, beside 2^-20 for what the lesser parts leave); the second product, up to 256 ranks, likewise, and the addition to y rounds once: |error| <= 2^-15 M + 2^-23 (|y| + M).
 """
 import numpy as np
 import pytest
