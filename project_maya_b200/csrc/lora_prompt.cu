@@ -553,6 +553,9 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
             if (g + 2 < g_end) issue();
         }
     }
+    // A block whose tiles have nothing to do waits too: were there no others, this launch would end ahead of the one in front, and who waits for this one alone
+    // would begin while tiles are still being looked up.
+    if (!waited) grid_dependency_wait();
     if (lost) {
         if (tid == 0) G.words[0] = 1;
         for (int m = made; m > 0 && m > made - 2; --m) mbar_wait(&ready[(m - 1) & 1], ((m - 1) >> 1) & 1);        // what is in flight gets its time

@@ -159,3 +159,17 @@ def test_more_tokens_than_the_scratch_is_for(cuda):
         ad.forward(T.zeros((5, 64), device="cuda"), T.zeros(5, dtype=T.int32, device="cuda"))
     assert e.value.status == -4
     assert ad.forward(T.zeros((0, 64), device="cuda"), T.zeros(0, dtype=T.int32, device="cuda")).shape == (0, 64)
+
+
+@pytest.mark.parametrize("rank", [16, 80])
+def test_calls_in_place_that_nobody_takes_part_in(cuda, rank):
+    """Every other call has nothing to do: none of its blocks may be a call ahead of the scratch that they look their tiles up in."""
+    import torch as T
+    from project_maya_b200 import api
+    ad, x, idx, y, out = check(T, 400, 512, 320, rank, 3, T.float32, T.bfloat16, kernel=api.LORA_MANY)
+    none, kept = T.full_like(idx, -1), y.clone()
+    got = [T.empty_like(out) for _ in range(20)]
+    for o in got:
+        ad.forward(x, none, y, out=y, kernel=api.LORA_MANY)
+        ad.forward(x, idx, y, out=o, kernel=api.LORA_MANY)
+    assert all(T.equal(o, out) for o in got) and T.equal(y, kept) and ad.error() == 0
