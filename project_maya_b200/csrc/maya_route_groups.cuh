@@ -194,7 +194,10 @@ template<int N> __device__ __forceinline__ void sort_descending(uint32_t (&v)[N]
 // The same where 32 bits decide; false: they do not, nothing is returned.
 // Errors: expf is within 2 ulp, its argument - for a softmax a difference, rounded - within 2^-24 of itself, at most 104 before the result is 0; quotient and sums round.
 // So a score without a bias is within 2^-16 of itself (sums of up to 2048 terms among them), a sigmoid with a bias within 2^-21 and the rounding
-// of the sum, a softmax with one within 2^-16; what lies below 2^-110 of the highest is not told apart.  kApart times these, the error of a sum of two among them, has to lie between two values.
+// of the sum, a softmax with one within 2^-16; what lies below 2^-110 of the highest is not told apart.  kApart times these has to lie between two values.
+// An error that grows with the value itself needs to be looked at between neighbours only: a value further off is off by more than its error grows.  That does not
+// hold for the sum of a group's two highest, whose error is that of the two - as large as their biases, when the sum of a large and a very negative one is near 0 - so
+// every kept group's sum less its error has to lie above every other group's sum and error.
 template<int PER>
 __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, float* keys, int lane, int (&id)[2], float (&w)[2]) {
     const float* l = A.logits + token * A.n_expert;
@@ -228,6 +231,10 @@ __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, 
     constexpr float kPlaces = (float) PER * 0x1p-23f;         // (what the places in the lowest bits take from a score)
     const float of_itself = kApart * (A.bias == nullptr ? 0x1p-16f : 0x1p-23f) + kPlaces, fixed = A.bias == nullptr ? 0x1p-110f : kApart * (A.sigmoid ? 0x1p-21f : 0x1p-16f);
     auto near = [&](float a, float b) { return !(a - b > fixed + of_itself * fmaxf(fabsf(a), fabsf(b))); };     // a >= b
+    auto ordered = [](float c) {
+        const uint32_t u = __float_as_uint(c);
+        return u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
+    };
     uint32_t o[PER];
     bool odd = false;
 #pragma unroll
@@ -237,8 +244,7 @@ __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, 
         if (e < A.n_expert) {
             const float c = (A.bias != nullptr ? s[j] + A.bias[e] : s[j]) + 0.0f;
             odd |= !(fabsf(c) < 1e30f);
-            const uint32_t u = __float_as_uint(c);
-            o[j] = u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
+            o[j] = ordered(c);
         }
     }
     if (__any_sync(0xffffffffu, odd)) return false;
@@ -277,10 +283,12 @@ __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, 
             const float other = __shfl_sync(0xffffffffu, score, q * lanes);
             rank += other > score || (other == score && q < g);
         }
-        const unsigned last = __ballot_sync(0xffffffffu, mine && rank == A.n_keep - 1), next = __ballot_sync(0xffffffffu, mine && rank == A.n_keep);
-        const float in = __shfl_sync(0xffffffffu, score, __ffs(last) - 1), out = __shfl_sync(0xffffffffu, score, __ffs(next) - 1);
-        const unsigned kept = __ballot_sync(0xffffffffu, mine && rank < A.n_keep);
-        if (near(in, out)) return false;       // (all lanes alike)
+        const bool keeps = mine && rank < A.n_keep;
+        const unsigned kept = __ballot_sync(0xffffffffu, keeps);
+        const float err = 0.5f * fixed + of_itself * (A.top2 && b != 0u ? fabsf(value(a)) + fabsf(value(b)) : fabsf(score));
+        const unsigned in = __reduce_min_sync(0xffffffffu, keeps ? ordered(score - err) : 0xffffffffu);
+        const unsigned out = __reduce_max_sync(0xffffffffu, mine && !keeps ? ordered(score + err) : 0u);
+        if (!(in > out)) return false;         // (all lanes alike)
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int e = j * 32 + lane;

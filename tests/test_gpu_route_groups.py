@@ -226,3 +226,27 @@ def test_layers_with_group_routing(cuda):
         token.forward_checked(logits[:1], x[:1], api.LAYER_STAGED)
     with pytest.raises(api.MayaError):
         token.forward(logits[:1], x[:1], hc=(x, x, x, x))
+
+
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("large", [64.0, 1e2, 1e3, 1e5, 1e6])
+@pytest.mark.parametrize("where", ["every group", "one group"])
+def test_large_biases_that_cancel_in_a_group(cuda, sigmoid, large, where):
+    """A pinned expert beside a banned one: the group's sum is small and the rounding of the two is not, 2^-24 of each bias in 32 bits.  In every group the borders
+    themselves are in doubt; in one, a group that stands away from the border may belong on its other side."""
+    import torch as T
+    from project_maya_b200 import api
+    T.manual_seed(int(large))
+    logits = (0.01 if where == "every group" else 0.5) * T.randn((100000, 16), device="cuda")
+    bias = T.zeros(16, device="cuda")
+    pairs = bias.view(8, 2)[:8 if where == "every group" else 1]
+    pairs[:, 0], pairs[:, 1] = large, -large
+    s = T.sigmoid(logits.double()) if sigmoid else T.softmax(logits.double(), -1)
+    c = s + bias.double()
+    groups = c.view(-1, 8, 2).sort(dim=-1, descending=True).values.sum(-1).sort(dim=-1, descending=True, stable=True).indices[:, :4]
+    seen = T.zeros((100000, 8), dtype=T.bool, device="cuda").scatter_(1, groups, True).repeat_interleave(2, 1)
+    want = c.masked_fill(~seen, -float("inf")).sort(dim=-1, descending=True, stable=True).indices[:, :3]
+    ids, w = api.router_groups(logits, 3, 8, 4, bias, sigmoid)
+    assert T.equal(ids.long(), want)
+    p = s.gather(1, want)
+    assert bool(((w.double() - p / p.sum(-1, keepdim=True)).abs() <= 2.0 ** -23).all())
