@@ -98,8 +98,10 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const KvView C, co
         lost = 0;
         mbar_fence_init();
     }
-    if (warp == kIssueWarp) tmem_alloc(&tmem_base, 512);
-    grid_launch_dependents();
+    if (warp == kIssueWarp) {
+        tmem_alloc(&tmem_base, 512);
+        grid_launch_dependents();                 // (by the warp that has its tensor memory)
+    }
     grid_dependency_wait();
 
     // ---- the rows, and the cache blocks they see

@@ -169,7 +169,6 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), set = warp >> 3, st = tid & 255;
     const int part = blockIdx.x % parts, tile = blockIdx.x / parts;
     grid_dependency_wait();
-    grid_launch_dependents();                  // (behind the wait: what the next launch reads ahead of its own is finished)
     if (tile >= G.words[1]) return;            // (the whole cluster)
     const int adapter = G.adapter[tile];
     if (adapter < 0) return;
@@ -187,6 +186,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    grid_launch_dependents();                  // (behind the wait: what the next launch reads ahead of its own is finished)
     const bool apart = rest_apart(rank);
     const uint32_t tmem = tmem_base, lead = tmem + (uint32_t) (set * set_cols(rank)), rest = lead + (apart ? (uint32_t) rank : 0u);
     const uint32_t idesc = kBf16 | ((uint32_t) (rank >> 3) << 17);
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         }
         fetch(g_first);
         if (adapter >= 0) weights(g_first);
-        if (!waited) { grid_launch_dependents(); grid_dependency_wait(); waited = true; }
+        if (!waited) { grid_dependency_wait(); waited = true; }
         if (adapter < 0) {
             for (int g = g_first; g < g_end; ++g) {
                 store(g);
@@ -469,6 +469,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
             __syncthreads();
             tc_fence_after();
             tmem = tmem_base | 0x80000000u;
+            grid_launch_dependents();                         // (a block that never gets here: when it ends)
         }
         const uint32_t tm = tmem & 0x7FFFFFFFu, z_tm = tm + 2 * kOutCols;
         // half of a row's terms: 32 values in 16 columns of its lane

@@ -11,6 +11,8 @@
 
 namespace maya {
 
+// A kernel asks for tensor memory before it lets its dependents start, so that no block of it still has to when they begin: they may take all of an SM's ahead of
+// their wait for it, and would wait for each other for good.
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {   // one whole warp
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
