@@ -130,10 +130,11 @@ MAYA_API int maya_mmvq(int ggml_type, const void* weights, const void* x_q8_1, f
 /* Low-rank adapters ------------------------------------------------------------------------------- */
 /* No counterpart in the reference: what adapters of many requests add beside a projection that all share,
  *   out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t], and out[t] = y[t] where idx[t] is outside 0 .. n_adapters - 1,
- * in f32 (prompts: matrix instructions over operands in as many parts as hold all their bits, sums in f32).  Which kernel serves a call goes by its sizes, so a token's
- * bits may differ between calls of other numbers of tokens; the same call gives the same bits.
+ * in f32 (prompts: matrix instructions over operands in as many parts as hold all their bits, sums in f32; the third part of x times the second of an f16 weight, below
+ * 2^-21 of their product, is left out).  Which kernel serves a call goes by its sizes, so a token's bits may differ between calls of other numbers of tokens; the same call gives the
+ * same bits.  Infinities and NaN of x and y come out as the formula's sums make them, in every kernel; a, b and scale are finite (others make inf or NaN).
  * x, out and y (NULL: zeros) are [n_tokens] rows ld_* elements (below 2^31) apart; out may be y (the same ld), otherwise they overlap nothing.  x, a and b are 16-byte
- * aligned, ld_x a multiple of 16 bytes; n_in % 32 == 0; rank a multiple of 16 (smaller ranks are padded with zeros).
+ * aligned, ld_x a multiple of 16 bytes; n_in % 32 == 0; rank a multiple of 16 (others are padded with zeros, with which an infinite x makes NaN).
  * scratch: maya_lora_scratch_bytes(n_in, rank, n_adapters, at least n_tokens) bytes, 256-byte aligned, its first 256 zeroed before the first use; one stream
  * at a time.  Waits are bounded: one that ran out sets its first word (sticky; the call's out is not valid), which maya_lora_error answers. */
 enum maya_lora_kernel {

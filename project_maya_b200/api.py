@@ -192,7 +192,7 @@ class LoraAdapters:
     """Low-rank adapters of one projection, of which every token uses its own or none: out[t] = y[t] + scale[i] * b[i] (a[i] x[t]), i = idx[t].
 
     a [n, rank, n_in] and b [n, n_out, rank] bf16 or f16, scale f32 [n] or None (1); they are kept as they are, or - where the rank is not a multiple
-    of 16 - as copies padded with zeros.  n_in % 32 == 0, rank <= 256.  max_tokens sizes the scratch, which belongs to this object: one thread and one
+    of 16 - as copies padded with zeros (an infinite x makes NaN with them).  n_in % 32 == 0, rank <= 256.  max_tokens sizes the scratch, which belongs to this object: one thread and one
     stream at a time."""
 
     def __init__(self, a, b, scale=None, max_tokens: int = 4096):

@@ -9,8 +9,10 @@
 //
 // Numbers.  The products run on bf16 matrix instructions.  An f32 is three bf16 terms cut off its mantissa, 8 bits each, exactly; an f16 weight
 // two (8 + 3 bits), a bf16 value one.  Terms that are 2^-8 and less of a product are added up apart from the leading ones, and those over two accumulators
-// in turn where tensor memory has room: the tensor cores cut every sum towards zero, and fewer and smaller sums are cut by less.  z is scaled in f32 and
-// again three terms.
+// in turn where tensor memory has room: the tensor cores cut every sum towards zero, and fewer and smaller sums are cut by less.  z is again three terms; scale
+// multiplies the sum behind it.
+// Infinities.  One of x leaves inf - inf behind its first term and meets the second term of a weight that is 0 (inf * 0): a z that is no number is done over in plain f32, from x
+// and A.  An infinite z stands in the third term, which meets weights' first terms alone: these are 0 where the weight is.
 #include "maya_lora.cuh"
 #include "maya_scan.cuh"
 #include "maya_tcgen05.cuh"
@@ -27,7 +29,7 @@ struct Tiles {
     int* words;                  // [0] error, [1] tiles
     int* adapter;                // [most] of a tile; -1: tokens without one
     int* token;                  // [most][128] of a row; -1: none
-    uint16_t* z;                 // [most][128][3][rank] bf16 terms of scale * z
+    uint16_t* z;                 // [most][128][3][rank] bf16 terms of z
     int most;
 };
 
@@ -154,6 +156,28 @@ __host__ __device__ inline int down_body(bool x_bf16, bool f16, int rank) {
 __host__ __device__ inline bool rest_apart(int rank) { return rank <= 128; }
 __host__ __device__ inline int set_cols(int rank) { return rest_apart(rank) ? 2 * rank : rank; }
 __host__ __device__ inline int pow2_cols(int c) { int p = 32; while (p < c) p *= 2; return p; }
+
+// Four z of one token by the calling warp, in plain f32.  x: its row, a: the first of four rows of A.
+template<bool XB, bool F16> __device__ __noinline__ float4 plain_z(const uint8_t* x, const uint16_t* a, int n_in, int lane) {
+    float z[4] = {};
+    for (int k = lane * 8; k < n_in; k += 256) {
+        float v[8];
+        if constexpr (XB) {
+            weights8<false>(*(const uint4*) (x + 2 * k), v);
+        } else {
+            const float4 p = *(const float4*) (x + 4 * k), q = *(const float4*) (x + 4 * k + 16);
+            v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float w[8];
+            weights8<F16>(*(const uint4*) (a + (size_t) r * n_in + k), w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[r] = __fmaf_rn(w[j], v[j], z[r]);
+        }
+    }
+    return make_float4(warp_sum(z[0]), warp_sum(z[1]), warp_sum(z[2]), warp_sum(z[3]));
+}
 
 // ---------------------------------------------------------------- z of a tile
 // XB: x is bf16.  F16: weights are.  WI: 16-byte pieces of a weight stage a thread brings (rank * 8 / 256, rounded up).
@@ -303,9 +327,8 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
     if (warp == 0) tmem_dealloc(tmem, (uint32_t) cols);      // (given back before the cluster is waited for: who waits for tensor memory waits for no cluster)
     cluster_arrive();
     cluster_wait();
-    const float scale = A.scale != nullptr ? A.scale[adapter] : 1.0f;
     const int quads = rank >> 2, rows = kLoraTile / parts;
-    for (int i = tid; i < rows * quads; i += kDownThreads) {
+    for (int i = tid; i < rows * quads; i += kDownThreads) {        // (whole warps: at least 16 rows of 4 quads)
         const int row = part * rows + i / quads, c = (i % quads) * 4;
         const uint32_t from = smem + (uint32_t) (row * stride + c) * 4u;
         float4 u[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -315,14 +338,25 @@ __global__ void __launch_bounds__(kDownThreads, 1) lora_down_kernel(const Lora A
 #pragma unroll
         for (int p = 0; p < 8; ++p)
             if (p < parts) { v.x += u[p].x; v.y += u[p].y; v.z += u[p].z; v.w += u[p].w; }
-        float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+        if constexpr (!XB || F16) {
+            const float sum = (v.x + v.y) + (v.z + v.w);
+            for (unsigned odd = __ballot_sync(0xffffffffu, sum != sum); odd != 0u; odd &= odd - 1u) {
+                const int who = __ffs(odd) - 1, r = __shfl_sync(0xffffffffu, row, who), q = __shfl_sync(0xffffffffu, c, who);
+                const int t = G.token[(size_t) tile * kLoraTile + r];
+                if (t < 0) continue;
+                const float4 u = plain_z<XB, F16>((const uint8_t*) A.x + (int64_t) t * A.ld_x * (XB ? 2 : 4), (const uint16_t*) A.a + ((size_t) adapter * rank + q) * A.n_in, A.n_in, lane);
+                if (lane == who) v = u;
+            }
+        }
+        float f[4] = {v.x, v.y, v.z, v.w};
         uint16_t* z = G.z + ((size_t) tile * kLoraTile + row) * 3 * rank + c;
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
             uint32_t o[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint32_t a = __float_as_uint(f[2 * j]), b = __float_as_uint(f[2 * j + 1]);
+                const uint32_t a = q < 2 && fabsf(f[2 * j]) == INFINITY ? 0u : __float_as_uint(f[2 * j]);
+                const uint32_t b = q < 2 && fabsf(f[2 * j + 1]) == INFINITY ? 0u : __float_as_uint(f[2 * j + 1]);
                 o[j] = __byte_perm(a, b, 0x7632);
                 f[2 * j] -= __uint_as_float(a & 0xFFFF0000u);
                 f[2 * j + 1] -= __uint_as_float(b & 0xFFFF0000u);
@@ -399,6 +433,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
     };
     uint4 wr[2];
     int adapter = -1;
+    float scale = 1.0f;
     auto fetch = [&](int g) {
         const int n = g * kOutCols + col0;
 #pragma unroll
@@ -446,6 +481,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
         u += g_end - g_first;
         adapter = __ldcg(G.adapter + tile);
         if (adapter < 0 && (A.y == A.out || k0 > 0)) continue;
+        if (adapter >= 0 && A.scale != nullptr) scale = __ldcg(A.scale + adapter);
         __syncthreads();                                      // (the last tile's rows have been looked up)
         if (tid < kLoraTile) tok[tid] = __ldcg(G.token + (size_t) tile * kLoraTile + tid);
         __syncthreads();
@@ -536,9 +572,10 @@ __global__ void __launch_bounds__(kUpThreads, 2) lora_up_kernel(const Lora A, co
                     if constexpr (VEC) {
                         const int row = row0 + 4 * r;
                         const float4 d = turn[row * 8 + ((lane & 7) ^ (row & 7))];
-                        y[4 * r] += d.x; y[4 * r + 1] += d.y; y[4 * r + 2] += d.z; y[4 * r + 3] += d.w;
+                        y[4 * r] = __fmaf_rn(scale, d.x, y[4 * r]); y[4 * r + 1] = __fmaf_rn(scale, d.y, y[4 * r + 1]);
+                        y[4 * r + 2] = __fmaf_rn(scale, d.z, y[4 * r + 2]); y[4 * r + 3] = __fmaf_rn(scale, d.w, y[4 * r + 3]);
                     } else {
-                        y[r] += ((const float*) (turn + r * 8 + ((lane >> 2) ^ (r & 7))))[lane & 3];
+                        y[r] = __fmaf_rn(scale, ((const float*) (turn + r * 8 + ((lane >> 2) ^ (r & 7))))[lane & 3], y[r]);
                     }
                 }
                 __syncwarp();

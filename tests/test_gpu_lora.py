@@ -173,3 +173,47 @@ def test_calls_in_place_that_nobody_takes_part_in(cuda, rank):
         ad.forward(x, none, y, out=y, kernel=api.LORA_MANY)
         ad.forward(x, idx, y, out=o, kernel=api.LORA_MANY)
     assert all(T.equal(o, out) for o in got) and T.equal(y, kept) and ad.error() == 0
+
+
+@pytest.mark.parametrize("act,weights", TYPES)
+@pytest.mark.parametrize("rank,n_out", [(16, 256), (80, 301)])
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_infinities_are_those_of_the_formula(cuda, act, weights, rank, n_out, kernel):
+    """An infinity stays one until it meets another sign, a zero or a NaN, whichever kernel serves the call.  Whether a sum is infinite or no number does not depend on
+    its order (nothing overflows here), so that 64 bits say it.  Adapter 0: positive A, an output's B of one sign; 1: weights of either sign; 2: positive A with zeros; 3:
+    scale 0; 4: all positive."""
+    import torch as T
+    from project_maya_b200 import api
+    g = T.Generator(device="cuda").manual_seed(rank)
+    n, n_in, tokens = 5, 544, 300
+    a, b = T.randn((n, rank, n_in), generator=g, device="cuda") / 16, T.randn((n, n_out, rank), generator=g, device="cuda") / 4
+    a[0], a[2] = a[0].abs() + 0.01, a[2].abs() + 0.01
+    b[0] = (b[0].abs() + 0.01) * T.where(T.arange(n_out, device="cuda") % 2 == 0, 1.0, -1.0)[:, None]
+    a[4], b[4] = a[4].abs() + 0.01, b[4].abs() + 0.01
+    a[0, :, ::2] = 0.125                                                           # (in f16: no second term)
+    a[2, 3, 7] = b[0, 5, 2] = 0.0
+    a, b = a.to(getattr(T, weights)), b.to(getattr(T, weights))
+    scale = T.tensor([0.5, 2.0, -1.0, 0.0, 3.0], device="cuda")
+    idx = (T.arange(tokens, device="cuda") % 7 - 1).int()                          # (-1 and 5: none)
+    clean = T.randn((tokens, n_in), generator=g, device="cuda").to(getattr(T, act))
+    x = clean.clone()
+    x[20:40, 4] = float("inf")
+    x[40:60, 7] = -float("inf")
+    x[60:70, 100], x[60:70, 101] = float("inf"), -float("inf")
+    x[70:80, 543] = float("nan")
+    x[80:100, 300:310] = float("inf")
+    y = T.randn((tokens, n_out), generator=g, device="cuda")
+    y[100:120, 3], y[20:30, 3] = float("inf"), -float("inf")
+    want = y.double()
+    for i in range(n):
+        rows = idx == i
+        want[rows] += float(scale[i]) * (x[rows].double() @ a[i].double().T @ b[i].double().T)
+    ad = api.LoraAdapters(a, b, scale, max_tokens=tokens)
+    out = ad.forward(x, idx, y, kernel=kernel)
+    assert T.equal(out.isnan(), want.isnan())
+    assert T.equal(out.isposinf(), want.isposinf()) and T.equal(out.isneginf(), want.isneginf())
+    assert bool(want[20:60].isposinf().any()) and bool(want[20:60].isneginf().any())
+    same = lambda u, v: T.allclose(u, v, rtol=0.0, atol=0.0, equal_nan=True)       # noqa: E731
+    assert same(out[120:], ad.forward(clean, idx, y, kernel=kernel)[120:])
+    twice = y.clone()
+    assert same(ad.forward(x, idx, twice, out=twice, kernel=kernel), out) and ad.error() == 0
