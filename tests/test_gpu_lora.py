@@ -217,3 +217,48 @@ def test_infinities_are_those_of_the_formula(cuda, act, weights, rank, n_out, ke
     assert same(out[120:], ad.forward(clean, idx, y, kernel=kernel)[120:])
     twice = y.clone()
     assert same(ad.forward(x, idx, twice, out=twice, kernel=kernel), out) and ad.error() == 0
+
+
+@pytest.mark.parametrize("act,weights", TYPES)
+@pytest.mark.parametrize("rank", [16, 64, 80, 256])
+@pytest.mark.parametrize("product", ["first", "second"])
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_operands_keep_their_last_bits(cuda, act, weights, rank, product, kernel):
+    """Pairs of terms that differ in their last bits alone, so that the leading parts cancel and only the least are left.  All values are whole numbers times one power of two,
+    every product and every sum of any order is one below 2^24: nothing rounds, and the result is equal to the whole numbers'."""
+    import torch as T
+    from project_maya_b200 import api
+    rng = np.random.default_rng(rank)
+    n, n_in, tokens = 3, 544, 300
+    at = rng.permutation(n_in)
+    idx = rng.integers(-1, n, tokens).astype(np.int32)
+    x_most, w_most = 24 if act == "float32" else 8, 11 if weights == "float16" else 8
+    half = rank // 2
+    ranks = rng.permutation(rank)
+    pairs = rank if product == "first" else half
+    p, q = (at[:rank], at[rank:2 * rank]) if product == "first" else (at[ranks[:half]], at[ranks[half:]])         # where a pair's values lie in x
+    whole = lambda bits, shape: rng.integers(1 << (bits - 1), 1 << bits, shape)    # noqa: E731
+    other = lambda v, low: (v >> low << low) + rng.integers(0, 1 << low, v.shape)  # noqa: E731
+    for x_bits, x_low, w_bits, w_low in ((x_most, x_most // 3, 1, 0), (1, 0, w_most, 3), (min(x_most, 12), 3, w_most, 3)):
+        X = np.where(rng.random((tokens, n_in)) < 0.5, 1, -1) * whole(x_bits, (tokens, n_in))
+        m, w = whole(x_bits, (tokens, pairs)), whole(w_bits, (n, pairs)) * np.where(rng.random((n, pairs)) < 0.5, 1, -1)
+        m2, w2 = other(m, x_low), np.sign(w) * other(abs(w), w_low)
+        X[:, p], X[:, q] = m, m2
+        A, B = np.zeros((n, rank, n_in), np.int64), np.zeros((n, rank + 3, rank), np.int64)
+        out_at = np.arange(pairs)
+        if product == "first":
+            A[:, out_at, p], A[:, out_at, q] = w, -w2
+            B[:, out_at, out_at] = 1
+        else:
+            A[:, np.arange(rank), at[:rank]] = 1
+            B[:, out_at, ranks[:half]], B[:, out_at, ranks[half:]] = w, -w2
+        want = np.zeros((tokens, rank + 3))
+        has = idx >= 0
+        want[has, :pairs] = (w[idx] * m - w2[idx] * m2)[has]
+        x, a, b = (T.from_numpy(v.astype(np.float64)).cuda().to(getattr(T, t)) for v, t in ((X * 2.0 ** -9, act), (A, weights), (B, weights)))
+        assert T.equal(x.double().cpu(), T.from_numpy(X * 2.0 ** -9)) and np.abs(want).max() < 2.0 ** 24
+        for n_out in (rank + 3, rank):
+            ad = api.LoraAdapters(a, b[:, :n_out].contiguous(), max_tokens=tokens)
+            out = ad.forward(x, T.from_numpy(idx).cuda(), kernel=kernel)
+            assert T.equal(out.double().cpu(), T.from_numpy(want[:, :n_out] * 2.0 ** -9))
+        assert ad.error() == 0 and bool((want != 0).any())
