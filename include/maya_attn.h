@@ -57,7 +57,7 @@ typedef struct maya_attn_batch {
  * table hold block b (0 or less: free); table entries of -1 hold none.  A call that needs blocks gets the free ones of the lowest numbers in the order of
  * asking: of those that are free when it begins, so that what a call frees can be had by the next.  When there are too few, the entries left without are -1 and
  * the scratch's error word is set (sticky).  Nothing here reads or writes a block or sequence outside what the descriptor says: such numbers in device
- * memory are passed over.  One scratch serves one stream at a time. */
+ * memory are passed over.  64 * table_ld is below 2^31.  One scratch serves one stream at a time. */
 #define MAYA_MAX_PAGES (1 << 20)   /* blocks of a descriptor */
 typedef struct maya_kv_layer {
     void* k;

@@ -54,6 +54,7 @@ int pages_check(const maya_kv_pages* p) {
     if (!p || !p->layers || !p->table || !p->refs || p->n_seq <= 0 || p->table_ld <= 0 || p->n_blocks <= 0 || p->n_layers <= 0 || p->n_kv <= 0) return MAYA_ERR_ARG;
     if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 192 && p->head_dim != 256) return MAYA_ERR_LIMIT;
     if (p->n_blocks > MAYA_MAX_PAGES || p->n_seq > 65535 || (int64_t) p->n_seq * p->table_ld > (1 << 28) || p->n_layers > 1024 || p->n_kv > 65535) return MAYA_ERR_LIMIT;
+    if ((int64_t) p->table_ld * kKvBlock > 0x7FFFFFFF) return MAYA_ERR_LIMIT;        // (tokens of a row are counted in an int)
     return MAYA_OK;
 }
 int pages_ready(const maya_kv_pages* p, Pages* v) {

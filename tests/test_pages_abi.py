@@ -72,3 +72,13 @@ def test_caches_of_other_tables_or_shapes_are_refused(monkeypatch):
         pages.compact()
     with pytest.raises(AssertionError):
         api.KvPages([a], refs=T.zeros(7, dtype=T.int32))
+
+
+def test_rows_of_more_tokens_than_an_int_counts_are_refused(lib):
+    """64 * table_ld is a number of tokens: at 2^25 blocks a row it would wrap, and a fork would leave the children nothing."""
+    assert lib.maya_pages_scratch_bytes(desc(n_seq=1, table_ld=(1 << 25) - 1)) > 0
+    for wide in (1 << 25, 1 << 26):
+        d = desc(n_seq=1, table_ld=wide)
+        assert lib.maya_pages_scratch_bytes(d) == 0
+        assert lib.maya_pages_fork(d, P, P, P, 1, None) == LIMIT and lib.maya_pages_reserve(d, batch(n_seq=1), None) == LIMIT
+        assert lib.maya_pages_free(d, P, 1, None) == LIMIT and lib.maya_pages_compact(d, 1, None) == LIMIT and lib.maya_pages_copy(d, P, P, 1, None) == LIMIT
