@@ -200,6 +200,7 @@ class LoraAdapters:
         n_out = b.shape[1]
         assert b.shape == (n, n_out, rank) and a.dtype is b.dtype and a.dtype in (torch.bfloat16, torch.float16)
         assert scale is None or (scale.dtype is torch.float32 and scale.shape == (n,))
+        assert b.device == a.device and (scale is None or scale.device == a.device), "a, b and scale of one device expected"
         wide = -(-rank // 16) * 16
         if wide != rank:
             a, b = torch.nn.functional.pad(a, (0, 0, 0, wide - rank)), torch.nn.functional.pad(b, (0, wide - rank))

@@ -48,3 +48,12 @@ def test_adapters_of_other_shapes_or_types_are_refused(monkeypatch):
         api.LoraAdapters(a[..., :40].contiguous(), b)
     with pytest.raises(api.MayaError):                       # tensors of the CPU
         ad.forward(T.zeros((1, 64)), T.zeros(1, dtype=T.int32))
+
+
+def test_adapters_on_two_devices_are_refused(monkeypatch):
+    """b and scale go to the kernels by address: they have to lie where a does."""
+    monkeypatch.setattr(api, "_ptr", lambda t: None if t is None else t.data_ptr())
+    a, b = T.zeros((2, 16, 64)).half(), T.zeros((2, 96, 16)).half()
+    for args in ((a, b.to("meta")), (a, b, T.ones(2, device="meta"))):
+        with pytest.raises(AssertionError):
+            api.LoraAdapters(*args)
