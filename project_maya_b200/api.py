@@ -893,6 +893,7 @@ class KvPages:
         shape = lambda c: (c.table.data_ptr(), c.table.shape, c.n_blocks, c.n_kv, c.head_dim, c.k_sum is None, c.k.device)   # noqa: E731
         assert all(shape(c) == shape(first) for c in caches), "caches of one table and one shape expected"
         dev, table = first.k.device, first.table
+        assert all(t is None or t.device == dev for c in caches for t in (c.v, c.k_scale, c.v_scale, c.table, c.k_sum)), "caches on one device expected"
         if refs is None:
             held = table[(table >= 0) & (table < first.n_blocks)].long()
             refs = torch.bincount(held, minlength=first.n_blocks).to(torch.int32)

@@ -82,3 +82,15 @@ def test_rows_of_more_tokens_than_an_int_counts_are_refused(lib):
         assert lib.maya_pages_scratch_bytes(d) == 0
         assert lib.maya_pages_fork(d, P, P, P, 1, None) == LIMIT and lib.maya_pages_reserve(d, batch(n_seq=1), None) == LIMIT
         assert lib.maya_pages_free(d, P, 1, None) == LIMIT and lib.maya_pages_compact(d, 1, None) == LIMIT and lib.maya_pages_copy(d, P, P, 1, None) == LIMIT
+
+
+def test_caches_in_parts_on_two_devices_are_refused(monkeypatch):
+    """A cache's buffers go to the kernels by address: they all have to lie where the table does."""
+    monkeypatch.setattr(api, "_ptr", lambda t: None if t is None else t.data_ptr())
+    table = T.full((2, 4), -1, dtype=T.int32)
+    c = api.KvCache.empty(8, 2, 64, table)
+    parts = dict(k=c.k, v=c.v, k_scale=c.k_scale, v_scale=c.v_scale, table=table, k_sum=c.k_sum)
+    assert api.KvPages([api.KvCache(**parts)]).n_blocks == 8
+    for name in parts:
+        with pytest.raises(AssertionError):
+            api.KvPages([api.KvCache(**{**parts, name: parts[name].to("meta")})], refs=T.zeros(8, dtype=T.int32))
