@@ -475,9 +475,9 @@ extern "C" int maya_pages_fork(const maya_kv_pages* p, const int* parents, const
     if (n < 0 || !parents || !children || !lens) return refuse(MAYA_ERR_ARG);
     if (n > p->n_seq) return refuse(MAYA_ERR_LIMIT);              // more pairs than children there are
     cudaStream_t s = as_stream(stream);
-    // A warp makes a row of up to 2048 blocks in the plan's launch (32 rows of 26, with the step behind it: 14.6 us, 15.3 in a launch of their own), longer or more ones take a launch with a
-    // thread block each.
-    const bool rows_too = (int64_t) n * p->table_ld <= 16384;
+    // A warp a row in the plan's launch while there is one for each and a row is three looks long, otherwise a launch with a thread block a row.  Both ways, plan's / own (the fork alone, us): 32
+    // rows of 64 blocks 9.3 / 9.3, one 8.3 / 8.6; 64 rows of 64 11.0 / 9.3; one row of 256 10.9 / 9.0, of 16384 222 / 45.
+    const bool rows_too = n <= kPlan / 32 && p->table_ld <= 96;
     launch_dependent(pages_fork_kernel, dim3(1), dim3(kPlan), 0, s, P, parents, children, lens, n, (int) rows_too);
     int launched = note_launch("kv_pages fork");
     if (launched != MAYA_OK) return launched;

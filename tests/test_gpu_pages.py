@@ -433,3 +433,21 @@ def test_forked_sequences_attend_as_if_they_had_their_own_blocks(cuda):
     pages.compact()
     step([1, 0, 1], [22, 0, 132])
     assert pages.error() == 0 and attn.error() == 0
+
+
+@pytest.mark.parametrize("wide,n", [(96, 32), (96, 33), (97, 32), (5000, 1)])
+def test_forks_on_both_sides_of_the_choice(cuda, wide, n):
+    """The most rows and blocks a row that the plan's thread block takes, one more of each, and a single long row."""
+    import torch as T
+    rng = np.random.default_rng(wide + n)
+    S, nb = 40, 6000
+    lens = [int(v) for v in rng.integers(1, min(wide, 100) * BLOCK, S)]
+    if n == 1:
+        lens[7] = 4000 * BLOCK + 5
+    host = Host(rng, S, wide, nb + 4000 * (n == 1), 1, 1, 64).fill(rng, lens)
+    pages = host.device(T)
+    p, c = ([7], [3]) if n == 1 else (rng.integers(0, S, n).tolist(), rng.permutation(S)[:n].tolist())
+    k = [lens[a] - 2 if lens[a] > 2 else lens[a] for a in p]
+    host.fork(p, c, k)
+    pages.fork(i32(T, p), i32(T, c), i32(T, k))
+    host.same(T, pages)
