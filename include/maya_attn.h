@@ -56,7 +56,9 @@ typedef struct maya_attn_batch {
 /* The blocks of the caches of n_layers layers that share one table, handed out and taken back on the device.  refs[b] says how many entries of the
  * table hold block b (0 or less: free); table entries of -1 hold none.  A call that needs blocks gets the free ones of the lowest numbers in the order of
  * asking: of those that are free when it begins, so that what a call frees can be had by the next.  When there are too few, the entries left without are -1 and
- * the scratch's error word is set (sticky).  Nothing here reads or writes a block or sequence outside what the descriptor says: such numbers in device
+ * the scratch's error word is set (sticky).  Tokens from before that such an entry was to go on with - in a shared block that reserve was to replace, in the last block
+ * of a fork - are then lost to the sequence, which is the one with -1 in front of its length; a later reserve gives it a block, not those tokens.  Free it and prefill it
+ * again, or ask with blocks to spare (a batch needs one for each shared block that it goes on in, and those for its new tokens).  Nothing here reads or writes a block or sequence outside what the descriptor says: such numbers in device
  * memory are passed over.  64 * table_ld is below 2^31.  One scratch serves one stream at a time. */
 #define MAYA_MAX_PAGES (1 << 20)   /* blocks of a descriptor */
 typedef struct maya_kv_layer {

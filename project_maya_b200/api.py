@@ -886,7 +886,8 @@ class KvPages:
     """The blocks of one or more layers' caches (KvCaches over one table, of one shape), handed out, shared and taken back on the device: nothing here
     waits for the GPU, and captured calls do in a replay what they would then do.  refs i32 [n_blocks]: how many entries of the table hold a block (0: free; None:
     counted from the table here).  Table entries without a block are -1.  A call that needs blocks gets the free ones of the lowest numbers, of those that are
-    free when it begins; too few leave -1 behind, and error() says so.  One thread and one stream at a time (include/maya_attn.h)."""
+    free when it begins; too few leave -1 behind, and error() says so: a sequence with -1 in front of its length has lost the tokens of that block - free it and prefill
+    it again.  One thread and one stream at a time (include/maya_attn.h)."""
 
     def __init__(self, caches, refs=None):
         first = caches[0]

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kPlan) pages_reserve_kernel(const Pages P, con
         const int fresh = r < got ? P.list[r] : -1;
         if (fresh >= 0) P.refs[fresh] = 1;
         if (is_block(P, e)) {
-            atomicSub(P.refs + e, 1);
+            atomicSub(P.refs + e, 1);                         // (also without a fresh one: new tokens must not go into a block that others hold)
             if (held && fresh >= 0) {
                 const int m = atomicAdd(&s_moves, 1);
                 P.src[m] = e;

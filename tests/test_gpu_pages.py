@@ -451,3 +451,29 @@ def test_forks_on_both_sides_of_the_choice(cuda, wide, n):
     host.fork(p, c, k)
     pages.fork(i32(T, p), i32(T, c), i32(T, k))
     host.same(T, pages)
+
+
+def test_a_shortage_loses_what_stood_in_a_block_that_was_to_be_replaced(cuda):
+    """Two sequences share the block that both go on in, and none is free: both entries are -1, the tokens in them are lost to both, a later reserve gives blocks and not
+    their tokens.  Who holds other blocks keeps them; prefilled from the start, the two are whole again."""
+    import torch as T
+    rng = np.random.default_rng(8)
+    host = Host(rng, 3, 3, 4, 1, 1, 64).fill(rng, [100, 0, 128])
+    pages = host.device(T)
+    host.fork([0], [1], [64])
+    pages.fork(i32(T, [0]), i32(T, [1]), i32(T, [64]))
+    host.table[1, 1] = host.table[0, 1]                                            # (shared by the caller)
+    host.refs[host.table[0, 1]] = 2
+    pages.table.copy_(T.from_numpy(host.table))
+    pages.refs.copy_(T.from_numpy(host.refs))
+    kept = host.table[2].copy()
+    host.reserve([1, 1, 0], [101, 101, 0])
+    pages.reserve(batch_of([1, 1, 0], [101, 101, 0]))
+    assert host.error == 1 and (host.table[:2, 1] == -1).all() and (host.table[2] == kept).all()
+    host.same(T, pages)
+    host.free([0, 1])
+    pages.free(i32(T, [0, 1]))
+    host.reserve([101, 0, 0], [101, 0, 0])
+    pages.reserve(batch_of([101, 0, 0], [101, 0, 0]))
+    assert host.error == 0 and (host.table[0, :2] >= 0).all() and (host.table[2] == kept).all()
+    host.same(T, pages)
