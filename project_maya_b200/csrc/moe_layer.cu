@@ -136,7 +136,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs P) {
             const int e = route.ids[tid];
             w = route.val[tid];
             if (e >= P.lo && e < P.hi) p = (unsigned long long) (P.experts + (size_t) e * P.stride);
-            if constexpr (RT != 2) {
+            if constexpr (RT == 2) {
+                if (p == 0ull) w = 0.0f;                         // (a skipped entry adds w * 0: the caller's may be no number)
+            } else {
                 P.ids[(size_t) t * P.k + tid] = e;
                 P.weights[(size_t) t * P.k + tid] = w;
             }

@@ -250,3 +250,24 @@ def test_large_biases_that_cancel_in_a_group(cuda, sigmoid, large, where):
     assert T.equal(ids.long(), want)
     p = s.gather(1, want)
     assert bool(((w.double() - p / p.sum(-1, keepdim=True)).abs() <= 2.0 ** -23).all())
+
+
+def test_routed_layer_takes_nothing_from_the_weights_of_ids_that_are_none(cuda):
+    """Whatever stands in a masked place - an infinity, NaN - the output is that of a weight of 0 there; an id given twice counts twice."""
+    import torch as T
+    from project_maya_b200 import api
+    cfg = layer_config(api)
+    blobs = experts_of(T, api, cfg)
+    x, w = T.randn((5, 512), device="cuda"), T.rand((5, 4), device="cuda")
+    ids = T.tensor([[1, -1, 5, 40], [-1, -7, 32, 1 << 30], [2, 3, 4, -1], [6, 6, 6, 6], [7, 1, 7, -1]], dtype=T.int32, device="cuda")
+    none = (ids < 0) | (ids >= 32)
+    for layer in (api.MoeLayer(cfg, blobs, staged=True), api.MoeLayer(cfg, blobs, expert_range=(0, 5))):
+        want = layer.forward_routed(ids, w.masked_fill(none, 0.0), x)
+        assert bool(want.isfinite().all()) and bool((want[1] == 0).all())
+        for odd in (float("nan"), float("inf"), -float("inf"), 3e38):
+            assert T.equal(layer.forward_routed(ids, w.masked_fill(none, odd), x), want)
+        assert layer.error() == 0
+    once = T.tensor([[6, -1, -1, -1]], dtype=T.int32, device="cuda")
+    layer = api.MoeLayer(cfg, blobs, staged=True)
+    four, one = layer.forward_routed(ids[3:4], w[3:4], x[3:4]), layer.forward_routed(once, T.stack([w[3].sum()] + [w[3, 0]] * 3)[None], x[3:4])
+    assert bool(((four - one).abs() <= 2.0 ** -21 * w[3].sum() * (one / w[3].sum()).abs()).all())        # (four products and sums of one sign, each rounded: 8 * 2^-24)
