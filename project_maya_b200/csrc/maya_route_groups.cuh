@@ -285,7 +285,7 @@ __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, 
         }
         const bool keeps = mine && rank < A.n_keep;
         const unsigned kept = __ballot_sync(0xffffffffu, keeps);
-        const float err = 0.5f * fixed + of_itself * (A.top2 && b != 0u ? fabsf(value(a)) + fabsf(value(b)) : fabsf(score));
+        const float err = 0.5f * (fixed + of_itself * (A.top2 && b != 0u ? fabsf(value(a)) + fabsf(value(b)) : fabsf(score)));        // (half of what two have to be apart)
         const unsigned in = __reduce_min_sync(0xffffffffu, keeps ? ordered(score - err) : 0xffffffffu);
         const unsigned out = __reduce_max_sync(0xffffffffu, mine && !keeps ? ordered(score + err) : 0u);
         if (!(in > out)) return false;         // (all lanes alike)
