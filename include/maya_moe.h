@@ -97,8 +97,8 @@ MAYA_API int maya_router_sigmoid(const float* logits, const float* bias, int n_t
  *   s = softmax(logits) or 1 / (1 + exp(-logit)); c = s + bias (bias NULL: s); a group of n_expert / n_group experts scores its highest c, or with top2
  *   the sum of its two highest; the n_keep best groups are kept (ties: the lower group), of their experts the k highest c are chosen (ties: the lower
  *   expert), in that order; weights = s, divided by max(their sum, 2^-14) when norm_w, times w_scale.  In 64 bits, the weights rounded once.
- * A score that is no number (a NaN logit; any logit of a softmax row with a NaN or +inf) ranks behind every other; a softmax row of nothing but -inf has
- * scores of 0.  n_group = n_keep = 1: no groups.  n_expert <= 2048, k <= 64, n_group <= 32 and a divisor of n_expert, k <= n_keep * n_expert / n_group. */
+ * A score that is no number (a NaN logit; any logit of a softmax row with a NaN or +inf) ranks behind every other; one that is chosen all the same leaves a
+ * normalised token no weight that is a number.  A softmax row of nothing but -inf has scores of 0.  n_group = n_keep = 1: no groups.  n_expert <= 2048, k <= 64, n_group <= 32 and a divisor of n_expert, k <= n_keep * n_expert / n_group. */
 typedef struct maya_route_args {
     const float* logits;         /* [n_tokens][n_expert] */
     const float* bias;           /* [n_expert] or NULL */

@@ -169,7 +169,7 @@ __device__ __noinline__ void route_exact(const RouteGroups& A, int64_t token, un
         for (int j = 0; j < PER; ++j)
             if (j * 32 + lane == e) o[j] = 0ull;
     }
-    const double div = A.norm_w ? fmax(sum, 6.103515625e-05) : 1.0;       // 2^-14
+    const double div = !A.norm_w ? 1.0 : sum < 6.103515625e-05 ? 6.103515625e-05 : sum;        // 2^-14; a sum that is no number stays one
 #pragma unroll
     for (int j = 0; j < 2; ++j) w[j] = (float) (mine[j] / div * (double) A.w_scale);
 }
@@ -328,7 +328,7 @@ __device__ __forceinline__ bool route_fast(const RouteGroups& A, int64_t token, 
     const double sum = warp_sum64(v[0] + v[1]);
     // a softmax's scores lack the division by the sum of all, which nothing but the least divisor asks for: far from it, or in 64 bits
     if (!A.sigmoid && !(sum > 2.0 * 6.103515625e-05 * (double) all)) return false;
-    const double div = A.sigmoid ? (A.norm_w ? fmax(sum, 6.103515625e-05) : 1.0) : sum;
+    const double div = A.sigmoid ? (A.norm_w ? fmax(sum, 6.103515625e-05) : 1.0) : sum;        // (scores are numbers here)
 #pragma unroll
     for (int j = 0; j < 2; ++j) w[j] = (float) (v[j] / div * (double) A.w_scale);
     return true;

@@ -271,3 +271,18 @@ def test_routed_layer_takes_nothing_from_the_weights_of_ids_that_are_none(cuda):
     layer = api.MoeLayer(cfg, blobs, staged=True)
     four, one = layer.forward_routed(ids[3:4], w[3:4], x[3:4]), layer.forward_routed(once, T.stack([w[3].sum()] + [w[3, 0]] * 3)[None], x[3:4])
     assert bool(((four - one).abs() <= 2.0 ** -21 * w[3].sum() * (one / w[3].sum()).abs()).all())        # (four products and sums of one sign, each rounded: 8 * 2^-24)
+
+
+@pytest.mark.parametrize("top2", [True, False])
+@pytest.mark.parametrize("keep,k", [(3, 30), (3, 31), (2, 20), (1, 10)])
+def test_choices_that_run_out_of_numbers(cuda, top2, keep, k):
+    """Fewer scores that are numbers than choices: NaN are chosen, and a sum with one is none, so no weight of a normalised token is a number."""
+    import torch as T
+    rng = np.random.default_rng(10 * keep + k)
+    logits = rng.standard_normal((20, 42)).astype(np.float32)
+    logits[:, ::4] = np.nan
+    logits[4, ::2] = np.nan
+    logits[7] = 0.5
+    for w_scale in (1.0, -1.0):
+        for norm_w in (True, False):
+            check(T, logits, k, n_group=3, n_keep=keep, norm_w=norm_w, top2=top2, w_scale=w_scale)
